@@ -1,0 +1,585 @@
+"""Tensor.topk, F.distillation_loss and F.sample_logits against plain numpy in
+64 bits."""
+import math
+import types
+
+import numpy as np
+import pytest
+
+gpu = pytest.mark.gpu
+U = 2.0 ** -24  # half a step of float32, relative
+
+
+# ------------------------------------------------------------------- oracles
+
+
+def topk_ref(x, k, largest=True):
+    """Indices [rows, k]: NaN the largest, equal values by ascending index."""
+    n = x.shape[1]
+    x = x.astype(np.float64) + 0.0
+    nan = np.isnan(x)
+    v = np.where(nan, 0.0, x)
+    idx = np.broadcast_to(np.arange(n), x.shape)
+    order = np.lexsort((idx, -v, ~nan) if largest else (idx, v, nan), axis=1)
+    return order[:, :k]
+
+
+def sample_ref(x, u, t=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """One row's index by the definition, each rule over the sorted row."""
+    x = x.astype(np.float64)
+    m = x.max()
+    if np.isnan(x).any() or not math.isfinite(m):
+        return -1
+    if not t > 0:
+        return int(np.argmax(x == m))
+    order = np.lexsort((np.arange(x.size), -x))
+    z = x[order] - m
+    with np.errstate(invalid="ignore"):
+        w = np.exp(np.where(np.isinf(z), -np.inf, z / t))
+    keep = np.ones(x.size, bool)
+    if 0 < top_k < x.size:
+        keep &= np.arange(x.size) < top_k
+    if top_p < 1:
+        before = np.concatenate([[0.0], np.cumsum(np.where(keep, w, 0.0))[:-1]])
+        keep &= before < max(top_p, 1e-300) * np.where(keep, w, 0.0).sum()
+    if min_p > 0:
+        keep &= z >= min(t * math.log(min_p), 0.0)
+    keep[0] = True
+    w = np.where(keep, w, 0.0)
+    kept = np.zeros(x.size)
+    kept[order] = w
+    cum = np.cumsum(kept)
+    hit = np.nonzero((cum > u * cum[-1]) & (kept > 0))[0]
+    return int(hit[0]) if hit.size else int(np.nonzero(kept > 0)[0][-1])
+
+
+def distill_ref(x, v, ids, t):
+    """(per-row loss, per-row gradient of it, valid rows, the sizes that
+    float32 roundings scale with: of the loss and of the gradient)."""
+    x, v = x.astype(np.float64), v.astype(np.float64)
+    rows, n = x.shape
+    loss, grad, valid = np.zeros(rows), np.zeros((rows, n)), np.zeros(rows, bool)
+    lsize, gsize = np.zeros(rows), np.zeros((rows, n))
+    for r in range(rows):
+        lq = x[r] / t - x[r].max() / t
+        lq = lq - np.log(np.exp(lq).sum())
+        at = [i for i in range(ids.shape[1]) if 0 <= ids[r, i] < n and v[r, i] > -np.inf]
+        if not at:
+            continue
+        valid[r] = True
+        lp = v[r, at] / t - v[r, at].max() / t
+        lp = lp - np.log(np.exp(lp).sum())
+        p = np.exp(lp)
+        loss[r] = t * t * (p * (lp - lq[ids[r, at]])).sum()
+        lsize[r] = t * t * (p * (np.abs(lp) + np.abs(lq[ids[r, at]]) + 1)).sum()
+        grad[r] = t * np.exp(lq)
+        gsize[r] = grad[r] * (1 + np.abs(lq))
+        np.add.at(grad[r], ids[r, at], -t * p)
+        np.add.at(gsize[r], ids[r, at], t * p * (1 + np.abs(lp)))
+    return loss, grad, valid, lsize, gsize
+
+
+# --------------------------------------------------------------------- top-k
+
+
+NS = [1, 2, 3, 5, 6, 7, 63, 255, 1000, 1023, 1024, 1025, 1029, 4096, 4097, 16384, 16387, 50257,
+      53248, 53249, 70001]
+
+
+@gpu
+@pytest.mark.parametrize("n", NS)
+def test_topk(torch, n):
+    rng = np.random.default_rng(n)
+    for k in sorted({1, 2, 20, 64, 255, 257, 1024, n // 2, n}):
+        if not 0 < k <= min(n, 1024):
+            continue
+        for largest in (True, False):
+            x = rng.standard_normal((3, n)).astype(np.float32) * 3
+            v, i = torch.tensor(x).topk(k, largest=largest)
+            ref = topk_ref(x, k, largest)
+            assert i.dtype == "int32" and v.shape == i.shape == (3, k)
+            np.testing.assert_array_equal(i.numpy(), ref, err_msg="k=%d %s" % (k, largest))
+            np.testing.assert_array_equal(v.numpy(), np.take_along_axis(x, ref, 1))
+
+
+@gpu
+@pytest.mark.parametrize("n", [6, 500, 3000, 9000, 50257, 60000])
+@pytest.mark.parametrize("kind", ["equal", "few", "zeros", "nan", "infinite", "masked", "sorted"])
+def test_topk_ties_and_specials(torch, n, kind):
+    rng = np.random.default_rng(n)
+    x = rng.standard_normal((2, n)).astype(np.float32)
+    if kind == "equal":
+        x[:] = 1.5
+    elif kind == "few":
+        x = rng.integers(-2, 3, (2, n)).astype(np.float32)
+    elif kind == "zeros":
+        x = np.where(rng.random((2, n)) < 0.5, np.float32(0.0), np.float32(-0.0))
+    elif kind == "nan":
+        x[:, :: 3] = np.nan
+    elif kind == "infinite":
+        x[:, :: 4], x[:, 1 :: 4] = np.inf, -np.inf
+    elif kind == "masked":
+        x[:, 5:] = -np.finfo(np.float32).max
+        x[1] = -np.inf
+    elif kind == "sorted":
+        x = np.sort(x, axis=1)
+    for k in (1, 3, min(n, 40), min(n, 700)):
+        for largest in (True, False):
+            v, i = torch.tensor(x).topk(k, largest=largest)
+            ref = topk_ref(x, k, largest)
+            np.testing.assert_array_equal(i.numpy(), ref, err_msg="k=%d %s" % (k, largest))
+            np.testing.assert_array_equal(v.numpy(), np.take_along_axis(x, ref, 1))
+
+
+@gpu
+def test_topk_layouts(torch):
+    rng = np.random.default_rng(0)
+    x = rng.standard_normal((4, 37, 11)).astype(np.float32)
+    t = torch.tensor(x)
+    for dim in (0, 1, 2, -1, -2):
+        v, i = t.topk(3, dim=dim)
+        ref = np.argsort(-x, axis=dim, kind="stable").take(range(3), axis=dim)
+        np.testing.assert_array_equal(i.numpy(), ref)
+        np.testing.assert_array_equal(v.numpy(), np.take_along_axis(x, ref, dim))
+    # rows at every alignment, and rows wider apart than they are long
+    w = rng.standard_normal((5, 1234)).astype(np.float32)
+    for lo in range(5):
+        view = torch.tensor(w)[:, lo:lo + 1001]
+        np.testing.assert_array_equal(view.topk(9)[1].numpy(), topk_ref(w[:, lo:lo + 1001], 9))
+    one = torch.tensor(w[0])
+    np.testing.assert_array_equal(one.topk(5)[1].numpy(), topk_ref(w[:1], 5)[0])
+    v, i = torch.tensor(np.float32(3.0).reshape(())).topk(1)
+    assert v.shape == i.shape == () and v.item() == 3.0 and i.item() == 0
+    assert torch.tensor(w).topk(0)[0].shape == (5, 0)
+    assert torch.zeros(0, 7).topk(2)[1].shape == (0, 2)
+    ints = torch.tensor(np.array([[3, 9, 9, 1]], np.int32))
+    assert ints.topk(2)[1].numpy().tolist() == [[1, 2]]
+
+
+@gpu
+@pytest.mark.parametrize("shape,k,dim", [((5, 1000), 8, -1), ((3, 50257), 64, -1), ((2, 6, 7), 3, 1),
+                                         ((1, 3), 3, -1)])
+def test_topk_gradient(torch, shape, k, dim):
+    rng = np.random.default_rng(k)
+    x = rng.standard_normal(shape).astype(np.float32)
+    t = torch.tensor(x, requires_grad=True)
+    v, i = t.topk(k, dim=dim)
+    g = rng.standard_normal(v.shape).astype(np.float32)
+    v.backward(torch.tensor(g))
+    ref = np.zeros(shape, np.float32)
+    np.put_along_axis(ref, i.numpy().astype(np.int64), g, dim)
+    np.testing.assert_array_equal(t.grad.numpy(), ref)
+    # through a differentiable backward: d/dx of (d sum v^2 / dx)^2
+    t2 = torch.tensor(x, requires_grad=True)
+    v2, _ = t2.topk(k, dim=dim)
+    (d,) = torch.autograd.grad((v2 * v2).sum(), t2, create_graph=True)
+    (dd,) = torch.autograd.grad((d * d).sum(), t2)
+    ref = np.zeros(shape, np.float32)
+    np.put_along_axis(ref, i.numpy().astype(np.int64), 8 * v.numpy(), dim)
+    np.testing.assert_allclose(dd.numpy(), ref, rtol=8 * U)
+
+
+# ------------------------------------------------------------------ sampling
+
+
+def _settings():
+    for top_k in (0, 1, 2, 50, 300, 2000):
+        for top_p in (1.0, 0.9, 0.3, 0.0):
+            for min_p in (0.0, 0.05, 1.0):
+                yield top_k, top_p, min_p
+
+
+@gpu
+@pytest.mark.parametrize("n", [1, 2, 3, 5, 7, 200, 1027, 4096, 4097, 4101, 16384, 16391, 50257, 53252,
+                               53253, 70001])
+def test_sample_logits(torch, n):
+    rng = np.random.default_rng(n)
+    rows = 4
+    for i, (top_k, top_p, min_p) in enumerate(_settings()):
+        t = (1.0, 0.7, 1.3)[i % 3]
+        x = (rng.standard_normal((rows, n)) * 2.5).astype(np.float32)
+        u = rng.random(rows).astype(np.float32)
+        got = torch.functional.sample_logits(torch.tensor(x), torch.tensor(u), t, top_k, top_p, min_p)
+        ref = [sample_ref(x[r], float(u[r]), t, top_k, top_p, min_p) for r in range(rows)]
+        assert got.dtype == "int32" and got.numpy().tolist() == ref, (top_k, top_p, min_p, t)
+
+
+@gpu
+@pytest.mark.parametrize("n", [5, 900, 5000, 50257, 60001])
+@pytest.mark.parametrize("kind", ["equal", "few", "one", "masked", "lowest", "flat", "sharp"])
+def test_sample_logits_ties_and_masks(torch, n, kind):
+    rng = np.random.default_rng(n)
+    rows = 3
+    x = rng.standard_normal((rows, n)).astype(np.float32)
+    if kind == "equal":
+        x[:] = -2.25
+    elif kind == "few":
+        x = rng.integers(0, 3, (rows, n)).astype(np.float32)
+    elif kind == "one":
+        x[:] = -np.inf
+        x[np.arange(rows), [0, n // 2, n - 1]] = 0.5
+    elif kind == "masked":
+        x[:, ::2] = -np.inf
+    elif kind == "lowest":
+        x[:, ::3] = -np.finfo(np.float32).max
+        x[1] = -np.finfo(np.float32).max
+    elif kind == "flat":
+        x *= 1e-4
+    elif kind == "sharp":
+        x *= 1e30
+    for top_k, top_p, min_p in ((0, 1.0, 0.0), (0, 0.7, 0.0), (3, 1.0, 0.0), (400, 0.5, 0.0),
+                                (1500, 0.9, 0.0), (0, 1.0, 0.5), (4, 0.6, 0.2)):
+        u = rng.random(rows).astype(np.float32)
+        got = torch.functional.sample_logits(torch.tensor(x), torch.tensor(u), 1.0, top_k, top_p, min_p)
+        ref = [sample_ref(x[r], float(u[r]), 1.0, top_k, top_p, min_p) for r in range(rows)]
+        assert got.numpy().tolist() == ref, (top_k, top_p, min_p)
+
+
+@gpu
+@pytest.mark.parametrize("n", [9, 4099, 50257, 60001])
+def test_sample_logits_ends(torch, n):
+    """The smallest and largest uniforms, greedy rows, extreme temperatures
+    and rows without a distribution."""
+    F = torch.functional
+    rng = np.random.default_rng(n)
+    x = rng.uniform(-3, 3, (6, n)).astype(np.float32)
+    for kw in ({}, {"top_k": 5}, {"top_p": 0.5}, {"min_p": 0.3}):
+        # u = 1 is past every running sum: the last kept index
+        for u in (0.0, 0.99999994, 1.0):
+            got = F.sample_logits(torch.tensor(x), np.full(6, u, np.float32), **kw)
+            ref = [sample_ref(r, float(np.float32(u)), 1.0, **kw) for r in x]
+            assert got.numpy().tolist() == ref, (kw, u)
+    y = x.copy()
+    y[:, [n // 3, n - 1]] = 4.0
+    assert F.sample_logits(torch.tensor(y), np.zeros(6, np.float32), 0.0).numpy().tolist() == [n // 3] * 6
+    u = rng.random(6).astype(np.float32)
+    for t in (1e-30, 1e-6, 1e30, math.inf):
+        for top_p in (1.0, 0.4):
+            got = F.sample_logits(torch.tensor(x), u, t, top_p=top_p).numpy().tolist()
+            assert got == [sample_ref(x[r], float(u[r]), t, top_p=top_p) for r in range(6)], (t, top_p)
+    bad = x.copy()
+    bad[0, n - 1], bad[1, 0], bad[2] = np.nan, np.inf, -np.inf
+    got = F.sample_logits(torch.tensor(bad), u, top_k=3, top_p=0.9).numpy().tolist()
+    assert got[:3] == [-1] * 3
+    assert got[3:] == [sample_ref(x[r], float(u[r]), 1.0, 3, 0.9) for r in range(3, 6)]
+
+
+@gpu
+@pytest.mark.parametrize("n", [50, 4099, 50257, 60001])
+def test_sample_logits_settings_of_each_row(torch, n):
+    rng = np.random.default_rng(n)
+    rows = 12
+    x = (rng.standard_normal((rows, n)) * 2.5).astype(np.float32)
+    u = rng.random(rows).astype(np.float32)
+    t = np.array([0.5, 1, 2, 0, -1, np.nan, 1, 1, 1, 0.9, 1, 1], np.float32)
+    k = np.array([0, 1, 20, 3, 3, 3, -5, n, 10 ** 6, 300, 1400, 7], np.int32)
+    p = np.array([1, 0.5, 0.9, 1, 1, 1, 2, np.nan, 0.9, -1, 0.8, 1], np.float32)
+    m = np.array([0, 0, 0.1, 0, 0, 0, -1, np.nan, 2, 0, 0, 0.2], np.float32)
+    got = torch.functional.sample_logits(torch.tensor(x), torch.tensor(u), torch.tensor(t), k, p, m)
+    ref = [sample_ref(x[r], float(u[r]), float(t[r]), int(k[r]), float(p[r]), float(m[r]))
+           for r in range(rows)]
+    assert got.numpy().tolist() == ref
+
+
+@gpu
+def test_sample_logits_layouts_and_frequencies(torch):
+    F = torch.functional
+    rng = np.random.default_rng(3)
+    w = (rng.standard_normal((5, 6000)) * 2).astype(np.float32)
+    u = rng.random(5).astype(np.float32)
+    for lo in range(5):  # rows at every alignment
+        x = w[:, lo:lo + 5003]
+        got = F.sample_logits(torch.tensor(w)[:, lo:lo + 5003], u, 0.9, 0, 0.8)
+        assert got.numpy().tolist() == [sample_ref(x[r], float(u[r]), 0.9, 0, 0.8) for r in range(5)]
+    got = F.sample_logits(torch.tensor(np.ascontiguousarray(w.T)).T, u)
+    assert got.numpy().tolist() == [sample_ref(w[r], float(u[r])) for r in range(5)]
+    one = F.sample_logits(torch.tensor(w[0]), np.float32(0.3), top_k=4)
+    assert one.shape == () and one.item() == sample_ref(w[0], float(np.float32(0.3)), 1.0, 4)
+    assert F.sample_logits(torch.zeros(0, 5), torch.zeros(0)).shape == (0,)
+    # drawn from the seeded stream: the same again, and in the right shares
+    x = np.log(np.array([0.5, 0.25, 0.125, 0.125], np.float32))
+    rows = torch.tensor(np.broadcast_to(x, (20000, 4)).copy())
+    torch.manual_seed(5)
+    a = F.sample_logits(rows).numpy()
+    torch.manual_seed(5)
+    assert (F.sample_logits(rows).numpy() == a).all()
+    share = np.bincount(a, minlength=4) / a.size
+    # five standard deviations of 20000 draws
+    assert (np.abs(share - np.exp(x)) < 5 * np.sqrt(np.exp(x) * (1 - np.exp(x)) / a.size)).all()
+
+
+@gpu
+def test_sample_logits_in_a_graph(torch):
+    F = torch.functional
+    rng = np.random.default_rng(8)
+    x, u = torch.zeros(3, 5003), torch.zeros(3)
+
+    def call():
+        return (F.sample_logits(x, u, 0.8, top_k=40, top_p=0.9), F.sample_logits(x, u, top_p=0.9),
+                x.topk(7)[1])
+    call()
+    g = torch.hip.Graph()
+    with torch.hip.graph(g):
+        got = call()
+    for _ in range(3):
+        hx = (rng.standard_normal((3, 5003)) * 2).astype(np.float32)
+        hu = rng.random(3).astype(np.float32)
+        x.copy_(torch.tensor(hx))
+        u.copy_(torch.tensor(hu))
+        torch.zeros(1000).add(1.0).numpy()  # work of the program's own between the replays
+        g.replay()
+        torch.synchronize()
+        assert got[0].numpy().tolist() == [sample_ref(hx[r], float(hu[r]), 0.8, 40, 0.9) for r in range(3)]
+        assert got[1].numpy().tolist() == [sample_ref(hx[r], float(hu[r]), 1.0, 0, 0.9) for r in range(3)]
+        np.testing.assert_array_equal(got[2].numpy(), topk_ref(hx, 7))
+
+
+# -------------------------------------------------------------- distillation
+
+
+def _distill_inputs(rng, rows, n, k, spread=2.5):
+    x = (rng.standard_normal((rows, n)) * spread).astype(np.float32)
+    v = (rng.standard_normal((rows, k)) * 3).astype(np.float32)
+    ids = np.stack([rng.permutation(max(n, k))[:k] for _ in range(rows)]).astype(np.int32)
+    return x, v, ids
+
+
+def _bounds(n, threads_terms):
+    """Half steps that a row's sums and exponentials can be off: the longest
+    chain of additions a thread makes (`threads_terms`), the tree over the
+    block, and the roundings of an exponential, a logarithm, a division and
+    the products around them; arguments of exponentials are off by two half
+    steps of their own size, which the sizes of distill_ref carry."""
+    return (threads_terms + 40) * U
+
+
+def _check_distill(torch, x, v, ids, t, reduction):
+    rows, n = x.shape
+    loss, grad, valid, lsize, gsize = distill_ref(x, v, ids, t)
+    c = _bounds(n, 4 * math.ceil(n / (4 * 64 if n <= 1024 else 4 * 256)) + 4)
+    den = {"mean": valid.sum(), "sum": 1, "batchmean": rows, "none": 1}[reduction]
+    tx = torch.tensor(x, requires_grad=True)
+    out = torch.functional.distillation_loss(tx, torch.tensor(v), torch.tensor(ids), t, reduction)
+    if reduction == "none":
+        assert (np.abs(out.numpy() - loss) <= c * lsize).all()
+        g = np.random.default_rng(1).standard_normal(rows).astype(np.float32)
+        out.backward(torch.tensor(g))
+        scale = g.astype(np.float64)[:, None]
+    else:
+        assert abs(out.item() - loss.sum() / den) <= (c + (rows / 1024 + 20) * U) * lsize.sum() / den
+        out.backward()
+        scale = np.full((rows, 1), 1.0 / den)
+    got = tx.grad.numpy()
+    assert got.shape == x.shape
+    assert (np.abs(got - grad * scale) <= c * gsize * np.abs(scale)).all()
+    assert (got[~valid] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("n,k", [(1, 1), (2, 3), (6, 2), (7, 5), (1000, 8), (1021, 64), (1024, 100),
+                                 (1025, 65), (4096, 7), (4099, 300), (16385, 1024), (32001, 37),
+                                 (50257, 64), (53248, 1), (53261, 200)])
+def test_distillation_loss(torch, n, k):
+    rng = np.random.default_rng(n)
+    for t in (1.0, 2.5):
+        x, v, ids = _distill_inputs(rng, 5, n, k)
+        ids[ids >= n] = -1
+        ids[1, k // 2:] = -1
+        ids[2] = n  # no entry
+        ids[3, 0] = -2 ** 31
+        if (ids[[0, 1, 3, 4]] >= 0).any():
+            for reduction in ("mean", "sum", "batchmean", "none"):
+                _check_distill(torch, x, v, ids, t, reduction)
+
+
+@gpu
+@pytest.mark.parametrize("n", [10, 900, 3000, 50257])
+@pytest.mark.parametrize("k", [5, 64, 130])
+def test_distillation_columns_given_twice(torch, n, k):
+    rng = np.random.default_rng(k)
+    x, v, _ = _distill_inputs(rng, 4, n, k)
+    ids = rng.integers(0, min(n, 9), (4, k)).astype(np.int32)
+    ids[3] = n - 1
+    for reduction in ("mean", "none"):
+        _check_distill(torch, x, v, ids, 1.5, reduction)
+    # the same bits on every run
+    def grads():
+        tx = torch.tensor(x, requires_grad=True)
+        torch.functional.distillation_loss(tx, torch.tensor(v), torch.tensor(ids)).backward()
+        return tx.grad.numpy()
+    np.testing.assert_array_equal(grads(), grads())
+
+
+@gpu
+def test_distillation_masks(torch):
+    """Logits and teacher entries of -infinity and of the lowest float."""
+    F = torch.functional
+    rng = np.random.default_rng(2)
+    x, v, ids = _distill_inputs(rng, 4, 5000, 20)
+    x[:, 3000:] = -np.inf
+    x[:, 2000:3000] = -np.finfo(np.float32).max
+    ids %= 2000
+    v[0, 10:], v[1, 5] = -np.inf, -np.finfo(np.float32).max
+    v[2] = -np.inf  # no entry above -infinity
+    _, grad, valid, _, gsize = distill_ref(x[:, :2000], v, ids, 1.0)
+    assert valid.tolist() == [True, True, False, True]
+    tx = torch.tensor(x, requires_grad=True)
+    out = F.distillation_loss(tx, torch.tensor(v), torch.tensor(ids), reduction="sum")
+    out.backward()
+    got = tx.grad.numpy()
+    assert math.isfinite(out.item()) and (got[:, 2000:] == 0).all()
+    assert (np.abs(got[:, :2000] - grad) <= _bounds(5000, 24) * gsize).all()
+    # a teacher's column that the student rules out costs without end
+    x[0, ids[0, 0]] = -np.inf
+    assert F.distillation_loss(torch.tensor(x), torch.tensor(v), torch.tensor(ids)).item() == math.inf
+    v[1, 0] = np.nan
+    per = F.distillation_loss(torch.tensor(x), torch.tensor(v), torch.tensor(ids), reduction="none")
+    assert np.isnan(per.numpy()).tolist() == [False, True, False, False]
+    none = F.distillation_loss(torch.tensor(x), torch.tensor(v), np.full((4, 20), -1, np.int32))
+    assert math.isnan(none.item())
+
+
+@gpu
+def test_distillation_shapes_and_differences(torch):
+    F = torch.functional
+    rng = np.random.default_rng(4)
+    x, v, ids = _distill_inputs(rng, 6, 77, 5)
+    want = F.distillation_loss(torch.tensor(x), torch.tensor(v), torch.tensor(ids), 2.0).item()
+    x3 = torch.tensor(x.reshape(2, 3, 77), requires_grad=True)
+    out = F.distillation_loss(x3, torch.tensor(v.reshape(2, 3, 5)), ids.reshape(2, 3, 5), 2.0)
+    assert out.item() == want
+    out.backward()
+    assert x3.grad.shape == (2, 3, 77)
+    mod = torch.nn.DistillationLoss(2.0)
+    assert mod(torch.tensor(x), torch.tensor(v), torch.tensor(ids)).item() == want
+    one = F.distillation_loss(torch.tensor(x[0]), torch.tensor(v[0]), torch.tensor(ids[0]), reduction="none")
+    assert one.shape == ()
+    # against central differences of the oracle's loss
+    h, g = 1e-4, x3.grad.numpy().reshape(6, 77)
+    for r, j in ((0, ids[0, 0]), (3, 5), (5, 76)):
+        lo, hi = x.astype(np.float64), x.astype(np.float64)
+        lo[r, j] -= h
+        hi[r, j] += h
+        d = (distill_ref(hi, v, ids, 2.0)[0].sum() - distill_ref(lo, v, ids, 2.0)[0].sum()) / (2 * h) / 6
+        # h^2 / 6 times a third derivative of at most 1 / T, and float32
+        assert abs(g[r, j] - d) <= h * h + 60 * U
+    # upstream gradients other than one, and twice through one graph
+    tx = torch.tensor(x, requires_grad=True)
+    out = F.distillation_loss(tx, torch.tensor(v), torch.tensor(ids), 2.0)
+    out.backward(torch.tensor(np.float32(3.0).reshape(())), retain_graph=True)
+    np.testing.assert_allclose(tx.grad.numpy(), 3 * g, rtol=4 * U, atol=0)
+    out.backward()
+    np.testing.assert_allclose(tx.grad.numpy(), 4 * g, rtol=8 * U, atol=0)
+
+
+@gpu
+def test_distillation_second_derivative(torch):
+    rng = np.random.default_rng(6)
+    x, v, ids = _distill_inputs(rng, 3, 9, 4)
+    ids[1, 2:] = -1
+    w = rng.standard_normal((3, 9)).astype(np.float32)
+    for red in ("mean", "none"):
+        tx = torch.tensor(x, requires_grad=True)
+        out = torch.functional.distillation_loss(tx, torch.tensor(v), torch.tensor(ids), 1.5, red)
+        (d,) = torch.autograd.grad(out.sum(), tx, create_graph=True)
+        (dd,) = torch.autograd.grad((d * torch.tensor(w)).sum(), tx)
+        s = 1 / 3 if red == "mean" else 1.0
+        q = np.exp(x / 1.5 - x.max(1, keepdims=True) / 1.5).astype(np.float64)
+        q /= q.sum(1, keepdims=True)
+        ref = s * q * (w - (q * w).sum(1, keepdims=True))
+        # a dozen float32 operations on values of at most 4
+        assert np.abs(dd.numpy() - ref).max() <= 100 * U
+
+
+@gpu
+def test_distillation_in_a_graph(torch):
+    F = torch.functional
+    rng = np.random.default_rng(9)
+    x = torch.zeros(6, 3001).requires_grad_(True)
+    v = torch.tensor(rng.standard_normal((6, 8)).astype(np.float32))
+    ids = torch.tensor(rng.integers(0, 3001, (6, 8)).astype(np.int32))
+
+    def call():
+        x.grad = None
+        loss = F.distillation_loss(x, v, ids, 2.0)
+        loss.backward()
+        return loss, x.grad
+    call()
+    g = torch.hip.Graph()
+    with torch.hip.graph(g):
+        loss, grad = call()
+    for _ in range(3):
+        hx = rng.standard_normal((6, 3001)).astype(np.float32)
+        x.detach().copy_(torch.tensor(hx))
+        g.replay()
+        torch.synchronize()
+        got = loss.item(), grad.numpy().copy()
+        e = torch.tensor(hx, requires_grad=True)
+        want = F.distillation_loss(e, v, ids, 2.0)
+        want.backward()
+        assert got[0] == want.item()
+        np.testing.assert_array_equal(got[1], e.grad.numpy())
+
+
+# ------------------------------------------------------------------ refusals
+
+
+def _fake(pkg, *shape, dtype="float32"):
+    """A tensor without a device: the checks come before anything reads it."""
+    return pkg.Tensor(types.SimpleNamespace(ptr=4096), shape, None, 0, dtype)
+
+
+def test_refusals(pkg):
+    F = pkg.functional
+    x = _fake(pkg, 4, 10)
+    for k in (-1, 11):
+        with pytest.raises(ValueError, match="topk"):
+            x.topk(k)
+    with pytest.raises(IndexError):
+        x.topk(1, dim=2)
+    u = _fake(pkg, 4)
+    for kw in (dict(temperature=-1.0), dict(temperature=math.nan), dict(top_k=-1), dict(top_p=1.5),
+               dict(top_p=-0.1), dict(min_p=2.0), dict(min_p=math.nan)):
+        with pytest.raises(ValueError, match="must lie in"):
+            F.sample_logits(x, u, **kw)
+    with pytest.raises(ValueError, match="uniforms"):
+        F.sample_logits(x, _fake(pkg, 3))
+    with pytest.raises(ValueError, match="has shape"):
+        F.sample_logits(x, u, temperature=_fake(pkg, 5))
+    for bad in (_fake(pkg, 2, 3, 4), _fake(pkg), _fake(pkg, 3, 0)):
+        with pytest.raises(ValueError, match="expected logits"):
+            F.sample_logits(bad, u)
+    v, ids = _fake(pkg, 4, 3), _fake(pkg, 4, 3, dtype="int32")
+    for t in (0.0, -1.0, math.inf, math.nan):
+        with pytest.raises(ValueError, match="temperature"):
+            F.distillation_loss(x, v, ids, t)
+    with pytest.raises(ValueError, match="reduction"):
+        F.distillation_loss(x, v, ids, reduction="max")
+    for bv, bi in ((_fake(pkg, 3, 3), ids), (v, _fake(pkg, 4, 2, dtype="int32")),
+                   (_fake(pkg, 4, 0), _fake(pkg, 4, 0, dtype="int32")),
+                   (_fake(pkg, 3), _fake(pkg, 3, dtype="int32"))):
+        with pytest.raises(ValueError, match="do not fit"):
+            F.distillation_loss(x, bv, bi)
+    with pytest.raises(ValueError, match="no classes"):
+        F.distillation_loss(_fake(pkg, 4, 0), v, ids)
+
+
+@gpu
+def test_refusals_of_the_library(torch):
+    from torchjs_amd import _lib as L
+    x = torch.zeros(2, 2000)
+    with pytest.raises(L.HipError, match="at most 1024"):
+        x.topk(1025)
+    with pytest.raises(L.HipError, match="at most 1024"):
+        torch.functional.distillation_loss(x, torch.zeros(2, 1025), np.zeros((2, 1025), np.int32))
+    big = torch.zeros(1).expand(1, 2 ** 20 + 1)
+    with pytest.raises(L.HipError, match="at most"):
+        torch.functional.sample_logits(big, torch.zeros(1))
+    lib, p = L.lib(), x.data_ptr()
+    assert lib.tjh_topk_forward(p, 1, 2, 2000, 1, 1, p, p) == 1
+    assert lib.tjh_topk_forward(None, 2000, 2, 2000, 1, 1, p, p) == 1
+    assert lib.tjh_topk_backward(p, p, 2, 5, 6, p) == 1
+    assert lib.tjh_sample_logits(p, 2000, 2, 2000, None, None, None, None, None, 1.0, 0, 1.0, 0.0, p) == 1
+    assert lib.tjh_distill(p, 2000, 2, 2000, p, p, 1, 1.0, 7, None, p, None, None, 0) == 1
+    assert lib.tjh_distill(p, 2000, 2, 2000, p, p, 1, 1.0, 0, None, None, None, p, 2000) == 1
+    assert lib.tjh_distill(p, 2000, 2, 2000, p, p, 1, 0.0, 1, None, p, p, None, 0) == 1

@@ -24,7 +24,7 @@ from .tensor import graph as _graph
 from .tensor import (Tensor, arange, cat, chunk, enable_grad, from_numpy, full, full_like,
                      inference_mode, init, is_grad_enabled, is_initialized, manual_seed, matmul,
                      multinomial, no_grad, ones, ones_like, rand, randn, set_grad_enabled, split,
-                     stack, synchronize, tensor, tril, triu, zeros, zeros_like, empty)
+                     stack, synchronize, tensor, topk, tril, triu, zeros, zeros_like, empty)
 
 nn.functional = functional
 F = functional
@@ -34,7 +34,7 @@ __all__ = [
     "full_like", "hip", "inference_mode", "init", "is_grad_enabled", "is_initialized", "load",
     "manual_seed", "matmul", "multinomial", "nn", "no_grad", "ones", "ones_like", "optim",
     "profiler", "rand",
-    "randn", "save", "set_grad_enabled", "split", "stack", "synchronize", "tensor", "tril",
+    "randn", "save", "set_grad_enabled", "split", "stack", "synchronize", "tensor", "topk", "tril",
     "triu", "webgpu",
     "zeros", "zeros_like",
 ]

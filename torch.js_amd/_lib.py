@@ -1,5 +1,5 @@
 """ctypes binding of libtorchjs_hip.so (the C ABI declared in
-include/torchjs_hip.h).
+include/torchjs_hip.h and include/torchjs_hip_lm.h).
 
 The library is required: importing the package works without it, but the
 first call that needs the device raises, naming the missing file.  Nothing
@@ -194,6 +194,12 @@ SIGNATURES = {
     "tjh_copy_strided_u8": [c_int, P_i64, c_vp, P_i64, c_vp, P_i64],
     "tjh_triangle": [c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_int],
     "tjh_multinomial": [c_vp, c_i64, c_i64, c_i64, c_int, c_u32, c_vp],
+    "tjh_topk_forward": [c_vp, c_i64, c_i64, c_i64, c_i64, c_int, c_vp, c_vp],
+    "tjh_topk_backward": [c_vp, c_vp, c_i64, c_i64, c_i64, c_vp],
+    "tjh_distill": [c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_f32, c_int, c_vp, c_vp, c_vp,
+                    c_vp, c_i64],
+    "tjh_sample_logits": [c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_f64, c_i64,
+                          c_f64, c_f64, c_vp],
     "tjh_adam_step": [c_int, ctypes.POINTER(c_vp), ctypes.POINTER(c_vp), ctypes.POINTER(c_vp),
                       ctypes.POINTER(c_vp), P_i64, P_i64, c_f64, c_f64, c_f64, c_f64, c_f64,
                       c_int],

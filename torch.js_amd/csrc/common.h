@@ -8,6 +8,7 @@
 #include <stddef.h>
 
 #include "../../include/torchjs_hip.h"
+#include "../../include/torchjs_hip_lm.h"
 
 namespace tjh {
 

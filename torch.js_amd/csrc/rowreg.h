@@ -1,0 +1,361 @@
+// One row of floats per workgroup, held in registers, with the block-wide
+// counts, scans and the selection of its largest values that the vocabulary
+// operators (topk.hip, sample_logits.hip, distill.hip) share.  Device only.
+//
+// Layout: the row's 16-byte aligned chunks of four go round the threads, so
+// every load is a whole chunk whatever the row's alignment and chunk order is
+// index order; the up to three elements before the first chunk and after the
+// last one are an extra element of the first six threads.  Rows that outgrow
+// the registers (NV == 0) are read again, from the L2, on every pass.
+#pragma once
+
+#include "common.h"
+#include "wave.h"
+
+namespace tjh {
+namespace rowreg {
+
+typedef unsigned long long u64;
+
+// Unsigned integer in the order of the floats, -0 and +0 equal; NaN has the
+// key `nan`, above or below all others.
+constexpr uint32_t kNanFirst = 0xffffffffu, kNanLast = 1u;
+__device__ __forceinline__ uint32_t order_key(float x, uint32_t nan = kNanFirst) {
+  const uint32_t u = __float_as_uint(x + 0.f);  // -0 becomes +0
+  const uint32_t k = (u >> 31) ? ~u : (u | 0x80000000u);
+  return x != x ? nan : k;
+}
+// the float of a number's key
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float((k >> 31) ? (k & 0x7fffffffu) : ~k);
+}
+
+// (value, index) as one integer: larger values first, of equal ones the
+// lower index.
+__device__ __forceinline__ u64 composite(uint32_t key, int i) {
+  return ((u64)key << 32) | (uint32_t)~(uint32_t)i;
+}
+__device__ __forceinline__ int index_of(u64 c) { return (int)~(uint32_t)c; }
+
+typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
+constexpr int kBufferFlags = 0x00020000;  // 32-bit data, raw addressing (gfx9)
+constexpr uint32_t kNegInf = 0xff800000u;
+
+template <int T, int NV>
+struct Row {
+  float v[NV > 0 ? 4 * NV : 1];
+  float edge;      // the extra element
+  int edge_index;  // and its place in the row
+  const float* p;
+  uint32_t sign;   // flipped in every element: 0x80000000 looks for the smallest
+  int n, head, n4; // elements, of them before the first chunk; chunks
+
+  __device__ __forceinline__ float at(int i) const {
+    return __uint_as_float(__float_as_uint(p[i]) ^ sign);
+  }
+
+  __device__ __forceinline__ void load(const float* row, int cols, uint32_t flip = 0) {
+    p = row;
+    n = cols;
+    sign = flip;
+    head = min(cols, (int)((16 - ((uintptr_t)row & 15)) & 15) / 4);
+    n4 = (n - head) >> 2;
+    const int t = threadIdx.x, tail = (n - head) & 3;
+    edge_index = t < 3 ? (t < head ? t : -1) : (t - 3 < tail ? head + 4 * n4 + t - 3 : -1);
+    if constexpr (NV > 0) {
+      // bounds-checked loads (chunks past the end give zeros), whose address
+      // is one register for all of them
+      const auto res = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<float*>(p + head), 0, 16 * n4, kBufferFlags);
+      uint4v x[NV];
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        x[j] = __builtin_amdgcn_raw_buffer_load_b128(res, 16 * t, 16 * j * T, 0);
+      edge = edge_index >= 0 ? at(edge_index) : -INFINITY;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const uint32_t past = t + j * T < n4 ? 0u : kNegInf;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[4 * j + u] = __uint_as_float((x[j][u] ^ sign) | past);
+      }
+    } else {
+      edge = edge_index >= 0 ? at(edge_index) : -INFINITY;
+    }
+  }
+
+  // place in the row of element u of this thread's j-th chunk; j < 0: the
+  // extra element's.  Not in [0, n): a place past the row.
+  __device__ __forceinline__ int index(int j, int u) const {
+    return j < 0 ? edge_index : head + 4 * ((int)threadIdx.x + j * T) + u;
+  }
+  __device__ __forceinline__ bool inside(int j, int u) const {
+    return j < 0 ? edge_index >= 0 : (int)threadIdx.x + j * T < n4;
+  }
+
+  // f(j, u, x) for the extra element (j = -1), then for each element u of
+  // this thread's j-th chunk; places past the row hold -infinity
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+    f(-1, 0, edge);
+    if constexpr (NV > 0) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) f(j, u, v[4 * j + u]);
+    } else {
+      int j = 0;
+      for (int c = threadIdx.x; c < n4; c += T, ++j) {
+        const uint4v x = *reinterpret_cast<const uint4v*>(p + head + 4 * c);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) f(j, u, __uint_as_float(x[u] ^ sign));
+      }
+    }
+  }
+};
+
+// Sum over the wave, in every lane.
+template <int CTRL>
+__device__ __forceinline__ u64 dpp_u64(u64 v) {
+  const int lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, 0xF, 0xF, false);
+  const int hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, 0xF, 0xF, false);
+  return ((u64)(uint32_t)hi << 32) | (uint32_t)lo;
+}
+__device__ __forceinline__ u64 lane_u64(u64 v, int lane) {
+  return ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
+__device__ __forceinline__ u64 wave_sum_u64(u64 v) {
+  v += dpp_u64<kDppXor1>(v);
+  v += dpp_u64<kDppXor2>(v);
+  v += dpp_u64<kDppRor4>(v);
+  v += dpp_u64<kDppRor8>(v);
+  return lane_u64(v, 0) + lane_u64(v, 16) + lane_u64(v, 32) + lane_u64(v, 48);
+}
+
+// Block-wide operations, one barrier each: consecutive ones use the two
+// halves of `sm` in turn, so nobody writes a half that is still being read.
+template <int T>
+struct Block {
+  static constexpr int W = T / 64;
+  u64* sm;  // [2 * W]
+  int half;
+  __device__ __forceinline__ explicit Block(u64* s) : sm(s), half(0) {}
+
+  // op over every wave's value, in wave order; the same in every thread
+  template <class V, class C>
+  __device__ __forceinline__ V across(V v, C op) {
+    if (W == 1) return v;
+    V* s = reinterpret_cast<V*>(sm + half * W);
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+    __syncthreads();
+    half ^= 1;
+    V r = s[0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) r = op(r, s[i]);
+    return r;
+  }
+  __device__ __forceinline__ float max(float v) { return across(wave_max(v), MaxOp{}); }
+  __device__ __forceinline__ float sum(float v) { return across(wave_sum(v), AddOp{}); }
+  __device__ __forceinline__ u64 sum64(u64 v) {
+    return across(wave_sum_u64(v), [](u64 x, u64 y) { return x + y; });
+  }
+  __device__ __forceinline__ bool any(bool p) {
+    return across((int)(__ballot(p) != 0), [](int x, int y) { return x | y; }) != 0;
+  }
+  __device__ __forceinline__ int sum_i(int v) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+    return across(v, [](int x, int y) { return x + y; });
+  }
+  // threads for which p holds, counted over `M` predicates of each
+  template <int M>
+  __device__ __forceinline__ int count(const bool (&p)[M]) {
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < M; ++i) c += __popcll(__ballot(p[i]));
+    return across(c, [](int x, int y) { return x + y; });
+  }
+  // sum of v over the threads before this one; total in *all
+  template <class V>
+  __device__ __forceinline__ V before(V v, V* all) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    V incl = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const V x = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += x;
+    }
+    if (W == 1) {
+      *all = __shfl(incl, 63, 64);
+      return incl - v;
+    }
+    V* s = reinterpret_cast<V*>(sm + half * W);
+    if (lane == 63) s[w] = incl;
+    __syncthreads();
+    half ^= 1;
+    V base = 0, tot = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      if (i == w) base = tot;
+      tot += s[i];
+    }
+    *all = tot;
+    return base + incl - v;
+  }
+};
+
+constexpr int kRank = 256;  // longest list sorted by counting
+
+// LDS of a selection: a list of CAP composites, a second one for the short
+// sort, and the block operations' slots.
+template <int T, int CAP>
+struct SelectLds {
+  u64 list[CAP];
+  u64 tmp[kRank];
+  int rank[kRank];
+  int count;
+  u64 sm[2 * (T / 64)];
+};
+
+// Sorts list[0, c) descending.  Up to 256 items each thread counts the items
+// above one of them (c * c / T comparisons, two barriers); longer lists take
+// a bitonic network over the next power of two, padded with zeros, which no
+// real item is below (c log^2 c / 4 T exchanges, log^2 c / 2 barriers).
+template <int T, int CAP>
+__device__ __forceinline__ void sort_list(SelectLds<T, CAP>& s, int c) {
+  if (c <= kRank) {
+    int pad = 64;
+    while (pad < c) pad <<= 1;
+    for (int i = threadIdx.x; i < c; i += T) s.rank[i] = 0;
+    __syncthreads();  // ranks cleared, list written
+    if (T >= pad) {
+      const int i = threadIdx.x & (pad - 1), g = threadIdx.x / pad, ng = T / pad;
+      if (i < c) {
+        const u64 me = s.list[i];
+        int r = 0;
+        for (int j = g; j < c; j += ng) r += s.list[j] > me;
+        if (ng > 1) atomicAdd(&s.rank[i], r);
+        else s.rank[i] = r;
+      }
+    } else {
+      for (int i = threadIdx.x; i < c; i += T) {
+        const u64 me = s.list[i];
+        int r = 0;
+        for (int j = 0; j < c; ++j) r += s.list[j] > me;
+        s.rank[i] = r;
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < c; i += T) s.tmp[s.rank[i]] = s.list[i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < c; i += T) s.list[i] = s.tmp[i];
+    __syncthreads();
+    return;
+  }
+  int p = 2 * kRank;
+  while (p < c) p <<= 1;  // <= CAP, a power of two
+  for (int i = c + threadIdx.x; i < p; i += T) s.list[i] = 0;
+  __syncthreads();
+  for (int len = 2; len <= p; len <<= 1) {
+    for (int o = len >> 1; o >= 1; o >>= 1) {
+      for (int q = threadIdx.x; q < p / 2; q += T) {
+        const int i = 2 * q - (q & (o - 1));  // the pair (i, i + o)
+        const u64 x = s.list[i], y = s.list[i + o];
+        const bool down = (i & len) == 0;  // descending run
+        if ((x < y) == down) {
+          s.list[i] = y;
+          s.list[i + o] = x;
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// The elements for which in(j, u, x) holds into the list, in no order (it is
+// sorted next): their number, of which the first CAP were stored.
+template <int T, int NV, int CAP, class In>
+__device__ __forceinline__ int gather_list(const Row<T, NV>& row, uint32_t nan, In in,
+                                           SelectLds<T, CAP>& s) {
+  if (threadIdx.x == 0) s.count = 0;
+  __syncthreads();
+  row.each([&](int j, int u, float x) {
+    if (in(j, u, x) && row.inside(j, u)) {  // few do
+      const int at = atomicAdd(&s.count, 1);
+      if (at < CAP) s.list[at] = composite(order_key(x, nan), row.index(j, u));
+    }
+  });
+  __syncthreads();
+  return s.count;
+}
+
+// The composite of the row's k-th largest element (1 <= k <= n) by bisection
+// over the keys, then over the indices of the elements that share the key:
+// 32 + log2(n) passes, for rows with more near-ties than the list holds, and
+// for any k.  Passes over memory: a pass over the registers would keep an
+// index and a mask of every element besides.
+template <int T>
+__device__ __forceinline__ u64 kth_by_bisection(const Row<T, 0>& row, int k, uint32_t nan,
+                                                Block<T>& b) {
+  const auto key = [&](int j, int u, float x) {  // 0: no element
+    return row.inside(j, u) ? order_key(x, nan) : 0u;
+  };
+  uint32_t t = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t c = t | (1u << bit);
+    int m = 0;
+    row.each([&](int j, int u, float x) { m += key(j, u, x) >= c; });
+    if (b.sum_i(m) >= k) t = c;
+  }
+  int above = 0;
+  row.each([&](int j, int u, float x) { above += key(j, u, x) > t; });
+  const int need = k - b.sum_i(above);  // of the elements with key t, >= 1
+  int lo = 0;                           // fewer than `need` of them lie before lo
+  for (int bit = 31 - __builtin_clz((unsigned)row.n); bit >= 0; --bit) {
+    const int c = lo + (1 << bit);
+    if (c > row.n) continue;  // the same for every thread
+    int m = 0;
+    row.each([&](int j, int u, float x) { m += key(j, u, x) == t && row.index(j, u) < c; });
+    if (b.sum_i(m) < need) lo = c;
+  }
+  return composite(t, lo);
+}
+
+// Sorts the row's k largest elements into list[0, k), 1 <= k <= min(n, CAP).
+// The k-th largest of the threads' own maxima (two of each thread) is a
+// lower bound of the k-th largest element, and few elements lie above it:
+// 50 of 50257 random values leave about 55.  The bound is taken to its 16
+// high bits, 16 counts instead of 32.  Where more than CAP elements remain
+// (ties), the exact bound comes from bisection.
+template <int T, int NV, int CAP>
+__device__ __forceinline__ void select_largest(const Row<T, NV>& row, int k, uint32_t nan,
+                                               SelectLds<T, CAP>& s, Block<T>& b) {
+  float mx[2] = {-INFINITY, -INFINITY};  // NaN takes no part: still a lower bound
+  row.each([&](int j, int, float x) { mx[j & 1] = fmaxf(mx[j & 1], x); });
+  const uint32_t mk[2] = {order_key(mx[0], nan), order_key(mx[1], nan)};
+  uint32_t lo = 0;
+#pragma unroll 1
+  for (int bit = 31; bit >= 16; --bit) {
+    const uint32_t c = lo | (1u << bit);
+    const bool p[2] = {mk[0] >= c, mk[1] >= c};
+    if (b.count(p) >= k) lo = c;
+  }
+  // below the key of -infinity everything is a candidate
+  const float bound = lo > 0x007fffffu ? key_value(lo) : -INFINITY;
+  const int c = gather_list(row, nan, [&](int, int, float x) { return !(x < bound); }, s);
+  if (c > CAP) {
+    Row<T, 0> again;
+    again.load(row.p, row.n, row.sign);
+    const u64 thr = kth_by_bisection(again, k, nan, b);
+    gather_list(
+        again, nan,
+        [&](int j, int u, float x) {
+          return composite(order_key(x, nan), again.index(j, u)) >= thr;
+        },
+        s);
+  }
+  sort_list(s, c > CAP ? k : c);
+}
+
+}  // namespace rowreg
+}  // namespace tjh

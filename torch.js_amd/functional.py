@@ -307,6 +307,177 @@ def nll_loss(input, target, weight=None, reduction="mean", *, ignore_index=-100)
     return _record(out, "NLLLoss", [x], bwd, gfn=gbwd)
 
 
+def _rows_2d(x):
+    """x as a float32 matrix of rows without a copy where its rows are dense:
+    (detached tensor, pointer, row stride, rows, columns)."""
+    xd = x.detach()
+    if xd.ndim != 2:
+        xd = reshape(xd.contiguous(), (-1, x.shape[-1]) if x.numel() else
+                     (_numel(x.shape[:-1]), x.shape[-1]))
+    rv = _rows_view(xd)
+    if rv is None:
+        xd = _k_contiguous(xd)
+        rv = _rows_view(xd)
+    return xd, rv[0], max(rv[1], xd.shape[1]), xd.shape[0], xd.shape[1]
+
+
+def distillation_loss(input, teacher_logits, teacher_ids, temperature=1.0, reduction="mean"):
+    """The loss of a student's logits against a teacher's largest ones
+    (beside F.cross_entropy, src/nn/losses.ts:129-168; torch.js has none):
+    input [..., C], teacher_logits and teacher_ids (int32 columns of input)
+    [..., K], as a teacher's logits.topk(K) gives them.  With T the
+    temperature, p = softmax(teacher_logits / T) over a row's entries and
+    q = softmax(input / T) over its columns, a row's loss is
+    T^2 sum p (ln p - ln q).  Entries whose id is outside [0, C) are none; a
+    row without any has loss 0 and gradient 0 and is not counted by "mean".
+    Reductions as cross_entropy's.  K up to 1024.  The gradient goes to
+    `input` only; for a scalar loss it is formed in the same pass over the
+    logits."""
+    red = _reduction_code(reduction)
+    temp = float(temperature)
+    if not (temp > 0.0 and math.isfinite(temp)):
+        raise ValueError("distillation_loss: temperature must be positive, got %r" % (temperature,))
+    x, v, ids = input, teacher_logits, _T._idx32(teacher_ids)
+    if not isinstance(v, Tensor):
+        v = _T.tensor(np.asarray(v, dtype=np.float32))
+    if x.ndim == 0 or x.shape[-1] == 0:
+        raise ValueError("distillation_loss: input of shape %s has no classes" % (list(x.shape),))
+    if v.ndim != x.ndim or v.shape[:-1] != x.shape[:-1] or ids.shape != v.shape or \
+            v.shape[-1] == 0:
+        raise ValueError("distillation_loss: teacher_logits %s and teacher_ids %s do not fit input "
+                         "%s" % (list(v.shape), list(ids.shape), list(x.shape)))
+    if x.dtype != "float32":
+        x = x.float()
+    v = (v if v.dtype == "float32" else v.float()).detach().contiguous()
+    xd, px, ld, rows, cols = _rows_2d(x)
+    k = v.shape[-1]
+    xs = x.shape
+    loss_rows = empty(xs[:-1])
+    out = empty(()) if red else loss_rows
+
+    def grad_buffer():
+        return _empty_padded(rows, cols) if cols % 4 else empty((rows, cols))
+    # the gradient for the unit seed of loss.backward(), as cross_entropy's
+    pre, me = [None], [None]
+    if red and _T._recorded(x):
+        pre[0] = grad_buffer()
+    d = pre[0]
+    L.check(L.lib().tjh_distill(px, ld, rows, cols, v.data_ptr(), ids.data_ptr(), k, temp, red,
+                                None, loss_rows.data_ptr(), out.data_ptr() if red else None,
+                                d.data_ptr() if d is not None else None,
+                                d._strides[0] if d is not None else 0), "distillation_loss")
+
+    def bwd(g):
+        d, pre[0] = pre[0], None  # handed out once (the engine may own it)
+        if d is None or g is not _T._unit_seed["g"] or me[0] != _T._unit_seed["node"]:
+            g = g.contiguous()
+            d = grad_buffer()
+            L.check(L.lib().tjh_distill(px, ld, rows, cols, v.data_ptr(), ids.data_ptr(), k, temp,
+                                        red, g.data_ptr(), None, None, d.data_ptr(),
+                                        d._strides[0]), "distillation_loss_backward")
+        return [reshape_raw(d, xs) if len(xs) != 2 else d]
+
+    def gbwd(g):  # log_softmax at the ids, weighted by the teacher's probabilities
+        p, lp, den = _teacher(v, ids, cols, temp, red, rows)
+
+        def ref(xx):
+            lq = _T.gather(log_softmax(mul(xx, 1.0 / temp), -1), -1, p[1])
+            per = mul(_T.reduce_sum(mul(p[0], sub(lp, lq)), -1), temp * temp)
+            return per if red == 0 else mul(_T.reduce_sum(per), 1.0 / den)
+        return _T._regrad(ref, [x], g)
+    res = _record(out, "Distillation", [x], bwd, gfn=gbwd)
+    me[0] = id(res.grad_fn) if res.grad_fn is not None else None
+    return res
+
+
+def _teacher(v, ids, cols, temp, red, rows):
+    """Constants of the distillation loss for its differentiable backward:
+    ((probabilities, ids inside [0, cols)), their logarithms, the divisor),
+    computed without recording.  Entries that are none have probability 0."""
+    with _T.no_grad():
+        h, hid = v.numpy().astype(np.float64) / temp, ids.numpy()
+        there = (hid >= 0) & (hid < cols)
+        h = np.where(there, h, -np.inf)
+        m = h.max(-1, keepdims=True)
+        valid = m > -np.inf
+        e = np.where(valid, np.exp(h - np.where(valid, m, 0.0)), 0.0)
+        p = e / np.where(valid, e.sum(-1, keepdims=True), 1.0)
+        lp = np.log(np.where(p > 0, p, 1.0))
+        den = max(int(valid.sum()), 1) if red == 1 else rows if red == 3 else 1
+        return ((_T.tensor(p.astype(np.float32)),
+                 _T.tensor(np.where(there, hid, 0).astype(np.int32), dtype="int32")),
+                _T.tensor(lp.astype(np.float32)), float(den))
+
+
+def _setting(name, value, rows, dtype, lo, hi):
+    """(tensor or None, number) of a sampling setting: a number in [lo, hi],
+    or one value a row."""
+    if isinstance(value, Tensor) or np.ndim(value):
+        t = value if isinstance(value, Tensor) else \
+            _T.tensor(np.asarray(value, dtype=_DT[dtype][1]), dtype=dtype)
+        if t.shape != (rows,):
+            raise ValueError("sample_logits: %s has shape %s for %d rows"
+                             % (name, list(t.shape), rows))
+        if t.dtype != dtype:
+            t = t.to(dtype)
+        return t.detach().contiguous(), lo
+    if not lo <= value <= hi:
+        raise ValueError("sample_logits: %s must lie in [%s, %s], got %r" % (name, lo, hi, value))
+    return None, value
+
+
+def sample_logits(logits, uniforms=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """Draws one int32 index from each row of logits [rows, C] (a number from
+    [C]) with the given uniforms [rows] in [0, 1) (None: the next of the
+    seeded stream), on the device and without a readback (beside
+    Tensor.multinomial, src/tensor/Tensor.ts:271-359).
+
+    The weight of an index is exp((x - max) / temperature).  In the order of
+    descending logits, equal ones by ascending index, kept are the first
+    `top_k` (0: all); of these the ones before which less than `top_p` of
+    their weight lies; of these the ones of at least `min_p` times the
+    largest's probability; always the first.  Drawn is the first kept index
+    whose running sum of weights, in index order, exceeds u times their sum.
+    temperature 0 takes the first index of the largest logit.
+
+    Each setting is a number or a tensor [rows] of each row's own; in a
+    tensor a temperature that is not above 0 stands for 0, and a setting out
+    of its range for none.  A row with NaN, +infinity or nothing above
+    -infinity gives -1.  C up to 2^20."""
+    x = logits
+    if x.ndim not in (1, 2) or x.shape[-1] == 0:
+        raise ValueError("sample_logits: expected logits [rows, C] or [C], got shape %s"
+                         % (list(x.shape),))
+    one = x.ndim == 1
+    if one:
+        x = reshape(x.detach(), (1, x.shape[0]))
+    if x.dtype != "float32":
+        x = x.float()
+    xd, px, ld, rows, cols = _rows_2d(x)
+    if uniforms is None:
+        u = _T.rand(rows)
+    else:
+        u = uniforms
+        if not isinstance(u, Tensor):
+            u = _T.tensor(np.asarray(u, dtype=np.float32))
+        if u.numel() != rows or u.ndim > 1 or (u.ndim == 0 and not one):
+            raise ValueError("sample_logits: uniforms of shape %s for %d rows"
+                             % (list(u.shape), rows))
+        u = (u if u.dtype == "float32" else u.float()).detach().contiguous()
+    t, t0 = _setting("temperature", temperature, rows, "float32", 0.0, math.inf)
+    k, k0 = _setting("top_k", top_k, rows, "int32", 0, 2 ** 31 - 1)
+    p, p0 = _setting("top_p", top_p, rows, "float32", 0.0, 1.0)
+    m, m0 = _setting("min_p", min_p, rows, "float32", 0.0, 1.0)
+    out = empty(() if one else (rows,), "int32")
+
+    def ptr(s):
+        return s.data_ptr() if s is not None else None
+    L.check(L.lib().tjh_sample_logits(px, ld, rows, cols, u.data_ptr(), ptr(t), ptr(k), ptr(p),
+                                      ptr(m), float(t0), int(k0), float(p0), float(m0),
+                                      out.data_ptr()), "sample_logits")
+    return out
+
+
 def mse_loss(input, target, reduction="mean"):
     """F.mse_loss (src/nn/losses.ts): mean((input - target)^2)."""
     d = sub(input, target)

@@ -446,6 +446,19 @@ class NLLLoss(Module):
                           ignore_index=self.ignore_index)
 
 
+class DistillationLoss(Module):
+    """F.distillation_loss as a module: forward(input, teacher_logits,
+    teacher_ids)."""
+
+    def __init__(self, temperature=1.0, reduction="mean"):
+        super().__init__()
+        self.temperature, self.reduction = temperature, reduction
+
+    def forward(self, input, teacher_logits, teacher_ids):
+        return F.distillation_loss(input, teacher_logits, teacher_ids, self.temperature,
+                                   self.reduction)
+
+
 class MSELoss(Module):
     def __init__(self, reduction="mean"):
         super().__init__()

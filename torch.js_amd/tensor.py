@@ -648,6 +648,9 @@ class Tensor:
     def gather(self, dim, index):
         return gather(self, dim, index)
 
+    def topk(self, k, dim=-1, largest=True):
+        return topk(self, k, dim, largest)
+
     def nonzero(self):
         return nonzero(self)
 
@@ -2713,6 +2716,49 @@ def _scatter_add_rec(xs, d, index, src):
                                     index.shape[d], src.data_ptr()), "scatter_add")
     return _record(z, "ScatterAdd", [src], lambda g: [gather(g, d, index)],
                    gfn=lambda g: [gather(g, d, index)])
+
+
+def topk(x, k, dim=-1, largest=True):
+    """Tensor.topk (Tensor.ts:3048-3178) on the device: (values, int32
+    indices) of the k largest (smallest) elements along `dim`, sorted by
+    value, equal ones by ascending index; NaN counts as the largest, as in
+    PyTorch.  k up to 1024.  The values' gradient goes back to the elements
+    they came from."""
+    k = int(k)
+    if x.ndim == 0:
+        v, i = topk(reshape(x, (1,)), k, 0, largest)
+        return (reshape(v, ()), reshape(i, ())) if k == 1 else (v, i)
+    d = _wrap_dim(dim, x.ndim)
+    n = x.shape[d]
+    if k < 0 or k > n:
+        raise ValueError("topk: k = %d is not in [0, %d], the elements along dim %d" % (k, n, d))
+    if d != x.ndim - 1:
+        perm = list(range(x.ndim))
+        perm[d], perm[-1] = perm[-1], perm[d]
+        v, i = topk(permute(x, perm), k, -1, largest)
+        return permute(v, perm), permute(i, perm)
+    if x.dtype != "float32":
+        x = x.float()
+    xd = x.detach()
+    if not (xd.ndim == 2 and xd._strides[1] == 1 and xd._strides[0] >= n):
+        xd = xd.contiguous()
+    ld = xd._strides[0] if xd.ndim == 2 else n
+    rows = _numel(x.shape[:-1])
+    oshape = x.shape[:-1] + (k,)
+    values, indices = empty(oshape), empty(oshape, "int32")
+    L.check(L.lib().tjh_topk_forward(xd.data_ptr(), max(ld, n), rows, n, k, 1 if largest else 0,
+                                     values.data_ptr(), indices.data_ptr()), "topk")
+    xs = x.shape
+
+    def bwd(g):
+        g = g.contiguous()
+        dx = empty(xs)
+        L.check(L.lib().tjh_topk_backward(g.data_ptr(), indices.data_ptr(), rows, n, k,
+                                          dx.data_ptr()), "topk_backward")
+        return [dx]
+    _record(values, "TopK", [x], bwd,
+            gfn=lambda g: [_scatter_add_rec(xs, len(xs) - 1, indices, g)])
+    return values, indices
 
 
 def _take_along(x, d, index):
