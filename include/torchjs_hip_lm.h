@@ -63,6 +63,29 @@ int tjh_sample_logits(const float* logits, int64_t ld, int64_t rows, int64_t col
                       const float* top_ps, const float* min_ps, double temperature,
                       int64_t top_k, double top_p, double min_p, int32_t* out);
 
+/* Attention over a sliding window with sinks.  q [B,H,Tq,D], k/v
+ * [B,Hkv,Tk,D], H a multiple of Hkv (query head h reads head h / (H / Hkv)),
+ * Tk >= Tq: the queries are the last Tq of the Tk positions, and the one at
+ * position i sees the keys j <= i with j > i - window or j < sinks (window >=
+ * 1).  o = softmax(scale q k^T over those) v; strides (elements) for the B, H
+ * and T axes, D contiguous, as tjh_sdpa_forward's.  lse [B,H,Tq] is saved for
+ * the backward, or NULL.  Keys and values that a query does not see have no
+ * part in its output, whatever they hold.  Head dims up to 128 that are
+ * multiples of 4, rows 16-byte aligned (else TJH_ERR_UNSUPPORTED). */
+int tjh_window_forward(const float* q, const float* k, const float* v, float* o, float* lse,
+                       int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t D,
+                       const int64_t* q_strides, const int64_t* k_strides,
+                       const int64_t* v_strides, const int64_t* o_strides, float scale,
+                       int64_t window, int64_t sinks);
+/* dq [B,H,Tq,D], dk/dv [B,Hkv,Tk,D] written (not accumulated; with Tq == 0
+ * nothing is), summed over the query heads of a key head.  strides[0..7] = q,
+ * k, v, o, do_, dq, dk, dv as tjh_sdpa_backward's. */
+int tjh_window_backward(const float* q, const float* k, const float* v, const float* o,
+                        const float* do_, const float* lse, float* dq, float* dk, float* dv,
+                        int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t D,
+                        const int64_t* const* strides, float scale, int64_t window,
+                        int64_t sinks);
+
 #ifdef __cplusplus
 }
 #endif

@@ -194,6 +194,11 @@ SIGNATURES = {
     "tjh_copy_strided_u8": [c_int, P_i64, c_vp, P_i64, c_vp, P_i64],
     "tjh_triangle": [c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_int],
     "tjh_multinomial": [c_vp, c_i64, c_i64, c_i64, c_int, c_u32, c_vp],
+    "tjh_window_forward": [c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64,
+                           P_i64, P_i64, P_i64, P_i64, c_f32, c_i64, c_i64],
+    "tjh_window_backward": [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64,
+                            c_i64, c_i64, c_i64, c_i64, ctypes.POINTER(P_i64), c_f32, c_i64,
+                            c_i64],
     "tjh_topk_forward": [c_vp, c_i64, c_i64, c_i64, c_i64, c_int, c_vp, c_vp],
     "tjh_topk_backward": [c_vp, c_vp, c_i64, c_i64, c_i64, c_vp],
     "tjh_distill": [c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_f32, c_int, c_vp, c_vp, c_vp,

@@ -1,0 +1,890 @@
+// Causal attention over a sliding window with sinks
+// (F.sliding_window_attention, beside the full attention of flash.hip behind
+// src/nn/functional.ts:866-890): the query at position i = Tk - Tq + t sees
+// the keys j <= i with j > i - window or j < sinks, H query heads share Hkv
+// heads of keys and values, and time and memory grow with the keys seen.
+//
+// The tiles, layouts and products are flash.hip's (flash_tile.h).  A block of
+// 128 queries walks the key tiles that hold sinks, then the ones from its
+// first query's window to its last query; a wave of 32 queries skips the
+// tiles that it sees nothing of and masks only the ones that it sees in part.
+// Backward: a key-block kernel walks the query heads that share its keys and
+// their query tiles, accumulating dV and dK and storing each 32x32 block of
+// dS in a band of `nsl` slots a query tile (sink tiles, then window tiles); a
+// query-block kernel turns those into dQ, so S and dP are formed once.  The
+// key blocks with sinks are seen by every later query: their query tiles are
+// cut into slices, whose sums a last kernel adds in order.  Deterministic, no
+// atomics.
+//
+// Keys that a query does not see may hold anything, infinities and NaN
+// included: their scores are replaced, never multiplied, and where a tile
+// that is seen in part holds such values of V (or of K, for dQ) they are kept
+// out of the products, in which 0 times them would be NaN.
+//
+// Bound by the fp32 matrix cores: 4 D operations forward and 10 D backward
+// for each key that a query sees, 8 floats moved a head and position.
+#include "flash_tile.h"
+
+#include <math.h>
+
+namespace tjh {
+namespace {
+
+struct WinArgs {
+  const float *q, *k, *v, *o, *dout, *lse, *dsum;
+  float *out, *out2, *lse_out;
+  Strides3 qs, ks, vs, os, gs, o1s, o2s;
+  int H, G;            // query heads, query heads to one of keys and values
+  int Tq, Tk, off;     // off = Tk - Tq: the first query's position
+  int D;
+  float scale;
+  int win, sinks, nst; // nst: key tiles that hold sinks
+  int nblk;            // row blocks of a head
+  // forward in slices of `kslice` key tiles (no lse is wanted): part
+  // [slice][b*H + h][Tq][D] unscaled sums, pml {maximum, sum}
+  float* part;
+  float2* pml;
+  int kslice;
+  // backward: dS blocks [bh - bh0][query tile][nsl], of the key heads from
+  // bkv0 on; slices of the key blocks with sinks
+  float* dsblk;
+  int nqt, nkt, nsl;
+  int bkv0, nbkv;
+  int nsb, nslice;     // key blocks with sinks, slices of their query tiles
+  float* sums;         // [slice][bkv - bkv0][nsb * PROWS][D] of dK, then dV
+};
+
+constexpr int PROWS = 64;  // keys of a workgroup of the key-block kernel
+
+// Workgroups go round the XCDs: neighbours in `i` are on one XCD, where they
+// find the keys and values that they share in its L2.
+__device__ __forceinline__ int xcd_item(int id, int n) {
+  const int per = n / kXcds, rem = n % kXcds, x = id % kXcds, j = id / kXcds;
+  return x * per + min(x, rem) + j;
+}
+
+// The key tiles that queries at positions [lo, hi] see: i -> tile.
+struct Tiles {
+  int ns, w0, n;  // sink tiles, the window's first tile, all
+  __device__ __forceinline__ Tiles(const WinArgs& a, int lo, int hi) {
+    w0 = max(0, lo - a.win + 1) / TILE;
+    ns = min(a.nst, w0);
+    n = ns + hi / TILE - w0 + 1;
+  }
+  __device__ __forceinline__ int operator()(int i) const { return i < ns ? i : w0 + i - ns; }
+};
+
+// Whether a query at a position in [lo, lo + 31] sees a key of tile kt, and
+// whether they all see all of it.
+__device__ __forceinline__ bool tile_seen(const WinArgs& a, int lo, int kt) {
+  const int k0 = kt * TILE;
+  return k0 <= lo + TILE - 1 && (k0 + TILE - 1 > lo - a.win || k0 < a.sinks);
+}
+__device__ __forceinline__ bool tile_whole(const WinArgs& a, int lo, int kt) {
+  const int k1 = kt * TILE + TILE - 1;
+  return k1 <= lo && (kt * TILE > lo + TILE - 1 - a.win || k1 < a.sinks);
+}
+__device__ __forceinline__ bool sees(const WinArgs& a, int pos, int key) {
+  return key <= pos && (key > pos - a.win || key < a.sinks);
+}
+// Slot of tile kt among the dS blocks of the queries at [lo, lo + 31].
+__device__ __forceinline__ int ds_slot(const WinArgs& a, int lo, int kt) {
+  return kt < a.nst ? kt : a.nst + kt - max(a.nst, max(0, lo - a.win + 1) / TILE);
+}
+
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+
+// Sets values that are not finite to 0; whether the wave had any.
+template <int NC>
+__device__ __forceinline__ bool drop_nonfinite(float (&x)[NC][16]) {
+  bool bad = false;
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int s = 0; s < 16; ++s) bad |= !finite(x[c][s]);
+  if (__ballot(bad) == 0) return false;
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int s = 0; s < 16; ++s) x[c][s] = finite(x[c][s]) ? x[c][s] : 0.f;
+  return true;
+}
+
+// ------------------------------------------------------------ forward
+
+// GUARD: Tk is not a multiple of 32, or D < HD.  PART: one slice of the key
+// tiles, joined by k_win_merge.
+template <int HD, bool GUARD, bool PART, int RUN>
+__global__ __launch_bounds__(256, occ_fwd<HD>()) void k_win_fwd(WinArgs a) {
+  using S_ = Hd<HD>;
+  __shared__ __attribute__((aligned(16))) float Ks[2][TILE * S_::W];
+  __shared__ __attribute__((aligned(16))) float Vs[2][TILE * S_::W];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int l32 = lane & 31, h = lane >> 5;
+  const int item = xcd_item(blockIdx.x, gridDim.x);
+  const int64_t bh = item / a.nblk;
+  const int qb = item % a.nblk;
+  const int64_t b = bh / a.H, hh = bh % a.H, kh = hh / a.G;
+  const float* Q = a.q + b * a.qs.b + hh * a.qs.h;
+  const float* K = a.k + b * a.ks.b + kh * a.ks.h;
+  const float* V = a.v + b * a.vs.b + kh * a.vs.h;
+  const int q0 = qb * ROWS + w * TILE;  // this wave's first query
+  const int myq = q0 + l32, lo = a.off + q0, pos = lo + l32;
+  const Tiles tiles(a, a.off + qb * ROWS, min(a.off + qb * ROWS + ROWS, a.Tk) - 1);
+  const int i0 = PART ? (int)blockIdx.y * a.kslice : 0;
+  const int i1 = PART ? min(tiles.n, i0 + a.kslice) : tiles.n;
+  if (PART && i0 >= i1) return;  // the same for the whole workgroup
+
+  float qf[RUN];
+  gl_run<HD, GUARD>(Q, a.qs.t, myq, a.Tq, a.D, h, a.scale * kLog2e, qf);
+  floatx16 acc[S_::NC];
+  zero_acc(acc);
+  float m = -INFINITY, lsum = 0.f;
+  floatx4 rk[S_::NC], rv[S_::NC];
+  load_tile<HD, GUARD>(K, a.ks.t, tiles(i0) * TILE, a.Tk, a.D, rk);
+  load_tile<HD, GUARD>(V, a.vs.t, tiles(i0) * TILE, a.Tk, a.D, rv);
+  store_tile<HD>(Ks[0], rk);
+  store_tile<HD>(Vs[0], rv);
+  __syncthreads();
+  for (int i = i0; i < i1; ++i) {
+    const int cur = (i - i0) & 1;
+    const bool more = i + 1 < i1;
+    if (more) {
+      load_tile<HD, GUARD>(K, a.ks.t, tiles(i + 1) * TILE, a.Tk, a.D, rk);
+      load_tile<HD, GUARD>(V, a.vs.t, tiles(i + 1) * TILE, a.Tk, a.D, rv);
+    }
+    const int kt = tiles(i), k0 = kt * TILE;
+    if (q0 < a.Tq && tile_seen(a, lo, kt)) {
+      float ka[RUN];
+      lds_run<HD>(Ks[cur], l32, h, ka);
+      floatx16 st = chain0<HD>(ka, qf);  // S^T[key][query], base-2 units
+      float va[S_::NC][16];
+      lds_cols<HD>(Vs[cur], l32, h, va);
+      bool bad = false;
+      if (!tile_whole(a, lo, kt)) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) st[j] = sees(a, pos, k0 + kappa(j, h)) ? st[j] : -INFINITY;
+        bad = drop_nonfinite(va);
+      }
+      float bm = st[0];
+#pragma unroll
+      for (int j = 1; j < 16; ++j) bm = fmaxf(bm, st[j]);
+      bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
+      const float mn = fmaxf(m, bm);
+      const float ms = mn == -INFINITY ? 0.f : mn;  // nothing seen so far
+      const float alpha = exp2_hw(m - ms);
+      float rs = 0.f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        st[j] = exp2_hw(st[j] - ms);
+        rs += st[j];
+      }
+      rs += __shfl_xor(rs, 32, 64);
+      lsum = lsum * alpha + rs;
+      m = mn;
+#pragma unroll
+      for (int c = 0; c < S_::NC; ++c) acc[c] *= alpha;
+#pragma unroll
+      for (int s = 0; s < 16; ++s)  // O^T += V^T P^T
+#pragma unroll
+        for (int c = 0; c < S_::NC; ++c) acc[c] = mfma(va[c][s], st[s], acc[c]);
+      if (bad) {  // values that are not finite, for the queries that see them
+#pragma unroll 1
+        for (int r = 0; r < TILE; ++r) {
+          if (!sees(a, pos, k0 + r)) continue;
+#pragma unroll
+          for (int c = 0; c < S_::NC; ++c)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float x = Vs[cur][r * S_::W + c * 32 + kappa(j, h)];
+              acc[c][j] += finite(x) ? 0.f : x;
+            }
+        }
+      }
+    }
+    if (more) {
+      store_tile<HD>(Ks[cur ^ 1], rk);
+      store_tile<HD>(Vs[cur ^ 1], rv);
+    }
+    __syncthreads();
+  }
+  float* buf = (w < 2 ? Ks[w] : Vs[w - 2]);
+  if constexpr (PART) {
+    const int64_t row0 = ((int64_t)blockIdx.y * (gridDim.x / a.nblk) + bh) * a.Tq;
+    write_rows<HD>(buf, acc, 1.0f, a.part + row0 * a.D, a.D, q0, a.Tq, a.D, l32, h, lane);
+    if (h == 0 && myq < a.Tq) a.pml[row0 + myq] = make_float2(m, lsum);
+    return;
+  }
+  const float inv = 1.0f / lsum;  // a query sees itself: the sum is at least 1
+  write_rows<HD>(buf, acc, inv, a.out + b * a.os.b + hh * a.os.h, a.os.t, q0, a.Tq, a.D, l32, h,
+                 lane);
+  if (a.lse_out && h == 0 && myq < a.Tq)
+    a.lse_out[bh * a.Tq + myq] = (m + __log2f(lsum)) * kLn2;
+}
+
+// Joins the slices of a query: o = sum 2^(m_s - m) acc_s / sum 2^(m_s - m)
+// l_s, in slice order.  One float4 a lane; n: slices of each row, or 0 and
+// those of its block of queries.
+__global__ __launch_bounds__(256) void k_win_merge(WinArgs a, int64_t n4, int nslices) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n4) return;
+  const int d4 = a.D / 4;
+  const int64_t row = i / d4, rows = n4 / d4;
+  const int c = (int)(i - row * d4);
+  const int64_t bh = row / a.Tq;
+  const int q = (int)(row - bh * a.Tq);
+  int n = nslices;
+  if (n == 0) {
+    const int lo = a.off + q / ROWS * ROWS;
+    const Tiles tiles(a, lo, min(lo + ROWS, a.Tk) - 1);
+    n = (tiles.n + a.kslice - 1) / a.kslice;
+  }
+  float top = -INFINITY;
+  for (int s = 0; s < n; ++s) top = fmaxf(top, a.pml[s * rows + row].x);
+  const float ts = top == -INFINITY ? 0.f : top;
+  floatx4 o = {0.f, 0.f, 0.f, 0.f};
+  float den = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < n; ++s) {
+    const float2 ml = a.pml[s * rows + row];
+    const float f = exp2_hw(ml.x - ts);
+    den = __builtin_fmaf(ml.y, f, den);
+    const floatx4 x = *reinterpret_cast<const floatx4*>(a.part + (s * rows + row) * a.D + 4 * c);
+    // a slice that this query sees nothing of has sums of 0 and a factor of
+    // 0, and infinities of other slices stay what they are
+    if (f != 0.f) o += f * x;
+  }
+  const int64_t b = bh / a.H, h = bh % a.H;
+  *reinterpret_cast<floatx4*>(a.out + b * a.os.b + h * a.os.h + q * a.os.t + 4 * c) =
+      o * (1.0f / den);
+}
+
+// Few queries (a decoding step): one query head and position a workgroup,
+// its keys over groups of 16 lanes, each with a running softmax of its own
+// over every NG-th key, joined once at the end in a fixed order.  grid.y
+// slices of the keys, joined by k_win_merge, where there are few rows.
+constexpr int kFewThreads = 512, kFewGroups = kFewThreads / 16, kFewUnroll = 4;
+
+template <int NC, bool PART>  // NC: 64-column pieces of the head dim
+__global__ __launch_bounds__(kFewThreads) void k_win_few(WinArgs a) {
+  __shared__ float sm[kFewGroups], sl[kFewGroups];
+  __shared__ __attribute__((aligned(16))) float so[kFewGroups][NC * 64];
+  const int64_t row = blockIdx.x;  // (b * H + h) * Tq + t
+  const int64_t bh = row / a.Tq, b = bh / a.H, hh = bh % a.H, kh = hh / a.G;
+  const int q = (int)(row - bh * a.Tq), pos = a.off + q;
+  const int g = threadIdx.x >> 4, l = threadIdx.x & 15;
+  const float* __restrict__ K = a.k + b * a.ks.b + kh * a.ks.h;
+  const float* __restrict__ V = a.v + b * a.vs.b + kh * a.vs.h;
+  // the i-th key that it sees
+  const int first = max(0, pos - a.win + 1), ns = min(a.sinks, first);
+  const int seen = ns + pos - first + 1;
+  const int i0 = PART ? (int)blockIdx.y * a.kslice : 0;
+  const int i1 = PART ? min(seen, i0 + a.kslice) : seen;
+  const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
+  floatx4 qv[NC], o[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int d = 64 * c + 4 * l;
+    o[c] = zero;
+    qv[c] = zero;
+    if (d < a.D)
+      qv[c] = *reinterpret_cast<const floatx4*>(a.q + b * a.qs.b + hh * a.qs.h + q * a.qs.t + d) *
+              (a.scale * kLog2e);
+  }
+  float m = -INFINITY, sum = 0.f;
+  for (int t0 = i0 + g; t0 < i1; t0 += kFewGroups * kFewUnroll) {
+    floatx4 kv[kFewUnroll][NC], vv[kFewUnroll][NC];
+#pragma unroll
+    for (int u = 0; u < kFewUnroll; ++u) {
+      // keys past the end repeat the last one with a score of -infinity
+      const int i = min(t0 + u * kFewGroups, i1 - 1);
+      const int64_t t = i < ns ? i : first + i - ns;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int d = 64 * c + 4 * l;
+        kv[u][c] = d < a.D ? *reinterpret_cast<const floatx4*>(K + t * a.ks.t + d) : zero;
+        vv[u][c] = d < a.D ? *reinterpret_cast<const floatx4*>(V + t * a.vs.t + d) : zero;
+      }
+    }
+    float s[kFewUnroll], mn = m;
+#pragma unroll
+    for (int u = 0; u < kFewUnroll; ++u) {
+      float x = 0.f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x = __builtin_fmaf(qv[c][e], kv[u][c][e], x);
+      x = row16_sum(x);
+      s[u] = t0 + u * kFewGroups < i1 ? x : -INFINITY;
+      mn = fmaxf(mn, s[u]);
+    }
+    const float ms = mn == -INFINITY ? 0.f : mn;
+    const float alpha = exp2_hw(m - ms);
+    m = mn;
+    sum *= alpha;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) o[c] *= alpha;
+#pragma unroll
+    for (int u = 0; u < kFewUnroll; ++u) {
+      const float p = exp2_hw(s[u] - ms);
+      sum += p;
+      if (t0 + u * kFewGroups < i1) {  // 0 times infinity of a repeated key stays out
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[c][e] = __builtin_fmaf(p, vv[u][c][e], o[c][e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < NC; ++c) *reinterpret_cast<floatx4*>(&so[g][64 * c + 4 * l]) = o[c];
+  if (l == 0) {
+    sm[g] = m;
+    sl[g] = sum;
+  }
+  __syncthreads();
+  const int d = threadIdx.x;
+  if (d >= NC * 64 || d >= a.D) return;
+  float top = -INFINITY;
+  for (int i = 0; i < kFewGroups; ++i) top = fmaxf(top, sm[i]);
+  const float ts = top == -INFINITY ? 0.f : top;
+  float den = 0.f, num = 0.f;
+#pragma unroll 8
+  for (int i = 0; i < kFewGroups; ++i) {
+    const float f = exp2_hw(sm[i] - ts);
+    den = __builtin_fmaf(sl[i], f, den);
+    num = __builtin_fmaf(so[i][d], f, num);
+  }
+  if constexpr (PART) {
+    const int64_t at = (int64_t)blockIdx.y * gridDim.x + row;
+    a.part[at * a.D + d] = num;
+    if (d == 0) a.pml[at] = make_float2(top, den);
+  } else {
+    a.out[b * a.os.b + hh * a.os.h + q * a.os.t + d] = num * (1.0f / den);
+    if (d == 0 && a.lse_out) a.lse_out[row] = (top + __log2f(den)) * kLn2;
+  }
+}
+
+// ------------------------------------------------------------ backward
+
+// Key-block kernel: 64 keys a workgroup, each 32 of them a pair of waves; wave
+// A forms P and accumulates dV^T += dO^T P, wave B forms dS = P (dP - D),
+// stores it and accumulates dK^T += Q^T dS (flash.hip's split of the work).
+// GUARD: Tq or Tk is not a multiple of 32, or D < HD.
+template <int HD, bool GUARD, int RUN>
+__global__ __launch_bounds__(256, occ_pair<HD>()) void k_win_dkv(WinArgs a) {
+  using S_ = Hd<HD>;
+  __shared__ __attribute__((aligned(16))) float Qs[2][TILE * S_::W];
+  __shared__ __attribute__((aligned(16))) float Gs[2][TILE * S_::W];
+  __shared__ __attribute__((aligned(16))) float Ps[2][16 * 64];
+  // unequal wave priorities keep a CU's workgroups out of step (flash.hip)
+  if (blockIdx.x % 3 == 0) __builtin_amdgcn_s_setprio(2);
+  else if (blockIdx.x % 3 == 1) __builtin_amdgcn_s_setprio(1);
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const int role = wv >> 1, pr = wv & 1;  // role 0: A (P, dV), 1: B (dS, dK)
+  const int l32 = lane & 31, h = lane >> 5;
+  // the slices of the sinks' blocks first: they are the longest
+  const int nlong = a.nbkv * a.nsb * a.nslice;
+  int bkv, kb, slice = 0;
+  const bool sunk = (int)blockIdx.x < nlong;
+  if (sunk) {
+    slice = blockIdx.x % a.nslice;
+    kb = blockIdx.x / a.nslice % a.nsb;
+    bkv = blockIdx.x / (a.nslice * a.nsb);
+  } else {
+    const int item = xcd_item(blockIdx.x - nlong, gridDim.x - nlong), per = a.nblk - a.nsb;
+    bkv = item / per;
+    kb = a.nsb + item % per;
+  }
+  const int hkv = a.H / a.G;
+  const int64_t b = (a.bkv0 + bkv) / hkv, kh = (a.bkv0 + bkv) % hkv;
+  const float* K = a.k + b * a.ks.b + kh * a.ks.h;
+  const float* V = a.v + b * a.vs.b + kh * a.vs.h;
+  const int k0 = kb * PROWS + pr * TILE, kt = k0 / TILE;  // the pair's keys
+  const int mykey = k0 + l32;
+
+  float kv[RUN];
+  if (role == 0)
+    gl_run<HD, GUARD>(K, a.ks.t, mykey, a.Tk, a.D, h, a.scale * kLog2e, kv);
+  else
+    gl_run<HD, GUARD>(V, a.vs.t, mykey, a.Tk, a.D, h, 1.0f, kv);
+  // complete the loads here: a wait for them inside the loop would also
+  // wait for every step's prefetch
+#pragma unroll
+  for (int i = 0; i < RUN; ++i) asm volatile("" : "+v"(kv[i]));
+  floatx16 acc[S_::NC];  // A: dV^T, B: dK^T
+  zero_acc(acc);
+  const float one = h == 0 ? 1.f : 0.f;
+  const float omul = role == 0 ? -kLog2e : -1.f;
+
+  // the query tiles that see some of the 64 keys
+  int qt0 = max(0, kb * PROWS - a.off) / TILE;
+  int last = a.Tq - 1;
+  if (!sunk) last = (int)min((int64_t)last, (int64_t)kb * PROWS + PROWS - 2 + a.win - a.off);
+  int qt1 = last < 0 ? qt0 : max(qt0, last / TILE + 1);
+  if (sunk && a.nslice > 1) {
+    const int per = (qt1 - qt0 + a.nslice - 1) / a.nslice;
+    qt0 = min(qt1, qt0 + slice * per);
+    qt1 = min(qt1, qt0 + per);
+  }
+  const int steps = (qt1 - qt0) * a.G;
+  // of the current and the next step: query head and tile
+  int hh = (int)kh * a.G, qt = qt0;
+  const auto qrows = [&](const float* x, const Strides3& s, int head) {
+    return x + b * s.b + (int64_t)head * s.h;
+  };
+  const auto row_raw = [&](int head, int t) {
+    const float* L = (role == 0 ? a.lse : a.dsum) + (b * a.H + head) * (int64_t)a.Tq;
+    return L[min(t * TILE + l32, a.Tq - 1)];
+  };
+  const auto row_fix = [&](int t, float raw) {
+    const bool in = !GUARD || t * TILE + l32 < a.Tq;
+    return (h == 0 && in) ? raw * omul : 0.f;
+  };
+  floatx4 rq[S_::NC], rg[S_::NC];
+  float off = 0.f, raw_n = 0.f;
+  if (steps > 0) {
+    load_tile<HD, GUARD>(qrows(a.q, a.qs, hh), a.qs.t, qt * TILE, a.Tq, a.D, rq);
+    load_tile<HD, GUARD>(qrows(a.dout, a.gs, hh), a.gs.t, qt * TILE, a.Tq, a.D, rg);
+    raw_n = row_raw(hh, qt);
+    store_tile<HD>(Qs[0], rq);
+    store_tile<HD>(Gs[0], rg);
+    off = row_fix(qt, raw_n);
+  }
+  __syncthreads();
+  float* pbuf = Ps[pr];
+  for (int step = 0; step < steps; ++step) {
+    const int cur = step & 1;
+    const bool more = step + 1 < steps;
+    int hn = hh, qn = qt + 1;
+    if (qn == qt1) {
+      qn = qt0;
+      ++hn;
+    }
+    if (more) {
+      load_tile<HD, GUARD>(qrows(a.q, a.qs, hn), a.qs.t, qn * TILE, a.Tq, a.D, rq);
+      load_tile<HD, GUARD>(qrows(a.dout, a.gs, hn), a.gs.t, qn * TILE, a.Tq, a.D, rg);
+      raw_n = row_raw(hn, qn);
+    }
+    const int lo = a.off + qt * TILE;  // the tile's first position
+    const bool seen = k0 < a.Tk && tile_seen(a, lo, kt);
+    const bool edge = !tile_whole(a, lo, kt) || (GUARD && qt * TILE + TILE > a.Tq);
+    const auto ok = [&](int j) {
+      const int r = kappa(j, h);
+      return (!GUARD || qt * TILE + r < a.Tq) && sees(a, lo + r, mykey);
+    };
+    floatx16 x = zero16();  // A: P; B: dP - D, then dS
+    if (seen) {
+      float xa[RUN];
+      // A: S[q][key] - lse[q] from Q rows; B: dP[q][key] - D[q] from dO rows
+      lds_run<HD>(role == 0 ? Qs[cur] : Gs[cur], l32, h, xa);
+      x = chain<HD>(off, one, xa, kv);
+      if (role == 0) {
+        if (edge) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) x[j] = ok(j) ? exp2_hw(x[j]) : 0.f;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) x[j] = exp2_hw(x[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) pbuf[j * 64 + lane] = x[j];
+      }
+    }
+    __syncthreads();
+    if (seen) {
+      float ct[S_::NC][16];
+      if (role == 0) {
+        lds_cols<HD>(Gs[cur], l32, h, ct);
+#pragma unroll
+        for (int s = 0; s < 16; ++s)  // dV^T += dO^T P
+#pragma unroll
+          for (int c = 0; c < S_::NC; ++c) acc[c] = mfma(ct[c][s], x[s], acc[c]);
+      } else {
+        if (edge) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) x[j] = ok(j) ? x[j] * pbuf[j * 64 + lane] : 0.f;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) x[j] *= pbuf[j * 64 + lane];
+        }
+        lds_cols<HD>(Qs[cur], l32, h, ct);
+#pragma unroll
+        for (int s = 0; s < 16; ++s)  // dK^T += Q^T dS
+#pragma unroll
+          for (int c = 0; c < S_::NC; ++c) acc[c] = mfma(ct[c][s], x[s], acc[c]);
+      }
+    }
+    if (more) {
+      store_tile<HD>(Qs[cur ^ 1], rq);
+      store_tile<HD>(Gs[cur ^ 1], rg);
+      off = row_fix(qn, raw_n);
+    }
+    if (seen && role == 1) {
+      const int64_t bh = (int64_t)bkv * a.G + hh - kh * a.G;
+      float* blk = a.dsblk + ((bh * a.nqt + qt) * a.nsl + ds_slot(a, lo, kt)) * (TILE * TILE) +
+                   ds_col(l32);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) __builtin_nontemporal_store(x[j], blk + kappa(j, h) * TILE);
+    }
+    hh = hn;
+    qt = qn;
+    __syncthreads();
+  }
+  float* buf = (wv < 2 ? Qs[wv] : Gs[wv - 2]);
+  if (sunk && a.nslice > 1) {
+    const int64_t rows = (int64_t)a.nsb * PROWS;
+    const int64_t all = a.nbkv * rows * a.D;
+    float* to = a.sums + (role == 0 ? a.nslice * all : 0) + slice * all + bkv * rows * a.D;
+    write_rows<HD>(buf, acc, role == 0 ? 1.0f : a.scale, to, a.D, k0, a.Tk, a.D, l32, h, lane);
+  } else if (role == 0) {
+    write_rows<HD>(buf, acc, 1.0f, a.out2 + b * a.o2s.b + kh * a.o2s.h, a.o2s.t, k0, a.Tk, a.D, l32,
+                   h, lane);
+  } else {
+    write_rows<HD>(buf, acc, a.scale, a.out + b * a.o1s.b + kh * a.o1s.h, a.o1s.t, k0, a.Tk, a.D,
+                   l32, h, lane);
+  }
+}
+
+// dK and dV of the key blocks with sinks: the slices' sums, in order.
+__global__ __launch_bounds__(256) void k_win_sums(WinArgs a, int64_t n4) {
+  int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= 2 * n4) return;
+  const bool v = i >= n4;
+  const int64_t rows = (int64_t)a.nsb * PROWS, all = a.nbkv * rows * a.D;
+  const float* src = a.sums + (v ? a.nslice * all : 0);
+  if (v) i -= n4;
+  const int d4 = a.D / 4;
+  const int64_t row = i / d4, bkv = row / rows, key = row - bkv * rows;
+  const int c = 4 * (int)(i - row * d4);
+  if (key >= a.Tk) return;
+  floatx4 x = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < a.nslice; ++s)
+    x += *reinterpret_cast<const floatx4*>(src + s * all + row * a.D + c);
+  const int hkv = a.H / a.G;
+  const int64_t b = (a.bkv0 + bkv) / hkv, kh = (a.bkv0 + bkv) % hkv;
+  const Strides3& st = v ? a.o2s : a.o1s;
+  *reinterpret_cast<floatx4*>((v ? a.out2 : a.out) + b * st.b + kh * st.h + key * st.t + c) = x;
+}
+
+// Query-block kernel: dQ^T += K^T dS^T for 128 queries from the stored dS
+// blocks; two groups of four waves take the even and the odd key tiles and
+// are added at the end (flash.hip's k_flash_dq_ds8).
+template <int HD, bool GUARD>
+__global__ __launch_bounds__(512, 1) void k_win_dq(WinArgs a) {
+  using S_ = Hd<HD>;
+  __shared__ __attribute__((aligned(16))) float Ks[WAVES][TILE * S_::W];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const int grp = wv >> 2, w = wv & 3, gt = threadIdx.x & 255;
+  const int l32 = lane & 31, h = lane >> 5;
+  const int item = xcd_item(blockIdx.x, gridDim.x);
+  const int64_t bhl = item / a.nblk;  // from the launch's first head on
+  const int qb = item % a.nblk;
+  const int64_t bh = (int64_t)a.bkv0 * a.G + bhl;
+  const int64_t b = bh / a.H, hh = bh % a.H;
+  const float* K = a.k + b * a.ks.b + (hh / a.G) * a.ks.h;
+  const int q0 = qb * ROWS + w * TILE, lo = a.off + q0;
+  const bool wave_in = q0 < a.Tq;
+  const float* dsrow = a.dsblk +
+                       (bhl * a.nqt + (wave_in ? q0 / TILE : 0)) * a.nsl * (TILE * TILE) +
+                       l32 * TILE + h * 16;
+  floatx16 dq[S_::NC];
+  zero_acc(dq);
+  const Tiles tiles(a, a.off + qb * ROWS, min(a.off + qb * ROWS + ROWS, a.Tk) - 1);
+  const int n = tiles.n, nst0 = (n + 1) / 2;
+  const auto idx = [&](int t) { return grp + 2 * t; };
+  const auto mine = [&](int i) { return i < n && wave_in && tile_seen(a, lo, tiles(i)); };
+  // every prefetch is issued, from slot 0 where the wave does not see the
+  // tile (its values are then not used): loads on conditional paths would
+  // make the waits of the current tile wait for them too
+  const auto fetch_ds = [&](int t, floatx4 (&d)[4]) {
+    const int i = idx(t);
+    const int slot = mine(i) ? ds_slot(a, lo, tiles(i)) : 0;
+    const floatx4* src = reinterpret_cast<const floatx4*>(dsrow + (int64_t)slot * (TILE * TILE));
+#pragma unroll
+    for (int u = 0; u < 4; ++u) d[u] = src[u];
+  };
+  floatx4 d0[4], d1[4], d2[4];
+  fetch_ds(0, d0);
+  fetch_ds(1, d1);
+  floatx4 rk[S_::NC];
+  if (idx(0) < n) {
+    load_tile<HD, GUARD>(K, a.ks.t, tiles(idx(0)) * TILE, a.Tk, a.D, rk, gt);
+    store_tile<HD>(Ks[2 * grp], rk, gt);
+  }
+  __syncthreads();
+  const auto step = [&](int t, const floatx4 (&use)[4], floatx4 (&into)[4]) {
+    const int cur = 2 * grp + (t & 1);
+    const int i = idx(t);
+    const bool more = i + 2 < n;
+    load_tile<HD, GUARD>(K, a.ks.t, tiles(more ? i + 2 : n - 1) * TILE, a.Tk, a.D, rk, gt);
+    fetch_ds(t + 2, into);
+    if (mine(i)) {
+      float ct[S_::NC][16];
+      lds_cols<HD>(Ks[cur], l32, h, ct);
+      // a query that sees a key that is not finite has NaN in dS already
+      if (!tile_whole(a, lo, tiles(i))) drop_nonfinite(ct);
+#pragma unroll
+      for (int s = 0; s < 16; ++s) {
+        const float d = use[s >> 2][s & 3];
+#pragma unroll
+        for (int c = 0; c < S_::NC; ++c) dq[c] = mfma(ct[c][s], d, dq[c]);
+      }
+    }
+    if (more) store_tile<HD>(Ks[2 * grp + ((t + 1) & 1)], rk, gt);
+    __syncthreads();
+  };
+  for (int t = 0; t < nst0; t += 3) {
+    step(t, d0, d2);
+    if (t + 1 >= nst0) break;
+    step(t + 1, d1, d0);
+    if (t + 2 >= nst0) break;
+    step(t + 2, d2, d1);
+  }
+  // even tiles' sum + odd tiles' sum
+  float* red = &Ks[0][0] + w * (S_::NC * 16 * 64);
+  if (grp == 1) {
+#pragma unroll
+    for (int c = 0; c < S_::NC; ++c)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) red[(c * 16 + j) * 64 + lane] = dq[c][j];
+  }
+  __syncthreads();
+  if (grp == 0) {
+#pragma unroll
+    for (int c = 0; c < S_::NC; ++c)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) dq[c][j] = dq[c][j] + red[(c * 16 + j) * 64 + lane];
+  }
+  __syncthreads();
+  if (grp == 0)
+    write_rows<HD>(Ks[w], dq, a.scale, a.out + b * a.o1s.b + hh * a.o1s.h, a.o1s.t, q0, a.Tq, a.D,
+                   l32, h, lane);
+  else
+    __syncthreads();  // the one barrier inside write_rows
+}
+
+// ------------------------------------------------------------ host
+
+Strides3 s3(const int64_t* s) { return Strides3{s[0], s[1], s[2]}; }
+
+// 16 or more of the padded columns empty: shorter products over the head dim
+template <int HD>
+bool short_run(const WinArgs& a) { return a.D <= HD - 16; }
+
+template <int HD, bool PART>
+void launch_fwd(const WinArgs& a, dim3 grid) {
+  if (short_run<HD>(a))
+    tjh_launch(k_win_fwd<HD, true, PART, HD / 2 - 8>, grid, dim3(256), 0, stream(), a);
+  else if (a.Tk % TILE || a.D != HD)
+    tjh_launch(k_win_fwd<HD, true, PART, HD / 2>, grid, dim3(256), 0, stream(), a);
+  else
+    tjh_launch(k_win_fwd<HD, false, PART, HD / 2>, grid, dim3(256), 0, stream(), a);
+}
+
+template <int HD>
+void launch_fwd(const WinArgs& a, dim3 grid, bool part) {
+  if (part) launch_fwd<HD, true>(a, grid);
+  else launch_fwd<HD, false>(a, grid);
+}
+
+template <int HD>
+int launch_bwd(WinArgs a, unsigned keys, float* dq, const int64_t* dq_st) {
+  if (short_run<HD>(a))
+    tjh_launch(k_win_dkv<HD, true, HD / 2 - 8>, dim3(keys), dim3(256), 0, stream(), a);
+  else if (a.Tq % TILE || a.Tk % TILE || a.D != HD)
+    tjh_launch(k_win_dkv<HD, true, HD / 2>, dim3(keys), dim3(256), 0, stream(), a);
+  else
+    tjh_launch(k_win_dkv<HD, false, HD / 2>, dim3(keys), dim3(256), 0, stream(), a);
+  int rc = check_launch("window_dkv");
+  if (rc != TJH_OK) return rc;
+  if (a.nslice > 1) {
+    const int64_t n4 = (int64_t)a.nbkv * a.nsb * PROWS * a.D / 4;
+    tjh_launch(k_win_sums, dim3((unsigned)cdiv(2 * n4, 256)), dim3(256), 0, stream(), a, n4);
+    if ((rc = check_launch("window_sums")) != TJH_OK) return rc;
+  }
+  a.nblk = (int)cdiv(a.Tq, ROWS);
+  a.out = dq;
+  a.o1s = s3(dq_st);
+  const unsigned grid = (unsigned)(a.nbkv * a.G * a.nblk);
+  if (a.Tk % TILE || a.D != HD)
+    tjh_launch(k_win_dq<HD, true>, dim3(grid), dim3(512), 0, stream(), a);
+  else
+    tjh_launch(k_win_dq<HD, false>, dim3(grid), dim3(512), 0, stream(), a);
+  return check_launch("window_dq");
+}
+
+int check_window(const char* who, int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk,
+                 int64_t D, int64_t window, int64_t sinks, const void* const* ptrs,
+                 const int64_t* const* strides, int n) {
+  TJH_ARG(B >= 0 && H >= 0 && Hkv >= 0 && Tq >= 0 && D > 0, "%s: bad sizes", who);
+  TJH_ARG(Tk >= Tq, "%s: %lld queries over %lld keys", who, (long long)Tq, (long long)Tk);
+  TJH_ARG(window >= 1 && sinks >= 0, "%s: window %lld, sinks %lld", who, (long long)window,
+          (long long)sinks);
+  TJH_ARG(H == 0 || (Hkv > 0 && H % Hkv == 0), "%s: %lld heads over %lld", who, (long long)H,
+          (long long)Hkv);
+  TJH_ARG(Tk < (int64_t(1) << 30) && H < (int64_t(1) << 30), "%s: too large", who);
+  TJH_ARG(B * H * cdiv(Tq, TILE) < (int64_t(1) << 31), "%s: grid too large", who);
+  for (int i = 0; i < n; ++i) TJH_ARG(strides[i], "%s: NULL strides", who);
+  if (B == 0 || H == 0 || Tq == 0) return TJH_OK;
+  for (int i = 0; i < n; ++i) TJH_ARG(ptrs[i], "%s: NULL pointer", who);
+  if (!flash_supported(D, ptrs, strides, n))
+    return set_error(TJH_ERR_UNSUPPORTED,
+                     "%s: head dims up to 128 that are multiples of 4, in 16-byte aligned rows "
+                     "(head dim %lld)", who, (long long)D);
+  return TJH_OK;
+}
+
+WinArgs win_args(int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t D, float scale,
+                 int64_t window, int64_t sinks) {
+  WinArgs a{};
+  a.H = (int)H; a.G = (int)(H / Hkv);
+  a.Tq = (int)Tq; a.Tk = (int)Tk; a.off = (int)(Tk - Tq); a.D = (int)D;
+  a.scale = scale;
+  a.win = (int)(window < Tk ? window : Tk);
+  a.sinks = (int)(sinks < Tk ? sinks : Tk);
+  // sinks that every query's window holds are none
+  if (a.win >= a.Tk) a.sinks = 0;
+  a.nst = (int)cdiv(a.sinks, TILE);
+  return a;
+}
+
+}  // namespace
+}  // namespace tjh
+
+using namespace tjh;
+
+extern "C" {
+
+int tjh_window_forward(const float* q, const float* k, const float* v, float* o, float* lse,
+                       int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t D,
+                       const int64_t* q_strides, const int64_t* k_strides,
+                       const int64_t* v_strides, const int64_t* o_strides, float scale,
+                       int64_t window, int64_t sinks) {
+  TJH_REQUIRE_INIT();
+  const void* ptrs[4] = {q, k, v, o};
+  const int64_t* sts[4] = {q_strides, k_strides, v_strides, o_strides};
+  int rc = check_window("tjh_window_forward", B, H, Hkv, Tq, Tk, D, window, sinks, ptrs, sts, 4);
+  if (rc != TJH_OK || B == 0 || H == 0 || Tq == 0) return rc;
+  WinArgs a = win_args(H, Hkv, Tq, Tk, D, scale, window, sinks);
+  a.q = q; a.k = k; a.v = v; a.out = o; a.lse_out = lse;
+  a.qs = s3(q_strides); a.ks = s3(k_strides); a.vs = s3(v_strides); a.os = s3(o_strides);
+  KernelScope ks("window_fwd");
+  const int64_t cus = num_cus() > 0 ? num_cus() : 256, rows = B * H * Tq;
+  // keys that a query sees at most
+  const int64_t most = a.win + a.sinks < a.Tk ? a.win + a.sinks : a.Tk;
+  const auto room = [&](Scratch& s, int64_t n) {
+    if (!s.ok()) return false;
+    a.part = s.as<float>();
+    a.pml = reinterpret_cast<float2*>(a.part + n * rows * D);
+    return true;
+  };
+  if (Tq <= 4) {
+    int64_t n = 1;
+    if (!lse && rows < cus && most > 512)
+      n = cdiv(most, 256) < cus / rows ? cdiv(most, 256) : cus / rows;
+    a.kslice = (int)cdiv(most, n);
+    n = cdiv(most, a.kslice);
+    Scratch s(n > 1 ? (size_t)(n * rows * (D + 2)) * sizeof(float) : 0);
+    const bool split = n > 1 && room(s, n);
+    const dim3 grid((unsigned)rows, split ? (unsigned)n : 1), block(kFewThreads);
+    if (split && D <= 64) tjh_launch(k_win_few<1, true>, grid, block, 0, stream(), a);
+    else if (split) tjh_launch(k_win_few<2, true>, grid, block, 0, stream(), a);
+    else if (D <= 64) tjh_launch(k_win_few<1, false>, grid, block, 0, stream(), a);
+    else tjh_launch(k_win_few<2, false>, grid, block, 0, stream(), a);
+    if ((rc = check_launch("window_few")) != TJH_OK || !split) return rc;
+    const int64_t n4 = rows * D / 4;
+    tjh_launch(k_win_merge, dim3((unsigned)cdiv(n4, 256)), dim3(256), 0, stream(), a, n4, (int)n);
+    return check_launch("window_merge");
+  }
+  a.nblk = (int)cdiv(Tq, ROWS);
+  const int64_t blocks = B * H * a.nblk;
+  // slices of the key tiles where the blocks of queries leave CUs idle and
+  // have enough tiles to pay for the join
+  const int64_t wt = cdiv((int64_t)a.win + ROWS - 2, TILE) + 1 + a.nst, all = cdiv(Tk, TILE);
+  const int64_t nt = wt < all ? wt : all;  // tiles of a block at most
+  int64_t n = 1;
+  if (!lse && blocks < cus && nt > 8) {
+    a.kslice = (int)(cdiv(nt * blocks, cus) < 4 ? 4 : cdiv(nt * blocks, cus));
+    n = cdiv(nt, a.kslice);
+  }
+  Scratch s(n > 1 ? (size_t)(n * rows * (D + 2)) * sizeof(float) : 0);
+  const bool split = n > 1 && room(s, n);
+  const dim3 grid((unsigned)blocks, split ? (unsigned)n : 1);
+  switch (cdiv(D, 32)) {
+    case 1: launch_fwd<32>(a, grid, split); break;
+    case 2: launch_fwd<64>(a, grid, split); break;
+    case 3: launch_fwd<96>(a, grid, split); break;
+    default: launch_fwd<128>(a, grid, split); break;
+  }
+  if ((rc = check_launch("window_fwd")) != TJH_OK || !split) return rc;
+  const int64_t n4 = rows * D / 4;
+  tjh_launch(k_win_merge, dim3((unsigned)cdiv(n4, 256)), dim3(256), 0, stream(), a, n4, 0);
+  return check_launch("window_merge");
+}
+
+int tjh_window_backward(const float* q, const float* k, const float* v, const float* o,
+                        const float* do_, const float* lse, float* dq, float* dk, float* dv,
+                        int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t D,
+                        const int64_t* const* strides, float scale, int64_t window,
+                        int64_t sinks) {
+  TJH_REQUIRE_INIT();
+  TJH_ARG(strides, "tjh_window_backward: NULL strides");
+  const void* ptrs[8] = {q, k, v, o, do_, dq, dk, dv};
+  int rc = check_window("tjh_window_backward", B, H, Hkv, Tq, Tk, D, window, sinks, ptrs, strides, 8);
+  if (rc != TJH_OK || B == 0 || H == 0 || Tq == 0) return rc;
+  TJH_ARG(lse, "tjh_window_backward: NULL pointer");
+  WinArgs a = win_args(H, Hkv, Tq, Tk, D, scale, window, sinks);
+  a.q = q; a.k = k; a.v = v; a.o = o; a.dout = do_; a.lse = lse; a.out = dk; a.out2 = dv;
+  a.qs = s3(strides[0]); a.ks = s3(strides[1]); a.vs = s3(strides[2]); a.os = s3(strides[3]);
+  a.gs = s3(strides[4]); a.o1s = s3(strides[6]); a.o2s = s3(strides[7]);
+  Scratch ds((size_t)(B * H * Tq) * sizeof(float));
+  if (!ds.ok()) return set_error(TJH_ERR_OOM, "tjh_window_backward: no scratch");
+  a.dsum = ds.as<float>();
+  KernelScope ks("window_bwd");
+  if ((rc = attn_dsum(do_, o, strides[4], strides[3], B, H, Tq, D, ds.as<float>())) != TJH_OK)
+    return rc;
+  a.nqt = (int)cdiv(Tq, TILE);
+  a.nkt = (int)cdiv(Tk, TILE);
+  // the window tiles of 32 queries: window + 31 keys from anywhere in a tile
+  const int64_t wt = cdiv((int64_t)a.win + 30, TILE) + 1;
+  a.nsl = (int)(a.nst + (wt < a.nkt ? wt : a.nkt));
+  a.nblk = (int)cdiv(Tk, PROWS);
+  a.nsb = (int)cdiv(a.sinks, PROWS);
+  // slices of the sinks' blocks about as long as the others' query tiles
+  const int64_t others = cdiv((int64_t)a.win + PROWS, TILE) + 1;
+  a.nslice = a.nsb ? (int)cdiv(a.nqt, others < 8 ? 8 : others) : 1;
+  // key heads at once: the dS blocks of all of them up to 4 GiB
+  const int64_t nbkv = B * Hkv;
+  const size_t per = (size_t)a.G * a.nqt * a.nsl * (TILE * TILE) * sizeof(float);
+  int64_t chunk = (int64_t)((size_t(4) << 30) / per);
+  chunk = chunk < 1 ? 1 : chunk > nbkv ? nbkv : chunk;
+  for (;;) {
+    Scratch blocks(per * chunk);
+    Scratch sums(a.nslice > 1
+                     ? (size_t)2 * a.nslice * chunk * a.nsb * PROWS * D * sizeof(float) : 0);
+    if (!blocks.ok() || (a.nslice > 1 && !sums.ok())) {
+      if (chunk == 1) return set_error(TJH_ERR_OOM, "tjh_window_backward: no scratch");
+      chunk = cdiv(chunk, 2);
+      continue;
+    }
+    a.dsblk = blocks.as<float>();
+    a.sums = sums.as<float>();
+    for (int64_t at = 0; at < nbkv; at += chunk) {
+      a.bkv0 = (int)at;
+      a.nbkv = (int)(nbkv - at < chunk ? nbkv - at : chunk);
+      const int64_t keys = (int64_t)a.nbkv * (a.nsb * a.nslice + a.nblk - a.nsb);
+      TJH_ARG(keys < (int64_t(1) << 31), "tjh_window_backward: grid too large");
+      switch (cdiv(D, 32)) {
+        case 1: rc = launch_bwd<32>(a, (unsigned)keys, dq, strides[5]); break;
+        case 2: rc = launch_bwd<64>(a, (unsigned)keys, dq, strides[5]); break;
+        case 3: rc = launch_bwd<96>(a, (unsigned)keys, dq, strides[5]); break;
+        default: rc = launch_bwd<128>(a, (unsigned)keys, dq, strides[5]); break;
+      }
+      if (rc != TJH_OK) return rc;
+    }
+    return TJH_OK;
+  }
+}
+
+}  // extern "C"

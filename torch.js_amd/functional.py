@@ -908,6 +908,45 @@ def _bhtd(t):
     return t
 
 
+def _grad_like(t):
+    """A gradient buffer for a [B, H, T, D] operand, laid out [B, T, H, D]."""
+    B, H, T, D = t.shape
+    return _alias(empty((B, T, H, D)), t.shape, (T * H * D, D, H * D, 1), 0)
+
+
+def _shared_grads(q, k, v):
+    """dq, dk, dv laid out exactly like q, k, v inside one new buffer when
+    the three are equally strided, disjoint views of one allocation (the
+    fused qkv projection split into heads): the gradient of that
+    projection's output is then that buffer, assembled with no copy."""
+    ts = (q, k, v)
+    if not all(t._storage is q._storage and t._strides == q._strides and
+               t.shape == q.shape for t in ts):
+        return None
+    # innermost dense run of the layout: each view is a set of runs of
+    # length `run` at offset + multiples of `period`
+    dims = sorted((st, n) for st, n in zip(q._strides, q.shape) if n > 1)
+    run, i = 1, 0
+    while i < len(dims) and dims[i][0] == run:
+        run *= dims[i][1]
+        i += 1
+    outer = [st for st, _ in dims[i:]]
+    if not outer:
+        return None
+    period = min(outer)
+    if run > period or any(st % period for st in outer):
+        return None
+    res = sorted(t._offset % period for t in ts)
+    gaps = [res[1] - res[0], res[2] - res[1], period - (res[2] - res[0])]
+    if min(gaps) < run:
+        return None  # the views share elements
+    ext = [t._offset + sum((n - 1) * st for n, st in zip(t.shape, t._strides)) + 1
+           for t in ts]
+    lo = min(t._offset for t in ts)
+    buf = empty((max(ext) - lo,))
+    return [_alias(buf, t.shape, t._strides, t._offset - lo) for t in ts]
+
+
 def scaled_dot_product_attention(query, key, value, attn_mask=None, dropout_p=0.0,
                                  is_causal=False, scale=None):
     """softmax(Q K^T * scale [causal] [mask]) V (src/nn/functional.ts:866-890).
@@ -943,51 +982,14 @@ def scaled_dot_product_attention(query, key, value, attn_mask=None, dropout_p=0.
                                      L.i64arr(v._strides[:3]), L.i64arr(o._strides[:3]), sc,
                                      1 if is_causal else 0), "sdpa")
 
-    def grad_like(t):
-        Bx, Hx, Tx, Dx = t.shape
-        buf = empty((Bx, Tx, Hx, Dx))
-        return _alias(buf, t.shape, (Tx * Hx * Dx, Dx, Hx * Dx, 1), 0)
-
-    def shared_grads():
-        """dq, dk, dv laid out exactly like q, k, v inside one new buffer when
-        the three are equally strided, disjoint views of one allocation (the
-        fused qkv projection split into heads): the gradient of that
-        projection's output is then that buffer, assembled with no copy."""
-        ts = (q, k, v)
-        if not all(t._storage is q._storage and t._strides == q._strides and
-                   t.shape == q.shape for t in ts):
-            return None
-        # innermost dense run of the layout: each view is a set of runs of
-        # length `run` at offset + multiples of `period`
-        dims = sorted((st, n) for st, n in zip(q._strides, q.shape) if n > 1)
-        run, i = 1, 0
-        while i < len(dims) and dims[i][0] == run:
-            run *= dims[i][1]
-            i += 1
-        outer = [st for st, _ in dims[i:]]
-        if not outer:
-            return None
-        period = min(outer)
-        if run > period or any(st % period for st in outer):
-            return None
-        res = sorted(t._offset % period for t in ts)
-        gaps = [res[1] - res[0], res[2] - res[1], period - (res[2] - res[0])]
-        if min(gaps) < run:
-            return None  # the views share elements
-        ext = [t._offset + sum((n - 1) * st for n, st in zip(t.shape, t._strides)) + 1
-               for t in ts]
-        lo = min(t._offset for t in ts)
-        buf = empty((max(ext) - lo,))
-        return [_alias(buf, t.shape, t._strides, t._offset - lo) for t in ts]
-
     def bwd(g):
         if three:
             g = _alias(g, (g.shape[0], 1) + g.shape[1:], (g._strides[0], 0) + g._strides[1:],
                        g._offset)
         if g._strides[3] != 1:
             g = _k_contiguous(g)
-        shared = shared_grads()
-        dq, dk, dv = shared if shared else (grad_like(q), grad_like(k), grad_like(v))
+        shared = _shared_grads(q, k, v)
+        dq, dk, dv = shared if shared else (_grad_like(q), _grad_like(k), _grad_like(v))
         arrs = [L.i64arr(t._strides[:3]) for t in (q, k, v, o, g, dq, dk, dv)]
         ptrs = (L.P_i64 * 8)(*[ctypes.cast(a, L.P_i64) for a in arrs])
         L.check(L.lib().tjh_sdpa_backward(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
@@ -1031,6 +1033,111 @@ def _sdpa_masked(query, key, value, attn_mask, scale):
     else:
         scores = scores + m.float() if m.dtype != "float32" else scores + m
     return _matmul(softmax(scores, -1), value)
+
+
+def _window_rows(t):
+    """[B, H, T, D] operand with dense, 16-byte aligned rows (a copy where
+    `t`'s are not)."""
+    st = t._strides
+    if t.numel() and ((st[3] != 1 and t.shape[3] > 1) or t.data_ptr() & 15 or
+                      any(s % 4 for s, n in zip(st[:3], t.shape) if n > 1)):
+        t = _k_contiguous(t)
+    # the stride of an axis of one element is free: one that the kernels take
+    return _alias(t, t.shape, tuple(0 if s % 4 else s for s in t._strides[:3]) + (1,), t._offset)
+
+
+def sliding_window_attention(query, key, value, window, sinks=0, scale=None):
+    """Causal attention over a sliding window, with a few first tokens that
+    stay visible (beside scaled_dot_product_attention,
+    src/nn/functional.ts:866-890; torch.js has none): query [B, H, Tq, D],
+    key and value [B, Hkv, Tk, D] (or all three [B, T, D]), where H is a
+    multiple of Hkv and query head h reads head h // (H // Hkv).  The queries
+    are the last Tq of the Tk positions: a whole sequence, the next part of
+    a prompt over a cache, or one decoding step.  The query at position i
+    sees the keys j <= i with j > i - window or j < sinks; what other keys
+    and values hold has no part in its output.  O(Tk) memory beside the
+    result, time by the keys seen.  Head dims up to 128; the gradients of
+    key and value are summed over the query heads that read them."""
+    window, sinks = _whole("window", window, 1), _whole("sinks", sinks, 0)
+    nd = query.ndim
+    if nd not in (3, 4) or key.ndim != nd or value.ndim != nd:
+        raise RuntimeError("sliding_window_attention expects three 3-D or three 4-D tensors")
+    three = nd == 3
+    if key.shape != value.shape or query.shape[0] != key.shape[0] or \
+            query.shape[-1] != key.shape[-1]:
+        raise RuntimeError("sliding_window_attention: shapes %s, %s, %s do not match"
+                           % (list(query.shape), list(key.shape), list(value.shape)))
+    D, Tq, Tk = query.shape[-1], query.shape[-2], key.shape[-2]
+    H, Hkv = (1, 1) if three else (query.shape[1], key.shape[1])
+    if (Hkv == 0) != (H == 0) or (Hkv and H % Hkv):
+        raise RuntimeError("sliding_window_attention: %d query heads over %d of keys" % (H, Hkv))
+    if Tq > Tk:
+        raise RuntimeError("sliding_window_attention: %d queries are not the last of %d positions"
+                           % (Tq, Tk))
+    if not 0 < D <= 128:
+        raise NotImplementedError("sliding_window_attention: head dims up to 128, got %d" % D)
+    sc = float(scale) if scale is not None else 1.0 / math.sqrt(D)
+    query, key, value = [t if t.dtype == "float32" else t.float() for t in (query, key, value)]
+    if D % 4:  # columns of zeros add nothing to any product
+        fill = 4 - D % 4
+        ts = [_T.cat([t, zeros(t.shape[:-1] + (fill,))], -1) for t in (query, key, value)]
+        return _T.narrow(sliding_window_attention(*ts, window, sinks, sc), -1, 0, D)
+    ins = [query, key, value]
+    q, k, v = [_window_rows(_bhtd(t.detach())) for t in ins]
+    B = q.shape[0]
+    rec = _T._recorded(*ins)
+    ob = empty((B, Tq, H, D))
+    o = _alias(ob, (B, H, Tq, D), (Tq * H * D, D, H * D, 1), 0)
+    lse = empty((B, H, Tq)) if rec else None
+    L.check(L.lib().tjh_window_forward(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+        lse.data_ptr() if lse is not None else None, B, H, Hkv, Tq, Tk, D, L.i64arr(q._strides[:3]),
+        L.i64arr(k._strides[:3]), L.i64arr(v._strides[:3]), L.i64arr(o._strides[:3]), sc, window,
+        sinks), "sliding_window_attention")
+
+    def bwd(g):
+        if three:
+            g = _alias(g, (B, 1) + g.shape[1:], (g._strides[0], 0) + g._strides[1:], g._offset)
+        g = _window_rows(g)
+        if not o.numel():
+            return [zeros(t.shape) for t in ins]
+        shared = _shared_grads(q, k, v)
+        dq, dk, dv = shared if shared else (_grad_like(q), _grad_like(k), _grad_like(v))
+        arrs = [L.i64arr(t._strides[:3]) for t in (q, k, v, o, g, dq, dk, dv)]
+        ptrs = (L.P_i64 * 8)(*[ctypes.cast(a, L.P_i64) for a in arrs])
+        L.check(L.lib().tjh_window_backward(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), g.data_ptr(), lse.data_ptr(),
+            dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, H, Hkv, Tq, Tk, D, ptrs, sc, window,
+            sinks), "sliding_window_attention_backward")
+        if three:
+            dq, dk, dv = [_alias(t, (B,) + t.shape[2:], (t._strides[0],) + t._strides[2:],
+                                 t._offset) for t in (dq, dk, dv)]
+        return [dq, dk, dv]
+
+    def gbwd(g):  # softmax over explicit scores with recording ops
+        i = np.arange(Tk - Tq, Tk)[:, None]
+        j = np.arange(Tk)
+        drop = _T.tensor(~((j <= i) & ((j > i - window) | (j < sinks))))
+
+        def ref(qq, kk, vv):
+            if H != Hkv:
+                kk, vv = [reshape(_T.expand(reshape(t, (B, Hkv, 1, Tk, D)),
+                                            (B, Hkv, H // Hkv, Tk, D)), (B, H, Tk, D))
+                          for t in (kk, vv)]
+            scores = mul(_T.matmul(qq, kk.transpose(-2, -1)), sc)
+            return _T.matmul(softmax(_T.masked_fill(scores, drop, float("-inf")), -1), vv)
+        return _T._regrad(ref, ins, g)
+    out = _alias(ob, (B, Tq, D), (Tq * D, D, 1), 0) if three else o
+    return _record(out, "WindowAttention", ins, bwd, gfn=gbwd)
+
+
+def _whole(name, value, least):
+    """`value` as a whole number of at least `least`."""
+    n = int(value)
+    if n != value or n < least:
+        raise ValueError("sliding_window_attention: %s must be a whole number of at least %d, "
+                         "got %r" % (name, least, value))
+    return min(n, 1 << 30)
 
 
 # ------------------------------------------------------------ one_hot
