@@ -274,13 +274,13 @@ __device__ __forceinline__ void sort_list(SelectLds<T, CAP>& s, int c) {
 
 // The elements for which in(j, u, x) holds into the list, in no order (it is
 // sorted next): their number, of which the first CAP were stored.
-template <int T, int NV, int CAP, class In>
-__device__ __forceinline__ int gather_list(const Row<T, NV>& row, uint32_t nan, In in,
+template <int T, int CAP, class In>
+__device__ __forceinline__ int gather_list(const Row<T, 0>& row, uint32_t nan, In in,
                                            SelectLds<T, CAP>& s) {
   if (threadIdx.x == 0) s.count = 0;
   __syncthreads();
   row.each([&](int j, int u, float x) {
-    if (in(j, u, x) && row.inside(j, u)) {  // few do
+    if (in(j, u, x) && row.inside(j, u)) {
       const int at = atomicAdd(&s.count, 1);
       if (at < CAP) s.list[at] = composite(order_key(x, nan), row.index(j, u));
     }
@@ -289,11 +289,61 @@ __device__ __forceinline__ int gather_list(const Row<T, NV>& row, uint32_t nan, 
   return s.count;
 }
 
+// The same for the elements that are not below `bound` (few of the row).
+// Those in registers are marked first and then read again, so that the rest
+// is one small loop and not a copy for every register.
+template <int T, int NV, int CAP>
+__device__ __forceinline__ int gather_above(const Row<T, NV>& row, uint32_t nan, float bound,
+                                            SelectLds<T, CAP>& s) {
+  if constexpr (NV == 0) {
+    return gather_list(row, nan, [&](int, int, float x) { return !(x < bound); }, s);
+  } else {
+    if (threadIdx.x == 0) s.count = 0;
+    constexpr int kWords = (4 * NV + 31) / 32;
+    uint32_t marks[kWords];
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) marks[i] = 0;
+#pragma unroll
+    for (int i = 0; i < 4 * NV; ++i) marks[i / 32] |= row.v[i] < bound ? 0u : 1u << (i % 32);
+    __syncthreads();  // the count is 0
+    const auto put = [&](int i) {
+      const int at = atomicAdd(&s.count, 1);
+      if (at < CAP) s.list[at] = composite(order_key(row.at(i), nan), i);
+    };
+    if (row.edge_index >= 0 && !(row.edge < bound)) put(row.edge_index);
+#pragma unroll
+    for (int i = 0; i < kWords; ++i)
+      for (uint32_t m = marks[i]; m; m &= m - 1) {
+        const int e = 32 * i + __ffs(m) - 1;
+        if (row.inside(e / 4, e % 4)) put(row.index(e / 4, e % 4));
+      }
+    __syncthreads();
+    return s.count;
+  }
+}
+
+// The index of the need-th element (in index order, need >= 1) of those for
+// which in(j, u, x) holds, by bisection: log2(n) passes.  Passes over memory
+// here and below: over the registers they would keep an index and a mask of
+// every element besides.
+template <int T, class In>
+__device__ __forceinline__ int nth_index(const Row<T, 0>& row, int need, In in, Block<T>& b) {
+  int lo = 0;  // fewer than `need` of them lie before lo
+  for (int bit = 31 - __builtin_clz((unsigned)row.n); bit >= 0; --bit) {
+    const int c = lo + (1 << bit);
+    if (c > row.n) continue;  // the same for every thread
+    int m = 0;
+    row.each([&](int j, int u, float x) {
+      m += row.inside(j, u) && row.index(j, u) < c && in(j, u, x);
+    });
+    if (b.sum_i(m) < need) lo = c;
+  }
+  return lo;
+}
+
 // The composite of the row's k-th largest element (1 <= k <= n) by bisection
 // over the keys, then over the indices of the elements that share the key:
-// 32 + log2(n) passes, for rows with more near-ties than the list holds, and
-// for any k.  Passes over memory: a pass over the registers would keep an
-// index and a mask of every element besides.
+// for rows with more near-ties than the list holds, and for any k.
 template <int T>
 __device__ __forceinline__ u64 kth_by_bisection(const Row<T, 0>& row, int k, uint32_t nan,
                                                 Block<T>& b) {
@@ -310,39 +360,45 @@ __device__ __forceinline__ u64 kth_by_bisection(const Row<T, 0>& row, int k, uin
   int above = 0;
   row.each([&](int j, int u, float x) { above += key(j, u, x) > t; });
   const int need = k - b.sum_i(above);  // of the elements with key t, >= 1
-  int lo = 0;                           // fewer than `need` of them lie before lo
-  for (int bit = 31 - __builtin_clz((unsigned)row.n); bit >= 0; --bit) {
-    const int c = lo + (1 << bit);
-    if (c > row.n) continue;  // the same for every thread
-    int m = 0;
-    row.each([&](int j, int u, float x) { m += key(j, u, x) == t && row.index(j, u) < c; });
-    if (b.sum_i(m) < need) lo = c;
+  return composite(
+      t, nth_index(row, need, [&](int j, int u, float x) { return key(j, u, x) == t; }, b));
+}
+
+// A bound that the row's k largest elements are not below and few others are
+// either: the k-th largest of the threads' own maxima (two of each thread),
+// to the 16 high bits of its key, found two at a time; -infinity where there
+// are fewer maxima.  50 of 50257 random values leave about 55.
+template <int T, int NV>
+__device__ __forceinline__ float kth_bound(const Row<T, NV>& row, int k, Block<T>& b) {
+  float mx[2] = {-INFINITY, -INFINITY};  // NaN takes no part: still a lower bound
+  row.each([&](int j, int, float x) { mx[j & 1] = fmaxf(mx[j & 1], x); });
+  const uint32_t mk[2] = {order_key(mx[0]), order_key(mx[1])};
+  uint32_t lo = 0;
+#pragma unroll 1
+  for (int bit = 30; bit >= 16; bit -= 2) {  // counts of three bounds a round
+    u64 c = 0;
+#pragma unroll
+    for (int i = 3; i >= 1; --i) {
+      const uint32_t bound = lo | ((uint32_t)i << bit);
+      c = (c << 20) | (u64)(__popcll(__ballot(mk[0] >= bound)) + __popcll(__ballot(mk[1] >= bound)));
+    }
+    c = b.across(c, [](u64 x, u64 y) { return x + y; });
+    uint32_t digit = 0;
+#pragma unroll
+    for (int i = 1; i <= 3; ++i)
+      if ((int)((c >> (20 * (i - 1))) & 0xfffff) >= k) digit = i;
+    lo |= digit << bit;
   }
-  return composite(t, lo);
+  return lo > 0x007fffffu ? key_value(lo) : -INFINITY;  // 0x007fffff: the key of -infinity
 }
 
 // Sorts the row's k largest elements into list[0, k), 1 <= k <= min(n, CAP).
-// The k-th largest of the threads' own maxima (two of each thread) is a
-// lower bound of the k-th largest element, and few elements lie above it:
-// 50 of 50257 random values leave about 55.  The bound is taken to its 16
-// high bits, 16 counts instead of 32.  Where more than CAP elements remain
-// (ties), the exact bound comes from bisection.
+// Where more than CAP elements are above the bound (ties), the exact one
+// comes from bisection.
 template <int T, int NV, int CAP>
 __device__ __forceinline__ void select_largest(const Row<T, NV>& row, int k, uint32_t nan,
                                                SelectLds<T, CAP>& s, Block<T>& b) {
-  float mx[2] = {-INFINITY, -INFINITY};  // NaN takes no part: still a lower bound
-  row.each([&](int j, int, float x) { mx[j & 1] = fmaxf(mx[j & 1], x); });
-  const uint32_t mk[2] = {order_key(mx[0], nan), order_key(mx[1], nan)};
-  uint32_t lo = 0;
-#pragma unroll 1
-  for (int bit = 31; bit >= 16; --bit) {
-    const uint32_t c = lo | (1u << bit);
-    const bool p[2] = {mk[0] >= c, mk[1] >= c};
-    if (b.count(p) >= k) lo = c;
-  }
-  // below the key of -infinity everything is a candidate
-  const float bound = lo > 0x007fffffu ? key_value(lo) : -INFINITY;
-  const int c = gather_list(row, nan, [&](int, int, float x) { return !(x < bound); }, s);
+  const int c = gather_above(row, nan, kth_bound(row, k, b), s);
   if (c > CAP) {
     Row<T, 0> again;
     again.load(row.p, row.n, row.sign);

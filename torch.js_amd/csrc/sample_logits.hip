@@ -16,20 +16,21 @@
 // Weights are integers, w_i * 2^s with the row's sum below 2^62 (s = 46 at
 // 50257 columns): sums are then the same in whatever order the atomics and
 // the waves add them, exact, and finer than 32-bit floats by 2^22.  They are
-// formed in 64 bits as 2^t = 2^(k / 128) 2^f, |f| <= 1 / 256, from a table and
-// the first five terms of 2^f (the sixth is below 2^-49): 32-bit ones would
+// formed in 64 bits as 2^t = 2^(k / 32) 2^f, |f| <= 1 / 64, from a table and
+// the first six terms of 2^f (the seventh is below 2^-48): 32-bit ones would
 // move one draw in some thousand over a border between two indices.
 //
-// One workgroup has a row, in registers (rowreg.h).  With top_k up to 256 the
-// largest elements are sorted in LDS and everything else happens on that
-// list.  Otherwise every element's weight is needed: a nucleus takes a pass
-// for the weights' sum, one that adds the weights of the elements that can
-// be in it to a histogram over x (an element of weight w_i is outside when
-// even n elements of its weight are no more than 1 - top_p of the sum), and
-// sorts the one bin that the nucleus ends in; then the draw adds the kept
-// weights up by wave and chunk, which is index order, and looks into one.
+// One workgroup has a row, in registers (rowreg.h).  Wherever the elements
+// that can be drawn fit (4096), they are moved into LDS and sorted, and
+// everything else happens on that list: the top_k largest; the elements
+// above min_p's bound; the nucleus, whose end comes from a histogram of the
+// weights over x, one pass in which every element's weight is formed.
+// Larger sets are a bound on (x, index), found in the histogram's last bin,
+// and a pass that adds the kept weights up by wave and chunk, which is index
+// order, and looks into one.
 #include "rowreg.h"
 
+#include <float.h>
 #include <math.h>
 
 namespace tjh {
@@ -37,8 +38,8 @@ namespace {
 
 using namespace rowreg;
 
-constexpr int kCap = 4096;    // sorted elements
-constexpr int kList = 256;    // top_k whose elements are drawn from in LDS
+constexpr int kCap = 4096;    // elements of a list
+constexpr int kMostK = 1024;  // top_k that is selected by the threads' maxima
 constexpr int kBins = 2048;   // of the nucleus's histogram
 constexpr int64_t kMaxCols = int64_t(1) << 20;
 
@@ -61,10 +62,11 @@ struct SampleLds {
   union {
     u64 bins[kBins];
     u64 seg[NV > 0 ? NV * (T / 64) : 4096];  // weight of each (chunk, wave)
-    u64 w[kList];
+    u64 w[kCap];                             // weights of the list
   };
-  double pow2[128];  // 2^(i / 128 + s)
+  double pow2[32];  // 2^(i / 32 + s)
   u64 edge_w[6];
+  u64 first;
   int pick;
 };
 
@@ -72,18 +74,44 @@ struct SampleLds {
 __device__ __forceinline__ u64 weight_of(double t, const double* pow2) {
   constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: its low word takes the integer
   constexpr double c1 = 6.93147180559945286e-01, c2 = 2.40226506959100694e-01,
-                   c3 = 5.55041086648215762e-02, c4 = 9.61812910762847687e-03;  // ln(2)^k / k!
+                   c3 = 5.55041086648215762e-02, c4 = 9.61812910762847687e-03,
+                   c5 = 1.33335581464284411e-03;  // ln(2)^k / k!
   t = fmax(t, -64.0);  // 2^(51 - 64) is 0
-  const double kd = __builtin_fma(t, 128.0, kMagic);
+  const double kd = __builtin_fma(t, 32.0, kMagic);
   const int k = (int)__double_as_longlong(kd);
-  const double f = __builtin_fma(kd - kMagic, -1.0 / 128, t);
-  double e = __builtin_fma(f, c4, c3);
+  const double f = __builtin_fma(kd - kMagic, -1.0 / 32, t);
+  double e = __builtin_fma(f, c5, c4);
+  e = __builtin_fma(f, e, c3);
   e = __builtin_fma(f, e, c2);
   e = __builtin_fma(f, e, c1);
-  const double tab = pow2[k & 127];
+  const double tab = pow2[k & 31];
   e = __builtin_fma(tab * f, e, tab);
-  e = ldexp(e, k >> 7) + 4503599627370496.0;  // 2^52: the integer is in the low 52 bits
+  e = ldexp(e, k >> 5) + 4503599627370496.0;  // 2^52: the integer is in the low 52 bits
   return (u64)__double_as_longlong(e) & 0xfffffffffffffull;
+}
+
+// A float that is not above x, nor far below it.
+__device__ __forceinline__ float float_below(double x) {
+  const float f = (float)x;
+  return f - (fabsf(f) * 2.4e-7f + FLT_MIN);
+}
+
+// Row::each with the work of one chunk kept together: all elements' weights
+// at once would take more registers than there are.
+template <int T, int NV, class F>
+__device__ __forceinline__ void each_chunk(const Row<T, NV>& row, F f) {
+  if constexpr (NV > 0) {
+    f(-1, 0, row.edge);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) f(j, u, row.v[4 * j + u]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  } else {
+    row.each(f);
+  }
 }
 
 template <int T, int NV>
@@ -91,6 +119,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
   __shared__ SampleLds<T, NV> lds;
   SelectLds<T, kCap>& s = lds.s;
   constexpr int W = T / 64;
+  constexpr int kNone = 0x7fffffff;
   const int64_t r = blockIdx.x;
   const int t = threadIdx.x;
   Block<T> b(s.sm);
@@ -111,7 +140,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
     return;
   }
   const double temp = a.temperature ? (double)a.temperature[r] : a.t0;
-  if (t == 0) lds.pick = 0x7fffffff;
+  if (t == 0) lds.pick = kNone;
   if (!(temp > 0.0)) {
     __syncthreads();
     row.each([&](int j, int u, float x) {
@@ -129,116 +158,111 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
   const double floor_z = min_p > 0.0 ? fmin(temp * log(min_p), 0.0) : -INFINITY;
   const double m = (double)mx;
   const double per_t = fmin(1.4426950408889634074 / temp, 1e300);
-  const double scale = ldexp(1.0, min(51, 62 - (32 - __clz(n))));
   const double u = (double)a.u[r];
-  if (t < 128) lds.pow2[t] = exp2((double)t / 128) * scale;
+  if (t < 32) lds.pow2[t] = ldexp(exp2((double)t / 32), min(51, 62 - (32 - __clz(n))));
   __syncthreads();
   const auto weight = [&](float x) { return weight_of(((double)x - m) * per_t, lds.pow2); };
 
   // elements of the order up to (tx, ti) are kept
   float tx = -INFINITY;
   int ti = n;
-  if (use_k && top_k <= kCap / 4) {
-    const int k = (int)top_k;
-    select_largest(row, k, kNanFirst, s, b);
-    if (k <= kList && k <= T) {
-      const u64 c = t < k ? s.list[t] : 0;
-      const float x = t < k ? key_value((uint32_t)(c >> 32)) : -INFINITY;
-      const u64 w = weight(x);
-      u64 all;
-      const u64 before = b.before(w, &all);
-      const bool keep = t < k && (!use_p || (double)before < p * (double)all) &&
-                        (double)x - m >= floor_z;
-      const u64 kept = b.sum64(keep ? w : 0);
-      const bool one[1] = {keep};
-      const int count = b.count(one);
-      if (t < k) lds.w[t] = w;
-      __syncthreads();
-      const double target = u * (double)kept;
-      if (keep && w) {
-        const int me = index_of(c);
-        u64 sum = 0;
-        for (int j = 0; j < count; ++j) sum += index_of(s.list[j]) <= me ? lds.w[j] : 0;
-        if ((double)sum > target) atomicMin(&lds.pick, me);
-      }
-      __syncthreads();
-      if (lds.pick == 0x7fffffff) {  // u is 1 or more: the last one of any weight
-        __syncthreads();
-        if (t == 0) lds.pick = -1;
-        __syncthreads();
-        if (keep && w) atomicMax(&lds.pick, index_of(c));
-        __syncthreads();
-      }
-      if (t == 0) a.out[r] = lds.pick;
-      return;
-    }
-    const u64 c = s.list[k - 1];
-    tx = key_value((uint32_t)(c >> 32));
-    ti = index_of(c);
-  } else if (use_k) {
-    Row<T, 0> again;
-    again.load(row.p, n);
-    const u64 c = kth_by_bisection(again, (int)top_k, kNanFirst, b);
-    tx = key_value((uint32_t)(c >> 32));
-    ti = index_of(c);
-  }
   const auto in_order = [&](const auto& of, int j, int e, float x) {
     return x > tx || (x == tx && of.index(j, e) <= ti);
   };
-
-  if (use_p) {
-    u64 mine = 0;
-    row.each([&](int j, int e, float x) { mine += in_order(row, j, e, x) ? weight(x) : 0; });
-    const u64 all = b.sum64(mine);
-    const double limit = p * (double)all;  // weight before an element that is in
-    // elements further than `far` below the maximum are outside
-    const double far =
-        fmax(temp * (log((double)n) - log1p(-p) - log((double)all / scale)) * 1.001, 0.0);
-    const float per = (float)((kBins - 1) / far);
+  const bool largest = use_k && top_k <= kMostK, cut = use_k && !largest;
+  if (cut) {
+    Row<T, 0> again;
+    again.load(row.p, n);
+    const u64 last = kth_by_bisection(again, (int)top_k, kNanFirst, b);
+    tx = key_value((uint32_t)(last >> 32));
+    ti = index_of(last);
+  }
+  // the elements that can be drawn are not below `bound`: where that is known
+  float bound = -INFINITY;
+  double limit = INFINITY;  // weight before an element that is in the nucleus
+  const auto bin_of = [&](float per, float x) {  // nondecreasing as x falls
+    const float z = (float)(m - (double)x) * per;
+    return z < (float)(kBins - 1) ? (int)z : kBins - 1;
+  };
+  float per = 0.f;
+  int last = -1;
+  if (largest) {
+    bound = kth_bound(row, (int)top_k, b);
+  } else if (use_p) {
+    // weights by bins of m - x, out to weights of e^-24 or the smallest x
+    float mn = mx;
+    row.each([&](int, int, float x) { mn = x > -INFINITY ? fminf(mn, x) : mn; });
+    mn = -b.max(-mn);
+    per = (float)(kBins / fmax(fmin(24.0 * temp, m - (double)mn), 1e-30));
     for (int i = t; i < kBins; i += T) lds.bins[i] = 0;
     __syncthreads();
-    const auto bin = [&](float x) {  // nondecreasing as x falls
-      const float z = (float)(m - (double)x) * per;
-      return z < (float)(kBins - 1) ? (int)z : kBins - 1;
-    };
-    row.each([&](int j, int e, float x) {
-      if (m - (double)x <= far && in_order(row, j, e, x)) atomicAdd(&lds.bins[bin(x)], weight(x));
+    each_chunk(row, [&](int j, int e, float x) {
+      const u64 w = !cut || in_order(row, j, e, x) ? weight(x) : 0;
+      if (w) atomicAdd(&lds.bins[bin_of(per, x)], w);
     });
     if (t == 0) lds.pick = -1;
     __syncthreads();
-    // the last bin before which less than `limit` lies
     u64 run = 0;
+    for (int i = t; i < kBins; i += T) run += lds.bins[i];
+    limit = p * (double)b.sum64(run);
+    // the last bin before which less than the limit lies
+    run = 0;
     for (int i0 = 0; i0 < kBins; i0 += T) {
       const u64 w = lds.bins[i0 + t];
       u64 part;
       const u64 before = run + b.before(w, &part);
-      if (w && (double)before < limit) {
-        atomicMax(&lds.pick, i0 + t);
-      }
+      if (w && (double)before < limit) atomicMax(&lds.pick, i0 + t);
       run += part;
     }
     __syncthreads();
-    const int last = lds.pick;
-    run = 0;
-    for (int i0 = 0; i0 < kBins; i0 += T) run += i0 + t < last ? lds.bins[i0 + t] : 0;
+    last = lds.pick;
+    // elements of later bins that are not below it do no harm
+    if (last < kBins - 1) bound = float_below(m - (last + 1.01) / per);
+  } else if (floor_z > -INFINITY) {
+    bound = float_below(m + floor_z);
+  }
+  int c = -1;  // elements of the list, if there is one
+  if (largest || bound > -INFINITY) {
+    c = gather_above(row, kNanFirst, bound, s);
+    if (c > kCap) c = -1;
+  }
+  if (largest) {
+    if (c < 0) {
+      Row<T, 0> again;
+      again.load(row.p, n);
+      const u64 thr = kth_by_bisection(again, (int)top_k, kNanFirst, b);
+      gather_list(
+          again, kNanFirst,
+          [&](int j, int e, float x) { return composite(order_key(x), again.index(j, e)) >= thr; },
+          s);
+      c = (int)top_k;
+    }
+    sort_list(s, c);
+    c = (int)top_k;
+  } else if (c >= 0 && use_p) {
+    sort_list(s, c);
+  } else if (c < 0 && use_p) {
+    // the nucleus ends in bin `last`: its elements alone
+    Row<T, 0> again;
+    again.load(row.p, n);
+    const auto in_bin = [&](int j, int e, float x) {
+      return bin_of(per, x) == last && x > -INFINITY && in_order(again, j, e, x);
+    };
+    u64 run = 0;
+    for (int i = t; i < last; i += T) run += lds.bins[i];
     const u64 above = b.sum64(run);
-    const int c = gather_list(
-        row, kNanFirst,
-        [&](int j, int e, float x) {
-          return m - (double)x <= far && bin(x) == last && in_order(row, j, e, x);
-        },
-        s);
-    if (c <= kCap) {
-      sort_list(s, c);
+    const int in = gather_list(again, kNanFirst, in_bin, s);
+    if (in <= kCap) {
+      sort_list(s, in);
       if (t == 0) lds.pick = 0;
       __syncthreads();
       u64 sum = above;
-      for (int i0 = 0; i0 < c; i0 += T) {
+      for (int i0 = 0; i0 < in; i0 += T) {
         const int i = i0 + t;
-        const u64 w = i < c ? weight(key_value((uint32_t)(s.list[i] >> 32))) : 0;
+        const u64 w = i < in ? weight(key_value((uint32_t)(s.list[i] >> 32))) : 0;
         u64 part;
         const u64 before = sum + b.before(w, &part);
-        if (i < c && (double)before < limit) atomicMax(&lds.pick, i);
+        if (i < in && (double)before < limit) atomicMax(&lds.pick, i);
         sum += part;
       }
       __syncthreads();
@@ -246,34 +270,115 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
       tx = key_value((uint32_t)(e >> 32));
       ti = index_of(e);
     } else {
-      // more equal logits than the list holds: the largest composite with at
-      // least `limit` above it, bit by bit, is the first one outside
-      Row<T, 0> again;
-      again.load(row.p, n);
-      u64 out = 0;
-      for (int bit = 63; bit >= 0; --bit) {
-        const u64 cand = out | (u64(1) << bit);
-        u64 w = 0;
-        again.each([&](int j, int e, float x) {
-          if (again.inside(j, e) && in_order(again, j, e, x) &&
-              composite(order_key(x), again.index(j, e)) > cand)
-            w += weight(x);
-        });
-        if ((double)b.sum64(w) >= limit) out = cand;
-      }
-      // the kept elements are the composites above `out`; the last one's
-      __syncthreads();
-      if (t == 0) s.list[0] = ~u64(0);
-      __syncthreads();
+      // more elements than the list holds.  All equal: as many of them as
+      // there is room for, by index; else the largest composite with at
+      // least the limit above it, bit by bit, is the first one outside
+      float lo = INFINITY, hi = -INFINITY;
       again.each([&](int j, int e, float x) {
-        const u64 c = composite(order_key(x), again.index(j, e));
-        if (again.inside(j, e) && c > out) atomicMin(&s.list[0], c);
+        if (in_bin(j, e, x)) {
+          lo = fminf(lo, x);
+          hi = fmaxf(hi, x);
+        }
       });
-      __syncthreads();
-      tx = key_value((uint32_t)(s.list[0] >> 32));
-      ti = index_of(s.list[0]);
+      lo = -b.max(-lo);
+      hi = b.max(hi);
+      if (lo == hi) {
+        // element i of them is in where above + i * w < limit
+        const double w = (double)weight(lo);
+        int q = (int)ceil((limit - (double)above) / w);
+        q = q < 1 ? 1 : q > in ? in : q;
+        while (q > 1 && !((double)above + (q - 1) * w < limit)) --q;
+        while (q < in && (double)above + q * w < limit) ++q;
+        ti = nth_index(
+            again, q, [&](int j, int e, float x) { return x == lo && in_order(again, j, e, x); }, b);
+        tx = lo;
+      } else {
+        u64 out = 0;
+        for (int bit = 63; bit >= 0; --bit) {
+          const u64 cand = out | (u64(1) << bit);
+          u64 w = 0;
+          again.each([&](int j, int e, float x) {
+            if (again.inside(j, e) && in_order(again, j, e, x) &&
+                composite(order_key(x), again.index(j, e)) > cand)
+              w += weight(x);
+          });
+          if ((double)b.sum64(w) >= limit) out = cand;
+        }
+        // the kept elements are the composites above `out`; the last one's
+        if (t == 0) lds.first = ~u64(0);
+        __syncthreads();
+        again.each([&](int j, int e, float x) {
+          const u64 at = composite(order_key(x), again.index(j, e));
+          if (again.inside(j, e) && at > out) atomicMin(&lds.first, at);
+        });
+        __syncthreads();
+        tx = key_value((uint32_t)(lds.first >> 32));
+        ti = index_of(lds.first);
+      }
     }
-    __syncthreads();  // bins and list are free
+    __syncthreads();  // bins are free
+  }
+
+  if (c >= 0) {
+    // the list's weights (none for elements that are not kept), the cut, and
+    // the rest in index order
+    u64 mine = 0;
+    for (int i = t; i < c; i += T) {
+      const u64 e = s.list[i];
+      const float x = key_value((uint32_t)(e >> 32));
+      const bool in = (double)x - m >= floor_z && (x > tx || (x == tx && index_of(e) <= ti));
+      const u64 w = in || largest ? weight(x) : 0;
+      lds.w[i] = w;
+      mine += w;
+    }
+    u64 all = b.sum64(mine);
+    int keep = c;
+    if (largest || use_p) {  // the list is sorted
+      if (largest && use_p) limit = p * (double)all;
+      int kept = 0;
+      u64 sum = 0, mine_kept = 0;
+      for (int i0 = 0; i0 < c; i0 += T) {
+        const int i = i0 + t;
+        const u64 w = i < c ? lds.w[i] : 0;
+        u64 part;
+        const u64 before = sum + b.before(w, &part);
+        sum += part;
+        const bool in = i < c && (double)before < limit &&
+                        (double)key_value((uint32_t)(s.list[i] >> 32)) - m >= floor_z;
+        kept += in;
+        mine_kept += in ? w : 0;
+      }
+      keep = b.sum_i(kept);
+      all = b.sum64(mine_kept);
+    }
+    // (index, place in the list), in ascending order of the index
+    if (t == 0) lds.pick = kNone;
+    for (int i = t; i < keep; i += T) s.list[i] = (s.list[i] << 32) | (uint32_t)i;
+    sort_list(s, keep);
+    const double target = u * (double)all;
+    u64 sum = 0;
+    int end = -1;  // the last one of any weight, where u is 1 or more
+    for (int i0 = 0; i0 < keep; i0 += T) {
+      const int i = i0 + t;
+      const u64 w = i < keep ? lds.w[(uint32_t)s.list[i]] : 0;
+      u64 part;
+      const u64 before = sum + b.before(w, &part);
+      sum += part;
+      if (w && (double)(before + w) > target) atomicMin(&lds.pick, i);
+      if (w) end = i;
+    }
+    __syncthreads();
+    int at = lds.pick;
+    if (at == kNone) {
+      __syncthreads();
+      if (t == 0) lds.pick = -1;
+      __syncthreads();
+      atomicMax(&lds.pick, end);
+      __syncthreads();
+      at = lds.pick;
+    }
+    if (t == 0) a.out[r] = (int)~(uint32_t)(s.list[at] >> 32);
+    return;
   }
 
   // the kept weight of every wave's part of every chunk, in index order
@@ -281,33 +386,20 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
     return in_order(of, j, e, x) && (double)x - m >= floor_z ? weight(x) : 0;
   };
   const int w = t >> 6, lane = t & 63;
-  const int chunks = NV > 0 ? NV : (row.n4 + T - 1) / T;
-  u64 part = 0;
-  const auto flush = [&](int j) {
+  const int chunks = (row.n4 + T - 1) / T;
+  for (int j = 0; j < chunks; ++j) {  // the row once more, from the L2
+    const int at = t + j * T;
+    u64 part = 0;
+    if (at < row.n4) {
+      const float4 x = *reinterpret_cast<const float4*>(row.p + row.head + 4 * at);
+      part = kept(row, j, 0, x.x) + kept(row, j, 1, x.y) + kept(row, j, 2, x.z) +
+             kept(row, j, 3, x.w);
+    }
     if (__ballot(part != 0)) part = wave_sum_u64(part);
     if (lane == 0) lds.seg[j * W + w] = part;
-    part = 0;
-  };
-  if constexpr (NV > 0) {
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) part += kept(row, j, e, row.v[4 * j + e]);
-      flush(j);
-    }
-  } else {
-    for (int j = 0; j < chunks; ++j) {
-      const int c = t + j * T;
-      if (c < row.n4) {
-        const float4 x = *reinterpret_cast<const float4*>(row.p + row.head + 4 * c);
-        part = kept(row, j, 0, x.x) + kept(row, j, 1, x.y) + kept(row, j, 2, x.z) +
-               kept(row, j, 3, x.w);
-      }
-      flush(j);
-    }
   }
   if (t < 6) lds.edge_w[t] = row.edge_index >= 0 ? kept(row, -1, 0, row.edge) : 0;
-  if (t == 0) lds.pick = 0x7fffffff;
+  if (t == 0) lds.pick = kNone;
   __syncthreads();
   const u64 first = lds.edge_w[0] + lds.edge_w[1] + lds.edge_w[2];
   u64 sum = 0;
@@ -316,19 +408,19 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
   const u64 all = first + inner + lds.edge_w[3] + lds.edge_w[4] + lds.edge_w[5];
   const double target = u * (double)all;
   // index order: the head's elements, the segments, the tail's elements
-  u64 run = first;
   if ((double)first > target && first) {
     if (t == 0) {
-      u64 c = 0;
+      u64 cum = 0;
       int i = 0;
       for (; i < 2; ++i) {
-        c += lds.edge_w[i];
-        if (lds.edge_w[i] && (double)c > target) break;
+        cum += lds.edge_w[i];
+        if (lds.edge_w[i] && (double)cum > target) break;
       }
       a.out[r] = i;
     }
     return;
   }
+  u64 run = first;
   for (int i0 = 0; i0 < chunks * W; i0 += T) {
     const int i = i0 + t;
     const u64 v = i < chunks * W ? lds.seg[i] : 0;
@@ -339,16 +431,16 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
   }
   __syncthreads();
   const int seg = lds.pick;
-  if (seg != 0x7fffffff) {
+  if (seg != kNone) {
     // the weight before the segment, then the segment by itself
     u64 sum_before = 0;
     for (int i = t; i < seg; i += T) sum_before += lds.seg[i];
     const u64 base = first + b.sum64(sum_before);
     if (w != 0) return;
-    const int j = seg / W, th = (seg % W) * 64 + lane, c = th + j * T;
+    const int j = seg / W, th = (seg % W) * 64 + lane, at = th + j * T;
     u64 wt[4] = {0, 0, 0, 0};
-    const int i = row.head + 4 * c;
-    if (c < row.n4) {
+    const int i = row.head + 4 * at;
+    if (at < row.n4) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float x = row.p[i + e];
@@ -377,17 +469,20 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
     return;
   }
   // among the tail's elements, or (u is 1 or more) the last one of any weight
-  u64 c = first + inner;
+  u64 cum = first + inner;
   int got = -1;
   for (int i = 3; i < 6; ++i) {
-    c += lds.edge_w[i];
-    if (got < 0 && lds.edge_w[i] && (double)c > target) got = row.head + 4 * row.n4 + i - 3;
+    cum += lds.edge_w[i];
+    if (got < 0 && lds.edge_w[i] && (double)cum > target) got = row.head + 4 * row.n4 + i - 3;
   }
   if (got < 0) {
+    __syncthreads();
     if (t == 0) lds.pick = -1;
     __syncthreads();
-    row.each([&](int j, int e, float x) {
-      if (row.inside(j, e) && kept(row, j, e, x)) atomicMax(&lds.pick, row.index(j, e));
+    Row<T, 0> again;
+    again.load(row.p, n);
+    again.each([&](int j, int e, float x) {
+      if (again.inside(j, e) && kept(again, j, e, x)) atomicMax(&lds.pick, again.index(j, e));
     });
     __syncthreads();
     got = lds.pick;

@@ -355,8 +355,8 @@ def distillation_loss(input, teacher_logits, teacher_ids, temperature=1.0, reduc
     loss_rows = empty(xs[:-1])
     out = empty(()) if red else loss_rows
 
-    def grad_buffer():
-        return _empty_padded(rows, cols) if cols % 4 else empty((rows, cols))
+    def grad_buffer():  # rows as far apart as the logits': of a layer's, padded to 16 bytes
+        return empty((rows, cols)) if ld == cols else _empty_padded(rows, cols)
     # the gradient for the unit seed of loss.backward(), as cross_entropy's
     pre, me = [None], [None]
     if red and _T._recorded(x):
@@ -914,6 +914,21 @@ def _grad_like(t):
     return _alias(empty((B, T, H, D)), t.shape, (T * H * D, D, H * D, 1), 0)
 
 
+def _grad_as(t):
+    """A gradient buffer laid out as a dense operand itself (a leaf's gradient
+    is then the buffer), as _grad_like where the operand's memory has gaps
+    or rows that the kernels do not take."""
+    run = 1
+    for s, n in sorted(zip(t._strides, t.shape)):
+        if n > 1:
+            if s != run:
+                return _grad_like(t)
+            run *= n
+    if t.shape[3] > 1 and t._strides[3] != 1:
+        return _grad_like(t)
+    return _alias(empty((max(run, 1),)), t.shape, t._strides, 0)
+
+
 def _shared_grads(q, k, v):
     """dq, dk, dv laid out exactly like q, k, v inside one new buffer when
     the three are equally strided, disjoint views of one allocation (the
@@ -1102,7 +1117,7 @@ def sliding_window_attention(query, key, value, window, sinks=0, scale=None):
         if not o.numel():
             return [zeros(t.shape) for t in ins]
         shared = _shared_grads(q, k, v)
-        dq, dk, dv = shared if shared else (_grad_like(q), _grad_like(k), _grad_like(v))
+        dq, dk, dv = shared if shared else (_grad_as(q), _grad_as(k), _grad_as(v))
         arrs = [L.i64arr(t._strides[:3]) for t in (q, k, v, o, g, dq, dk, dv)]
         ptrs = (L.P_i64 * 8)(*[ctypes.cast(a, L.P_i64) for a in arrs])
         L.check(L.lib().tjh_window_backward(
