@@ -206,50 +206,56 @@ struct Block {
 
 constexpr int kRank = 256;  // longest list sorted by counting
 
-// LDS of a selection: a list of CAP composites, a second one for the short
-// sort, and the block operations' slots.
+// LDS of a selection: a list of CAP composites, room for the short sort, and
+// the block operations' slots.
 template <int T, int CAP>
 struct SelectLds {
   u64 list[CAP];
-  u64 tmp[kRank];
+  u64 sorted[kRank];
   int rank[kRank];
   int count;
   u64 sm[2 * (T / 64)];
 };
 
-// Sorts list[0, c) descending.  Up to 256 items each thread counts the items
-// above one of them (c * c / T comparisons, two barriers); longer lists take
-// a bitonic network over the next power of two, padded with zeros, which no
-// real item is below (c log^2 c / 4 T exchanges, log^2 c / 2 barriers).
+// Sorts list[0, c) descending, c <= 256: each thread counts the items above
+// one of them (c * c / T comparisons, four barriers).
+template <int T, int CAP>
+__device__ __forceinline__ void sort_short(u64* list, int c, SelectLds<T, CAP>& s) {
+  int pad = 64;
+  while (pad < c) pad <<= 1;
+  for (int i = threadIdx.x; i < c; i += T) s.rank[i] = 0;
+  __syncthreads();  // ranks cleared, list written
+  if (T >= pad) {
+    const int i = threadIdx.x & (pad - 1), g = threadIdx.x / pad, ng = T / pad;
+    if (i < c) {
+      const u64 me = list[i];
+      int r = 0;
+      for (int j = g; j < c; j += ng) r += list[j] > me;
+      if (ng > 1) atomicAdd(&s.rank[i], r);
+      else s.rank[i] = r;
+    }
+  } else {
+    for (int i = threadIdx.x; i < c; i += T) {
+      const u64 me = list[i];
+      int r = 0;
+      for (int j = 0; j < c; ++j) r += list[j] > me;
+      s.rank[i] = r;
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < c; i += T) s.sorted[s.rank[i]] = list[i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < c; i += T) list[i] = s.sorted[i];
+  __syncthreads();
+}
+
+// Sorts s.list[0, c) descending.  Over 256 items a bitonic network over the
+// next power of two, padded with zeros, which no real item is below
+// (c log^2 c / 4 T exchanges, log^2 c / 2 barriers).
 template <int T, int CAP>
 __device__ __forceinline__ void sort_list(SelectLds<T, CAP>& s, int c) {
   if (c <= kRank) {
-    int pad = 64;
-    while (pad < c) pad <<= 1;
-    for (int i = threadIdx.x; i < c; i += T) s.rank[i] = 0;
-    __syncthreads();  // ranks cleared, list written
-    if (T >= pad) {
-      const int i = threadIdx.x & (pad - 1), g = threadIdx.x / pad, ng = T / pad;
-      if (i < c) {
-        const u64 me = s.list[i];
-        int r = 0;
-        for (int j = g; j < c; j += ng) r += s.list[j] > me;
-        if (ng > 1) atomicAdd(&s.rank[i], r);
-        else s.rank[i] = r;
-      }
-    } else {
-      for (int i = threadIdx.x; i < c; i += T) {
-        const u64 me = s.list[i];
-        int r = 0;
-        for (int j = 0; j < c; ++j) r += s.list[j] > me;
-        s.rank[i] = r;
-      }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < c; i += T) s.tmp[s.rank[i]] = s.list[i];
-    __syncthreads();
-    for (int i = threadIdx.x; i < c; i += T) s.list[i] = s.tmp[i];
-    __syncthreads();
+    sort_short(s.list, c, s);
     return;
   }
   int p = 2 * kRank;
@@ -290,33 +296,38 @@ __device__ __forceinline__ int gather_list(const Row<T, 0>& row, uint32_t nan, I
 }
 
 // The same for the elements that are not below `bound` (few of the row).
-// Those in registers are marked first and then read again, so that the rest
-// is one small loop and not a copy for every register.
+// Chunks with one are marked first and then read again, so that the rest is
+// one small loop and not a copy for every register.
 template <int T, int NV, int CAP>
 __device__ __forceinline__ int gather_above(const Row<T, NV>& row, uint32_t nan, float bound,
                                             SelectLds<T, CAP>& s) {
   if constexpr (NV == 0) {
     return gather_list(row, nan, [&](int, int, float x) { return !(x < bound); }, s);
   } else {
+    static_assert(NV <= 32, "marks");
     if (threadIdx.x == 0) s.count = 0;
-    constexpr int kWords = (4 * NV + 31) / 32;
-    uint32_t marks[kWords];
+    uint32_t marks = 0;
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) marks[i] = 0;
-#pragma unroll
-    for (int i = 0; i < 4 * NV; ++i) marks[i / 32] |= row.v[i] < bound ? 0u : 1u << (i % 32);
+    for (int j = 0; j < NV; ++j) {
+      // the maximum that NaN is larger than everything for
+      const float x = __builtin_elementwise_maximum(
+          __builtin_elementwise_maximum(row.v[4 * j], row.v[4 * j + 1]),
+          __builtin_elementwise_maximum(row.v[4 * j + 2], row.v[4 * j + 3]));
+      marks |= x < bound ? 0u : 1u << j;
+    }
     __syncthreads();  // the count is 0
     const auto put = [&](int i) {
+      const float x = row.at(i);
+      if (x < bound) return;
       const int at = atomicAdd(&s.count, 1);
-      if (at < CAP) s.list[at] = composite(order_key(row.at(i), nan), i);
+      if (at < CAP) s.list[at] = composite(order_key(x, nan), i);
     };
-    if (row.edge_index >= 0 && !(row.edge < bound)) put(row.edge_index);
-#pragma unroll
-    for (int i = 0; i < kWords; ++i)
-      for (uint32_t m = marks[i]; m; m &= m - 1) {
-        const int e = 32 * i + __ffs(m) - 1;
-        if (row.inside(e / 4, e % 4)) put(row.index(e / 4, e % 4));
-      }
+    if (row.edge_index >= 0) put(row.edge_index);
+    for (; marks; marks &= marks - 1) {
+      const int j = __ffs(marks) - 1;
+      if (row.inside(j, 0))
+        for (int u = 0; u < 4; ++u) put(row.index(j, u));
+    }
     __syncthreads();
     return s.count;
   }
@@ -365,14 +376,17 @@ __device__ __forceinline__ u64 kth_by_bisection(const Row<T, 0>& row, int k, uin
 }
 
 // A bound that the row's k largest elements are not below and few others are
-// either: the k-th largest of the threads' own maxima (two of each thread),
+// either: the k-th largest of the threads' own maxima (four of each thread),
 // to the 16 high bits of its key, found two at a time; -infinity where there
 // are fewer maxima.  50 of 50257 random values leave about 55.
 template <int T, int NV>
 __device__ __forceinline__ float kth_bound(const Row<T, NV>& row, int k, Block<T>& b) {
-  float mx[2] = {-INFINITY, -INFINITY};  // NaN takes no part: still a lower bound
-  row.each([&](int j, int, float x) { mx[j & 1] = fmaxf(mx[j & 1], x); });
-  const uint32_t mk[2] = {order_key(mx[0]), order_key(mx[1])};
+  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  // NaN takes no part: still a lower bound
+  row.each([&](int, int u, float x) { mx[u] = fmaxf(mx[u], x); });
+  uint32_t mk[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) mk[u] = order_key(mx[u]);
   uint32_t lo = 0;
 #pragma unroll 1
   for (int bit = 30; bit >= 16; bit -= 2) {  // counts of three bounds a round
@@ -380,7 +394,10 @@ __device__ __forceinline__ float kth_bound(const Row<T, NV>& row, int k, Block<T
 #pragma unroll
     for (int i = 3; i >= 1; --i) {
       const uint32_t bound = lo | ((uint32_t)i << bit);
-      c = (c << 20) | (u64)(__popcll(__ballot(mk[0] >= bound)) + __popcll(__ballot(mk[1] >= bound)));
+      int n = 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) n += __popcll(__ballot(mk[u] >= bound));
+      c = (c << 20) | (u64)n;
     }
     c = b.across(c, [](u64 x, u64 y) { return x + y; });
     uint32_t digit = 0;

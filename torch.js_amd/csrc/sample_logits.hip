@@ -16,18 +16,19 @@
 // Weights are integers, w_i * 2^s with the row's sum below 2^62 (s = 46 at
 // 50257 columns): sums are then the same in whatever order the atomics and
 // the waves add them, exact, and finer than 32-bit floats by 2^22.  They are
-// formed in 64 bits as 2^t = 2^(k / 32) 2^f, |f| <= 1 / 64, from a table and
-// the first six terms of 2^f (the seventh is below 2^-48): 32-bit ones would
-// move one draw in some thousand over a border between two indices.
+// formed in 64 bits as 2^(k / 32) 2^(f / 32), |f| <= 1 / 2, from a table and
+// the first six terms of the second (the seventh is below 2^-48): 32-bit ones
+// would move one draw in some thousand over a border between two indices.
 //
 // One workgroup has a row, in registers (rowreg.h).  Wherever the elements
-// that can be drawn fit (4096), they are moved into LDS and sorted, and
-// everything else happens on that list: the top_k largest; the elements
-// above min_p's bound; the nucleus, whose end comes from a histogram of the
-// weights over x, one pass in which every element's weight is formed.
-// Larger sets are a bound on (x, index), found in the histogram's last bin,
-// and a pass that adds the kept weights up by wave and chunk, which is index
-// order, and looks into one.
+// that can be drawn fit (4096), they are moved into LDS and everything else
+// happens on that list: the top_k largest; the elements above min_p's bound;
+// the nucleus, which ends in a bin of a histogram of the weights over x (one
+// pass in which every element's weight is formed).  Only the nucleus's last
+// bin and the part of the list around the draw are sorted: lists longer than
+// 256 are added up by parts of the index range first.  Larger sets are a
+// bound on (x, index), and a pass that adds the kept weights up by wave and
+// chunk, which is index order, and looks into one.
 #include "rowreg.h"
 
 #include <float.h>
@@ -62,33 +63,49 @@ struct SampleLds {
   union {
     u64 bins[kBins];
     u64 seg[NV > 0 ? NV * (T / 64) : 4096];  // weight of each (chunk, wave)
-    u64 w[kCap];                             // weights of the list
   };
+  u64 w[kCap];     // weights of the list
+  u64 few[kRank];  // a part of the list
   double pow2[32];  // 2^(i / 32 + s)
   u64 edge_w[6];
   u64 first;
   int pick;
 };
 
-// 2^(t + s) rounded to an integer, for t <= 0 (or NaN: 0) and s <= 51.
-__device__ __forceinline__ u64 weight_of(double t, const double* pow2) {
-  constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: its low word takes the integer
-  constexpr double c1 = 6.93147180559945286e-01, c2 = 2.40226506959100694e-01,
-                   c3 = 5.55041086648215762e-02, c4 = 9.61812910762847687e-03,
-                   c5 = 1.33335581464284411e-03;  // ln(2)^k / k!
-  t = fmax(t, -64.0);  // 2^(51 - 64) is 0
-  const double kd = __builtin_fma(t, 32.0, kMagic);
-  const int k = (int)__double_as_longlong(kd);
-  const double f = __builtin_fma(kd - kMagic, -1.0 / 32, t);
-  double e = __builtin_fma(f, c5, c4);
-  e = __builtin_fma(f, e, c3);
-  e = __builtin_fma(f, e, c2);
-  e = __builtin_fma(f, e, c1);
-  const double tab = pow2[k & 31];
-  e = __builtin_fma(tab * f, e, tab);
-  e = ldexp(e, k >> 5) + 4503599627370496.0;  // 2^52: the integer is in the low 52 bits
-  return (u64)__double_as_longlong(e) & 0xfffffffffffffull;
-}
+// Weights of a row: 2^(d * per_t + s) rounded to an integer, d = x - m <= 0
+// (NaN: 0), s <= 51.  Constants are scalar registers of their own: literals
+// would each be moved into vector registers for every weight.
+struct Weights {
+  double m, scale, lowest, magic, c1, c2, c3, c4, c5, top;
+  const double* pow2;
+  __device__ __forceinline__ Weights(double max, double per_t, const double* table)
+      : m(max), scale(per_t * 32.0), pow2(table) {
+    constexpr double l = 6.93147180559945286e-01 / 32;  // 2^(f / 32) = sum (l f)^k / k!
+    lowest = -2048.0 / scale;      // 2^(51 - 64) is 0
+    magic = 6755399441055744.0;    // 1.5 * 2^52: its low word takes the integer
+    top = 4503599627370496.0;      // 2^52: the integer is in the low 52 bits
+    c1 = l;
+    c2 = l * l / 2;
+    c3 = l * l * l / 6;
+    c4 = l * l * l * l / 24;
+    c5 = l * l * l * l * l / 120;
+    asm volatile("" : "+s"(magic), "+s"(top), "+s"(c1), "+s"(c2), "+s"(c3), "+s"(c4), "+s"(c5));
+  }
+  __device__ __forceinline__ u64 operator()(float x) const {
+    const double d = fmax((double)x - m, lowest);
+    const double kd = __builtin_fma(d, scale, magic);
+    const int k = (int)__double_as_longlong(kd);
+    const double f = __builtin_fma(d, scale, -(kd - magic));  // |f| <= 1 / 2
+    const double tab = pow2[k & 31];
+    double e = __builtin_fma(f, c5, c4);
+    e = __builtin_fma(f, e, c3);
+    e = __builtin_fma(f, e, c2);
+    e = __builtin_fma(f, e, c1);
+    e = __builtin_fma(tab * f, e, tab);
+    e = ldexp(e, k >> 5) + top;
+    return (u64)__double_as_longlong(e) & 0xfffffffffffffull;
+  }
+};
 
 // A float that is not above x, nor far below it.
 __device__ __forceinline__ float float_below(double x) {
@@ -157,11 +174,11 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
   const double p = top_p > 0.0 ? top_p : 1e-300;  // the first element at least
   const double floor_z = min_p > 0.0 ? fmin(temp * log(min_p), 0.0) : -INFINITY;
   const double m = (double)mx;
-  const double per_t = fmin(1.4426950408889634074 / temp, 1e300);
+  const double per_t = fmax(fmin(1.4426950408889634074 / temp, 1e300), 1e-300);
   const double u = (double)a.u[r];
   if (t < 32) lds.pow2[t] = ldexp(exp2((double)t / 32), min(51, 62 - (32 - __clz(n))));
   __syncthreads();
-  const auto weight = [&](float x) { return weight_of(((double)x - m) * per_t, lds.pow2); };
+  const Weights weight(m, per_t, lds.pow2);
 
   // elements of the order up to (tx, ti) are kept
   float tx = -INFINITY;
@@ -196,10 +213,19 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
     per = (float)(kBins / fmax(fmin(24.0 * temp, m - (double)mn), 1e-30));
     for (int i = t; i < kBins; i += T) lds.bins[i] = 0;
     __syncthreads();
-    each_chunk(row, [&](int j, int e, float x) {
-      const u64 w = !cut || in_order(row, j, e, x) ? weight(x) : 0;
-      if (w) atomicAdd(&lds.bins[bin_of(per, x)], w);
-    });
+    if (!cut) {
+      each_chunk(row, [&](int, int, float x) {
+        const u64 w = weight(x);
+        if (w) atomicAdd(&lds.bins[bin_of(per, x)], w);
+      });
+    } else {
+      Row<T, 0> again;
+      again.load(row.p, n);
+      again.each([&](int j, int e, float x) {
+        const u64 w = in_order(again, j, e, x) ? weight(x) : 0;
+        if (w) atomicAdd(&lds.bins[bin_of(per, x)], w);
+      });
+    }
     if (t == 0) lds.pick = -1;
     __syncthreads();
     u64 run = 0;
@@ -239,43 +265,64 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
     }
     sort_list(s, c);
     c = (int)top_k;
-  } else if (c >= 0 && use_p) {
-    sort_list(s, c);
-  } else if (c < 0 && use_p) {
-    // the nucleus ends in bin `last`: its elements alone
-    Row<T, 0> again;
-    again.load(row.p, n);
-    const auto in_bin = [&](int j, int e, float x) {
-      return bin_of(per, x) == last && x > -INFINITY && in_order(again, j, e, x);
-    };
+  } else if (use_p) {
+    // the nucleus ends in bin `last`: (tx, ti) from that bin's elements
     u64 run = 0;
     for (int i = t; i < last; i += T) run += lds.bins[i];
     const u64 above = b.sum64(run);
-    const int in = gather_list(again, kNanFirst, in_bin, s);
+    if (t == 0) s.count = 0;
+    __syncthreads();
+    for (int i = t; i < c; i += T) {
+      const u64 e = s.list[i];
+      const float x = key_value((uint32_t)(e >> 32));
+      if (bin_of(per, x) == last && (x > tx || (x == tx && index_of(e) <= ti))) {
+        const int at = atomicAdd(&s.count, 1);
+        if (at < kRank) lds.few[at] = e;
+      }
+    }
+    __syncthreads();
+    int in = s.count;
+    u64* part = lds.few;
+    if (c >= 0 && in <= kRank) {
+      sort_short(part, in, s);
+    } else {
+      c = -1;  // no list: the bin alone
+      Row<T, 0> again;
+      again.load(row.p, n);
+      in = gather_list(
+          again, kNanFirst,
+          [&](int j, int e, float x) {
+            return bin_of(per, x) == last && x > -INFINITY && in_order(again, j, e, x);
+          },
+          s);
+      part = s.list;
+      if (in <= kCap) sort_list(s, in);
+    }
     if (in <= kCap) {
-      sort_list(s, in);
       if (t == 0) lds.pick = 0;
       __syncthreads();
       u64 sum = above;
       for (int i0 = 0; i0 < in; i0 += T) {
         const int i = i0 + t;
-        const u64 w = i < in ? weight(key_value((uint32_t)(s.list[i] >> 32))) : 0;
-        u64 part;
-        const u64 before = sum + b.before(w, &part);
+        const u64 w = i < in ? weight(key_value((uint32_t)(part[i] >> 32))) : 0;
+        u64 all;
+        const u64 before = sum + b.before(w, &all);
         if (i < in && (double)before < limit) atomicMax(&lds.pick, i);
-        sum += part;
+        sum += all;
       }
       __syncthreads();
-      const u64 e = s.list[lds.pick];
+      const u64 e = part[lds.pick];
       tx = key_value((uint32_t)(e >> 32));
       ti = index_of(e);
     } else {
       // more elements than the list holds.  All equal: as many of them as
       // there is room for, by index; else the largest composite with at
       // least the limit above it, bit by bit, is the first one outside
+      Row<T, 0> again;
+      again.load(row.p, n);
       float lo = INFINITY, hi = -INFINITY;
       again.each([&](int j, int e, float x) {
-        if (in_bin(j, e, x)) {
+        if (bin_of(per, x) == last && x > -INFINITY && in_order(again, j, e, x)) {
           lo = fminf(lo, x);
           hi = fmaxf(hi, x);
         }
@@ -316,25 +363,25 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
         ti = index_of(lds.first);
       }
     }
-    __syncthreads();  // bins are free
+    __syncthreads();  // bins and parts are free
   }
 
   if (c >= 0) {
-    // the list's weights (none for elements that are not kept), the cut, and
-    // the rest in index order
+    // the list's weights, none for elements that are not kept
     u64 mine = 0;
     for (int i = t; i < c; i += T) {
       const u64 e = s.list[i];
       const float x = key_value((uint32_t)(e >> 32));
-      const bool in = (double)x - m >= floor_z && (x > tx || (x == tx && index_of(e) <= ti));
-      const u64 w = in || largest ? weight(x) : 0;
+      const bool in = largest || ((double)x - m >= floor_z &&
+                                  (x > tx || (x == tx && index_of(e) <= ti)));
+      const u64 w = in ? weight(x) : 0;
       lds.w[i] = w;
       mine += w;
     }
     u64 all = b.sum64(mine);
     int keep = c;
-    if (largest || use_p) {  // the list is sorted
-      if (largest && use_p) limit = p * (double)all;
+    if (largest && (use_p || floor_z > -INFINITY)) {  // a sorted list, to be cut
+      if (use_p) limit = p * (double)all;
       int kept = 0;
       u64 sum = 0, mine_kept = 0;
       for (int i0 = 0; i0 < c; i0 += T) {
@@ -351,34 +398,94 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
       keep = b.sum_i(kept);
       all = b.sum64(mine_kept);
     }
-    // (index, place in the list), in ascending order of the index
-    if (t == 0) lds.pick = kNone;
-    for (int i = t; i < keep; i += T) s.list[i] = (s.list[i] << 32) | (uint32_t)i;
-    sort_list(s, keep);
     const double target = u * (double)all;
-    u64 sum = 0;
-    int end = -1;  // the last one of any weight, where u is 1 or more
-    for (int i0 = 0; i0 < keep; i0 += T) {
-      const int i = i0 + t;
-      const u64 w = i < keep ? lds.w[(uint32_t)s.list[i]] : 0;
-      u64 part;
-      const u64 before = sum + b.before(w, &part);
-      sum += part;
-      if (w && (double)(before + w) > target) atomicMin(&lds.pick, i);
-      if (w) end = i;
+    u64 sum = 0;  // weight of the indices before the ones looked into
+    u64* part = s.list;
+    int in = keep;
+    if (keep > kRank) {
+      // by parts of the index range: the first with the target, or, where u
+      // is 1 or more, the last of any weight
+      constexpr int kParts = 1024;
+      const int shift = max(0, 32 - __clz(n - 1) - 10);  // 2^10 parts
+      __syncthreads();
+      for (int i = t; i < kParts; i += T) lds.bins[i] = 0;
+      if (t == 0) {
+        lds.pick = kNone;
+        s.count = 0;
+      }
+      __syncthreads();
+      for (int i = t; i < keep; i += T)
+        if (lds.w[i]) atomicAdd(&lds.bins[index_of(s.list[i]) >> shift], lds.w[i]);
+      __syncthreads();
+      u64 run = 0;
+      int end = -1;
+      for (int i0 = 0; i0 < kParts; i0 += T) {
+        const u64 w = lds.bins[i0 + t];
+        u64 here;
+        const u64 before = run + b.before(w, &here);
+        if (w && (double)(before + w) > target) atomicMin(&lds.pick, i0 + t);
+        if (w) end = i0 + t;
+        run += here;
+      }
+      __syncthreads();
+      int at = lds.pick;
+      if (at == kNone) {
+        __syncthreads();
+        if (t == 0) lds.pick = -1;
+        __syncthreads();
+        atomicMax(&lds.pick, end);
+        __syncthreads();
+        at = lds.pick;
+      }
+      run = 0;
+      for (int i = t; i < at; i += T) run += lds.bins[i];
+      sum = b.sum64(run);
+      for (int i = t; i < keep; i += T)
+        if (lds.w[i] && index_of(s.list[i]) >> shift == at) {
+          const int put = atomicAdd(&s.count, 1);
+          if (put < kRank) lds.few[put] = (s.list[i] << 32) | (uint32_t)i;
+        }
+      __syncthreads();
+      in = s.count;
+      part = lds.few;
+    } else {
+      __syncthreads();
+      for (int i = t; i < keep; i += T) s.list[i] = (s.list[i] << 32) | (uint32_t)i;
+    }
+    if (in <= kRank) {
+      // (index, place in the list), in ascending order of the index
+      if (t == 0) lds.pick = kNone;
+      sort_short(part, in, s);
+      int end = -1;
+      for (int i0 = 0; i0 < in; i0 += T) {
+        const int i = i0 + t;
+        const u64 w = i < in ? lds.w[(uint32_t)part[i]] : 0;
+        u64 here;
+        const u64 before = sum + b.before(w, &here);
+        sum += here;
+        if (w && (double)(before + w) > target) atomicMin(&lds.pick, i);
+        if (w) end = i;
+      }
+      __syncthreads();
+      int at = lds.pick;
+      if (at == kNone) {  // the last one of any weight
+        __syncthreads();
+        if (t == 0) lds.pick = -1;
+        __syncthreads();
+        atomicMax(&lds.pick, end);
+        __syncthreads();
+        at = lds.pick;
+      }
+      if (t == 0) a.out[r] = (int)~(uint32_t)(part[at] >> 32);
+      return;
+    }
+    // more than 256 in one part: the pass over the row, down to the last kept
+    if (largest) {
+      const u64 e = s.list[keep - 1];
+      tx = key_value((uint32_t)(e >> 32));
+      ti = index_of(e);
     }
     __syncthreads();
-    int at = lds.pick;
-    if (at == kNone) {
-      __syncthreads();
-      if (t == 0) lds.pick = -1;
-      __syncthreads();
-      atomicMax(&lds.pick, end);
-      __syncthreads();
-      at = lds.pick;
-    }
-    if (t == 0) a.out[r] = (int)~(uint32_t)(s.list[at] >> 32);
-    return;
   }
 
   // the kept weight of every wave's part of every chunk, in index order
@@ -387,14 +494,17 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
   };
   const int w = t >> 6, lane = t & 63;
   const int chunks = (row.n4 + T - 1) / T;
-  for (int j = 0; j < chunks; ++j) {  // the row once more, from the L2
-    const int at = t + j * T;
-    u64 part = 0;
-    if (at < row.n4) {
-      const float4 x = *reinterpret_cast<const float4*>(row.p + row.head + 4 * at);
-      part = kept(row, j, 0, x.x) + kept(row, j, 1, x.y) + kept(row, j, 2, x.z) +
-             kept(row, j, 3, x.w);
-    }
+  const auto chunk = [&](int j) {  // the row once more, from the L2
+    return t + j * T < row.n4
+               ? *reinterpret_cast<const float4*>(row.p + row.head + 4 * (t + j * T))
+               : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+  };
+  float4 next = chunk(0);
+  for (int j = 0; j < chunks; ++j) {
+    const float4 x = next;
+    next = chunk(j + 1);
+    u64 part = kept(row, j, 0, x.x) + kept(row, j, 1, x.y) + kept(row, j, 2, x.z) +
+               kept(row, j, 3, x.w);
     if (__ballot(part != 0)) part = wave_sum_u64(part);
     if (lane == 0) lds.seg[j * W + w] = part;
   }
@@ -513,8 +623,8 @@ extern "C" int tjh_sample_logits(const float* logits, int64_t ld, int64_t rows, 
   KernelScope ks("sample_logits");
   const dim3 grid((unsigned)rows);
   if (cols <= 4096) tjh_launch(k_sample<256, 4>, grid, dim3(256), 0, stream(), a);
-  else if (cols <= 16384) tjh_launch(k_sample<1024, 4>, grid, dim3(1024), 0, stream(), a);
-  else if (cols <= 53248) tjh_launch(k_sample<1024, 13>, grid, dim3(1024), 0, stream(), a);
+  else if (cols <= 16384) tjh_launch(k_sample<512, 8>, grid, dim3(512), 0, stream(), a);
+  else if (cols <= 53248) tjh_launch(k_sample<512, 26>, grid, dim3(512), 0, stream(), a);
   else tjh_launch(k_sample<1024, 0>, grid, dim3(1024), 0, stream(), a);
   return check_launch("sample_logits");
 }
