@@ -68,8 +68,9 @@ int tjh_sample_logits(const float* logits, int64_t ld, int64_t rows, int64_t col
  * Tk >= Tq: the queries are the last Tq of the Tk positions, and the one at
  * position i sees the keys j <= i with j > i - window or j < sinks (window >=
  * 1).  o = softmax(scale q k^T over those) v; strides (elements) for the B, H
- * and T axes, D contiguous, as tjh_sdpa_forward's.  lse [B,H,Tq] is saved for
- * the backward, or NULL.  Keys and values that a query does not see have no
+ * and T axes, D contiguous, as tjh_sdpa_forward's.  lse [B,H,Tq],
+ * the logarithm to base 2 of a query's sum of exponentials, is saved for the
+ * backward, or NULL.  Keys and values that a query does not see have no
  * part in its output, whatever they hold.  Head dims up to 128 that are
  * multiples of 4, rows 16-byte aligned (else TJH_ERR_UNSUPPORTED). */
 int tjh_window_forward(const float* q, const float* k, const float* v, float* o, float* lse,

@@ -27,8 +27,8 @@
 // pass in which every element's weight is formed).  Only the nucleus's last
 // bin and the part of the list around the draw are sorted: lists longer than
 // 256 are added up by parts of the index range first.  Larger sets are a
-// bound on (x, index), and a pass that adds the kept weights up by wave and
-// chunk, which is index order, and looks into one.
+// bound on (x, index), and passes that add the kept weights up by runs of the
+// index range, one a wave, and look into one.
 #include "rowreg.h"
 
 #include <float.h>
@@ -57,13 +57,10 @@ struct SampleArgs {
   int32_t* out;
 };
 
-template <int T, int NV>
+template <int T>
 struct SampleLds {
   SelectLds<T, kCap> s;
-  union {
-    u64 bins[kBins];
-    u64 seg[NV > 0 ? NV * (T / 64) : 4096];  // weight of each (chunk, wave)
-  };
+  u64 bins[kBins];
   u64 w[kCap];     // weights of the list
   u64 few[kRank];  // a part of the list
   double pow2[32];  // 2^(i / 32 + s)
@@ -113,27 +110,31 @@ __device__ __forceinline__ float float_below(double x) {
   return f - (fabsf(f) * 2.4e-7f + FLT_MIN);
 }
 
-// Row::each with the work of one chunk kept together: all elements' weights
-// at once would take more registers than there are.
+// f(x0, x1, x2, x3) for each chunk of the row and its extra element (with
+// -infinity), a chunk's work kept together: that of all of them at once would
+// take more registers than there are.
 template <int T, int NV, class F>
-__device__ __forceinline__ void each_chunk(const Row<T, NV>& row, F f) {
+__device__ __forceinline__ void each_four(const Row<T, NV>& row, F f) {
+  f(row.edge, -INFINITY, -INFINITY, -INFINITY);
   if constexpr (NV > 0) {
-    f(-1, 0, row.edge);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) f(j, u, row.v[4 * j + u]);
+      f(row.v[4 * j], row.v[4 * j + 1], row.v[4 * j + 2], row.v[4 * j + 3]);
     }
     __builtin_amdgcn_sched_barrier(0);
   } else {
-    row.each(f);
+#pragma unroll 2
+    for (int c = threadIdx.x; c < row.n4; c += T) {
+      const float4 x = *reinterpret_cast<const float4*>(row.p + row.head + 4 * c);
+      f(x.x, x.y, x.z, x.w);
+    }
   }
 }
 
 template <int T, int NV>
 __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
-  __shared__ SampleLds<T, NV> lds;
+  __shared__ SampleLds<T> lds;
   SelectLds<T, kCap>& s = lds.s;
   constexpr int W = T / 64;
   constexpr int kNone = 0x7fffffff;
@@ -214,9 +215,14 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
     for (int i = t; i < kBins; i += T) lds.bins[i] = 0;
     __syncthreads();
     if (!cut) {
-      each_chunk(row, [&](int, int, float x) {
-        const u64 w = weight(x);
-        if (w) atomicAdd(&lds.bins[bin_of(per, x)], w);
+      each_four(row, [&](float x0, float x1, float x2, float x3) {
+        const float x[4] = {x0, x1, x2, x3};
+        u64 w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = weight(x[e]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (w[e]) atomicAdd(&lds.bins[bin_of(per, x[e])], w[e]);
       });
     } else {
       Row<T, 0> again;
@@ -249,7 +255,8 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
   }
   int c = -1;  // elements of the list, if there is one
   if (largest || bound > -INFINITY) {
-    c = gather_above(row, kNanFirst, bound, s);
+    c = use_p && !largest ? gather_above<false>(row, kNanFirst, bound, s, b)
+                          : gather_above<true>(row, kNanFirst, bound, s, b);
     if (c > kCap) c = -1;
   }
   if (largest) {
@@ -488,75 +495,86 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
     __syncthreads();
   }
 
-  // the kept weight of every wave's part of every chunk, in index order
-  const auto kept = [&](const auto& of, int j, int e, float x) -> u64 {
-    return in_order(of, j, e, x) && (double)x - m >= floor_z ? weight(x) : 0;
+  // index order: the head's elements, the chunks, the tail's elements.  Each
+  // wave adds a run of the chunks up; the first one with the target is cut
+  // into runs again, until one wave's lanes have a chunk each
+  const auto in = [&](int i, float x) {
+    return (x > tx || (x == tx && i <= ti)) && (double)x - m >= floor_z;
   };
+  const auto kept = [&](int i, float x) -> u64 { return in(i, x) ? weight(x) : 0; };
   const int w = t >> 6, lane = t & 63;
-  const int chunks = (row.n4 + T - 1) / T;
-  const auto chunk = [&](int j) {  // the row once more, from the L2
-    return t + j * T < row.n4
-               ? *reinterpret_cast<const float4*>(row.p + row.head + 4 * (t + j * T))
-               : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-  };
-  float4 next = chunk(0);
-  for (int j = 0; j < chunks; ++j) {
-    const float4 x = next;
-    next = chunk(j + 1);
-    u64 part = kept(row, j, 0, x.x) + kept(row, j, 1, x.y) + kept(row, j, 2, x.z) +
-               kept(row, j, 3, x.w);
-    if (__ballot(part != 0)) part = wave_sum_u64(part);
-    if (lane == 0) lds.seg[j * W + w] = part;
-  }
-  if (t < 6) lds.edge_w[t] = row.edge_index >= 0 ? kept(row, -1, 0, row.edge) : 0;
-  if (t == 0) lds.pick = kNone;
-  __syncthreads();
-  const u64 first = lds.edge_w[0] + lds.edge_w[1] + lds.edge_w[2];
-  u64 sum = 0;
-  for (int i = t; i < chunks * W; i += T) sum += lds.seg[i];
-  const u64 inner = b.sum64(sum);
-  const u64 all = first + inner + lds.edge_w[3] + lds.edge_w[4] + lds.edge_w[5];
-  const double target = u * (double)all;
-  // index order: the head's elements, the segments, the tail's elements
-  if ((double)first > target && first) {
-    if (t == 0) {
-      u64 cum = 0;
-      int i = 0;
-      for (; i < 2; ++i) {
-        cum += lds.edge_w[i];
-        if (lds.edge_w[i] && (double)cum > target) break;
-      }
-      a.out[r] = i;
-    }
-    return;
-  }
-  u64 run = first;
-  for (int i0 = 0; i0 < chunks * W; i0 += T) {
-    const int i = i0 + t;
-    const u64 v = i < chunks * W ? lds.seg[i] : 0;
-    u64 part_all;
-    const u64 before = run + b.before(v, &part_all);
-    if (v && (double)(before + v) > target) atomicMin(&lds.pick, i);
-    run += part_all;
-  }
-  __syncthreads();
-  const int seg = lds.pick;
-  if (seg != kNone) {
-    // the weight before the segment, then the segment by itself
-    u64 sum_before = 0;
-    for (int i = t; i < seg; i += T) sum_before += lds.seg[i];
-    const u64 base = first + b.sum64(sum_before);
-    if (w != 0) return;
-    const int j = seg / W, th = (seg % W) * 64 + lane, at = th + j * T;
-    u64 wt[4] = {0, 0, 0, 0};
-    const int i = row.head + 4 * at;
-    if (at < row.n4) {
+  if (t < 6) lds.edge_w[t] = row.edge_index >= 0 ? kept(row.edge_index, row.edge) : 0;
+  u64 base = 0, all = 0;
+  double target = 0.0;
+  int lo = 0, count = row.n4;
+  for (bool whole = true; whole || count > 64; whole = false) {
+    const int per = (count + W - 1) / W;
+    const int c0 = lo + w * per, c1 = min(lo + count, c0 + per);
+    u64 sum = 0;
+    for (int c = c0 + lane; c < c1; c += 256) {
+      float4 x[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = row.p[i + e];
-        const bool in = x > tx || (x == tx && i + e <= ti);
-        wt[e] = in && (double)x - m >= floor_z ? weight(x) : 0;
+      for (int v = 0; v < 4; ++v)  // past the run the last chunk, not counted
+        x[v] = *reinterpret_cast<const float4*>(row.p + row.head + 4 * min(c + 64 * v, c1 - 1));
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int i = row.head + 4 * (c + 64 * v);
+        const float e[4] = {x[v].x, x[v].y, x[v].z, x[v].w};
+        bool k[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) k[y] = c + 64 * v < c1 && in(i + y, e[y]);
+        if (__ballot(k[0] || k[1] || k[2] || k[3])) {  // four weights at a time, no branches
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const u64 wy = weight(e[y]);
+            sum += k[y] ? wy : 0;
+          }
+        }
       }
+    }
+    sum = wave_sum_u64(sum);
+    __syncthreads();  // the last round's runs are read, the edges written
+    if (lane == 0) lds.bins[w] = sum;
+    __syncthreads();
+    if (whole) {
+      base = lds.edge_w[0] + lds.edge_w[1] + lds.edge_w[2];
+      for (int i = 0; i < W; ++i) all += lds.bins[i];
+      all += base + lds.edge_w[3] + lds.edge_w[4] + lds.edge_w[5];
+      target = u * (double)all;
+      if (base && (double)base > target) {
+        u64 cum = 0;
+        int i = 0;
+        for (; i < 2; ++i) {
+          cum += lds.edge_w[i];
+          if (lds.edge_w[i] && (double)cum > target) break;
+        }
+        if (t == 0) a.out[r] = i;
+        return;
+      }
+    }
+    int run = -1;
+    for (int i = 0; i < W; ++i) {
+      const u64 v = lds.bins[i];
+      if (v && (double)(base + v) > target) {
+        run = i;
+        break;
+      }
+      base += v;
+    }
+    if (run < 0) {  // not among the chunks (in the first round)
+      count = -1;
+      break;
+    }
+    lo += run * per;
+    count = min(per, count - run * per);
+  }
+  if (count > 0) {
+    if (w != 0) return;
+    u64 wt[4] = {0, 0, 0, 0};
+    const int i = row.head + 4 * (lo + lane);
+    if (lane < count) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) wt[e] = kept(i + e, row.p[i + e]);
     }
     const u64 mine = wt[0] + wt[1] + wt[2] + wt[3];
     u64 incl = mine;
@@ -579,7 +597,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
     return;
   }
   // among the tail's elements, or (u is 1 or more) the last one of any weight
-  u64 cum = first + inner;
+  u64 cum = base;
   int got = -1;
   for (int i = 3; i < 6; ++i) {
     cum += lds.edge_w[i];
@@ -592,7 +610,8 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
     Row<T, 0> again;
     again.load(row.p, n);
     again.each([&](int j, int e, float x) {
-      if (again.inside(j, e) && kept(again, j, e, x)) atomicMax(&lds.pick, again.index(j, e));
+      if (again.inside(j, e) && kept(again.index(j, e), x))
+        atomicMax(&lds.pick, again.index(j, e));
     });
     __syncthreads();
     got = lds.pick;

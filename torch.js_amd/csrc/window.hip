@@ -218,8 +218,7 @@ __global__ __launch_bounds__(256, occ_fwd<HD>()) void k_win_fwd(WinArgs a) {
   const float inv = 1.0f / lsum;  // a query sees itself: the sum is at least 1
   write_rows<HD>(buf, acc, inv, a.out + b * a.os.b + hh * a.os.h, a.os.t, q0, a.Tq, a.D, l32, h,
                  lane);
-  if (a.lse_out && h == 0 && myq < a.Tq)
-    a.lse_out[bh * a.Tq + myq] = (m + __log2f(lsum)) * kLn2;
+  if (a.lse_out && h == 0 && myq < a.Tq) a.lse_out[bh * a.Tq + myq] = m + __log2f(lsum);
 }
 
 // Joins the slices of a query: o = sum 2^(m_s - m) acc_s / sum 2^(m_s - m)
@@ -361,7 +360,7 @@ __global__ __launch_bounds__(kFewThreads) void k_win_few(WinArgs a) {
     if (d == 0) a.pml[at] = make_float2(top, den);
   } else {
     a.out[b * a.os.b + hh * a.os.h + q * a.os.t + d] = num * (1.0f / den);
-    if (d == 0 && a.lse_out) a.lse_out[row] = (top + __log2f(den)) * kLn2;
+    if (d == 0 && a.lse_out) a.lse_out[row] = top + __log2f(den);
   }
 }
 
@@ -377,6 +376,7 @@ __global__ __launch_bounds__(256, occ_pair<HD>()) void k_win_dkv(WinArgs a) {
   __shared__ __attribute__((aligned(16))) float Qs[2][TILE * S_::W];
   __shared__ __attribute__((aligned(16))) float Gs[2][TILE * S_::W];
   __shared__ __attribute__((aligned(16))) float Ps[2][16 * 64];
+  __shared__ __attribute__((aligned(16))) float Rs[2][2][TILE];  // [role][tile][row]: lse, D
   // unequal wave priorities keep a CU's workgroups out of step (flash.hip)
   if (blockIdx.x % 3 == 0) __builtin_amdgcn_s_setprio(2);
   else if (blockIdx.x % 3 == 1) __builtin_amdgcn_s_setprio(1);
@@ -414,8 +414,6 @@ __global__ __launch_bounds__(256, occ_pair<HD>()) void k_win_dkv(WinArgs a) {
   for (int i = 0; i < RUN; ++i) asm volatile("" : "+v"(kv[i]));
   floatx16 acc[S_::NC];  // A: dV^T, B: dK^T
   zero_acc(acc);
-  const float one = h == 0 ? 1.f : 0.f;
-  const float omul = role == 0 ? -kLog2e : -1.f;
 
   // the query tiles that see some of the 64 keys
   int qt0 = max(0, kb * PROWS - a.off) / TILE;
@@ -433,23 +431,22 @@ __global__ __launch_bounds__(256, occ_pair<HD>()) void k_win_dkv(WinArgs a) {
   const auto qrows = [&](const float* x, const Strides3& s, int head) {
     return x + b * s.b + (int64_t)head * s.h;
   };
-  const auto row_raw = [&](int head, int t) {
+  // lse (A) or D (B) of the tile's rows: subtracted after the products.  As
+  // the products' first term, as in flash.hip, they would have every later
+  // sum rounded at their own size, three times the error in P at 260 keys
+  const auto row_term = [&](int head, int t) {
     const float* L = (role == 0 ? a.lse : a.dsum) + (b * a.H + head) * (int64_t)a.Tq;
     return L[min(t * TILE + l32, a.Tq - 1)];
   };
-  const auto row_fix = [&](int t, float raw) {
-    const bool in = !GUARD || t * TILE + l32 < a.Tq;
-    return (h == 0 && in) ? raw * omul : 0.f;
-  };
   floatx4 rq[S_::NC], rg[S_::NC];
-  float off = 0.f, raw_n = 0.f;
+  float term = 0.f;
   if (steps > 0) {
     load_tile<HD, GUARD>(qrows(a.q, a.qs, hh), a.qs.t, qt * TILE, a.Tq, a.D, rq);
     load_tile<HD, GUARD>(qrows(a.dout, a.gs, hh), a.gs.t, qt * TILE, a.Tq, a.D, rg);
-    raw_n = row_raw(hh, qt);
+    term = row_term(hh, qt);
     store_tile<HD>(Qs[0], rq);
     store_tile<HD>(Gs[0], rg);
-    off = row_fix(qt, raw_n);
+    if (pr == 0 && h == 0) Rs[role][0][l32] = term;
   }
   __syncthreads();
   float* pbuf = Ps[pr];
@@ -464,7 +461,7 @@ __global__ __launch_bounds__(256, occ_pair<HD>()) void k_win_dkv(WinArgs a) {
     if (more) {
       load_tile<HD, GUARD>(qrows(a.q, a.qs, hn), a.qs.t, qn * TILE, a.Tq, a.D, rq);
       load_tile<HD, GUARD>(qrows(a.dout, a.gs, hn), a.gs.t, qn * TILE, a.Tq, a.D, rg);
-      raw_n = row_raw(hn, qn);
+      term = row_term(hn, qn);
     }
     const int lo = a.off + qt * TILE;  // the tile's first position
     const bool seen = k0 < a.Tk && tile_seen(a, lo, kt);
@@ -478,7 +475,13 @@ __global__ __launch_bounds__(256, occ_pair<HD>()) void k_win_dkv(WinArgs a) {
       float xa[RUN];
       // A: S[q][key] - lse[q] from Q rows; B: dP[q][key] - D[q] from dO rows
       lds_run<HD>(role == 0 ? Qs[cur] : Gs[cur], l32, h, xa);
-      x = chain<HD>(off, one, xa, kv);
+      x = chain0<HD>(xa, kv);
+#pragma unroll
+      for (int j = 0; j < 16; j += 4) {
+        const floatx4 r = *reinterpret_cast<const floatx4*>(&Rs[role][cur][kappa(j, h)]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[j + e] -= r[e];
+      }
       if (role == 0) {
         if (edge) {
 #pragma unroll
@@ -518,7 +521,7 @@ __global__ __launch_bounds__(256, occ_pair<HD>()) void k_win_dkv(WinArgs a) {
     if (more) {
       store_tile<HD>(Qs[cur ^ 1], rq);
       store_tile<HD>(Gs[cur ^ 1], rg);
-      off = row_fix(qn, raw_n);
+      if (pr == 0 && h == 0) Rs[role][cur ^ 1][l32] = term;
     }
     if (seen && role == 1) {
       const int64_t bh = (int64_t)bkv * a.G + hh - kh * a.G;
