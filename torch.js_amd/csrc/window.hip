@@ -807,8 +807,8 @@ int tjh_window_forward(const float* q, const float* k, const float* v, float* o,
   const int64_t wt = cdiv((int64_t)a.win + ROWS - 2, TILE) + 1 + a.nst, all = cdiv(Tk, TILE);
   const int64_t nt = wt < all ? wt : all;  // tiles of a block at most
   int64_t n = 1;
-  if (!lse && blocks < cus && nt > 8) {
-    a.kslice = (int)(cdiv(nt * blocks, cus) < 4 ? 4 : cdiv(nt * blocks, cus));
+  if (!lse && blocks < cus && nt > 4) {
+    a.kslice = (int)(cdiv(nt * blocks, cus) < 2 ? 2 : cdiv(nt * blocks, cus));
     n = cdiv(nt, a.kslice);
   }
   Scratch s(n > 1 ? (size_t)(n * rows * (D + 2)) * sizeof(float) : 0);

@@ -3,6 +3,7 @@ src/nn/losses.ts): the hot-path ops as fused kernels with their
 backward passes.
 """
 import ctypes
+import functools
 import math
 
 import numpy as np
@@ -308,17 +309,13 @@ def nll_loss(input, target, weight=None, reduction="mean", *, ignore_index=-100)
 
 
 def _rows_2d(x):
-    """x as a float32 matrix of rows without a copy where its rows are dense:
-    (detached tensor, pointer, row stride, rows, columns)."""
-    xd = x.detach()
-    if xd.ndim != 2:
-        xd = reshape(xd.contiguous(), (-1, x.shape[-1]) if x.numel() else
-                     (_numel(x.shape[:-1]), x.shape[-1]))
-    rv = _rows_view(xd)
-    if rv is None:
-        xd = _k_contiguous(xd)
-        rv = _rows_view(xd)
-    return xd, rv[0], max(rv[1], xd.shape[1]), xd.shape[0], xd.shape[1]
+    """x as a matrix of rows, without a copy where its rows are dense: (tensor
+    that holds them, pointer, row stride, rows, columns)."""
+    st, (rows, cols) = x._strides, (_numel(x.shape[:-1]), x.shape[-1])
+    if len(st) == 2 and st[1] == 1 and st[0] >= cols:
+        return x, x.data_ptr(), st[0], rows, cols
+    xd = x.detach().contiguous()
+    return xd, xd.data_ptr(), cols, rows, cols
 
 
 def distillation_loss(input, teacher_logits, teacher_ids, temperature=1.0, reduction="mean"):
@@ -349,7 +346,7 @@ def distillation_loss(input, teacher_logits, teacher_ids, temperature=1.0, reduc
     if x.dtype != "float32":
         x = x.float()
     v = (v if v.dtype == "float32" else v.float()).detach().contiguous()
-    xd, px, ld, rows, cols = _rows_2d(x)
+    xd, px, ld, rows, cols = _rows_2d(x.detach())
     k = v.shape[-1]
     xs = x.shape
     loss_rows = empty(xs[:-1])
@@ -410,20 +407,20 @@ def _teacher(v, ids, cols, temp, red, rows):
 
 
 def _setting(name, value, rows, dtype, lo, hi):
-    """(tensor or None, number) of a sampling setting: a number in [lo, hi],
-    or one value a row."""
-    if isinstance(value, Tensor) or np.ndim(value):
-        t = value if isinstance(value, Tensor) else \
-            _T.tensor(np.asarray(value, dtype=_DT[dtype][1]), dtype=dtype)
-        if t.shape != (rows,):
-            raise ValueError("sample_logits: %s has shape %s for %d rows"
-                             % (name, list(t.shape), rows))
-        if t.dtype != dtype:
-            t = t.to(dtype)
-        return t.detach().contiguous(), lo
-    if not lo <= value <= hi:
-        raise ValueError("sample_logits: %s must lie in [%s, %s], got %r" % (name, lo, hi, value))
-    return None, value
+    """(pointer or None, number, tensor or None) of a sampling setting: a
+    number in [lo, hi], or one value a row."""
+    if isinstance(value, (int, float)) or (not isinstance(value, Tensor) and np.ndim(value) == 0):
+        if not lo <= value <= hi:
+            raise ValueError("sample_logits: %s must lie in [%s, %s], got %r"
+                             % (name, lo, hi, value))
+        return None, value, None
+    t = value if isinstance(value, Tensor) else \
+        _T.tensor(np.asarray(value, dtype=_DT[dtype][1]), dtype=dtype)
+    if t.shape != (rows,):
+        raise ValueError("sample_logits: %s has shape %s for %d rows"
+                         % (name, list(t.shape), rows))
+    t = (t if t.dtype == dtype else t.to(dtype)).contiguous()
+    return t.data_ptr(), lo, t
 
 
 def sample_logits(logits, uniforms=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
@@ -463,18 +460,16 @@ def sample_logits(logits, uniforms=None, temperature=1.0, top_k=0, top_p=1.0, mi
         if u.numel() != rows or u.ndim > 1 or (u.ndim == 0 and not one):
             raise ValueError("sample_logits: uniforms of shape %s for %d rows"
                              % (list(u.shape), rows))
-        u = (u if u.dtype == "float32" else u.float()).detach().contiguous()
-    t, t0 = _setting("temperature", temperature, rows, "float32", 0.0, math.inf)
-    k, k0 = _setting("top_k", top_k, rows, "int32", 0, 2 ** 31 - 1)
-    p, p0 = _setting("top_p", top_p, rows, "float32", 0.0, 1.0)
-    m, m0 = _setting("min_p", min_p, rows, "float32", 0.0, 1.0)
+        u = (u if u.dtype == "float32" else u.float()).contiguous()
+    # the tensors live until the launch is queued
+    t, t0, _t = _setting("temperature", temperature, rows, "float32", 0.0, math.inf)
+    k, k0, _k = _setting("top_k", top_k, rows, "int32", 0, 2 ** 31 - 1)
+    p, p0, _p = _setting("top_p", top_p, rows, "float32", 0.0, 1.0)
+    m, m0, _m = _setting("min_p", min_p, rows, "float32", 0.0, 1.0)
     out = empty(() if one else (rows,), "int32")
-
-    def ptr(s):
-        return s.data_ptr() if s is not None else None
-    L.check(L.lib().tjh_sample_logits(px, ld, rows, cols, u.data_ptr(), ptr(t), ptr(k), ptr(p),
-                                      ptr(m), float(t0), int(k0), float(p0), float(m0),
-                                      out.data_ptr()), "sample_logits")
+    L.check(L.lib().tjh_sample_logits(px, ld, rows, cols, u.data_ptr(), t, k, p, m, float(t0),
+                                      int(k0), float(p0), float(m0), out.data_ptr()),
+            "sample_logits")
     return out
 
 
@@ -1051,14 +1046,23 @@ def _sdpa_masked(query, key, value, attn_mask, scale):
 
 
 def _window_rows(t):
-    """[B, H, T, D] operand with dense, 16-byte aligned rows (a copy where
-    `t`'s are not)."""
+    """A [B, H, T, D] operand with dense, 16-byte aligned rows: `t` itself, or
+    a copy where its rows are not."""
     st = t._strides
+    if st[3] == 1 and not (st[0] | st[1] | st[2]) & 3 and not t.data_ptr() & 15:
+        return t
+    t = t.detach()
     if t.numel() and ((st[3] != 1 and t.shape[3] > 1) or t.data_ptr() & 15 or
                       any(s % 4 for s, n in zip(st[:3], t.shape) if n > 1)):
         t = _k_contiguous(t)
     # the stride of an axis of one element is free: one that the kernels take
     return _alias(t, t.shape, tuple(0 if s % 4 else s for s in t._strides[:3]) + (1,), t._offset)
+
+
+@functools.lru_cache(maxsize=1024)
+def _strides3(st):
+    """The first three strides as the C entry points take them."""
+    return L.i64arr(st[:3])
 
 
 def sliding_window_attention(query, key, value, window, sinks=0, scale=None):
@@ -1073,17 +1077,20 @@ def sliding_window_attention(query, key, value, window, sinks=0, scale=None):
     and values hold has no part in its output.  O(Tk) memory beside the
     result, time by the keys seen.  Head dims up to 128; the gradients of
     key and value are summed over the query heads that read them."""
-    window, sinks = _whole("window", window, 1), _whole("sinks", sinks, 0)
-    nd = query.ndim
-    if nd not in (3, 4) or key.ndim != nd or value.ndim != nd:
+    if type(window) is not int or window < 1 or window > 1 << 30:
+        window = _whole("window", window, 1)
+    if type(sinks) is not int or sinks < 0 or sinks > 1 << 30:
+        sinks = _whole("sinks", sinks, 0)
+    qs, ks = query.shape, key.shape
+    nd = len(qs)
+    if nd not in (3, 4) or len(ks) != nd or value.ndim != nd:
         raise RuntimeError("sliding_window_attention expects three 3-D or three 4-D tensors")
     three = nd == 3
-    if key.shape != value.shape or query.shape[0] != key.shape[0] or \
-            query.shape[-1] != key.shape[-1]:
+    if ks != value.shape or qs[0] != ks[0] or qs[-1] != ks[-1]:
         raise RuntimeError("sliding_window_attention: shapes %s, %s, %s do not match"
-                           % (list(query.shape), list(key.shape), list(value.shape)))
-    D, Tq, Tk = query.shape[-1], query.shape[-2], key.shape[-2]
-    H, Hkv = (1, 1) if three else (query.shape[1], key.shape[1])
+                           % (list(qs), list(ks), list(value.shape)))
+    B, D, Tq, Tk = qs[0], qs[-1], qs[-2], ks[-2]
+    H, Hkv = (1, 1) if three else (qs[1], ks[1])
     if (Hkv == 0) != (H == 0) or (Hkv and H % Hkv):
         raise RuntimeError("sliding_window_attention: %d query heads over %d of keys" % (H, Hkv))
     if Tq > Tk:
@@ -1091,34 +1098,39 @@ def sliding_window_attention(query, key, value, window, sinks=0, scale=None):
                            % (Tq, Tk))
     if not 0 < D <= 128:
         raise NotImplementedError("sliding_window_attention: head dims up to 128, got %d" % D)
-    sc = float(scale) if scale is not None else 1.0 / math.sqrt(D)
-    query, key, value = [t if t.dtype == "float32" else t.float() for t in (query, key, value)]
+    sc = float(scale) if scale is not None else D ** -0.5
+    if not (query._dtype == key._dtype == value._dtype == "float32"):
+        query, key, value = [t if t.dtype == "float32" else t.float() for t in (query, key, value)]
     if D % 4:  # columns of zeros add nothing to any product
         fill = 4 - D % 4
         ts = [_T.cat([t, zeros(t.shape[:-1] + (fill,))], -1) for t in (query, key, value)]
         return _T.narrow(sliding_window_attention(*ts, window, sinks, sc), -1, 0, D)
     ins = [query, key, value]
-    q, k, v = [_window_rows(_bhtd(t.detach())) for t in ins]
-    B = q.shape[0]
+    q, k, v = [_window_rows(_bhtd(t.detach()) if three else t) for t in ins]
     rec = _T._recorded(*ins)
     ob = empty((B, Tq, H, D))
-    o = _alias(ob, (B, H, Tq, D), (Tq * H * D, D, H * D, 1), 0)
+    ost = (Tq * H * D, D, H * D, 1)
     lse = empty((B, H, Tq)) if rec else None
     L.check(L.lib().tjh_window_forward(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-        lse.data_ptr() if lse is not None else None, B, H, Hkv, Tq, Tk, D, L.i64arr(q._strides[:3]),
-        L.i64arr(k._strides[:3]), L.i64arr(v._strides[:3]), L.i64arr(o._strides[:3]), sc, window,
-        sinks), "sliding_window_attention")
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), ob.data_ptr(),
+        lse.data_ptr() if rec else None, B, H, Hkv, Tq, Tk, D, _strides3(q._strides),
+        _strides3(k._strides), _strides3(v._strides), _strides3(ost), sc, window, sinks),
+        "sliding_window_attention")
+    out = Tensor(ob._st, (B, Tq, D), (Tq * D, D, 1)) if three else Tensor(ob._st, qs, ost)
+    if not rec:
+        return out
+    q, k, v = q.detach(), k.detach(), v.detach()
+    o = _alias(ob, (B, H, Tq, D), ost, 0)
 
     def bwd(g):
         if three:
             g = _alias(g, (B, 1) + g.shape[1:], (g._strides[0], 0) + g._strides[1:], g._offset)
         g = _window_rows(g)
         if not o.numel():
-            return [zeros(t.shape) for t in ins]
+            return [zeros(s) for s in (qs, ks, ks)]
         shared = _shared_grads(q, k, v)
         dq, dk, dv = shared if shared else (_grad_as(q), _grad_as(k), _grad_as(v))
-        arrs = [L.i64arr(t._strides[:3]) for t in (q, k, v, o, g, dq, dk, dv)]
+        arrs = [_strides3(t._strides) for t in (q, k, v, o, g, dq, dk, dv)]
         ptrs = (L.P_i64 * 8)(*[ctypes.cast(a, L.P_i64) for a in arrs])
         L.check(L.lib().tjh_window_backward(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), g.data_ptr(), lse.data_ptr(),
@@ -1142,7 +1154,6 @@ def sliding_window_attention(query, key, value, window, sinks=0, scale=None):
             scores = mul(_T.matmul(qq, kk.transpose(-2, -1)), sc)
             return _T.matmul(softmax(_T.masked_fill(scores, drop, float("-inf")), -1), vv)
         return _T._regrad(ref, ins, g)
-    out = _alias(ob, (B, Tq, D), (Tq * D, D, 1), 0) if three else o
     return _record(out, "WindowAttention", ins, bwd, gfn=gbwd)
 
 

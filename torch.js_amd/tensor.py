@@ -2737,18 +2737,23 @@ def topk(x, k, dim=-1, largest=True):
         perm[d], perm[-1] = perm[-1], perm[d]
         v, i = topk(permute(x, perm), k, -1, largest)
         return permute(v, perm), permute(i, perm)
-    if x.dtype != "float32":
+    if x._dtype != "float32":
         x = x.float()
-    xd = x.detach()
-    if not (xd.ndim == 2 and xd._strides[1] == 1 and xd._strides[0] >= n):
-        xd = xd.contiguous()
-    ld = xd._strides[0] if xd.ndim == 2 else n
-    rows = _numel(x.shape[:-1])
-    oshape = x.shape[:-1] + (k,)
-    values, indices = empty(oshape), empty(oshape, "int32")
-    L.check(L.lib().tjh_topk_forward(xd.data_ptr(), max(ld, n), rows, n, k, 1 if largest else 0,
+    xs, st, xd, ld = x._shape, x._strides, x, n
+    if len(st) == 2 and st[1] == 1 and st[0] >= n:
+        ld = st[0]
+    else:
+        xd = x.detach().contiguous()
+    rows = _numel(xs[:-1])
+    oshape = xs[:-1] + (k,)
+    # both in one allocation, the indices after the values
+    both = Storage(max(1, 2 * rows * k) * 4)
+    values = Tensor(both, oshape)
+    indices = Tensor(both, oshape, None, rows * k, "int32")
+    L.check(L.lib().tjh_topk_forward(xd.data_ptr(), ld, rows, n, k, 1 if largest else 0,
                                      values.data_ptr(), indices.data_ptr()), "topk")
-    xs = x.shape
+    if not _recorded(x):
+        return values, indices
 
     def bwd(g):
         g = g.contiguous()
