@@ -72,7 +72,8 @@ int tjh_sample_logits(const float* logits, int64_t ld, int64_t rows, int64_t col
  * the logarithm to base 2 of a query's sum of exponentials, is saved for the
  * backward, or NULL.  Keys and values that a query does not see have no
  * part in its output, whatever they hold.  Head dims up to 128 that are
- * multiples of 4, rows 16-byte aligned (else TJH_ERR_UNSUPPORTED). */
+ * multiples of 4, rows 16-byte aligned and less than 2^23 elements apart (else
+ * TJH_ERR_UNSUPPORTED). */
 int tjh_window_forward(const float* q, const float* k, const float* v, float* o, float* lse,
                        int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t D,
                        const int64_t* q_strides, const int64_t* k_strides,

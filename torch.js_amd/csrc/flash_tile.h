@@ -184,8 +184,10 @@ __device__ __forceinline__ floatx16 chain0(const float (&a)[RUN],
 
 // Writes transposed accumulators acc[c][j] = X[row = l32][d] (d = c*32 +
 // 8(j/4)+4h+j%4) for the wave's 32 rows through LDS (buf, 32 x W floats)
-// into dst rows r0.. (stride st, columns < D), times `mul`.
-template <int HD>
+// into dst rows r0.. (stride st, columns < D), times `mul`.  BLOCK: every wave
+// of the workgroup calls this the same number of times (one barrier);
+// otherwise each wave by itself.
+template <int HD, bool BLOCK = true>
 __device__ __forceinline__ void write_rows(float* __restrict__ buf,
                                            const floatx16 (&acc)[Hd<HD>::NC], float mul,
                                            float* __restrict__ dst, int64_t st, int r0, int T,
@@ -195,7 +197,8 @@ __device__ __forceinline__ void write_rows(float* __restrict__ buf,
 #pragma unroll
     for (int c = 0; c < Hd<HD>::NC; ++c)
       buf[l32 * Hd<HD>::W + c * 32 + 8 * (j >> 2) + 4 * h + (j & 3)] = acc[c][j] * mul;
-  __syncthreads();  // every wave of the workgroup calls this the same number of times
+  if constexpr (BLOCK) __syncthreads();
+  else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // one wave's LDS accesses are in order
   // 32 rows x HD/4 float4: HD/8 float4 per lane
 #pragma unroll
   for (int i = 0; i < HD / 8; ++i) {

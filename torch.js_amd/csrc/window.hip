@@ -106,20 +106,78 @@ __device__ __forceinline__ bool drop_nonfinite(float (&x)[NC][16]) {
 #pragma unroll
   for (int c = 0; c < NC; ++c)
 #pragma unroll
-    for (int s = 0; s < 16; ++s) x[c][s] = finite(x[c][s]) ? x[c][s] : 0.f;
+    for (int s = 0; s < 16; ++s) {
+      asm volatile("" : "+v"(x[c][s]));  // compared anew: else every mask is kept
+      x[c][s] = finite(x[c][s]) ? x[c][s] : 0.f;
+    }
   return true;
+}
+
+// Operands straight from memory, with no LDS between: the waves of a
+// workgroup then need no barriers, and each walks just the tiles that its own
+// 32 queries see (a 128-query block's list is a third longer at a window of
+// 256).  What they share comes from the L1.
+
+// One 32-row tile of a [T, D] matrix with row stride st, as a buffer from the
+// tile's first element to the last one of its rows: loads past that give 0,
+// and addresses are one register and scalars.  Row strides are below 2^23, so
+// that a tile's offsets fit 32 bits.
+constexpr int kBufferFlags = 0x00020000;  // 32-bit data, raw addressing (gfx9)
+constexpr int64_t kMaxRowStride = int64_t(1) << 23;
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_buffer(const float* tile, int64_t st,
+                                                              int left, int D) {
+  const int rows = min(left, TILE);
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(tile), 0,
+                                           4 * ((rows - 1) * (int)st + D), kBufferFlags);
+}
+
+typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
+
+// Operand of a product over the head dim, row l32 of the tile: lane (l32, h)
+// has row[8 i + 4 h + e] as x[4 i + e].  GUARD: columns >= D are zero (read
+// past the buffer).
+template <int HD, bool GUARD, int RUN>
+__device__ __forceinline__ void row_operand(__amdgpu_buffer_rsrc_t tile, int st, int D, int l32,
+                                            int h, float (&x)[RUN]) {
+  const int at = 4 * (l32 * st + 4 * h);
+#pragma unroll
+  for (int i = 0; i < RUN / 4; ++i) {
+    const bool in = !GUARD || 8 * i + 4 * h < D;
+    const uint4v v = __builtin_amdgcn_raw_buffer_load_b128(tile, in ? at : 0x7ffffff0, 32 * i, 0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[4 * i + e] = __uint_as_float(v[e]);
+  }
+}
+
+// Operand of a product over the tile's rows (lds_cols's): x[c][s] is column
+// c * 32 + l32 of row kappa(s, h).  Columns past D hold anything: they go to
+// columns of the result that are not written.
+template <int HD>
+__device__ __forceinline__ void col_operand(__amdgpu_buffer_rsrc_t tile, int st, int l32, int h,
+                                            float (&x)[Hd<HD>::NC][16]) {
+  const int at = 4 * (4 * h * st + l32);
+#pragma unroll
+  for (int s = 0; s < 16; ++s)
+#pragma unroll
+    for (int c = 0; c < Hd<HD>::NC; ++c)
+      x[c][s] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+          tile, at + 128 * c, 4 * kappa(s, 0) * st, 0));
 }
 
 // ------------------------------------------------------------ forward
 
-// GUARD: Tk is not a multiple of 32, or D < HD.  PART: one slice of the key
-// tiles, joined by k_win_merge.
+// Waves per SIMD the registers leave room for.
+template <int HD> constexpr int waves_fwd() { return HD <= 64 ? 3 : HD <= 96 ? 2 : 1; }
+
+// One wave 32 queries.  GUARD: D < HD.  PART: one slice of the key tiles,
+// joined by k_win_merge.
 template <int HD, bool GUARD, bool PART, int RUN>
-__global__ __launch_bounds__(256, occ_fwd<HD>()) void k_win_fwd(WinArgs a) {
+__global__ __launch_bounds__(256, waves_fwd<HD>()) void k_win_fwd(WinArgs a) {
   using S_ = Hd<HD>;
-  __shared__ __attribute__((aligned(16))) float Ks[2][TILE * S_::W];
-  __shared__ __attribute__((aligned(16))) float Vs[2][TILE * S_::W];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  __shared__ __attribute__((aligned(16))) float buf[WAVES][TILE * S_::W];  // the output's rows
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l32 = lane & 31, h = lane >> 5;
   const int item = xcd_item(blockIdx.x, gridDim.x);
   const int64_t bh = item / a.nblk;
@@ -129,101 +187,95 @@ __global__ __launch_bounds__(256, occ_fwd<HD>()) void k_win_fwd(WinArgs a) {
   const float* K = a.k + b * a.ks.b + kh * a.ks.h;
   const float* V = a.v + b * a.vs.b + kh * a.vs.h;
   const int q0 = qb * ROWS + w * TILE;  // this wave's first query
+  if (q0 >= a.Tq) return;
   const int myq = q0 + l32, lo = a.off + q0, pos = lo + l32;
-  const Tiles tiles(a, a.off + qb * ROWS, min(a.off + qb * ROWS + ROWS, a.Tk) - 1);
+  const Tiles tiles(a, lo, min(lo + TILE, a.Tk) - 1);
   const int i0 = PART ? (int)blockIdx.y * a.kslice : 0;
   const int i1 = PART ? min(tiles.n, i0 + a.kslice) : tiles.n;
-  if (PART && i0 >= i1) return;  // the same for the whole workgroup
+  if (PART && i0 >= i1) return;
 
   float qf[RUN];
-  gl_run<HD, GUARD>(Q, a.qs.t, myq, a.Tq, a.D, h, a.scale * kLog2e, qf);
+  row_operand<HD, GUARD>(tile_buffer(Q + q0 * a.qs.t, a.qs.t, a.Tq - q0, a.D), (int)a.qs.t, a.D,
+                         l32, h, qf);
+#pragma unroll
+  for (int s = 0; s < RUN; ++s) qf[s] *= a.scale * kLog2e;
+  const auto load_keys = [&](int kt, float (&x)[RUN]) {
+    const int k0 = kt * TILE;
+    row_operand<HD, GUARD>(tile_buffer(K + k0 * a.ks.t, a.ks.t, a.Tk - k0, a.D), (int)a.ks.t, a.D,
+                           l32, h, x);
+  };
   floatx16 acc[S_::NC];
   zero_acc(acc);
   float m = -INFINITY, lsum = 0.f;
-  floatx4 rk[S_::NC], rv[S_::NC];
-  load_tile<HD, GUARD>(K, a.ks.t, tiles(i0) * TILE, a.Tk, a.D, rk);
-  load_tile<HD, GUARD>(V, a.vs.t, tiles(i0) * TILE, a.Tk, a.D, rv);
-  store_tile<HD>(Ks[0], rk);
-  store_tile<HD>(Vs[0], rv);
-  __syncthreads();
+  float ka[RUN];
+  load_keys(tiles(i0), ka);
   for (int i = i0; i < i1; ++i) {
-    const int cur = (i - i0) & 1;
-    const bool more = i + 1 < i1;
-    if (more) {
-      load_tile<HD, GUARD>(K, a.ks.t, tiles(i + 1) * TILE, a.Tk, a.D, rk);
-      load_tile<HD, GUARD>(V, a.vs.t, tiles(i + 1) * TILE, a.Tk, a.D, rv);
-    }
     const int kt = tiles(i), k0 = kt * TILE;
-    if (q0 < a.Tq && tile_seen(a, lo, kt)) {
-      float ka[RUN];
-      lds_run<HD>(Ks[cur], l32, h, ka);
-      floatx16 st = chain0<HD>(ka, qf);  // S^T[key][query], base-2 units
-      float va[S_::NC][16];
-      lds_cols<HD>(Vs[cur], l32, h, va);
-      bool bad = false;
-      if (!tile_whole(a, lo, kt)) {
+    // values on their way during the first product, the next keys during the
+    // second
+    float va[S_::NC][16];
+    col_operand<HD>(tile_buffer(V + k0 * a.vs.t, a.vs.t, a.Tk - k0, a.D), (int)a.vs.t, l32, h, va);
+    floatx16 st = chain0<HD>(ka, qf);  // S^T[key][query], base-2 units
+    load_keys(tiles(min(i + 1, i1 - 1)), ka);
+    bool bad = false;
+    if (!tile_whole(a, lo, kt)) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) st[j] = sees(a, pos, k0 + kappa(j, h)) ? st[j] : -INFINITY;
-        bad = drop_nonfinite(va);
-      }
-      float bm = st[0];
+      for (int j = 0; j < 16; ++j) st[j] = sees(a, pos, k0 + kappa(j, h)) ? st[j] : -INFINITY;
+      bad = drop_nonfinite(va);
+    }
+    float bm = st[0];
 #pragma unroll
-      for (int j = 1; j < 16; ++j) bm = fmaxf(bm, st[j]);
-      bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
-      const float mn = fmaxf(m, bm);
-      const float ms = mn == -INFINITY ? 0.f : mn;  // nothing seen so far
-      const float alpha = exp2_hw(m - ms);
-      float rs = 0.f;
+    for (int j = 1; j < 16; ++j) bm = fmaxf(bm, st[j]);
+    bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
+    const float mn = fmaxf(m, bm);
+    const float ms = mn == -INFINITY ? 0.f : mn;  // nothing seen so far
+    const float alpha = exp2_hw(m - ms);
+    float rs = 0.f;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        st[j] = exp2_hw(st[j] - ms);
-        rs += st[j];
-      }
-      rs += __shfl_xor(rs, 32, 64);
-      lsum = lsum * alpha + rs;
-      m = mn;
+    for (int j = 0; j < 16; ++j) {
+      st[j] = exp2_hw(st[j] - ms);
+      rs += st[j];
+    }
+    rs += __shfl_xor(rs, 32, 64);
+    lsum = lsum * alpha + rs;
+    m = mn;
 #pragma unroll
-      for (int c = 0; c < S_::NC; ++c) acc[c] *= alpha;
+    for (int c = 0; c < S_::NC; ++c) acc[c] *= alpha;
 #pragma unroll
-      for (int s = 0; s < 16; ++s)  // O^T += V^T P^T
+    for (int s = 0; s < 16; ++s)  // O^T += V^T P^T
 #pragma unroll
-        for (int c = 0; c < S_::NC; ++c) acc[c] = mfma(va[c][s], st[s], acc[c]);
-      if (bad) {  // values that are not finite, for the queries that see them
+      for (int c = 0; c < S_::NC; ++c) acc[c] = mfma(va[c][s], st[s], acc[c]);
+    if (bad) {  // values that are not finite, for the queries that see them
 #pragma unroll 1
-        for (int r = 0; r < TILE; ++r) {
-          if (!sees(a, pos, k0 + r)) continue;
+      for (int r = 0; r < TILE; ++r) {
+        if (!sees(a, pos, k0 + r) || k0 + r >= a.Tk) continue;
+        const float* row = V + (int64_t)(k0 + r) * a.vs.t;
 #pragma unroll
-          for (int c = 0; c < S_::NC; ++c)
+        for (int c = 0; c < S_::NC; ++c)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const float x = Vs[cur][r * S_::W + c * 32 + kappa(j, h)];
-              acc[c][j] += finite(x) ? 0.f : x;
-            }
-        }
+          for (int j = 0; j < 16; ++j) {
+            const int d = c * 32 + kappa(j, h);
+            const float x = d < a.D ? row[d] : 0.f;
+            acc[c][j] += finite(x) ? 0.f : x;
+          }
       }
     }
-    if (more) {
-      store_tile<HD>(Ks[cur ^ 1], rk);
-      store_tile<HD>(Vs[cur ^ 1], rv);
-    }
-    __syncthreads();
   }
-  float* buf = (w < 2 ? Ks[w] : Vs[w - 2]);
   if constexpr (PART) {
     const int64_t row0 = ((int64_t)blockIdx.y * (gridDim.x / a.nblk) + bh) * a.Tq;
-    write_rows<HD>(buf, acc, 1.0f, a.part + row0 * a.D, a.D, q0, a.Tq, a.D, l32, h, lane);
+    write_rows<HD, false>(buf[w], acc, 1.0f, a.part + row0 * a.D, a.D, q0, a.Tq, a.D, l32, h, lane);
     if (h == 0 && myq < a.Tq) a.pml[row0 + myq] = make_float2(m, lsum);
     return;
   }
   const float inv = 1.0f / lsum;  // a query sees itself: the sum is at least 1
-  write_rows<HD>(buf, acc, inv, a.out + b * a.os.b + hh * a.os.h, a.os.t, q0, a.Tq, a.D, l32, h,
-                 lane);
+  write_rows<HD, false>(buf[w], acc, inv, a.out + b * a.os.b + hh * a.os.h, a.os.t, q0, a.Tq, a.D,
+                        l32, h, lane);
   if (a.lse_out && h == 0 && myq < a.Tq) a.lse_out[bh * a.Tq + myq] = m + __log2f(lsum);
 }
 
 // Joins the slices of a query: o = sum 2^(m_s - m) acc_s / sum 2^(m_s - m)
 // l_s, in slice order.  One float4 a lane; n: slices of each row, or 0 and
-// those of its block of queries.
+// those of its 32 queries.
 __global__ __launch_bounds__(256) void k_win_merge(WinArgs a, int64_t n4, int nslices) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= n4) return;
@@ -234,8 +286,8 @@ __global__ __launch_bounds__(256) void k_win_merge(WinArgs a, int64_t n4, int ns
   const int q = (int)(row - bh * a.Tq);
   int n = nslices;
   if (n == 0) {
-    const int lo = a.off + q / ROWS * ROWS;
-    const Tiles tiles(a, lo, min(lo + ROWS, a.Tk) - 1);
+    const int lo = a.off + q / TILE * TILE;
+    const Tiles tiles(a, lo, min(lo + TILE, a.Tk) - 1);
     n = (tiles.n + a.kslice - 1) / a.kslice;
   }
   float top = -INFINITY;
@@ -570,15 +622,14 @@ __global__ __launch_bounds__(256) void k_win_sums(WinArgs a, int64_t n4) {
   *reinterpret_cast<floatx4*>((v ? a.out2 : a.out) + b * st.b + kh * st.h + key * st.t + c) = x;
 }
 
-// Query-block kernel: dQ^T += K^T dS^T for 128 queries from the stored dS
-// blocks; two groups of four waves take the even and the odd key tiles and
-// are added at the end (flash.hip's k_flash_dq_ds8).
-template <int HD, bool GUARD>
-__global__ __launch_bounds__(512, 1) void k_win_dq(WinArgs a) {
+// Query kernel: dQ^T += K^T dS^T from the stored dS blocks, one wave 32
+// queries, the next tile's operands on their way during a tile's products.
+template <int HD>
+__global__ __launch_bounds__(256, HD <= 64 ? 3 : HD <= 96 ? 2 : 1) void k_win_dq(WinArgs a) {
   using S_ = Hd<HD>;
-  __shared__ __attribute__((aligned(16))) float Ks[WAVES][TILE * S_::W];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  const int grp = wv >> 2, w = wv & 3, gt = threadIdx.x & 255;
+  __shared__ __attribute__((aligned(16))) float buf[WAVES][TILE * S_::W];
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l32 = lane & 31, h = lane >> 5;
   const int item = xcd_item(blockIdx.x, gridDim.x);
   const int64_t bhl = item / a.nblk;  // from the launch's first head on
@@ -587,84 +638,39 @@ __global__ __launch_bounds__(512, 1) void k_win_dq(WinArgs a) {
   const int64_t b = bh / a.H, hh = bh % a.H;
   const float* K = a.k + b * a.ks.b + (hh / a.G) * a.ks.h;
   const int q0 = qb * ROWS + w * TILE, lo = a.off + q0;
-  const bool wave_in = q0 < a.Tq;
-  const float* dsrow = a.dsblk +
-                       (bhl * a.nqt + (wave_in ? q0 / TILE : 0)) * a.nsl * (TILE * TILE) +
-                       l32 * TILE + h * 16;
-  floatx16 dq[S_::NC];
-  zero_acc(dq);
-  const Tiles tiles(a, a.off + qb * ROWS, min(a.off + qb * ROWS + ROWS, a.Tk) - 1);
-  const int n = tiles.n, nst0 = (n + 1) / 2;
-  const auto idx = [&](int t) { return grp + 2 * t; };
-  const auto mine = [&](int i) { return i < n && wave_in && tile_seen(a, lo, tiles(i)); };
-  // every prefetch is issued, from slot 0 where the wave does not see the
-  // tile (its values are then not used): loads on conditional paths would
-  // make the waits of the current tile wait for them too
-  const auto fetch_ds = [&](int t, floatx4 (&d)[4]) {
-    const int i = idx(t);
-    const int slot = mine(i) ? ds_slot(a, lo, tiles(i)) : 0;
-    const floatx4* src = reinterpret_cast<const floatx4*>(dsrow + (int64_t)slot * (TILE * TILE));
+  if (q0 >= a.Tq) return;
+  const float* dsrow = a.dsblk + (bhl * a.nqt + q0 / TILE) * a.nsl * (TILE * TILE) + l32 * TILE +
+                       h * 16;
+  const Tiles tiles(a, lo, min(lo + TILE, a.Tk) - 1);
+  const auto load = [&](int kt, float (&k)[S_::NC][16], floatx4 (&d)[4]) {
+    const int k0 = kt * TILE;
+    col_operand<HD>(tile_buffer(K + k0 * a.ks.t, a.ks.t, a.Tk - k0, a.D), (int)a.ks.t, l32, h, k);
+    const floatx4* src =
+        reinterpret_cast<const floatx4*>(dsrow + (int64_t)ds_slot(a, lo, kt) * (TILE * TILE));
 #pragma unroll
     for (int u = 0; u < 4; ++u) d[u] = src[u];
   };
-  floatx4 d0[4], d1[4], d2[4];
-  fetch_ds(0, d0);
-  fetch_ds(1, d1);
-  floatx4 rk[S_::NC];
-  if (idx(0) < n) {
-    load_tile<HD, GUARD>(K, a.ks.t, tiles(idx(0)) * TILE, a.Tk, a.D, rk, gt);
-    store_tile<HD>(Ks[2 * grp], rk, gt);
-  }
-  __syncthreads();
-  const auto step = [&](int t, const floatx4 (&use)[4], floatx4 (&into)[4]) {
-    const int cur = 2 * grp + (t & 1);
-    const int i = idx(t);
-    const bool more = i + 2 < n;
-    load_tile<HD, GUARD>(K, a.ks.t, tiles(more ? i + 2 : n - 1) * TILE, a.Tk, a.D, rk, gt);
-    fetch_ds(t + 2, into);
-    if (mine(i)) {
-      float ct[S_::NC][16];
-      lds_cols<HD>(Ks[cur], l32, h, ct);
-      // a query that sees a key that is not finite has NaN in dS already
-      if (!tile_whole(a, lo, tiles(i))) drop_nonfinite(ct);
+  floatx16 dq[S_::NC];
+  zero_acc(dq);
+  const auto products = [&](int kt, float (&k)[S_::NC][16], const floatx4 (&d)[4]) {
+    // a query that sees a key that is not finite has NaN in dS already
+    if (!tile_whole(a, lo, kt)) drop_nonfinite(k);
 #pragma unroll
-      for (int s = 0; s < 16; ++s) {
-        const float d = use[s >> 2][s & 3];
+    for (int s = 0; s < 16; ++s)
 #pragma unroll
-        for (int c = 0; c < S_::NC; ++c) dq[c] = mfma(ct[c][s], d, dq[c]);
-      }
-    }
-    if (more) store_tile<HD>(Ks[2 * grp + ((t + 1) & 1)], rk, gt);
-    __syncthreads();
+      for (int c = 0; c < S_::NC; ++c) dq[c] = mfma(k[c][s], d[s >> 2][s & 3], dq[c]);
   };
-  for (int t = 0; t < nst0; t += 3) {
-    step(t, d0, d2);
-    if (t + 1 >= nst0) break;
-    step(t + 1, d1, d0);
-    if (t + 2 >= nst0) break;
-    step(t + 2, d2, d1);
+  float k0[S_::NC][16], k1[S_::NC][16];
+  floatx4 d0[4], d1[4];
+  load(tiles(0), k0, d0);
+  for (int i = 0; i < tiles.n; i += 2) {
+    load(tiles(min(i + 1, tiles.n - 1)), k1, d1);
+    products(tiles(i), k0, d0);
+    load(tiles(min(i + 2, tiles.n - 1)), k0, d0);
+    if (i + 1 < tiles.n) products(tiles(i + 1), k1, d1);
   }
-  // even tiles' sum + odd tiles' sum
-  float* red = &Ks[0][0] + w * (S_::NC * 16 * 64);
-  if (grp == 1) {
-#pragma unroll
-    for (int c = 0; c < S_::NC; ++c)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) red[(c * 16 + j) * 64 + lane] = dq[c][j];
-  }
-  __syncthreads();
-  if (grp == 0) {
-#pragma unroll
-    for (int c = 0; c < S_::NC; ++c)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) dq[c][j] = dq[c][j] + red[(c * 16 + j) * 64 + lane];
-  }
-  __syncthreads();
-  if (grp == 0)
-    write_rows<HD>(Ks[w], dq, a.scale, a.out + b * a.o1s.b + hh * a.o1s.h, a.o1s.t, q0, a.Tq, a.D,
-                   l32, h, lane);
-  else
-    __syncthreads();  // the one barrier inside write_rows
+  write_rows<HD, false>(buf[w], dq, a.scale, a.out + b * a.o1s.b + hh * a.o1s.h, a.o1s.t, q0, a.Tq,
+                        a.D, l32, h, lane);
 }
 
 // ------------------------------------------------------------ host
@@ -679,7 +685,7 @@ template <int HD, bool PART>
 void launch_fwd(const WinArgs& a, dim3 grid) {
   if (short_run<HD>(a))
     tjh_launch(k_win_fwd<HD, true, PART, HD / 2 - 8>, grid, dim3(256), 0, stream(), a);
-  else if (a.Tk % TILE || a.D != HD)
+  else if (a.D != HD)
     tjh_launch(k_win_fwd<HD, true, PART, HD / 2>, grid, dim3(256), 0, stream(), a);
   else
     tjh_launch(k_win_fwd<HD, false, PART, HD / 2>, grid, dim3(256), 0, stream(), a);
@@ -710,10 +716,7 @@ int launch_bwd(WinArgs a, unsigned keys, float* dq, const int64_t* dq_st) {
   a.out = dq;
   a.o1s = s3(dq_st);
   const unsigned grid = (unsigned)(a.nbkv * a.G * a.nblk);
-  if (a.Tk % TILE || a.D != HD)
-    tjh_launch(k_win_dq<HD, true>, dim3(grid), dim3(512), 0, stream(), a);
-  else
-    tjh_launch(k_win_dq<HD, false>, dim3(grid), dim3(512), 0, stream(), a);
+  tjh_launch(k_win_dq<HD>, dim3(grid), dim3(256), 0, stream(), a);
   return check_launch("window_dq");
 }
 
@@ -729,12 +732,14 @@ int check_window(const char* who, int64_t B, int64_t H, int64_t Hkv, int64_t Tq,
   TJH_ARG(Tk < (int64_t(1) << 30) && H < (int64_t(1) << 30), "%s: too large", who);
   TJH_ARG(B * H * cdiv(Tq, TILE) < (int64_t(1) << 31), "%s: grid too large", who);
   for (int i = 0; i < n; ++i) TJH_ARG(strides[i], "%s: NULL strides", who);
+  bool wide = false;
+  for (int i = 0; i < n; ++i) wide |= strides[i][2] >= kMaxRowStride || strides[i][2] < 0;
   if (B == 0 || H == 0 || Tq == 0) return TJH_OK;
   for (int i = 0; i < n; ++i) TJH_ARG(ptrs[i], "%s: NULL pointer", who);
-  if (!flash_supported(D, ptrs, strides, n))
+  if (wide || !flash_supported(D, ptrs, strides, n))
     return set_error(TJH_ERR_UNSUPPORTED,
                      "%s: head dims up to 128 that are multiples of 4, in 16-byte aligned rows "
-                     "(head dim %lld)", who, (long long)D);
+                     "less than 2^23 apart (head dim %lld)", who, (long long)D);
   return TJH_OK;
 }
 
@@ -804,8 +809,8 @@ int tjh_window_forward(const float* q, const float* k, const float* v, float* o,
   const int64_t blocks = B * H * a.nblk;
   // slices of the key tiles where the blocks of queries leave CUs idle and
   // have enough tiles to pay for the join
-  const int64_t wt = cdiv((int64_t)a.win + ROWS - 2, TILE) + 1 + a.nst, all = cdiv(Tk, TILE);
-  const int64_t nt = wt < all ? wt : all;  // tiles of a block at most
+  const int64_t wt = cdiv((int64_t)a.win + TILE - 2, TILE) + 1 + a.nst, all = cdiv(Tk, TILE);
+  const int64_t nt = wt < all ? wt : all;  // tiles of 32 queries at most
   int64_t n = 1;
   if (!lse && blocks < cus && nt > 4) {
     a.kslice = (int)(cdiv(nt * blocks, cus) < 2 ? 2 : cdiv(nt * blocks, cus));

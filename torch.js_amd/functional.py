@@ -1049,10 +1049,11 @@ def _window_rows(t):
     """A [B, H, T, D] operand with dense, 16-byte aligned rows: `t` itself, or
     a copy where its rows are not."""
     st = t._strides
-    if st[3] == 1 and not (st[0] | st[1] | st[2]) & 3 and not t.data_ptr() & 15:
+    if st[3] == 1 and not (st[0] | st[1] | st[2]) & 3 and not t.data_ptr() & 15 and \
+            st[2] < 1 << 23:
         return t
     t = t.detach()
-    if t.numel() and ((st[3] != 1 and t.shape[3] > 1) or t.data_ptr() & 15 or
+    if t.numel() and ((st[3] != 1 and t.shape[3] > 1) or t.data_ptr() & 15 or st[2] >= 1 << 23 or
                       any(s % 4 for s, n in zip(st[:3], t.shape) if n > 1)):
         t = _k_contiguous(t)
     # the stride of an axis of one element is free: one that the kernels take
