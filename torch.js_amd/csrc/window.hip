@@ -4,17 +4,16 @@
 // the keys j <= i with j > i - window or j < sinks, H query heads share Hkv
 // heads of keys and values, and time and memory grow with the keys seen.
 //
-// The tiles, layouts and products are flash.hip's (flash_tile.h).  A block of
-// 128 queries walks the key tiles that hold sinks, then the ones from its
-// first query's window to its last query; a wave of 32 queries skips the
-// tiles that it sees nothing of and masks only the ones that it sees in part.
-// Backward: a key-block kernel walks the query heads that share its keys and
-// their query tiles, accumulating dV and dK and storing each 32x32 block of
-// dS in a band of `nsl` slots a query tile (sink tiles, then window tiles); a
-// query-block kernel turns those into dQ, so S and dP are formed once.  The
-// key blocks with sinks are seen by every later query: their query tiles are
-// cut into slices, whose sums a last kernel adds in order.  Deterministic, no
-// atomics.
+// Layouts and products are flash.hip's (flash_tile.h).  Forward and dQ: a wave
+// has 32 queries, its operands straight from memory, and walks the tiles of
+// keys that those see: the ones that hold sinks, then the window's.  It masks
+// only the tiles that it sees in part.  dK and dV: a key-block kernel walks
+// the query heads that share its keys and their query tiles, accumulating dV
+// and dK and storing each 32x32 block of dS in a band of `nsl` slots a query
+// tile (sink tiles, then window tiles); the query kernel turns those into dQ,
+// so S and dP are formed once.  The key blocks with sinks are seen by every
+// later query: their steps are cut into slices, whose sums a last kernel adds
+// in order.  Deterministic, no atomics.
 //
 // Keys that a query does not see may hold anything, infinities and NaN
 // included: their scores are replaced, never multiplied, and where a tile
@@ -46,12 +45,14 @@ struct WinArgs {
   float2* pml;
   int kslice;
   // backward: dS blocks [bh - bh0][query tile][nsl], of the key heads from
-  // bkv0 on; slices of the key blocks with sinks
+  // bkv0 on
   float* dsblk;
   int nqt, nkt, nsl;
   int bkv0, nbkv;
-  int nsb, nslice;     // key blocks with sinks, slices of their query tiles
-  float* sums;         // [slice][bkv - bkv0][nsb * PROWS][D] of dK, then dV
+  // slices of the steps of the nsb key blocks with sinks and of the others;
+  // sums [slice][bkv - bkv0][keys of those blocks][D] of dK, then dV, of each
+  int nsb, nslice, nsplit;
+  float* sums;
 };
 
 constexpr int PROWS = 64;  // keys of a workgroup of the key-block kernel
@@ -85,7 +86,11 @@ __device__ __forceinline__ bool tile_whole(const WinArgs& a, int lo, int kt) {
   return k1 <= lo && (kt * TILE > lo + TILE - 1 - a.win || k1 < a.sinks);
 }
 __device__ __forceinline__ bool sees(const WinArgs& a, int pos, int key) {
-  return key <= pos && (key > pos - a.win || key < a.sinks);
+  // key <= pos and key > pos - win as one comparison.  No short circuits here
+  // or where this is used: a branch around one element of an accumulator has
+  // been compiled wrongly (ROCm 7.2: the element's other value went to every
+  // lane that took the branch)
+  return ((unsigned)(pos - key) < (unsigned)a.win) | ((key < a.sinks) & (key <= pos));
 }
 // Slot of tile kt among the dS blocks of the queries at [lo, lo + 31].
 __device__ __forceinline__ int ds_slot(const WinArgs& a, int lo, int kt) {
@@ -97,12 +102,14 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 // Sets values that are not finite to 0; whether the wave had any.
 template <int NC>
 __device__ __forceinline__ bool drop_nonfinite(float (&x)[NC][16]) {
-  bool bad = false;
+  float top = 0.f;  // the maximum that NaN is larger than everything for
 #pragma unroll
   for (int c = 0; c < NC; ++c)
 #pragma unroll
-    for (int s = 0; s < 16; ++s) bad |= !finite(x[c][s]);
-  if (__ballot(bad) == 0) return false;
+    for (int s = 0; s < 16; s += 2)
+      top = __builtin_elementwise_maximum(
+          __builtin_elementwise_maximum(top, fabsf(x[c][s])), fabsf(x[c][s + 1]));
+  if (__ballot(!finite(top)) == 0) return false;
 #pragma unroll
   for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -220,7 +227,10 @@ __global__ __launch_bounds__(256, waves_fwd<HD>()) void k_win_fwd(WinArgs a) {
     bool bad = false;
     if (!tile_whole(a, lo, kt)) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) st[j] = sees(a, pos, k0 + kappa(j, h)) ? st[j] : -INFINITY;
+      for (int j = 0; j < 16; ++j) {
+        const bool in = sees(a, pos, k0 + kappa(j, h));
+        st[j] = in ? st[j] : -INFINITY;
+      }
       bad = drop_nonfinite(va);
     }
     float bm = st[0];
@@ -418,10 +428,17 @@ __global__ __launch_bounds__(kFewThreads) void k_win_few(WinArgs a) {
 
 // ------------------------------------------------------------ backward
 
+// Where the sums of the key blocks without sinks begin.
+__host__ __device__ inline int64_t sums_at(const WinArgs& a) {
+  return a.nslice > 1 ? (int64_t)2 * a.nslice * a.nbkv * a.nsb * PROWS * a.D : 0;
+}
+
 // Key-block kernel: 64 keys a workgroup, each 32 of them a pair of waves; wave
 // A forms P and accumulates dV^T += dO^T P, wave B forms dS = P (dP - D),
-// stores it and accumulates dK^T += Q^T dS (flash.hip's split of the work).
-// GUARD: Tq or Tk is not a multiple of 32, or D < HD.
+// stores it and accumulates dK^T += Q^T dS (flash.hip's split of the work, the
+// tiles of Q and dO through LDS: straight from memory they took 2 % less at a
+// head dim of 64 and a sixth more at 128).  GUARD: Tq or Tk is not a multiple
+// of 32, or D < HD.
 template <int HD, bool GUARD, int RUN>
 __global__ __launch_bounds__(256, occ_pair<HD>()) void k_win_dkv(WinArgs a) {
   using S_ = Hd<HD>;
@@ -435,19 +452,15 @@ __global__ __launch_bounds__(256, occ_pair<HD>()) void k_win_dkv(WinArgs a) {
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const int role = wv >> 1, pr = wv & 1;  // role 0: A (P, dV), 1: B (dS, dK)
   const int l32 = lane & 31, h = lane >> 5;
-  // the slices of the sinks' blocks first: they are the longest
+  // the slices of the sinks' blocks first, then the blocks by position: the
+  // last ones are seen by fewer queries and fill the CUs at the end
   const int nlong = a.nbkv * a.nsb * a.nslice;
-  int bkv, kb, slice = 0;
   const bool sunk = (int)blockIdx.x < nlong;
-  if (sunk) {
-    slice = blockIdx.x % a.nslice;
-    kb = blockIdx.x / a.nslice % a.nsb;
-    bkv = blockIdx.x / (a.nslice * a.nsb);
-  } else {
-    const int item = xcd_item(blockIdx.x - nlong, gridDim.x - nlong), per = a.nblk - a.nsb;
-    bkv = item / per;
-    kb = a.nsb + item % per;
-  }
+  const int slices = sunk ? a.nslice : a.nsplit;
+  int id = sunk ? blockIdx.x : blockIdx.x - nlong;
+  const int bkv = id % a.nbkv;
+  id /= a.nbkv;
+  const int slice = id % slices, kb = (sunk ? 0 : a.nsb) + id / slices;
   const int hkv = a.H / a.G;
   const int64_t b = (a.bkv0 + bkv) / hkv, kh = (a.bkv0 + bkv) % hkv;
   const float* K = a.k + b * a.ks.b + kh * a.ks.h;
@@ -468,18 +481,15 @@ __global__ __launch_bounds__(256, occ_pair<HD>()) void k_win_dkv(WinArgs a) {
   zero_acc(acc);
 
   // the query tiles that see some of the 64 keys
-  int qt0 = max(0, kb * PROWS - a.off) / TILE;
+  const int qt0 = max(0, kb * PROWS - a.off) / TILE;
   int last = a.Tq - 1;
   if (!sunk) last = (int)min((int64_t)last, (int64_t)kb * PROWS + PROWS - 2 + a.win - a.off);
-  int qt1 = last < 0 ? qt0 : max(qt0, last / TILE + 1);
-  if (sunk && a.nslice > 1) {
-    const int per = (qt1 - qt0 + a.nslice - 1) / a.nslice;
-    qt0 = min(qt1, qt0 + slice * per);
-    qt1 = min(qt1, qt0 + per);
-  }
-  const int steps = (qt1 - qt0) * a.G;
+  const int qt1 = last < 0 ? qt0 : max(qt0, last / TILE + 1), nt = qt1 - qt0;
+  // this slice of the steps, the query heads' tiles one head after the other
+  const int per = (nt * a.G + slices - 1) / slices;
+  const int f0 = min(nt * a.G, slice * per), steps = min(nt * a.G - f0, per);
   // of the current and the next step: query head and tile
-  int hh = (int)kh * a.G, qt = qt0;
+  int hh = (int)kh * a.G + (nt ? f0 / nt : 0), qt = qt0 + (nt ? f0 % nt : 0);
   const auto qrows = [&](const float* x, const Strides3& s, int head) {
     return x + b * s.b + (int64_t)head * s.h;
   };
@@ -520,7 +530,7 @@ __global__ __launch_bounds__(256, occ_pair<HD>()) void k_win_dkv(WinArgs a) {
     const bool edge = !tile_whole(a, lo, kt) || (GUARD && qt * TILE + TILE > a.Tq);
     const auto ok = [&](int j) {
       const int r = kappa(j, h);
-      return (!GUARD || qt * TILE + r < a.Tq) && sees(a, lo + r, mykey);
+      return (!GUARD | (qt * TILE + r < a.Tq)) & sees(a, lo + r, mykey);
     };
     floatx16 x = zero16();  // A: P; B: dP - D, then dS
     if (seen) {
@@ -537,7 +547,10 @@ __global__ __launch_bounds__(256, occ_pair<HD>()) void k_win_dkv(WinArgs a) {
       if (role == 0) {
         if (edge) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) x[j] = ok(j) ? exp2_hw(x[j]) : 0.f;
+          for (int j = 0; j < 16; ++j) {
+            const float e = exp2_hw(x[j]);
+            x[j] = ok(j) ? e : 0.f;
+          }
         } else {
 #pragma unroll
           for (int j = 0; j < 16; ++j) x[j] = exp2_hw(x[j]);
@@ -558,7 +571,10 @@ __global__ __launch_bounds__(256, occ_pair<HD>()) void k_win_dkv(WinArgs a) {
       } else {
         if (edge) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) x[j] = ok(j) ? x[j] * pbuf[j * 64 + lane] : 0.f;
+          for (int j = 0; j < 16; ++j) {
+            const float ds = x[j] * pbuf[j * 64 + lane];
+            x[j] = ok(j) ? ds : 0.f;
+          }
         } else {
 #pragma unroll
           for (int j = 0; j < 16; ++j) x[j] *= pbuf[j * 64 + lane];
@@ -587,34 +603,36 @@ __global__ __launch_bounds__(256, occ_pair<HD>()) void k_win_dkv(WinArgs a) {
     __syncthreads();
   }
   float* buf = (wv < 2 ? Qs[wv] : Gs[wv - 2]);
-  if (sunk && a.nslice > 1) {
-    const int64_t rows = (int64_t)a.nsb * PROWS;
-    const int64_t all = a.nbkv * rows * a.D;
-    float* to = a.sums + (role == 0 ? a.nslice * all : 0) + slice * all + bkv * rows * a.D;
-    write_rows<HD>(buf, acc, role == 0 ? 1.0f : a.scale, to, a.D, k0, a.Tk, a.D, l32, h, lane);
-  } else if (role == 0) {
-    write_rows<HD>(buf, acc, 1.0f, a.out2 + b * a.o2s.b + kh * a.o2s.h, a.o2s.t, k0, a.Tk, a.D, l32,
-                   h, lane);
+  const float mul = role == 0 ? 1.0f : a.scale;
+  if (slices > 1) {  // rows of `sums`: the sinks' blocks, then the others
+    const int64_t rows = (int64_t)(sunk ? a.nsb : a.nblk - a.nsb) * PROWS;
+    float* to = a.sums + (sunk ? 0 : sums_at(a)) +
+                (((int64_t)(role == 0 ? slices : 0) + slice) * a.nbkv + bkv) * rows * a.D;
+    write_rows<HD>(buf, acc, mul, to - (sunk ? 0 : (int64_t)a.nsb * PROWS * a.D), a.D, k0, a.Tk,
+                   a.D, l32, h, lane);
   } else {
-    write_rows<HD>(buf, acc, a.scale, a.out + b * a.o1s.b + kh * a.o1s.h, a.o1s.t, k0, a.Tk, a.D,
-                   l32, h, lane);
+    const Strides3& st = role == 0 ? a.o2s : a.o1s;
+    write_rows<HD>(buf, acc, mul, (role == 0 ? a.out2 : a.out) + b * st.b + kh * st.h, st.t, k0,
+                   a.Tk, a.D, l32, h, lane);
   }
 }
 
-// dK and dV of the key blocks with sinks: the slices' sums, in order.
-__global__ __launch_bounds__(256) void k_win_sums(WinArgs a, int64_t n4) {
+// dK and dV of the key blocks whose steps were cut into slices: the slices'
+// sums, in order.  Blocks [blk0, blk0 + nb) and their part of `sums`.
+__global__ __launch_bounds__(256) void k_win_sums(WinArgs a, const float* __restrict__ sums,
+                                                  int blk0, int nb, int slices, int64_t n4) {
   int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= 2 * n4) return;
   const bool v = i >= n4;
-  const int64_t rows = (int64_t)a.nsb * PROWS, all = a.nbkv * rows * a.D;
-  const float* src = a.sums + (v ? a.nslice * all : 0);
+  const int64_t rows = (int64_t)nb * PROWS, all = a.nbkv * rows * a.D;
+  const float* src = sums + (v ? slices * all : 0);
   if (v) i -= n4;
   const int d4 = a.D / 4;
-  const int64_t row = i / d4, bkv = row / rows, key = row - bkv * rows;
+  const int64_t row = i / d4, bkv = row / rows, key = row - bkv * rows + (int64_t)blk0 * PROWS;
   const int c = 4 * (int)(i - row * d4);
   if (key >= a.Tk) return;
   floatx4 x = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < a.nslice; ++s)
+  for (int s = 0; s < slices; ++s)
     x += *reinterpret_cast<const floatx4*>(src + s * all + row * a.D + c);
   const int hkv = a.H / a.G;
   const int64_t b = (a.bkv0 + bkv) / hkv, kh = (a.bkv0 + bkv) % hkv;
@@ -707,9 +725,12 @@ int launch_bwd(WinArgs a, unsigned keys, float* dq, const int64_t* dq_st) {
     tjh_launch(k_win_dkv<HD, false, HD / 2>, dim3(keys), dim3(256), 0, stream(), a);
   int rc = check_launch("window_dkv");
   if (rc != TJH_OK) return rc;
-  if (a.nslice > 1) {
-    const int64_t n4 = (int64_t)a.nbkv * a.nsb * PROWS * a.D / 4;
-    tjh_launch(k_win_sums, dim3((unsigned)cdiv(2 * n4, 256)), dim3(256), 0, stream(), a, n4);
+  for (int sunk = 0; sunk < 2; ++sunk) {
+    const int nb = sunk ? a.nsb : a.nblk - a.nsb, slices = sunk ? a.nslice : a.nsplit;
+    if (slices < 2 || nb == 0) continue;
+    const int64_t n4 = (int64_t)a.nbkv * nb * PROWS * a.D / 4;
+    tjh_launch(k_win_sums, dim3((unsigned)cdiv(2 * n4, 256)), dim3(256), 0, stream(), a,
+               (const float*)(a.sums + (sunk ? 0 : sums_at(a))), sunk ? 0 : a.nsb, nb, slices, n4);
     if ((rc = check_launch("window_sums")) != TJH_OK) return rc;
   }
   a.nblk = (int)cdiv(a.Tq, ROWS);
@@ -718,6 +739,28 @@ int launch_bwd(WinArgs a, unsigned keys, float* dq, const int64_t* dq_st) {
   const unsigned grid = (unsigned)(a.nbkv * a.G * a.nblk);
   tjh_launch(k_win_dq<HD>, dim3(grid), dim3(256), 0, stream(), a);
   return check_launch("window_dq");
+}
+
+// Over how many workgroups the query heads of a key block are split: all
+// workgroups are about as long as each other, so the last of the rounds that
+// they fill the CUs in may be nearly empty.  Each split costs a prologue of
+// some 3 steps and the sums' way through memory (2 steps a split: dK and dV
+// written and read).  4 key heads of 8192, 4 query heads each, are 540
+// workgroups of 140 steps on 512 places: two rounds, 1780 us; as four splits
+// five rounds of 35 steps, measured below.
+int key_splits(const WinArgs& a, int64_t nbkv, int64_t tiles) {
+  const int64_t cus = num_cus() > 0 ? num_cus() : 256, places = cus * (a.D <= 64 ? 3 : 2);
+  int best = 1;
+  int64_t cost = 0;
+  for (int n = 1; n <= a.G && n <= 8; ++n) {
+    const int64_t each = cdiv(tiles * a.G, n);
+    const int64_t c = cdiv(nbkv * a.nblk * n, places) * (each + 3) + (n > 1 ? 2 * n : 0);
+    if (n == 1 || c < cost) {
+      cost = c;
+      best = n;
+    }
+  }
+  return best;
 }
 
 int check_window(const char* who, int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk,
@@ -859,19 +902,26 @@ int tjh_window_backward(const float* q, const float* k, const float* v, const fl
   a.nsl = (int)(a.nst + (wt < a.nkt ? wt : a.nkt));
   a.nblk = (int)cdiv(Tk, PROWS);
   a.nsb = (int)cdiv(a.sinks, PROWS);
-  // slices of the sinks' blocks about as long as the others' query tiles
-  const int64_t others = cdiv((int64_t)a.win + PROWS, TILE) + 1;
-  a.nslice = a.nsb ? (int)cdiv(a.nqt, others < 8 ? 8 : others) : 1;
+  // steps (32 queries of a head) of a key block without sinks, at most
+  const int64_t tiles = cdiv((int64_t)a.win + PROWS, TILE) + 1;
+  const int64_t tq = tiles < a.nqt ? tiles : a.nqt;
   // key heads at once: the dS blocks of all of them up to 4 GiB
   const int64_t nbkv = B * Hkv;
   const size_t per = (size_t)a.G * a.nqt * a.nsl * (TILE * TILE) * sizeof(float);
   int64_t chunk = (int64_t)((size_t(4) << 30) / per);
   chunk = chunk < 1 ? 1 : chunk > nbkv ? nbkv : chunk;
   for (;;) {
+    a.nsplit = key_splits(a, chunk, tq);
+    // slices of the sinks' blocks about as long as the others' steps
+    const int64_t each = cdiv(tq * a.G, a.nsplit);
+    a.nslice = a.nsb ? (int)cdiv((int64_t)a.nqt * a.G, each < 8 ? 8 : each) : 1;
+    a.nbkv = (int)chunk;
+    const int64_t rest = a.nsplit > 1
+                             ? (int64_t)2 * a.nsplit * chunk * (a.nblk - a.nsb) * PROWS * D : 0;
+    const size_t room = (size_t)(sums_at(a) + rest) * sizeof(float);
     Scratch blocks(per * chunk);
-    Scratch sums(a.nslice > 1
-                     ? (size_t)2 * a.nslice * chunk * a.nsb * PROWS * D * sizeof(float) : 0);
-    if (!blocks.ok() || (a.nslice > 1 && !sums.ok())) {
+    Scratch sums(room);
+    if (!blocks.ok() || (room && !sums.ok())) {
       if (chunk == 1) return set_error(TJH_ERR_OOM, "tjh_window_backward: no scratch");
       chunk = cdiv(chunk, 2);
       continue;
@@ -881,7 +931,8 @@ int tjh_window_backward(const float* q, const float* k, const float* v, const fl
     for (int64_t at = 0; at < nbkv; at += chunk) {
       a.bkv0 = (int)at;
       a.nbkv = (int)(nbkv - at < chunk ? nbkv - at : chunk);
-      const int64_t keys = (int64_t)a.nbkv * (a.nsb * a.nslice + a.nblk - a.nsb);
+      const int64_t keys =
+          (int64_t)a.nbkv * (a.nsb * a.nslice + (a.nblk - a.nsb) * (int64_t)a.nsplit);
       TJH_ARG(keys < (int64_t(1) << 31), "tjh_window_backward: grid too large");
       switch (cdiv(D, 32)) {
         case 1: rc = launch_bwd<32>(a, (unsigned)keys, dq, strides[5]); break;
