@@ -741,20 +741,19 @@ int launch_bwd(WinArgs a, unsigned keys, float* dq, const int64_t* dq_st) {
   return check_launch("window_dq");
 }
 
-// Over how many workgroups the query heads of a key block are split: all
-// workgroups are about as long as each other, so the last of the rounds that
-// they fill the CUs in may be nearly empty.  Each split costs a prologue of
-// some 3 steps and the sums' way through memory (2 steps a split: dK and dV
-// written and read).  4 key heads of 8192, 4 query heads each, are 540
-// workgroups of 140 steps on 512 places: two rounds, 1780 us; as four splits
-// five rounds of 35 steps, measured below.
+// Over how many workgroups the query heads of a key block are split.  The
+// workgroups are about equally long, so the last round that they fill the CUs
+// in stands half empty on average; each split costs a prologue of some 3
+// steps, and its sums' way through memory about 2.  4 key heads of 8192, 4
+// query heads each (508 workgroups of 140 steps on 512 places): 1424 us, as
+// two splits 1315, as four 1292.
 int key_splits(const WinArgs& a, int64_t nbkv, int64_t tiles) {
   const int64_t cus = num_cus() > 0 ? num_cus() : 256, places = cus * (a.D <= 64 ? 3 : 2);
   int best = 1;
   int64_t cost = 0;
   for (int n = 1; n <= a.G && n <= 8; ++n) {
-    const int64_t each = cdiv(tiles * a.G, n);
-    const int64_t c = cdiv(nbkv * a.nblk * n, places) * (each + 3) + (n > 1 ? 2 * n : 0);
+    const int64_t each = cdiv(tiles * a.G, n) + 3;
+    const int64_t c = 2 * nbkv * a.nblk * n * each / places + each + (n > 1 ? 4 * n : 0);
     if (n == 1 || c < cost) {
       cost = c;
       best = n;

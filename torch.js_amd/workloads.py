@@ -49,9 +49,14 @@ class CNN(nn.Module):
 
 
 class CausalSelfAttention(nn.Module):
-    def __init__(self, d, heads, fused=True):
+    """With `window`, each position sees the last `window` positions and the
+    first `sinks` ones (F.sliding_window_attention) in place of all earlier
+    ones."""
+
+    def __init__(self, d, heads, fused=True, window=None, sinks=0):
         super().__init__()
         self.d, self.heads, self.fused = d, heads, fused
+        self.window, self.sinks = window, sinks
         self.c_attn = nn.Linear(d, 3 * d)
         self.c_proj = nn.Linear(d, d)
 
@@ -65,7 +70,10 @@ class CausalSelfAttention(nn.Module):
         q = q.view(B, T, self.heads, hd).transpose(1, 2)
         k = k.view(B, T, self.heads, hd).transpose(1, 2)
         v = v.view(B, T, self.heads, hd).transpose(1, 2)
-        y = F.scaled_dot_product_attention(q, k, v, is_causal=True)
+        if self.window is None:
+            y = F.scaled_dot_product_attention(q, k, v, is_causal=True)
+        else:
+            y = F.sliding_window_attention(q, k, v, self.window, self.sinks)
         y = y.transpose(1, 2).contiguous().view(B, T, C)
         return self._project(y, residual)
 
@@ -74,7 +82,7 @@ class CausalSelfAttention(nn.Module):
         cached keys / values of positions [0, pos) plus their own; the new
         keys and values are appended to the cache.  A prompt (pos 0) is
         causal over itself; a single new token attends to every cached
-        position."""
+        position.  With a window, a prompt may also come in parts."""
         B, T, C = x.shape
         hd = C // self.heads
         q, k, v = self.c_attn(x).split(C, dim=2)
@@ -82,7 +90,9 @@ class CausalSelfAttention(nn.Module):
         k = k.view(B, T, self.heads, hd).transpose(1, 2)
         v = v.view(B, T, self.heads, hd).transpose(1, 2)
         keys, values = cache.append(layer, k, v, pos)
-        if pos == 0:
+        if self.window is not None:
+            y = F.sliding_window_attention(q, keys, values, self.window, self.sinks)
+        elif pos == 0:
             y = F.scaled_dot_product_attention(q, keys, values, is_causal=True)
         elif T == 1:
             y = F.scaled_dot_product_attention(q, keys, values, is_causal=False)
@@ -122,10 +132,10 @@ class Block(nn.Module):
     would; fused=True routes the GELU and the residual adds through the
     GEMM epilogues (the same values, bit for bit)."""
 
-    def __init__(self, d, heads, fused=True):
+    def __init__(self, d, heads, fused=True, window=None, sinks=0):
         super().__init__()
         self.ln_1 = nn.LayerNorm(d)
-        self.attn = CausalSelfAttention(d, heads, fused)
+        self.attn = CausalSelfAttention(d, heads, fused, window, sinks)
         self.ln_2 = nn.LayerNorm(d)
         self.mlp = MLPBlock(d, fused)
 
@@ -144,7 +154,8 @@ class Block(nn.Module):
         graph is recorded and the block is made of the plain layers in
         float32; None anywhere else."""
         at, mlp = self.attn, self.mlp
-        if type(at) is not CausalSelfAttention or type(mlp) is not MLPBlock:
+        if type(at) is not CausalSelfAttention or type(mlp) is not MLPBlock or \
+                at.window is not None:
             return None
         mods = (self.ln_1, at, at.c_attn, at.c_proj, self.ln_2, mlp, mlp.c_fc, mlp.c_proj)
         if not (tuple(map(type, mods)) == _BLOCK_MODULES and at.fused and mlp.fused and
@@ -239,15 +250,17 @@ class KVCache:
 
 
 class GPT2(nn.Module):
-    """GPT-2 with the LM head tied to the token embedding."""
+    """GPT-2 with the LM head tied to the token embedding; with `window` and
+    `sinks`, attention over a sliding window (CausalSelfAttention)."""
 
-    def __init__(self, vocab=50257, ctx=1024, d=768, heads=12, layers=12, fused=True):
+    def __init__(self, vocab=50257, ctx=1024, d=768, heads=12, layers=12, fused=True, window=None,
+                 sinks=0):
         super().__init__()
         self.vocab, self.ctx = vocab, ctx
         self.fused = fused
         self.wte = nn.Embedding(vocab, d)
         self.wpe = nn.Embedding(ctx, d)
-        self.h = nn.ModuleList([Block(d, heads, fused) for _ in range(layers)])
+        self.h = nn.ModuleList([Block(d, heads, fused, window, sinks) for _ in range(layers)])
         self.ln_f = nn.LayerNorm(d)
 
     def forward(self, ids):
@@ -269,6 +282,11 @@ class GPT2(nn.Module):
         logits = self(ids)
         return F.cross_entropy(logits.view(-1, self.vocab), targets.reshape(-1))
 
+    def distillation_loss(self, ids, teacher_logits, teacher_ids, temperature=1.0):
+        """F.distillation_loss of this model's logits for ids [B, T] against a
+        teacher's largest ones [B, T, K] (`teacher(ids).topk(K)`)."""
+        return F.distillation_loss(self(ids), teacher_logits, teacher_ids, temperature)
+
     def new_cache(self, batch, max_len=None):
         blk = self.h[0].attn
         return KVCache(len(self.h), batch, blk.heads, max_len or self.ctx, blk.d // blk.heads)
@@ -283,17 +301,22 @@ class GPT2(nn.Module):
         x = self.ln_f(x)
         return F.linear(x, self.wte.weight)
 
-    def generate(self, ids, max_new_tokens, temperature=1.0, greedy=False):
+    def generate(self, ids, max_new_tokens, temperature=1.0, greedy=False, top_k=0, top_p=1.0,
+                 min_p=0.0):
         """Autoregressive decoding with a KV cache (the inference side of the
         GPT-2 path, tests/gpt2.test.ts): the prompt runs once, then each
         new token is one cached step; the next token is drawn by
         multinomial from softmax(logits / temperature) (or argmax when
-        greedy).  Returns the [B, T + max_new_tokens] int32 ids."""
+        greedy).  With top_k, top_p or min_p it is drawn by F.sample_logits
+        from the logits, without a readback in the loop; logits without a
+        distribution (NaN) raise at the end.  Returns the
+        [B, T + max_new_tokens] int32 ids."""
         from .tensor import cat
         B, T = ids.shape
         total = T + max_new_tokens
         if total > self.ctx:
             raise ValueError("generate: %d positions exceed the context of %d" % (total, self.ctx))
+        cut = top_k != 0 or top_p != 1.0 or min_p != 0.0
         with no_grad():
             cache = self.new_cache(B, total)
             logits = self.forward_cached(ids, cache, 0)
@@ -303,13 +326,18 @@ class GPT2(nn.Module):
                 last = logits[:, -1, :]
                 if greedy:
                     nxt = last.argmax(-1, keepdim=True)
+                elif cut:
+                    nxt = F.sample_logits(last, None, temperature, top_k, top_p, min_p).view(B, 1)
                 else:
                     probs = F.softmax(last * (1.0 / temperature), -1)
                     nxt = probs.multinomial(1)
                 out.append(nxt)
                 logits = self.forward_cached(nxt, cache, pos)
                 pos += 1
-            return cat(out, 1)
+            res = cat(out, 1)
+            if cut and not greedy and (res.numpy() < 0).any():
+                raise RuntimeError("generate: logits hold NaN, infinity or nothing to draw")
+            return res
 
 
 def load_params(model, params):
