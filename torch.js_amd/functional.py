@@ -909,19 +909,26 @@ def _grad_like(t):
     return _alias(empty((B, T, H, D)), t.shape, (T * H * D, D, H * D, 1), 0)
 
 
+@functools.lru_cache(maxsize=1024)
+def _dense(shape, strides):
+    """Whether a [B, H, T, D] layout is some order of the axes without gaps,
+    its last one dense."""
+    run = 1
+    for s, n in sorted(zip(strides, shape)):
+        if n > 1:
+            if s != run:
+                return False
+            run *= n
+    return shape[3] <= 1 or strides[3] == 1
+
+
 def _grad_as(t):
     """A gradient buffer laid out as a dense operand itself (a leaf's gradient
     is then the buffer), as _grad_like where the operand's memory has gaps
     or rows that the kernels do not take."""
-    run = 1
-    for s, n in sorted(zip(t._strides, t.shape)):
-        if n > 1:
-            if s != run:
-                return _grad_like(t)
-            run *= n
-    if t.shape[3] > 1 and t._strides[3] != 1:
+    if not _dense(t._shape, t._strides):
         return _grad_like(t)
-    return _alias(empty((max(run, 1),)), t.shape, t._strides, 0)
+    return Tensor(empty(t._shape)._st, t._shape, t._strides)
 
 
 def _shared_grads(q, k, v):
@@ -1066,6 +1073,14 @@ def _strides3(st):
     return L.i64arr(st[:3])
 
 
+@functools.lru_cache(maxsize=1024)
+def _strides8(sts):
+    """Eight tensors' first three strides for tjh_window_backward, and the
+    arrays that they stand in."""
+    arrs = [_strides3(st) for st in sts]
+    return (L.P_i64 * 8)(*[ctypes.cast(a, L.P_i64) for a in arrs]), arrs
+
+
 def sliding_window_attention(query, key, value, window, sinks=0, scale=None):
     """Causal attention over a sliding window, with a few first tokens that
     stay visible (beside scaled_dot_product_attention,
@@ -1131,8 +1146,7 @@ def sliding_window_attention(query, key, value, window, sinks=0, scale=None):
             return [zeros(s) for s in (qs, ks, ks)]
         shared = _shared_grads(q, k, v)
         dq, dk, dv = shared if shared else (_grad_as(q), _grad_as(k), _grad_as(v))
-        arrs = [_strides3(t._strides) for t in (q, k, v, o, g, dq, dk, dv)]
-        ptrs = (L.P_i64 * 8)(*[ctypes.cast(a, L.P_i64) for a in arrs])
+        ptrs, _ = _strides8(tuple(t._strides for t in (q, k, v, o, g, dq, dk, dv)))
         L.check(L.lib().tjh_window_backward(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), g.data_ptr(), lse.data_ptr(),
             dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, H, Hkv, Tq, Tk, D, ptrs, sc, window,
