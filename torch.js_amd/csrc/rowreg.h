@@ -224,10 +224,10 @@ struct SelectLds {
   u64 sm[2 * (T / 64)];
 };
 
-// Sorts list[0, c) descending, c <= 256: each thread counts the items above
-// one of them (c * c / T comparisons, four barriers).
+// list[0, c) in descending order in s.sorted, c <= 256: each thread counts the
+// items above one of them (c * c / T comparisons, three barriers).
 template <int T, int CAP>
-__device__ __forceinline__ void sort_short(u64* list, int c, SelectLds<T, CAP>& s) {
+__device__ __forceinline__ void sort_short(const u64* list, int c, SelectLds<T, CAP>& s) {
   int pad = 64;
   while (pad < c) pad <<= 1;
   for (int i = threadIdx.x; i < c; i += T) s.rank[i] = 0;
@@ -252,18 +252,16 @@ __device__ __forceinline__ void sort_short(u64* list, int c, SelectLds<T, CAP>& 
   __syncthreads();
   for (int i = threadIdx.x; i < c; i += T) s.sorted[s.rank[i]] = list[i];
   __syncthreads();
-  for (int i = threadIdx.x; i < c; i += T) list[i] = s.sorted[i];
-  __syncthreads();
 }
 
-// Sorts s.list[0, c) descending.  Over 256 items a bitonic network over the
-// next power of two, padded with zeros, which no real item is below
-// (c log^2 c / 4 T exchanges, log^2 c / 2 barriers).
+// s.list[0, c) in descending order: where it stands.  Over 256 items a bitonic
+// network in place over the next power of two, padded with zeros, which no
+// real item is below (c log^2 c / 4 T exchanges, log^2 c / 2 barriers).
 template <int T, int CAP>
-__device__ __forceinline__ void sort_list(SelectLds<T, CAP>& s, int c) {
+__device__ __forceinline__ u64* sort_list(SelectLds<T, CAP>& s, int c) {
   if (c <= kRank) {
     sort_short(s.list, c, s);
-    return;
+    return s.sorted;
   }
   int p = 2 * kRank;
   while (p < c) p <<= 1;  // <= CAP, a power of two
@@ -283,6 +281,7 @@ __device__ __forceinline__ void sort_list(SelectLds<T, CAP>& s, int c) {
       __syncthreads();
     }
   }
+  return s.list;
 }
 
 // The elements for which in(j, u, x) holds into the list, in no order (it is
@@ -427,11 +426,12 @@ __device__ __forceinline__ float kth_bound(const Row<T, NV>& row, int k, Block<T
   return lo > 0x007fffffu ? key_value(lo) : -INFINITY;  // 0x007fffff: the key of -infinity
 }
 
-// Sorts the row's k largest elements into list[0, k), 1 <= k <= min(n, CAP).
+// The row's k largest elements in order, 1 <= k <= min(n, CAP): where they
+// stand.
 // Where more than CAP elements are above the bound (ties), the exact one
 // comes from bisection.
 template <int T, int NV, int CAP>
-__device__ __forceinline__ void select_largest(const Row<T, NV>& row, int k, uint32_t nan,
+__device__ __forceinline__ u64* select_largest(const Row<T, NV>& row, int k, uint32_t nan,
                                                SelectLds<T, CAP>& s, Block<T>& b) {
   const int c = gather_above<true>(row, nan, kth_bound(row, k, b), s, b);
   if (c > CAP) {
@@ -445,7 +445,7 @@ __device__ __forceinline__ void select_largest(const Row<T, NV>& row, int k, uin
         },
         s);
   }
-  sort_list(s, c > CAP ? k : c);
+  return sort_list(s, c > CAP ? k : c);
 }
 
 }  // namespace rowreg

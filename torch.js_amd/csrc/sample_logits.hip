@@ -21,7 +21,7 @@
 // would move one draw in some thousand over a border between two indices.
 //
 // One workgroup has a row, in registers (rowreg.h).  Wherever the elements
-// that can be drawn fit (4096), they are moved into LDS and everything else
+// that can be drawn fit (8192), they are moved into LDS and everything else
 // happens on that list: the top_k largest; the elements above min_p's bound;
 // the nucleus, which ends in a bin of a histogram of the weights over x (one
 // pass in which every element's weight is formed).  Only the nucleus's last
@@ -39,7 +39,7 @@ namespace {
 
 using namespace rowreg;
 
-constexpr int kCap = 4096;    // elements of a list
+constexpr int kCap = 8192;    // elements of a list
 constexpr int kMostK = 1024;  // top_k that is selected by the threads' maxima
 constexpr int kBins = 2048;   // of the nucleus's histogram
 constexpr int64_t kMaxCols = int64_t(1) << 20;
@@ -204,6 +204,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
   };
   float per = 0.f;
   int last = -1;
+  u64 above = 0;  // weight of the bins before `last`
   if (largest) {
     bound = kth_bound(row, (int)top_k, b);
   } else if (use_p) {
@@ -234,19 +235,29 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
     }
     if (t == 0) lds.pick = -1;
     __syncthreads();
-    u64 run = 0;
-    for (int i = t; i < kBins; i += T) run += lds.bins[i];
-    limit = p * (double)b.sum64(run);
     // the last bin before which less than the limit lies
-    run = 0;
-    for (int i0 = 0; i0 < kBins; i0 += T) {
-      const u64 w = lds.bins[i0 + t];
-      u64 part;
-      const u64 before = run + b.before(w, &part);
-      if (w && (double)before < limit) atomicMax(&lds.pick, i0 + t);
-      run += part;
+    constexpr int kEach = (kBins + T - 1) / T;
+    u64 mine = 0, all;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) mine += lds.bins[t * kEach + i];
+    above = b.before(mine, &all);
+    limit = p * (double)all;
+    int found = -1;
+    u64 before = above;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const u64 w = lds.bins[t * kEach + i];
+      if (w && (double)before < limit) {
+        found = t * kEach + i;
+        above = before;
+      }
+      before += w;
     }
+    if (found >= 0) atomicMax(&lds.pick, found);
     __syncthreads();
+    if (lds.pick == found) lds.first = above;  // one thread: the bins are its own
+    __syncthreads();
+    above = lds.first;
     last = lds.pick;
     // elements of later bins that are not below it do no harm
     if (last < kBins - 1) bound = float_below(m - (last + 1.01) / per);
@@ -254,6 +265,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
     bound = float_below(m + floor_z);
   }
   int c = -1;  // elements of the list, if there is one
+  const u64* list = s.list;
   if (largest || bound > -INFINITY) {
     c = use_p && !largest ? gather_above<false>(row, kNanFirst, bound, s, b)
                           : gather_above<true>(row, kNanFirst, bound, s, b);
@@ -270,13 +282,10 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
           s);
       c = (int)top_k;
     }
-    sort_list(s, c);
+    list = sort_list(s, c);
     c = (int)top_k;
   } else if (use_p) {
     // the nucleus ends in bin `last`: (tx, ti) from that bin's elements
-    u64 run = 0;
-    for (int i = t; i < last; i += T) run += lds.bins[i];
-    const u64 above = b.sum64(run);
     if (t == 0) s.count = 0;
     __syncthreads();
     for (int i = t; i < c; i += T) {
@@ -289,9 +298,9 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
     }
     __syncthreads();
     int in = s.count;
-    u64* part = lds.few;
+    const u64* part = s.sorted;
     if (c >= 0 && in <= kRank) {
-      sort_short(part, in, s);
+      sort_short(lds.few, in, s);
     } else {
       c = -1;  // no list: the bin alone
       Row<T, 0> again;
@@ -302,8 +311,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
             return bin_of(per, x) == last && x > -INFINITY && in_order(again, j, e, x);
           },
           s);
-      part = s.list;
-      if (in <= kCap) sort_list(s, in);
+      if (in <= kCap) part = sort_list(s, in);
     }
     if (in <= kCap) {
       if (t == 0) lds.pick = 0;
@@ -377,7 +385,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
     // the list's weights, none for elements that are not kept
     u64 mine = 0;
     for (int i = t; i < c; i += T) {
-      const u64 e = s.list[i];
+      const u64 e = list[i];
       const float x = key_value((uint32_t)(e >> 32));
       const bool in = largest || ((double)x - m >= floor_z &&
                                   (x > tx || (x == tx && index_of(e) <= ti)));
@@ -398,7 +406,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
         const u64 before = sum + b.before(w, &part);
         sum += part;
         const bool in = i < c && (double)before < limit &&
-                        (double)key_value((uint32_t)(s.list[i] >> 32)) - m >= floor_z;
+                        (double)key_value((uint32_t)(list[i] >> 32)) - m >= floor_z;
         kept += in;
         mine_kept += in ? w : 0;
       }
@@ -407,12 +415,11 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
     }
     const double target = u * (double)all;
     u64 sum = 0;  // weight of the indices before the ones looked into
-    u64* part = s.list;
     int in = keep;
     if (keep > kRank) {
       // by parts of the index range: the first with the target, or, where u
       // is 1 or more, the last of any weight
-      constexpr int kParts = 1024;
+      constexpr int kParts = 1024, kEach = (kParts + T - 1) / T;
       const int shift = max(0, 32 - __clz(n - 1) - 10);  // 2^10 parts
       __syncthreads();
       for (int i = t; i < kParts; i += T) lds.bins[i] = 0;
@@ -422,18 +429,26 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
       }
       __syncthreads();
       for (int i = t; i < keep; i += T)
-        if (lds.w[i]) atomicAdd(&lds.bins[index_of(s.list[i]) >> shift], lds.w[i]);
+        if (lds.w[i]) atomicAdd(&lds.bins[index_of(list[i]) >> shift], lds.w[i]);
       __syncthreads();
-      u64 run = 0;
-      int end = -1;
-      for (int i0 = 0; i0 < kParts; i0 += T) {
-        const u64 w = lds.bins[i0 + t];
-        u64 here;
-        const u64 before = run + b.before(w, &here);
-        if (w && (double)(before + w) > target) atomicMin(&lds.pick, i0 + t);
-        if (w) end = i0 + t;
-        run += here;
+      u64 own = 0, total;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (T <= kParts || t < kParts) own += lds.bins[t * kEach + i];
+      u64 before = b.before(own, &total);
+      int first = kNone, end = -1;
+      u64 start = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const u64 w = lds.bins[t * kEach + i];
+        if (w && first == kNone && (double)(before + w) > target) {
+          first = t * kEach + i;
+          start = before;
+        }
+        if (w) end = t * kEach + i;
+        before += w;
       }
+      if (first != kNone) atomicMin(&lds.pick, first);
       __syncthreads();
       int at = lds.pick;
       if (at == kNone) {
@@ -443,30 +458,29 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
         atomicMax(&lds.pick, end);
         __syncthreads();
         at = lds.pick;
+        if (end == at) lds.first = total - lds.bins[at];
+      } else if (first == at) {
+        lds.first = start;
       }
-      run = 0;
-      for (int i = t; i < at; i += T) run += lds.bins[i];
-      sum = b.sum64(run);
       for (int i = t; i < keep; i += T)
-        if (lds.w[i] && index_of(s.list[i]) >> shift == at) {
+        if (lds.w[i] && index_of(list[i]) >> shift == at) {
           const int put = atomicAdd(&s.count, 1);
-          if (put < kRank) lds.few[put] = (s.list[i] << 32) | (uint32_t)i;
+          if (put < kRank) lds.few[put] = (list[i] << 32) | (uint32_t)i;
         }
       __syncthreads();
+      sum = lds.first;
       in = s.count;
-      part = lds.few;
     } else {
-      __syncthreads();
-      for (int i = t; i < keep; i += T) s.list[i] = (s.list[i] << 32) | (uint32_t)i;
+      for (int i = t; i < keep; i += T) lds.few[i] = (list[i] << 32) | (uint32_t)i;
     }
     if (in <= kRank) {
       // (index, place in the list), in ascending order of the index
       if (t == 0) lds.pick = kNone;
-      sort_short(part, in, s);
+      sort_short(lds.few, in, s);
       int end = -1;
       for (int i0 = 0; i0 < in; i0 += T) {
         const int i = i0 + t;
-        const u64 w = i < in ? lds.w[(uint32_t)part[i]] : 0;
+        const u64 w = i < in ? lds.w[(uint32_t)s.sorted[i]] : 0;
         u64 here;
         const u64 before = sum + b.before(w, &here);
         sum += here;
@@ -483,12 +497,12 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
         __syncthreads();
         at = lds.pick;
       }
-      if (t == 0) a.out[r] = (int)~(uint32_t)(part[at] >> 32);
+      if (t == 0) a.out[r] = (int)~(uint32_t)(s.sorted[at] >> 32);
       return;
     }
     // more than 256 in one part: the pass over the row, down to the last kept
     if (largest) {
-      const u64 e = s.list[keep - 1];
+      const u64 e = list[keep - 1];
       tx = key_value((uint32_t)(e >> 32));
       ti = index_of(e);
     }

@@ -25,9 +25,9 @@ __global__ __launch_bounds__(T, T == 512 ? 4 : 1) void k_topk(const float* __res
   Block<T> b(s.sm);
   Row<T, NV> row;
   row.load(x + r * ld, n, largest ? 0u : 0x80000000u);
-  select_largest(row, k, largest ? kNanFirst : kNanLast, s, b);
+  const u64* best = select_largest(row, k, largest ? kNanFirst : kNanLast, s, b);
   for (int i = threadIdx.x; i < k; i += T) {
-    const int at = index_of(s.list[i]);
+    const int at = index_of(best[i]);
     indices[r * k + i] = at;
     values[r * k + i] = row.p[at];
   }

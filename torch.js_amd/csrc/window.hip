@@ -300,20 +300,36 @@ __global__ __launch_bounds__(256) void k_win_merge(WinArgs a, int64_t n4, int ns
     const Tiles tiles(a, lo, min(lo + TILE, a.Tk) - 1);
     n = (tiles.n + a.kslice - 1) / a.kslice;
   }
-  float top = -INFINITY;
-  for (int s = 0; s < n; ++s) top = fmaxf(top, a.pml[s * rows + row].x);
-  const float ts = top == -INFINITY ? 0.f : top;
+  // eight slices at a time, their loads together: they come from other XCDs
   floatx4 o = {0.f, 0.f, 0.f, 0.f};
-  float den = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < n; ++s) {
-    const float2 ml = a.pml[s * rows + row];
-    const float f = exp2_hw(ml.x - ts);
-    den = __builtin_fmaf(ml.y, f, den);
-    const floatx4 x = *reinterpret_cast<const floatx4*>(a.part + (s * rows + row) * a.D + 4 * c);
-    // a slice that this query sees nothing of has sums of 0 and a factor of
-    // 0, and infinities of other slices stay what they are
-    if (f != 0.f) o += f * x;
+  float top = -INFINITY, den = 0.f;
+  for (int s0 = 0; s0 < n; s0 += 8) {
+    float2 ml[8];
+    floatx4 x[8];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const int64_t at = min(s0 + s, n - 1) * rows + row;  // past the end: not used
+      ml[s] = a.pml[at];
+      x[s] = *reinterpret_cast<const floatx4*>(a.part + at * a.D + 4 * c);
+    }
+    float m = top;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) m = fmaxf(m, ml[s].x);
+    const float ms = m == -INFINITY ? 0.f : m;
+    const float alpha = exp2_hw(top - ms);
+    top = m;
+    den *= alpha;
+    o *= alpha;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const float f = s0 + s < n ? exp2_hw(ml[s].x - ms) : 0.f;
+      // a slice that this query sees nothing of has sums of 0 and a factor of
+      // 0, and infinities of other slices stay what they are
+      if (f != 0.f) {
+        den = __builtin_fmaf(ml[s].y, f, den);
+        o += f * x[s];
+      }
+    }
   }
   const int64_t b = bh / a.H, h = bh % a.H;
   *reinterpret_cast<floatx4*>(a.out + b * a.os.b + h * a.os.h + q * a.os.t + 4 * c) =
