@@ -282,6 +282,35 @@ def test_sample_logits_settings_of_each_row(torch, n):
 
 
 @gpu
+@pytest.mark.parametrize("n", [50257, 60001])
+def test_sample_logits_nucleus_in_one_bin(torch, n):
+    """One far outlier below: the whole nucleus falls into one bin of the
+    histogram, more different logits than a list holds."""
+    rng = np.random.default_rng(n)
+    x = (rng.standard_normal((3, n)) * 1e-4).astype(np.float32)
+    x[0, 5], x[1, n - 1], x[2, n // 2] = -100, -100, -np.finfo(np.float32).max
+    u = rng.random(3).astype(np.float32)
+    for kw in (dict(top_p=0.7), dict(top_p=0.05), dict(top_p=0.6, top_k=20000), dict(top_p=0.9, min_p=0.9999)):
+        got = torch.functional.sample_logits(torch.tensor(x), torch.tensor(u), **kw)
+        assert got.numpy().tolist() == [sample_ref(x[r], float(u[r]), **kw) for r in range(3)], kw
+
+
+@gpu
+@pytest.mark.parametrize("n", [9001, 600000, 2 ** 20])
+def test_sample_logits_of_neighbours(torch, n):
+    """All that can be drawn stands side by side."""
+    rng = np.random.default_rng(n)
+    x = np.full((4, n), -8, np.float32) + rng.random((4, n)).astype(np.float32) / 8
+    for r, at in enumerate((0, 5001, n - 2000, n // 2)):
+        x[r, at:at + 2000] = rng.standard_normal(min(2000, n - at)) / 10
+    for kw in (dict(min_p=0.2), dict(top_p=0.6), dict(top_k=900), dict(top_k=1500), dict(top_k=1000, top_p=0.9),
+               dict(top_p=0.8, min_p=0.9)):
+        for u in (rng.random(4).astype(np.float32), np.zeros(4, np.float32), np.ones(4, np.float32)):
+            got = torch.functional.sample_logits(torch.tensor(x), torch.tensor(u), **kw)
+            assert got.numpy().tolist() == [sample_ref(x[r], float(u[r]), **kw) for r in range(4)], (kw, u)
+
+
+@gpu
 def test_sample_logits_layouts_and_frequencies(torch):
     F = torch.functional
     rng = np.random.default_rng(3)
@@ -473,6 +502,58 @@ def test_distillation_shapes_and_differences(torch):
 
 
 @gpu
+@pytest.mark.parametrize("n", [50, 3000, 50257])
+def test_distillation_of_many_rows(torch, n):
+    """The count of rows with entries, where a launch of its own takes it."""
+    rng = np.random.default_rng(n)
+    rows = 1500
+    x, v, ids = _distill_inputs(rng, rows, n, 7)
+    ids[rng.random(rows) < 0.3] = -1
+    _check_distill(torch, x, v, ids, 1.5, "mean")
+
+
+@gpu
+def test_rows_of_a_padded_output(torch):
+    """Logits [B, T, C] whose rows are padded, as a linear layer's output of
+    an odd width, are read where they stand."""
+    F = torch.functional
+    rng = np.random.default_rng(1)
+    b, t, n = 2, 3, 1003
+    w = rng.standard_normal((b, t, n + 5)).astype(np.float32)
+    x = np.ascontiguousarray(w[:, :, :n])
+    _, v, ids = _distill_inputs(rng, b * t, n, 6)
+    v, ids = v.reshape(b, t, 6), ids.reshape(b, t, 6)
+    for pick in (np.s_[:, :], np.s_[:, 1:2], np.s_[1:, :], np.s_[:, 1]):
+        tx, tw = torch.tensor(x, requires_grad=True), torch.tensor(w, requires_grad=True)
+        tv, ti = v[pick], ids[pick]
+        for y in (tx, tw):
+            z = y[:, :, :n][pick]
+            F.distillation_loss(z, torch.tensor(np.ascontiguousarray(tv)), np.ascontiguousarray(ti)).backward()
+        np.testing.assert_allclose(tw.grad.numpy()[:, :, :n], tx.grad.numpy(), rtol=0, atol=60 * U)
+        assert (tw.grad.numpy()[:, :, n:] == 0).all()
+        val, idx = tw.detach()[:, :, :n][pick].topk(5)
+        flat = x[pick].reshape(-1, n)
+        ref = topk_ref(flat, 5)
+        np.testing.assert_array_equal(idx.numpy().reshape(-1, 5), ref)
+        np.testing.assert_array_equal(val.numpy().reshape(-1, 5), np.take_along_axis(flat, ref, 1))
+
+
+@gpu
+def test_topk_of_more_rows_than_a_grid(torch):
+    rng = np.random.default_rng(3)
+    rows = 2 ** 21 + 3
+    x = rng.integers(0, 50, (rows, 5)).astype(np.float32)
+    tx = torch.tensor(x, requires_grad=True)
+    v, i = tx.topk(2)
+    ref = topk_ref(x, 2)
+    np.testing.assert_array_equal(i.numpy(), ref)
+    v.backward(torch.tensor(np.arange(2 * rows, dtype=np.float32).reshape(rows, 2)))
+    want = np.zeros_like(x)
+    np.put_along_axis(want, ref, np.arange(2 * rows, dtype=np.float32).reshape(rows, 2), 1)
+    np.testing.assert_array_equal(tx.grad.numpy(), want)
+
+
+@gpu
 def test_distillation_second_derivative(torch):
     rng = np.random.default_rng(6)
     x, v, ids = _distill_inputs(rng, 3, 9, 4)
@@ -542,6 +623,8 @@ def test_refusals(pkg):
                dict(top_p=-0.1), dict(min_p=2.0), dict(min_p=math.nan)):
         with pytest.raises(ValueError, match="must lie in"):
             F.sample_logits(x, u, **kw)
+    with pytest.raises(ValueError, match="whole number"):
+        F.sample_logits(x, u, top_k=0.5)
     with pytest.raises(ValueError, match="uniforms"):
         F.sample_logits(x, _fake(pkg, 3))
     with pytest.raises(ValueError, match="has shape"):
@@ -579,6 +662,8 @@ def test_refusals_of_the_library(torch):
     assert lib.tjh_topk_forward(p, 1, 2, 2000, 1, 1, p, p) == 1
     assert lib.tjh_topk_forward(None, 2000, 2, 2000, 1, 1, p, p) == 1
     assert lib.tjh_topk_backward(p, p, 2, 5, 6, p) == 1
+    assert lib.tjh_sample_logits(p, 2000, 2 ** 22, 2000, p, None, None, None, None, 1.0, 0, 1.0, 0.0, p) == 1
+    assert lib.tjh_distill(p, 2000, 2 ** 24, 2000, p, p, 1, 1.0, 1, None, p, p, None, 0) == 1
     assert lib.tjh_sample_logits(p, 2000, 2, 2000, None, None, None, None, None, 1.0, 0, 1.0, 0.0, p) == 1
     assert lib.tjh_distill(p, 2000, 2, 2000, p, p, 1, 1.0, 7, None, p, None, None, 0) == 1
     assert lib.tjh_distill(p, 2000, 2, 2000, p, p, 1, 1.0, 0, None, None, None, p, 2000) == 1

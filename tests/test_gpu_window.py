@@ -297,6 +297,100 @@ def test_in_a_graph(torch, tq, tk):
             np.testing.assert_array_equal(a, e.numpy())
 
 
+@gpu
+def test_one_tensor_as_queries_keys_and_values(torch):
+    x, _, _, g = inputs(8, 2, 2, 2, 45, 45, 16)
+    want, bound = reference(x, x, x, 10, 2, g)
+    t = torch.tensor(x, requires_grad=True)
+    for n in (1, 2):  # and a second pass adds to the first one's gradient
+        o = torch.functional.sliding_window_attention(t, t, t, 10, 2)
+        near(o.numpy(), want[0], bound[0], "output")
+        o.backward(torch.tensor(g))
+        # three parts in two additions a pass, each off by half a step of the sum
+        size = n * sum(np.abs(w) for w in want[1:])
+        near(t.grad.numpy(), n * sum(want[1:]), n * sum(bound[1:]) + 3 * n * U * size, "gradient")
+
+
+@gpu
+@pytest.mark.parametrize("row", [2 ** 23 - 8, 2 ** 23])
+def test_rows_far_apart(torch, row):
+    """Offsets past 32 bits, and rows farther apart than the kernels take."""
+    n, d, window, sinks = 300, 8, 40, 3
+    q, k, v, g = (x[0] for x in inputs(9, 1, 2, 2, n, n, d))
+    want, bound = reference(q[None], k[None], v[None], window, sinks, g[None])
+    ts = []
+    for i, x in enumerate((q, k, v)):
+        if i == 1:
+            base = torch.zeros(n, row)
+            y = base[:, 4:4 + 2 * d]
+            y.copy_(torch.tensor(np.ascontiguousarray(x.transpose(1, 0, 2).reshape(n, 2 * d))))
+            y = y.view(n, 2, d).transpose(0, 1)
+            assert y.stride() == (d, row, 1)
+        else:
+            y = torch.tensor(x)
+        ts.append(y.requires_grad_(True))
+    f = torch.functional.sliding_window_attention
+    o = f(*ts, window, sinks)
+    near(o.numpy(), want[0][0], bound[0][0], "output")
+    o.backward(torch.tensor(g))
+    for name, t, w, e in zip(("dq", "dk", "dv"), ts, want[1:], bound[1:]):
+        near(t.grad.numpy(), w[0], e[0], name)
+    o = f(ts[0].detach()[:, -1:], ts[1].detach(), ts[2].detach(), window, sinks)
+    near(o.numpy(), want[0][0][:, -1:], bound[0][0][:, -1:], "last position")
+
+
+@gpu
+@pytest.mark.parametrize("h,hkv", [(260, 260), (320, 160)])
+def test_backward_in_parts_of_the_heads(torch, h, hkv):
+    """More heads than the backward's memory takes at once."""
+    n, d, window, sinks = 2048, 4, 2040, 1
+    q, k, v, g = inputs(10, 1, h, hkv, n, n, d)
+    ts = [torch.tensor(x, requires_grad=True) for x in (q, k, v)]
+    torch.functional.sliding_window_attention(*ts, window, sinks).backward(torch.tensor(g))
+    grads = [t.grad.numpy() for t in ts]
+    grp = h // hkv
+    for kv in (0, hkv // 2, hkv - 1):
+        a, b = slice(kv * grp, (kv + 1) * grp), slice(kv, kv + 1)
+        want, bound = reference(q[:, a], k[:, b], v[:, b], window, sinks, g[:, a])
+        for name, got, w, e in zip(("dq", "dk", "dv"), (grads[0][:, a], grads[1][:, b], grads[2][:, b]),
+                                   want[1:], bound[1:]):
+            near(got, w, e, "%s of key head %d" % (name, kv))
+
+
+@gpu
+def test_graphs_and_eager_work_between(torch):
+    """Two captured graphs and eager calls share the library's workspaces."""
+    f = torch.functional.sliding_window_attention
+    q, k, v, g = inputs(12, 1, 4, 2, 200, 200, 64)
+    hosts = [(q, k, v), tuple(np.ascontiguousarray(x[:, :, ::-1]) for x in (q, k, v))]
+    tg = torch.tensor(g)
+
+    def call(ts):
+        for t in ts:
+            t.grad = None
+        o = f(*ts, 70, 5)
+        o.backward(tg)
+        return [o] + [t.grad for t in ts]
+
+    leaves = [[torch.tensor(x, requires_grad=True) for x in xs] for xs in hosts]
+    want = [[t.numpy().copy() for t in call(ts)] for ts in leaves]
+    long = torch.tensor(np.random.default_rng(1).standard_normal((1, 1, 4000, 64)).astype(np.float32))
+    one = f(long[:, :, -1:], long, long, 4000).numpy()
+    graphs, got = [], []
+    for ts in leaves:
+        graph = torch.hip.Graph()
+        with torch.hip.graph(graph):
+            got.append(call(ts))
+        graphs.append(graph)
+    for order in ((0, 1), (1, 0), (0, 1)):
+        for i in order:
+            graphs[i].replay()
+            np.testing.assert_array_equal(f(long[:, :, -1:], long, long, 4000).numpy(), one)
+        for i in (0, 1):
+            for a, w in zip(got[i], want[i]):
+                np.testing.assert_array_equal(a.numpy(), w)
+
+
 # ------------------------------------------------------------------ refusals
 
 

@@ -234,6 +234,8 @@ extern "C" int tjh_distill(const float* logits, int64_t ld, int64_t rows, int64_
   TJH_REQUIRE_INIT();
   TJH_ARG(rows >= 0 && cols > 0 && k > 0 && ld >= cols, "tjh_distill: bad sizes");
   TJH_ARG(rows < (int64_t(1) << 31) && cols < (int64_t(1) << 30), "tjh_distill: too large");
+  const int threads = cols <= 1024 ? 64 : cols <= 4096 ? 256 : cols <= 53248 ? 512 : 1024;
+  TJH_ARG(rows * threads < (int64_t(1) << 32), "tjh_distill: too many rows");  // of a grid
   TJH_ARG(reduction >= 0 && reduction <= 3, "tjh_distill: reduction %d", reduction);
   TJH_ARG(temperature > 0.f && temperature < INFINITY, "tjh_distill: temperature must be positive");
   if (k > kMaxK)
@@ -258,7 +260,6 @@ extern "C" int tjh_distill(const float* logits, int64_t ld, int64_t rows, int64_
   // the count of valid rows: up to two per thread every workgroup adds their
   // flags up itself, which saves a launch (2 of 40 us at 509 rows; at 2048 the
   // launch is 4 us faster)
-  const int threads = cols <= 1024 ? 64 : cols <= 4096 ? 256 : cols <= 53248 ? 512 : 1024;
   const float* valid = mean && rows <= 2 * threads ? denom + 1 : nullptr;
   int rc = TJH_OK;
   if (batch) {

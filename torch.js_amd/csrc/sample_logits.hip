@@ -39,9 +39,7 @@ namespace {
 
 using namespace rowreg;
 
-constexpr int kCap = 8192;    // elements of a list
 constexpr int kMostK = 1024;  // top_k that is selected by the threads' maxima
-constexpr int kBins = 2048;   // of the nucleus's histogram
 constexpr int64_t kMaxCols = int64_t(1) << 20;
 
 struct SampleArgs {
@@ -57,7 +55,8 @@ struct SampleArgs {
   int32_t* out;
 };
 
-template <int T>
+// kCap: elements of a list, kBins: of the nucleus's histogram.
+template <int T, int kCap, int kBins>
 struct SampleLds {
   SelectLds<T, kCap> s;
   u64 bins[kBins];
@@ -134,7 +133,9 @@ __device__ __forceinline__ void each_four(const Row<T, NV>& row, F f) {
 
 template <int T, int NV>
 __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
-  __shared__ SampleLds<T> lds;
+  // rows of 4096 at most: two workgroups fit a CU
+  constexpr int kCap = NV == 4 ? 4096 : 8192, kBins = NV == 4 ? 1024 : 2048;
+  __shared__ SampleLds<T, kCap, kBins> lds;
   SelectLds<T, kCap>& s = lds.s;
   constexpr int W = T / 64;
   constexpr int kNone = 0x7fffffff;
@@ -645,7 +646,7 @@ extern "C" int tjh_sample_logits(const float* logits, int64_t ld, int64_t rows, 
                                  int32_t* out) {
   TJH_REQUIRE_INIT();
   TJH_ARG(rows >= 0 && cols > 0 && ld >= cols, "tjh_sample_logits: bad sizes");
-  TJH_ARG(rows < (int64_t(1) << 31), "tjh_sample_logits: too many rows");
+  TJH_ARG(rows < (int64_t(1) << 22), "tjh_sample_logits: too many rows");  // of a grid
   if (rows == 0) return TJH_OK;
   if (cols > kMaxCols)
     return set_error(TJH_ERR_UNSUPPORTED, "tjh_sample_logits: %lld columns, at most %lld",

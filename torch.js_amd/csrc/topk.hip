@@ -54,6 +54,7 @@ __global__ __launch_bounds__(256) void k_topk_bwd(const float* __restrict__ g,
 }
 
 constexpr int kMaxK = 1024;
+constexpr int64_t kGrid = 1 << 21;  // workgroups of a launch: a grid has less than 2^32 threads
 
 }  // namespace
 }  // namespace tjh
@@ -74,23 +75,23 @@ int tjh_topk_forward(const float* x, int64_t ld, int64_t rows, int64_t cols, int
   TJH_ARG(rows < (int64_t(1) << 31) && cols < (int64_t(1) << 30), "tjh_topk_forward: too large");
   TJH_ARG(x && values && indices, "tjh_topk_forward: NULL pointer");
   KernelScope ks("topk");
-  const dim3 grid((unsigned)rows);
   const int n = (int)cols, kk = (int)k;
-  if (n <= 1024 - 3)
-    tjh_launch(k_topk<64, 4, 1024>, grid, dim3(64), 0, stream(), x, ld, n, kk, largest, values,
-               indices);
-  else if (n <= 4096 - 3)
-    tjh_launch(k_topk<256, 4, 4096>, grid, dim3(256), 0, stream(), x, ld, n, kk, largest, values,
-               indices);
-  else if (n <= 16384 - 3)
-    tjh_launch(k_topk<512, 8, 8192>, grid, dim3(512), 0, stream(), x, ld, n, kk, largest, values,
-               indices);
-  else if (n <= 53248 - 3)
-    tjh_launch(k_topk<512, 26, 8192>, grid, dim3(512), 0, stream(), x, ld, n, kk, largest, values,
-               indices);
-  else
-    tjh_launch(k_topk<1024, 0, 8192>, grid, dim3(1024), 0, stream(), x, ld, n, kk, largest, values,
-               indices);
+  for (int64_t at = 0; at < rows; at += kGrid) {
+    const dim3 grid((unsigned)(rows - at < kGrid ? rows - at : kGrid));
+    const float* p = x + at * ld;
+    float* v = values + at * k;
+    int32_t* ix = indices + at * k;
+    if (n <= 1024 - 3)
+      tjh_launch(k_topk<64, 4, 1024>, grid, dim3(64), 0, stream(), p, ld, n, kk, largest, v, ix);
+    else if (n <= 4096 - 3)
+      tjh_launch(k_topk<256, 4, 4096>, grid, dim3(256), 0, stream(), p, ld, n, kk, largest, v, ix);
+    else if (n <= 16384 - 3)
+      tjh_launch(k_topk<512, 8, 8192>, grid, dim3(512), 0, stream(), p, ld, n, kk, largest, v, ix);
+    else if (n <= 53248 - 3)
+      tjh_launch(k_topk<512, 26, 8192>, grid, dim3(512), 0, stream(), p, ld, n, kk, largest, v, ix);
+    else
+      tjh_launch(k_topk<1024, 0, 8192>, grid, dim3(1024), 0, stream(), p, ld, n, kk, largest, v, ix);
+  }
   return check_launch("topk");
 }
 
@@ -102,8 +103,9 @@ int tjh_topk_backward(const float* g, const int32_t* indices, int64_t rows, int6
   TJH_ARG(rows < (int64_t(1) << 31) && cols < (int64_t(1) << 30), "tjh_topk_backward: too large");
   TJH_ARG(dx && (k == 0 || (g && indices)), "tjh_topk_backward: NULL pointer");
   KernelScope ks("topk_bwd");
-  tjh_launch(k_topk_bwd, dim3((unsigned)rows), dim3(256), 0, stream(), g, indices, (int)cols,
-             (int)k, dx);
+  for (int64_t at = 0; at < rows; at += kGrid)
+    tjh_launch(k_topk_bwd, dim3((unsigned)(rows - at < kGrid ? rows - at : kGrid)), dim3(256), 0,
+               stream(), g + at * k, indices + at * k, (int)cols, (int)k, dx + at * cols);
   return check_launch("topk_bwd");
 }
 

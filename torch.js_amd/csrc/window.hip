@@ -788,7 +788,8 @@ int check_window(const char* who, int64_t B, int64_t H, int64_t Hkv, int64_t Tq,
   TJH_ARG(H == 0 || (Hkv > 0 && H % Hkv == 0), "%s: %lld heads over %lld", who, (long long)H,
           (long long)Hkv);
   TJH_ARG(Tk < (int64_t(1) << 30) && H < (int64_t(1) << 30), "%s: too large", who);
-  TJH_ARG(B * H * cdiv(Tq, TILE) < (int64_t(1) << 31), "%s: grid too large", who);
+  // a grid has less than 2^32 threads, and Tq <= 4 takes a workgroup of 256 a query
+  TJH_ARG(B * H * (Tq <= 4 ? Tq : cdiv(Tq, TILE)) < (int64_t(1) << 24), "%s: too large", who);
   for (int i = 0; i < n; ++i) TJH_ARG(strides[i], "%s: NULL strides", who);
   bool wide = false;
   for (int i = 0; i < n; ++i) wide |= strides[i][2] >= kMaxRowStride || strides[i][2] < 0;
@@ -948,7 +949,7 @@ int tjh_window_backward(const float* q, const float* k, const float* v, const fl
       a.nbkv = (int)(nbkv - at < chunk ? nbkv - at : chunk);
       const int64_t keys =
           (int64_t)a.nbkv * (a.nsb * a.nslice + (a.nblk - a.nsb) * (int64_t)a.nsplit);
-      TJH_ARG(keys < (int64_t(1) << 31), "tjh_window_backward: grid too large");
+      TJH_ARG(keys < (int64_t(1) << 24), "tjh_window_backward: too large");
       switch (cdiv(D, 32)) {
         case 1: rc = launch_bwd<32>(a, (unsigned)keys, dq, strides[5]); break;
         case 2: rc = launch_bwd<64>(a, (unsigned)keys, dq, strides[5]); break;

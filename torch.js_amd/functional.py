@@ -308,16 +308,6 @@ def nll_loss(input, target, weight=None, reduction="mean", *, ignore_index=-100)
     return _record(out, "NLLLoss", [x], bwd, gfn=gbwd)
 
 
-def _rows_2d(x):
-    """x as a matrix of rows, without a copy where its rows are dense: (tensor
-    that holds them, pointer, row stride, rows, columns)."""
-    st, (rows, cols) = x._strides, (_numel(x.shape[:-1]), x.shape[-1])
-    if len(st) == 2 and st[1] == 1 and st[0] >= cols:
-        return x, x.data_ptr(), st[0], rows, cols
-    xd = x.detach().contiguous()
-    return xd, xd.data_ptr(), cols, rows, cols
-
-
 def distillation_loss(input, teacher_logits, teacher_ids, temperature=1.0, reduction="mean"):
     """The loss of a student's logits against a teacher's largest ones
     (beside F.cross_entropy, src/nn/losses.ts:129-168; torch.js has none):
@@ -346,7 +336,7 @@ def distillation_loss(input, teacher_logits, teacher_ids, temperature=1.0, reduc
     if x.dtype != "float32":
         x = x.float()
     v = (v if v.dtype == "float32" else v.float()).detach().contiguous()
-    xd, px, ld, rows, cols = _rows_2d(x.detach())
+    xd, px, ld, rows, cols = _T._rows_2d(x.detach())
     k = v.shape[-1]
     xs = x.shape
     loss_rows = empty(xs[:-1])
@@ -450,7 +440,7 @@ def sample_logits(logits, uniforms=None, temperature=1.0, top_k=0, top_p=1.0, mi
         x = reshape(x.detach(), (1, x.shape[0]))
     if x.dtype != "float32":
         x = x.float()
-    xd, px, ld, rows, cols = _rows_2d(x)
+    xd, px, ld, rows, cols = _T._rows_2d(x)
     if uniforms is None:
         u = _T.rand(rows)
     else:
@@ -463,6 +453,8 @@ def sample_logits(logits, uniforms=None, temperature=1.0, top_k=0, top_p=1.0, mi
         u = (u if u.dtype == "float32" else u.float()).contiguous()
     # the tensors live until the launch is queued
     t, t0, _t = _setting("temperature", temperature, rows, "float32", 0.0, math.inf)
+    if isinstance(top_k, float) and top_k != int(top_k):
+        raise ValueError("sample_logits: top_k must be a whole number, got %r" % (top_k,))
     k, k0, _k = _setting("top_k", top_k, rows, "int32", 0, 2 ** 31 - 1)
     p, p0, _p = _setting("top_p", top_p, rows, "float32", 0.0, 1.0)
     m, m0, _m = _setting("min_p", min_p, rows, "float32", 0.0, 1.0)

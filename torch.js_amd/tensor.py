@@ -762,6 +762,21 @@ def _empty_padded(rows, cols):
     return Tensor(st, (rows, cols), (ld, 1), 0, "float32")
 
 
+def _rows_2d(x):
+    """x [..., n] as a matrix of rows, without a copy where its rows are dense
+    and evenly spaced (a layer's padded output in any number of dims): (tensor
+    that holds them, pointer, row stride, rows, columns)."""
+    sh, st = x._shape, x._strides
+    cols, rows = sh[-1], _numel(sh[:-1])
+    lead = [(s, n) for s, n in zip(st[:-1], sh[:-1]) if n != 1]
+    ld = lead[-1][0] if lead else cols
+    if st[-1] == 1 and ld >= cols and \
+            all(a[0] == b[0] * b[1] for a, b in zip(lead, lead[1:])):
+        return x, x.data_ptr(), ld, rows, cols
+    x = x.detach().contiguous()
+    return x, x.data_ptr(), cols, rows, cols
+
+
 def _fill_view(t, value):
     _before_write(t)
     lib = L.lib()
@@ -2739,18 +2754,14 @@ def topk(x, k, dim=-1, largest=True):
         return permute(v, perm), permute(i, perm)
     if x._dtype != "float32":
         x = x.float()
-    xs, st, xd, ld = x._shape, x._strides, x, n
-    if len(st) == 2 and st[1] == 1 and st[0] >= n:
-        ld = st[0]
-    else:
-        xd = x.detach().contiguous()
-    rows = _numel(xs[:-1])
+    xs = x._shape
+    xd, px, ld, rows, _ = _rows_2d(x)
     oshape = xs[:-1] + (k,)
     # both in one allocation, the indices after the values
     both = Storage(max(1, 2 * rows * k) * 4)
     values = Tensor(both, oshape)
     indices = Tensor(both, oshape, None, rows * k, "int32")
-    L.check(L.lib().tjh_topk_forward(xd.data_ptr(), ld, rows, n, k, 1 if largest else 0,
+    L.check(L.lib().tjh_topk_forward(px, ld, rows, n, k, 1 if largest else 0,
                                      values.data_ptr(), indices.data_ptr()), "topk")
     if not _recorded(x):
         return values, indices
