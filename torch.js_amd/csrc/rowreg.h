@@ -225,29 +225,38 @@ struct SelectLds {
 };
 
 // list[0, c) in descending order in s.sorted, c <= 256: each thread counts the
-// items above one of them (c * c / T comparisons, three barriers).
+// items above one of them (c * c / T comparisons, three barriers), eight of
+// them read at a time: the list has room for 256 and is padded with zeros,
+// which no item is below.
 template <int T, int CAP>
-__device__ __forceinline__ void sort_short(const u64* list, int c, SelectLds<T, CAP>& s) {
+__device__ __forceinline__ void sort_short(u64* list, int c, SelectLds<T, CAP>& s) {
   int pad = 64;
   while (pad < c) pad <<= 1;
+  const int ng = T >= pad ? T / pad : 1;  // threads an item
+  const int end = (c + 8 * ng - 1) / (8 * ng) * (8 * ng);  // <= 256
   for (int i = threadIdx.x; i < c; i += T) s.rank[i] = 0;
+  for (int i = c + threadIdx.x; i < end; i += T) list[i] = 0;
   __syncthreads();  // ranks cleared, list written
+  const auto above = [&](u64 me, int g) {
+    int r = 0;
+    for (int j = g; j < end; j += 8 * ng) {
+      u64 x[8];
+#pragma unroll
+      for (int v = 0; v < 8; ++v) x[v] = list[j + v * ng];
+#pragma unroll
+      for (int v = 0; v < 8; ++v) r += x[v] > me;
+    }
+    return r;
+  };
   if (T >= pad) {
-    const int i = threadIdx.x & (pad - 1), g = threadIdx.x / pad, ng = T / pad;
+    const int i = threadIdx.x & (pad - 1);
     if (i < c) {
-      const u64 me = list[i];
-      int r = 0;
-      for (int j = g; j < c; j += ng) r += list[j] > me;
+      const int r = above(list[i], threadIdx.x / pad);
       if (ng > 1) atomicAdd(&s.rank[i], r);
       else s.rank[i] = r;
     }
   } else {
-    for (int i = threadIdx.x; i < c; i += T) {
-      const u64 me = list[i];
-      int r = 0;
-      for (int j = 0; j < c; ++j) r += list[j] > me;
-      s.rank[i] = r;
-    }
+    for (int i = threadIdx.x; i < c; i += T) s.rank[i] = above(list[i], 0);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < c; i += T) s.sorted[s.rank[i]] = list[i];
@@ -256,15 +265,18 @@ __device__ __forceinline__ void sort_short(const u64* list, int c, SelectLds<T, 
 
 // s.list[0, c) in descending order: where it stands.  Over 256 items a bitonic
 // network in place over the next power of two, padded with zeros, which no
-// real item is below (c log^2 c / 4 T exchanges, log^2 c / 2 barriers).
+// real item is below (c log^2 c / 4 T exchanges, log^2 c / 2 rounds).  The
+// pairs of a wave's 64 threads stay within 128 items while the distance is 64
+// or less, so that barriers stand only around the rounds of larger ones.
 template <int T, int CAP>
 __device__ __forceinline__ u64* sort_list(SelectLds<T, CAP>& s, int c) {
+  static_assert((CAP & (CAP - 1)) == 0 && CAP >= 2 * kRank, "padded to a power of two");
   if (c <= kRank) {
     sort_short(s.list, c, s);
     return s.sorted;
   }
   int p = 2 * kRank;
-  while (p < c) p <<= 1;  // <= CAP, a power of two
+  while (p < c) p <<= 1;  // <= CAP
   for (int i = c + threadIdx.x; i < p; i += T) s.list[i] = 0;
   __syncthreads();
   for (int len = 2; len <= p; len <<= 1) {
@@ -278,7 +290,13 @@ __device__ __forceinline__ u64* sort_list(SelectLds<T, CAP>& s, int c) {
           s.list[i + o] = x;
         }
       }
-      __syncthreads();
+      const int next = o > 1 ? o >> 1 : len;
+      if (o > 64 || next > 64) {
+        __syncthreads();
+      } else {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      }
     }
   }
   return s.list;

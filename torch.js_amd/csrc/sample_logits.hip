@@ -98,7 +98,8 @@ struct Weights {
     e = __builtin_fma(f, e, c2);
     e = __builtin_fma(f, e, c1);
     e = __builtin_fma(tab * f, e, tab);
-    e = ldexp(e, k >> 5) + top;
+    // times 2^(k >> 5): normal numbers of 2^-14 to 2^52
+    e = __hiloint2double(__double2hiint(e) + ((k & ~31) << 15), __double2loint(e)) + top;
     return (u64)__double_as_longlong(e) & 0xfffffffffffffull;
   }
 };
@@ -134,7 +135,7 @@ __device__ __forceinline__ void each_four(const Row<T, NV>& row, F f) {
 template <int T, int NV>
 __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
   // rows of 4096 at most: two workgroups fit a CU
-  constexpr int kCap = NV == 4 ? 4096 : 8192, kBins = NV == 4 ? 1024 : 2048;
+  constexpr int kCap = T == 256 ? 4096 : 8192, kBins = T == 256 ? 1024 : 2048;
   __shared__ SampleLds<T, kCap, kBins> lds;
   SelectLds<T, kCap>& s = lds.s;
   constexpr int W = T / 64;
@@ -200,8 +201,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
   float bound = -INFINITY;
   double limit = INFINITY;  // weight before an element that is in the nucleus
   const auto bin_of = [&](float per, float x) {  // nondecreasing as x falls
-    const float z = (float)(m - (double)x) * per;
-    return z < (float)(kBins - 1) ? (int)z : kBins - 1;
+    return (int)fminf((mx - x) * per, (float)(kBins - 1));
   };
   float per = 0.f;
   int last = -1;
