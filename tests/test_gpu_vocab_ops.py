@@ -539,6 +539,26 @@ def test_rows_of_a_padded_output(torch):
 
 
 @gpu
+@pytest.mark.parametrize("n,ks", [(300, (33, 100, 128, 300)), (1000, (90, 128, 129, 700)), (1021, (64, 1021)),
+                                  (4093, (512, 513)), (16000, (250, 640))])
+def test_topk_of_many_rows(torch, n, ks):
+    """Sizes at which the rows' number and k choose between kernels and ways
+    to sort, and lists much longer than k."""
+    rng = np.random.default_rng(n)
+    for spread in (False, True):
+        x = rng.standard_normal((1025, n)).astype(np.float32)
+        if spread:  # a few values: ties by index
+            x = np.rint(x * 3).astype(np.float32)
+        tx = torch.tensor(x)
+        for k in ks:
+            for largest in (True, False):
+                v, i = tx.topk(k, largest=largest)
+                ref = topk_ref(x, k, largest)
+                np.testing.assert_array_equal(i.numpy(), ref)
+                np.testing.assert_array_equal(v.numpy(), np.take_along_axis(x, ref, 1))
+
+
+@gpu
 def test_topk_of_more_rows_than_a_grid(torch):
     rng = np.random.default_rng(3)
     rows = 2 ** 21 + 3

@@ -76,14 +76,19 @@ int tjh_topk_forward(const float* x, int64_t ld, int64_t rows, int64_t cols, int
   TJH_ARG(x && values && indices, "tjh_topk_forward: NULL pointer");
   KernelScope ks("topk");
   const int n = (int)cols, kk = (int)k;
+  // The fewest threads that hold the row, but with enough of their maxima for
+  // the k: with too few the bound lets most of the row into the list.  (4096,
+  // 1000), k 64: one wave 16 us, four 27; 256: 124, 49.  Few rows leave the
+  // CUs idle anyway: (64, 1000), k 32: 6, 6; 64: 8, 6.  (2048, 4000), k 500:
+  // four waves 52 us, eight 66; 1000: 211, 87.
   for (int64_t at = 0; at < rows; at += kGrid) {
     const dim3 grid((unsigned)(rows - at < kGrid ? rows - at : kGrid));
     const float* p = x + at * ld;
     float* v = values + at * k;
     int32_t* ix = indices + at * k;
-    if (n <= 1024 - 3)
+    if (n <= 1024 - 3 && kk <= (rows < 1024 ? 32 : 128))
       tjh_launch(k_topk<64, 4, 1024>, grid, dim3(64), 0, stream(), p, ld, n, kk, largest, v, ix);
-    else if (n <= 4096 - 3)
+    else if (n <= 4096 - 3 && kk <= 512)
       tjh_launch(k_topk<256, 4, 4096>, grid, dim3(256), 0, stream(), p, ld, n, kk, largest, v, ix);
     else if (n <= 16384 - 3)
       tjh_launch(k_topk<512, 8, 8192>, grid, dim3(512), 0, stream(), p, ld, n, kk, largest, v, ix);
