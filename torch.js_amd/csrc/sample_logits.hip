@@ -18,7 +18,8 @@
 // the waves add them, exact, and finer than 32-bit floats by 2^22.  They are
 // formed in 64 bits as 2^(k / 32) 2^(f / 32), |f| <= 1 / 2, from a table and
 // the first six terms of the second (the seventh is below 2^-48): 32-bit ones
-// would move one draw in some thousand over a border between two indices.
+// would move one draw in some thousand over a border between two indices.  A
+// weight below half of 2^-s counts as 0.
 //
 // One workgroup has a row, in registers (rowreg.h).  Wherever the elements
 // that can be drawn fit (8192), they are moved into LDS and everything else
@@ -29,6 +30,11 @@
 // 256 are added up by parts of the index range first.  Larger sets are a
 // bound on (x, index), and passes that add the kept weights up by runs of the
 // index range, one a wave, and look into one.
+//
+// Bound by the work of a row on its one CU, far from memory (10 us for 256
+// rows of 50257).  Up to 256 rows of 50257: greedy 7 us (the load and the
+// maximum), top_k 50 16, min_p 0.01 24, no rule 31 (of it some 15 the
+// weights), top_k 1000 39, top_p 0.9 49; of 32001, top_p 0.9 43.
 #include "rowreg.h"
 
 #include <float.h>

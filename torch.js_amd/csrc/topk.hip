@@ -8,7 +8,9 @@
 //
 // Bound by reading the rows once: a workgroup keeps its row in registers,
 // takes a lower bound of the k-th value from the threads' maxima, moves the
-// few elements above it into LDS and sorts those (rowreg.h).
+// few elements above it into LDS and sorts those (rowreg.h).  64 of each of
+// 2048 rows of 50257: 75 us, 5.5 TB/s; 20 of one row: 9 us, a chain of loads,
+// rounds of the bound and the sort on one CU.
 #include "rowreg.h"
 
 namespace tjh {
@@ -34,7 +36,7 @@ __global__ __launch_bounds__(T, T == 512 ? 4 : 1) void k_topk(const float* __res
 }
 
 // dx = 0 but dx[r, indices[r, i]] = g[r, i]: the row's zeros, then its k
-// values, one workgroup a row.
+// values, one workgroup a row.  (4099, 1000), 8 values: 5.1 us, 3.2 TB/s.
 __global__ __launch_bounds__(256) void k_topk_bwd(const float* __restrict__ g,
                                                   const int32_t* __restrict__ indices, int n, int k,
                                                   float* __restrict__ dx) {

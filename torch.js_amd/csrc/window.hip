@@ -178,7 +178,10 @@ __device__ __forceinline__ void col_operand(__amdgpu_buffer_rsrc_t tile, int st,
 template <int HD> constexpr int waves_fwd() { return HD <= 64 ? 3 : HD <= 96 ? 2 : 1; }
 
 // One wave 32 queries.  GUARD: D < HD.  PART: one slice of the key tiles,
-// joined by k_win_merge.
+// joined by k_win_merge.  96 heads of 1024 positions, D 64, window 256: 87 us,
+// 66 TFLOP/s of the keys seen (80 of the tiles formed); 16 of 8192, D 128,
+// window 1024: 718 us, 91.  A part of a prompt, 16 heads of 93 positions, D
+// 80, window 300, in slices: 15 us and 4 for the join.
 template <int HD, bool GUARD, bool PART, int RUN>
 __global__ __launch_bounds__(256, waves_fwd<HD>()) void k_win_fwd(WinArgs a) {
   using S_ = Hd<HD>;
@@ -340,6 +343,7 @@ __global__ __launch_bounds__(256) void k_win_merge(WinArgs a, int64_t n4, int ns
 // its keys over groups of 16 lanes, each with a running softmax of its own
 // over every NG-th key, joined once at the end in a fixed order.  grid.y
 // slices of the keys, joined by k_win_merge, where there are few rows.
+// Bound by the latency of its loads: 48 rows of 260 keys, D 64, 5.7 us.
 constexpr int kFewThreads = 512, kFewGroups = kFewThreads / 16, kFewUnroll = 4;
 
 template <int NC, bool PART>  // NC: 64-column pieces of the head dim
@@ -454,7 +458,8 @@ __host__ __device__ inline int64_t sums_at(const WinArgs& a) {
 // stores it and accumulates dK^T += Q^T dS (flash.hip's split of the work, the
 // tiles of Q and dO through LDS: straight from memory they took 2 % less at a
 // head dim of 64 and a sixth more at 128).  GUARD: Tq or Tk is not a multiple
-// of 32, or D < HD.
+// of 32, or D < HD.  The sizes of k_win_fwd: 168 us, 68 TFLOP/s of the keys
+// seen; 1239 us, 105.
 template <int HD, bool GUARD, int RUN>
 __global__ __launch_bounds__(256, occ_pair<HD>()) void k_win_dkv(WinArgs a) {
   using S_ = Hd<HD>;
@@ -658,6 +663,8 @@ __global__ __launch_bounds__(256) void k_win_sums(WinArgs a, const float* __rest
 
 // Query kernel: dQ^T += K^T dS^T from the stored dS blocks, one wave 32
 // queries, the next tile's operands on their way during a tile's products.
+// Half the products of a tile for the same loads as the forward's: the sizes
+// of k_win_fwd, 58 us, 49 TFLOP/s of the keys seen; 375 us, 87.
 template <int HD>
 __global__ __launch_bounds__(256, HD <= 64 ? 3 : HD <= 96 ? 2 : 1) void k_win_dq(WinArgs a) {
   using S_ = Hd<HD>;
