@@ -139,6 +139,31 @@ __device__ __forceinline__ u64 wave_sum_u64(u64 v) {
   return lane_u64(v, 0) + lane_u64(v, 16) + lane_u64(v, 32) + lane_u64(v, 48);
 }
 
+// Inclusive sums over the lanes by the DPP network: within rows of 16, then
+// their last lanes' to the rows after them.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_shift(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp_shift(u64 v) {
+  const int lo = dpp_shift<CTRL, ROWS>((int)(uint32_t)v);
+  const int hi = dpp_shift<CTRL, ROWS>((int)(v >> 32));
+  return ((u64)(uint32_t)hi << 32) | (uint32_t)lo;
+}
+template <class V>
+__device__ __forceinline__ V wave_scan(V v) {
+  v += dpp_shift<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
+  v += dpp_shift<0x112, 0xF>(v);
+  v += dpp_shift<0x114, 0xF>(v);
+  v += dpp_shift<0x118, 0xF>(v);
+  v += dpp_shift<0x142, 0xA>(v);  // row_bcast:15 to rows 1 and 3
+  v += dpp_shift<0x143, 0xC>(v);  // row_bcast:31 to rows 2 and 3
+  return v;
+}
+__device__ __forceinline__ int last_lane(int v) { return __builtin_amdgcn_readlane(v, 63); }
+__device__ __forceinline__ u64 last_lane(u64 v) { return lane_u64(v, 63); }
+
 // Block-wide operations, one barrier each: consecutive ones use the two
 // halves of `sm` in turn, so nobody writes a half that is still being read.
 template <int T>
@@ -170,9 +195,7 @@ struct Block {
     return across((int)(__ballot(p) != 0), [](int x, int y) { return x | y; }) != 0;
   }
   __device__ __forceinline__ int sum_i(int v) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-    return across(v, [](int x, int y) { return x + y; });
+    return across(last_lane(wave_scan(v)), [](int x, int y) { return x + y; });
   }
   // threads for which p holds, counted over `M` predicates of each
   template <int M>
@@ -186,14 +209,9 @@ struct Block {
   template <class V>
   __device__ __forceinline__ V before(V v, V* all) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    V incl = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const V x = __shfl_up(incl, o, 64);
-      if (lane >= o) incl += x;
-    }
+    const V incl = wave_scan(v);
     if (W == 1) {
-      *all = __shfl(incl, 63, 64);
+      *all = last_lane(incl);
       return incl - v;
     }
     V* s = reinterpret_cast<V*>(sm + half * W);
@@ -401,36 +419,20 @@ __device__ __forceinline__ int gather_list(const Row<T, 0>& row, uint32_t nan, I
   return s.count;
 }
 
-// The same for the elements that are not below `bound`, straight from the
-// registers.  FEW: some ten or hundred of the row, each of which takes a
-// place by itself; otherwise they are counted first, so that each thread
-// knows its places (an 11th of 32001 elements: 5 us less; 50 of them: 3 us
-// more).
-template <bool FEW, int T, int NV, int CAP>
+// The same for the elements that are not below `bound`, some ten or hundred of
+// the row, straight from the registers.
+template <int T, int NV, int CAP>
 __device__ __forceinline__ int gather_above(const Row<T, NV>& row, uint32_t nan, float bound,
-                                            SelectLds<T, CAP>& s, Block<T>& b) {
+                                            SelectLds<T, CAP>& s) {
   if constexpr (NV == 0) {
     return gather_list(row, nan, [&](int, int, float x) { return !(x < bound); }, s);
   } else {
-    int at = 0, total = 0;
-    if constexpr (FEW) {
-      if (threadIdx.x == 0) s.count = 0;
-      __syncthreads();
-    } else {
-      // places past the row (-infinity) count where the bound is -infinity
-      const bool all_in = !(bound > -INFINITY);
-      int mine = 0;
-      row.each([&](int j, int u, float x) {
-        mine += !(x < bound) && (!all_in || row.inside(j, u));
-      });
-      at = b.before(mine, &total);
-      if (total > CAP) return total;
-      asm volatile("" : "+v"(bound));  // compared anew: else every comparison's mask is kept
-    }
+    if (threadIdx.x == 0) s.count = 0;
+    __syncthreads();
     const auto put = [&](int j, int u, float x) {
       if (!(x < bound) && row.inside(j, u)) {
-        const int to = FEW ? atomicAdd(&s.count, 1) : at++;
-        if (!FEW || to < CAP) s.list[to] = composite(order_key(x, nan), row.index(j, u));
+        const int to = atomicAdd(&s.count, 1);
+        if (to < CAP) s.list[to] = composite(order_key(x, nan), row.index(j, u));
       }
     };
     put(-1, 0, row.edge);
@@ -446,8 +448,48 @@ __device__ __forceinline__ int gather_above(const Row<T, NV>& row, uint32_t nan,
       }
     }
     __syncthreads();
-    return FEW ? s.count : total;
+    return s.count;
   }
+}
+
+// (x, index) as they are
+__device__ __forceinline__ u64 pair_of(float x, int i) {
+  return ((u64)__float_as_uint(x) << 32) | (uint32_t)i;
+}
+__device__ __forceinline__ float pair_value(u64 e) { return __uint_as_float((uint32_t)(e >> 32)); }
+__device__ __forceinline__ int pair_index(u64 e) { return (int)(uint32_t)e; }
+
+// Pairs of the elements that are not below `bound`, above -infinity, of a row
+// without NaN into the list, if it holds them: their number.  They are counted
+// first, so that each thread knows its places: an 11th of a row's elements
+// would wait for each other's increments of one count.
+template <int T, int NV, int CAP>
+__device__ __forceinline__ int gather_pairs(const Row<T, NV>& row, float bound,
+                                            SelectLds<T, CAP>& s, Block<T>& b) {
+  int at = 0, total = 0;
+  row.each([&](int, int, float x) { at += x >= bound; });
+  at = b.before(at, &total);
+  if (total > CAP) return total;
+  asm volatile("" : "+v"(bound));  // compared anew: else every comparison's mask is kept
+  const auto put = [&](int j, int u, float x) {
+    if (x >= bound) s.list[at++] = pair_of(x, row.index(j, u));
+  };
+  if constexpr (NV == 0) {
+    row.each(put);
+  } else {
+    put(-1, 0, row.edge);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const float x = fmaxf(fmaxf(row.v[4 * j], row.v[4 * j + 1]),
+                            fmaxf(row.v[4 * j + 2], row.v[4 * j + 3]));
+      if (x >= bound) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) put(j, u, row.v[4 * j + u]);
+      }
+    }
+  }
+  __syncthreads();
+  return total;
 }
 
 // The index of the need-th element (in index order, need >= 1) of those for
@@ -533,7 +575,7 @@ __device__ __forceinline__ float kth_bound(const Row<T, NV>& row, int k, Block<T
 template <int T, int NV, int CAP>
 __device__ __forceinline__ u64* select_largest(const Row<T, NV>& row, int k, uint32_t nan,
                                                SelectLds<T, CAP>& s, Block<T>& b) {
-  const int c = gather_above<true>(row, nan, kth_bound(row, k, b), s, b);
+  const int c = gather_above(row, nan, kth_bound(row, k, b), s);
   if (c > CAP) {
     Row<T, 0> again;
     again.load(row.p, row.n, row.sign);

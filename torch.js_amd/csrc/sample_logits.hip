@@ -138,6 +138,25 @@ __device__ __forceinline__ void each_four(const Row<T, NV>& row, F f) {
   }
 }
 
+// f(i, list[i]) for i < c, four of a thread's items at a time, their reads
+// together.
+template <int T, class F>
+__device__ __forceinline__ void each_listed_of(const u64* list, int c, F f) {
+  for (int i0 = threadIdx.x; i0 < c; i0 += 4 * T) {
+    u64 e[4];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) e[v] = list[min(i0 + v * T, c - 1)];
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+      if (i0 + v * T < c) f(i0 + v * T, e[v]);
+  }
+}
+
+// (~index, place in the list) of a pair: in descending order by the index
+__device__ __forceinline__ u64 by_index(u64 e, int i) {
+  return ((u64)(uint32_t)~pair_index(e) << 32) | (uint32_t)i;
+}
+
 template <int T, int NV>
 __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
   // rows of 4096 at most: two workgroups fit a CU
@@ -153,22 +172,39 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
   row.load(a.x + r * a.ld, a.n);
   const int n = a.n;
 
-  float mx = -INFINITY;
-  uint32_t mag = 0;  // largest |x| as bits: above infinity's is NaN
+  const double temp = a.temperature ? (double)a.temperature[r] : a.t0;
+  const int64_t top_k = a.top_k ? (int64_t)a.top_k[r] : a.k0;
+  const double top_p = a.top_p ? (double)a.top_p[r] : a.p0;
+  const double min_p = a.min_p ? (double)a.min_p[r] : a.m0;
+  const double u = (double)a.u[r];
+  const bool use_k = top_k > 0 && top_k < n, use_p = top_p < 1.0;
+  const bool largest = use_k && top_k <= kMostK, cut = use_k && !largest;
+  const bool nucleus = use_p && !largest;  // by the histogram
+
+  float mx = -INFINITY, mn = INFINITY;  // mn: the smallest above -infinity, for the nucleus
+  uint32_t mag = 0;                     // largest |x| as bits: above infinity's is NaN
   row.each([&](int, int, float x) {
     mx = fmaxf(mx, x);
     const uint32_t u = __float_as_uint(x) << 1;
     mag = u > mag ? u : mag;
   });
-  mx = b.max(mx);
-  if (b.any(mag > 0xff000000u) || !(fabsf(mx) < INFINITY)) {
+  if (nucleus) {
+    row.each([&](int, int, float x) { mn = x > -INFINITY ? fminf(mn, x) : mn; });
+    for (int i = t; i < kBins; i += T) lds.bins[i] = 0;
+  }
+  if (t < 32) lds.pow2[t] = ldexp(exp2((double)t / 32), min(51, 62 - (32 - __clz(n))));
+  if (t == 0) lds.pick = kNone;
+  mx = __ballot(mag > 0xff000000u) ? INFINITY : wave_max(mx);
+  const float2 ends = b.across(make_float2(mx, wave_max(-mn)), [](float2 x, float2 y) {
+    return make_float2(fmaxf(x.x, y.x), fmaxf(x.y, y.y));
+  });
+  mx = ends.x;
+  mn = -ends.y;
+  if (!(fabsf(mx) < INFINITY)) {
     if (t == 0) a.out[r] = -1;
     return;
   }
-  const double temp = a.temperature ? (double)a.temperature[r] : a.t0;
-  if (t == 0) lds.pick = kNone;
   if (!(temp > 0.0)) {
-    __syncthreads();
     row.each([&](int j, int u, float x) {
       if (x == mx && row.inside(j, u)) atomicMin(&lds.pick, row.index(j, u));
     });
@@ -176,17 +212,10 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
     if (t == 0) a.out[r] = lds.pick;
     return;
   }
-  const int64_t top_k = a.top_k ? (int64_t)a.top_k[r] : a.k0;
-  const double top_p = a.top_p ? (double)a.top_p[r] : a.p0;
-  const double min_p = a.min_p ? (double)a.min_p[r] : a.m0;
-  const bool use_k = top_k > 0 && top_k < n, use_p = top_p < 1.0;
   const double p = top_p > 0.0 ? top_p : 1e-300;  // the first element at least
   const double floor_z = min_p > 0.0 ? fmin(temp * log(min_p), 0.0) : -INFINITY;
   const double m = (double)mx;
   const double per_t = fmax(fmin(1.4426950408889634074 / temp, 1e300), 1e-300);
-  const double u = (double)a.u[r];
-  if (t < 32) lds.pow2[t] = ldexp(exp2((double)t / 32), min(51, 62 - (32 - __clz(n))));
-  __syncthreads();
   const Weights weight(m, per_t, lds.pow2);
 
   // elements of the order up to (tx, ti) are kept
@@ -195,7 +224,6 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
   const auto in_order = [&](const auto& of, int j, int e, float x) {
     return x > tx || (x == tx && of.index(j, e) <= ti);
   };
-  const bool largest = use_k && top_k <= kMostK, cut = use_k && !largest;
   if (cut) {
     Row<T, 0> again;
     again.load(row.p, n);
@@ -214,14 +242,9 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
   u64 above = 0;  // weight of the bins before `last`
   if (largest) {
     bound = kth_bound(row, (int)top_k, b);
-  } else if (use_p) {
+  } else if (nucleus) {
     // weights by bins of m - x, out to weights of e^-24 or the smallest x
-    float mn = mx;
-    row.each([&](int, int, float x) { mn = x > -INFINITY ? fminf(mn, x) : mn; });
-    mn = -b.max(-mn);
     per = (float)(kBins / fmax(fmin(24.0 * temp, m - (double)mn), 1e-30));
-    for (int i = t; i < kBins; i += T) lds.bins[i] = 0;
-    __syncthreads();
     if (!cut) {
       each_four(row, [&](float x0, float x1, float x2, float x3) {
         const float x[4] = {x0, x1, x2, x3};
@@ -272,12 +295,10 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
     bound = float_below(m + floor_z);
   }
   int c = -1;  // elements of the list, if there is one
-  const u64* list = s.list;
-  if (largest || bound > -INFINITY) {
-    c = use_p && !largest ? gather_above<false>(row, kNanFirst, bound, s, b)
-                          : gather_above<true>(row, kNanFirst, bound, s, b);
-    if (c > kCap) c = -1;
-  }
+  u64* list = s.list;
+  if (largest) c = gather_above(row, kNanFirst, bound, s);
+  else if (bound > -INFINITY) c = gather_pairs(row, bound, s, b);
+  if (c > kCap) c = -1;
   if (largest) {
     if (c < 0) {
       Row<T, 0> again;
@@ -295,14 +316,13 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
     // the nucleus ends in bin `last`: (tx, ti) from that bin's elements
     if (t == 0) s.count = 0;
     __syncthreads();
-    for (int i = t; i < c; i += T) {
-      const u64 e = s.list[i];
-      const float x = key_value((uint32_t)(e >> 32));
-      if (bin_of(per, x) == last && (x > tx || (x == tx && index_of(e) <= ti))) {
+    each_listed_of<T>(s.list, c, [&](int, u64 e) {
+      const float x = pair_value(e);
+      if (bin_of(per, x) == last && (x > tx || (x == tx && pair_index(e) <= ti))) {
         const int at = atomicAdd(&s.count, 1);
-        if (at < kRank) lds.few[at] = e;
+        if (at < kRank) lds.few[at] = composite(order_key(x), pair_index(e));
       }
-    }
+    });
     __syncthreads();
     int in = s.count;
     const u64* part = s.sorted;
@@ -389,18 +409,32 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
   }
 
   if (c >= 0) {
-    // the list's weights, none for elements that are not kept
+    // the list's weights, none for elements that are not kept; those of more
+    // than 256 by parts of the index range too
+    constexpr int kParts = 1024, kEach = (kParts + T - 1) / T;
+    const int shift = max(0, 32 - __clz(n - 1) - 10);  // 2^10 parts
+    bool parts = !largest && c > kRank;
+    const auto clear = [&]() {
+      for (int i = t; i < kParts; i += T) lds.bins[i] = 0;
+      if (t == 0) {
+        lds.pick = kNone;
+        s.count = 0;
+      }
+      __syncthreads();
+    };
+    if (parts) clear();
     u64 mine = 0;
-    for (int i = t; i < c; i += T) {
-      const u64 e = list[i];
-      const float x = key_value((uint32_t)(e >> 32));
+    each_listed_of<T>(list, c, [&](int i, u64 e) {
+      if (largest) list[i] = e = pair_of(key_value((uint32_t)(e >> 32)), index_of(e));
+      const float x = pair_value(e);
       const bool in = largest || ((double)x - m >= floor_z &&
-                                  (x > tx || (x == tx && index_of(e) <= ti)));
+                                  (x > tx || (x == tx && pair_index(e) <= ti)));
       const u64 w = in ? weight(x) : 0;
       lds.w[i] = w;
       mine += w;
-    }
-    u64 all = b.sum64(mine);
+      if (parts && w) atomicAdd(&lds.bins[pair_index(e) >> shift], w);
+    });
+    u64 all = parts ? 0 : b.sum64(mine);
     int keep = c;
     if (largest && (use_p || floor_z > -INFINITY)) {  // a sorted list, to be cut
       if (use_p) limit = p * (double)all;
@@ -412,37 +446,34 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
         u64 part;
         const u64 before = sum + b.before(w, &part);
         sum += part;
-        const bool in = i < c && (double)before < limit &&
-                        (double)key_value((uint32_t)(list[i] >> 32)) - m >= floor_z;
+        const bool in =
+            i < c && (double)before < limit && (double)pair_value(list[i]) - m >= floor_z;
         kept += in;
         mine_kept += in ? w : 0;
       }
       keep = b.sum_i(kept);
       all = b.sum64(mine_kept);
     }
-    const double target = u * (double)all;
+    if (largest && keep > kRank) {
+      parts = true;
+      __syncthreads();
+      clear();
+      for (int i = t; i < keep; i += T)
+        if (lds.w[i]) atomicAdd(&lds.bins[pair_index(list[i]) >> shift], lds.w[i]);
+    }
+    double target = u * (double)all;
     u64 sum = 0;  // weight of the indices before the ones looked into
     int in = keep;
-    if (keep > kRank) {
-      // by parts of the index range: the first with the target, or, where u
-      // is 1 or more, the last of any weight
-      constexpr int kParts = 1024, kEach = (kParts + T - 1) / T;
-      const int shift = max(0, 32 - __clz(n - 1) - 10);  // 2^10 parts
-      __syncthreads();
-      for (int i = t; i < kParts; i += T) lds.bins[i] = 0;
-      if (t == 0) {
-        lds.pick = kNone;
-        s.count = 0;
-      }
-      __syncthreads();
-      for (int i = t; i < keep; i += T)
-        if (lds.w[i]) atomicAdd(&lds.bins[index_of(list[i]) >> shift], lds.w[i]);
+    if (parts) {
+      // the first part with the target, or, where u is 1 or more, the last of
+      // any weight
       __syncthreads();
       u64 own = 0, total;
 #pragma unroll
       for (int i = 0; i < kEach; ++i)
         if (T <= kParts || t < kParts) own += lds.bins[t * kEach + i];
       u64 before = b.before(own, &total);
+      target = u * (double)total;
       int first = kNone, end = -1;
       u64 start = 0;
 #pragma unroll
@@ -469,16 +500,17 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
       } else if (first == at) {
         lds.first = start;
       }
-      for (int i = t; i < keep; i += T)
-        if (lds.w[i] && index_of(list[i]) >> shift == at) {
+      each_listed_of<T>(list, keep, [&](int i, u64 e) {
+        if (pair_index(e) >> shift == at && lds.w[i]) {
           const int put = atomicAdd(&s.count, 1);
-          if (put < kRank) lds.few[put] = (list[i] << 32) | (uint32_t)i;
+          if (put < kRank) lds.few[put] = by_index(e, i);
         }
+      });
       __syncthreads();
       sum = lds.first;
       in = s.count;
     } else {
-      for (int i = t; i < keep; i += T) lds.few[i] = (list[i] << 32) | (uint32_t)i;
+      for (int i = t; i < keep; i += T) lds.few[i] = by_index(list[i], i);
     }
     if (in <= kRank) {
       // (index, place in the list), in ascending order of the index
@@ -510,8 +542,8 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
     // more than 256 in one part: the pass over the row, down to the last kept
     if (largest) {
       const u64 e = list[keep - 1];
-      tx = key_value((uint32_t)(e >> 32));
-      ti = index_of(e);
+      tx = pair_value(e);
+      ti = pair_index(e);
     }
     __syncthreads();
   }
