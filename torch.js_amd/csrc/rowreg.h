@@ -480,11 +480,16 @@ __device__ __forceinline__ int gather_pairs(const Row<T, NV>& row, float bound,
     put(-1, 0, row.edge);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const float x = fmaxf(fmaxf(row.v[4 * j], row.v[4 * j + 1]),
-                            fmaxf(row.v[4 * j + 2], row.v[4 * j + 3]));
+      const float x = __builtin_elementwise_maximum(
+          __builtin_elementwise_maximum(row.v[4 * j], row.v[4 * j + 1]),
+          __builtin_elementwise_maximum(row.v[4 * j + 2], row.v[4 * j + 3]));
       if (x >= bound) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) put(j, u, row.v[4 * j + u]);
+        for (int u = 0; u < 4; ++u) {
+          float x = row.v[4 * j + u];
+          asm volatile("" : "+v"(x));  // a copy: else every value of the row takes half a pair
+          put(j, u, x);
+        }
       }
     }
   }

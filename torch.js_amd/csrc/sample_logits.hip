@@ -126,7 +126,7 @@ __device__ __forceinline__ void each_four(const Row<T, NV>& row, F f) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       __builtin_amdgcn_sched_barrier(0);
-      f(row.v[4 * j], row.v[4 * j + 1], row.v[4 * j + 2], row.v[4 * j + 3]);
+      if (j * T < row.n4) f(row.v[4 * j], row.v[4 * j + 1], row.v[4 * j + 2], row.v[4 * j + 3]);
     }
     __builtin_amdgcn_sched_barrier(0);
   } else {
@@ -548,9 +548,11 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
     __syncthreads();
   }
 
-  // index order: the head's elements, the chunks, the tail's elements.  Each
-  // wave adds a run of the chunks up; the first one with the target is cut
-  // into runs again, until one wave's lanes have a chunk each
+  // index order: the head's elements, the chunks, the tail's elements.  The
+  // chunks' weights are added up by runs, and the first run with the target is
+  // looked into.  In registers a wave's 64 chunks of each round are a run;
+  // otherwise each wave adds a run of the chunks up, and the one with the
+  // target is cut into runs again, until one wave's lanes have a chunk each
   const auto in = [&](int i, float x) {
     return (x > tx || (x == tx && i <= ti)) && (double)x - m >= floor_z;
   };
@@ -560,66 +562,109 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
   u64 base = 0, all = 0;
   double target = 0.0;
   int lo = 0, count = row.n4;
-  for (bool whole = true; whole || count > 64; whole = false) {
-    const int per = (count + W - 1) / W;
-    const int c0 = lo + w * per, c1 = min(lo + count, c0 + per);
-    u64 sum = 0;
-    for (int c = c0 + lane; c < c1; c += 256) {
-      float4 x[4];
+  // the head's weight and the target; whether an element of the head is drawn
+  const auto in_head = [&](u64 chunks) {
+    base = lds.edge_w[0] + lds.edge_w[1] + lds.edge_w[2];
+    all = chunks + base + lds.edge_w[3] + lds.edge_w[4] + lds.edge_w[5];
+    target = u * (double)all;
+    if (!base || !((double)base > target)) return false;
+    u64 cum = 0;
+    int i = 0;
+    for (; i < 2; ++i) {
+      cum += lds.edge_w[i];
+      if (lds.edge_w[i] && (double)cum > target) break;
+    }
+    if (t == 0) a.out[r] = i;
+    return true;
+  };
+  if constexpr (NV > 0) {
+    static_assert(NV * W <= T && NV * W <= kBins, "a run a thread");
 #pragma unroll
-      for (int v = 0; v < 4; ++v)  // past the run the last chunk, not counted
-        x[v] = *reinterpret_cast<const float4*>(row.p + row.head + 4 * min(c + 64 * v, c1 - 1));
+    for (int j = 0; j < NV; ++j) {
+      __builtin_amdgcn_sched_barrier(0);
+      u64 sum = 0;
+      if (j * T < row.n4) {
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const int i = row.head + 4 * (c + 64 * v);
-        const float e[4] = {x[v].x, x[v].y, x[v].z, x[v].w};
-        bool k[4];
+        for (int e = 0; e < 4; ++e) {
+          const float x = row.v[4 * j + e];  // past the row -infinity, of weight 0
+          const u64 wx = weight(x);
+          sum += in(row.index(j, e), x) ? wx : 0;
+        }
+        sum = wave_sum_u64(sum);
+      }
+      if (lane == 0) lds.bins[j * W + w] = sum;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (t == 0) lds.pick = kNone;
+    __syncthreads();
+    const u64 mine = t < NV * W ? lds.bins[t] : 0;
+    u64 chunks;
+    const u64 before = b.before(mine, &chunks);
+    if (in_head(chunks)) return;
+    if (mine && (double)(base + before + mine) > target) atomicMin(&lds.pick, t);
+    __syncthreads();
+    const int run = lds.pick;
+    if (run == kNone) {
+      base += chunks;
+      count = -1;
+    } else {
+      if (t == run) lds.first = base + before;
+      __syncthreads();
+      base = lds.first;
+      lo = 64 * run;
+      count = min(64, row.n4 - lo);
+    }
+  } else {
+    for (bool whole = true; whole || count > 64; whole = false) {
+      const int per = (count + W - 1) / W;
+      const int c0 = lo + w * per, c1 = min(lo + count, c0 + per);
+      u64 sum = 0;
+      for (int c = c0 + lane; c < c1; c += 256) {
+        float4 x[4];
 #pragma unroll
-        for (int y = 0; y < 4; ++y) k[y] = c + 64 * v < c1 && in(i + y, e[y]);
-        if (__ballot(k[0] || k[1] || k[2] || k[3])) {  // four weights at a time, no branches
+        for (int v = 0; v < 4; ++v)  // past the run the last chunk, not counted
+          x[v] = *reinterpret_cast<const float4*>(row.p + row.head + 4 * min(c + 64 * v, c1 - 1));
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const u64 wy = weight(e[y]);
-            sum += k[y] ? wy : 0;
+        for (int v = 0; v < 4; ++v) {
+          const int i = row.head + 4 * (c + 64 * v);
+          const float e[4] = {x[v].x, x[v].y, x[v].z, x[v].w};
+          bool k[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) k[y] = c + 64 * v < c1 && in(i + y, e[y]);
+          if (__ballot(k[0] || k[1] || k[2] || k[3])) {  // four weights at a time, no branches
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const u64 wy = weight(e[y]);
+              sum += k[y] ? wy : 0;
+            }
           }
         }
       }
-    }
-    sum = wave_sum_u64(sum);
-    __syncthreads();  // the last round's runs are read, the edges written
-    if (lane == 0) lds.bins[w] = sum;
-    __syncthreads();
-    if (whole) {
-      base = lds.edge_w[0] + lds.edge_w[1] + lds.edge_w[2];
-      for (int i = 0; i < W; ++i) all += lds.bins[i];
-      all += base + lds.edge_w[3] + lds.edge_w[4] + lds.edge_w[5];
-      target = u * (double)all;
-      if (base && (double)base > target) {
-        u64 cum = 0;
-        int i = 0;
-        for (; i < 2; ++i) {
-          cum += lds.edge_w[i];
-          if (lds.edge_w[i] && (double)cum > target) break;
-        }
-        if (t == 0) a.out[r] = i;
-        return;
+      sum = wave_sum_u64(sum);
+      __syncthreads();  // the last round's runs are read, the edges written
+      if (lane == 0) lds.bins[w] = sum;
+      __syncthreads();
+      if (whole) {
+        u64 chunks = 0;
+        for (int i = 0; i < W; ++i) chunks += lds.bins[i];
+        if (in_head(chunks)) return;
       }
-    }
-    int run = -1;
-    for (int i = 0; i < W; ++i) {
-      const u64 v = lds.bins[i];
-      if (v && (double)(base + v) > target) {
-        run = i;
+      int run = -1;
+      for (int i = 0; i < W; ++i) {
+        const u64 v = lds.bins[i];
+        if (v && (double)(base + v) > target) {
+          run = i;
+          break;
+        }
+        base += v;
+      }
+      if (run < 0) {  // not among the chunks (in the first round)
+        count = -1;
         break;
       }
-      base += v;
+      lo += run * per;
+      count = min(per, count - run * per);
     }
-    if (run < 0) {  // not among the chunks (in the first round)
-      count = -1;
-      break;
-    }
-    lo += run * per;
-    count = min(per, count - run * per);
   }
   if (count > 0) {
     if (w != 0) return;
