@@ -107,6 +107,29 @@ def test_forward_and_gradients(torch, case):
 
 
 @gpu
+@pytest.mark.parametrize("case", [(1, 1, 1, 900, 900, 64, 700, 3), (1, 2, 1, 301, 777, 128, 400, 70),
+                                  (2, 1, 1, 270, 270, 20, 256, 0), (1, 1, 1, 2, 1300, 64, 1200, 1)], ids=str)
+def test_slices_with_gradients(torch, case):
+    """Few heads: keys in slices forward, steps in slices backward; the same
+    bits on every run and with or without a gradient."""
+    b, h, hkv, tq, tk, d, window, sinks = case
+    q, k, v, g = inputs(sum(case), b, h, hkv, tq, tk, d)
+    want, bound = reference(q, k, v, window, sinks, g)
+    f = torch.functional.sliding_window_attention
+    runs = []
+    for _ in range(2):
+        ts = [torch.tensor(x, requires_grad=True) for x in (q, k, v)]
+        o = f(*ts, window, sinks)
+        o.backward(torch.tensor(g))
+        runs.append([o.numpy()] + [t.grad.numpy() for t in ts])
+    for name, a, again, w, e in zip(("output", "dq", "dk", "dv"), *runs, want, bound):
+        near(a, w, e, name)
+        np.testing.assert_array_equal(a, again)
+    with torch.no_grad():
+        np.testing.assert_array_equal(f(*ts, window, sinks).numpy(), runs[0][0])
+
+
+@gpu
 @pytest.mark.parametrize("case", [(1, 2, 2, 100, 100, 64), (2, 4, 2, 77, 77, 32)], ids=str)
 def test_equals_full_attention_where_the_window_holds_all(torch, case):
     b, h, hkv, tq, tk, d = case

@@ -39,7 +39,7 @@ struct WinArgs {
   float scale;
   int win, sinks, nst; // nst: key tiles that hold sinks
   int nblk;            // row blocks of a head
-  // forward in slices of `kslice` key tiles (no lse is wanted): part
+  // forward in slices of `kslice` key tiles: part
   // [slice][b*H + h][Tq][D] unscaled sums, pml {maximum, sum}
   float* part;
   float2* pml;
@@ -337,6 +337,7 @@ __global__ __launch_bounds__(256) void k_win_merge(WinArgs a, int64_t n4, int ns
   const int64_t b = bh / a.H, h = bh % a.H;
   *reinterpret_cast<floatx4*>(a.out + b * a.os.b + h * a.os.h + q * a.os.t + 4 * c) =
       o * (1.0f / den);
+  if (a.lse_out && c == 0) a.lse_out[row] = top + __log2f(den);
 }
 
 // Few queries (a decoding step): one query head and position a workgroup,
@@ -764,17 +765,18 @@ int launch_bwd(WinArgs a, unsigned keys, float* dq, const int64_t* dq_st) {
   return check_launch("window_dq");
 }
 
-// Over how many workgroups the query heads of a key block are split.  The
+// Over how many workgroups the steps of a key block are split.  The
 // workgroups are about equally long, so the last round that they fill the CUs
 // in stands half empty on average; each split costs a prologue of some 3
 // steps, and its sums' way through memory about 2.  4 key heads of 8192, 4
 // query heads each (508 workgroups of 140 steps on 512 places): 1424 us, as
-// two splits 1315, as four 1292.
+// two splits 1315, as four 1292; one head of 4096, D 64, window 2000, the
+// whole backward: 300 us, split 171.
 int key_splits(const WinArgs& a, int64_t nbkv, int64_t tiles) {
   const int64_t cus = num_cus() > 0 ? num_cus() : 256, places = cus * (a.D <= 64 ? 3 : 2);
   int best = 1;
   int64_t cost = 0;
-  for (int n = 1; n <= a.G && n <= 8; ++n) {
+  for (int n = 1; n <= 8 && n <= tiles * a.G; ++n) {
     const int64_t each = cdiv(tiles * a.G, n) + 3;
     const int64_t c = 2 * nbkv * a.nblk * n * each / places + each + (n > 1 ? 4 * n : 0);
     if (n == 1 || c < cost) {
@@ -855,7 +857,7 @@ int tjh_window_forward(const float* q, const float* k, const float* v, float* o,
   };
   if (Tq <= 4) {
     int64_t n = 1;
-    if (!lse && rows < cus && most > 512)
+    if (rows < cus && most > 512)
       n = cdiv(most, 256) < cus / rows ? cdiv(most, 256) : cus / rows;
     a.kslice = (int)cdiv(most, n);
     n = cdiv(most, a.kslice);
@@ -874,14 +876,14 @@ int tjh_window_forward(const float* q, const float* k, const float* v, float* o,
   a.nblk = (int)cdiv(Tq, ROWS);
   const int64_t blocks = B * H * a.nblk;
   // slices of the key tiles where the blocks of queries leave CUs idle and
-  // have enough tiles to pay for the join
+  // a wave is spared four tiles or more, some 3 us each, for the join.  2 heads
+  // of 3000, D 128, window 1000: 173 us, in slices 54; 3 of 300, D 64, window
+  // 100 (4 spared): 22, 16; 16 of 1500, D 64, window 300 (3 spared): 39, 46
   const int64_t wt = cdiv((int64_t)a.win + TILE - 2, TILE) + 1 + a.nst, all = cdiv(Tk, TILE);
   const int64_t nt = wt < all ? wt : all;  // tiles of 32 queries at most
   int64_t n = 1;
-  if (!lse && blocks < cus && nt > 4) {
-    a.kslice = (int)(cdiv(nt * blocks, cus) < 2 ? 2 : cdiv(nt * blocks, cus));
-    n = cdiv(nt, a.kslice);
-  }
+  a.kslice = (int)(cdiv(nt * blocks, cus) < 2 ? 2 : cdiv(nt * blocks, cus));
+  if (blocks < cus && nt - a.kslice >= 4) n = cdiv(nt, a.kslice);
   Scratch s(n > 1 ? (size_t)(n * rows * (D + 2)) * sizeof(float) : 0);
   const bool split = n > 1 && room(s, n);
   const dim3 grid((unsigned)blocks, split ? (unsigned)n : 1);

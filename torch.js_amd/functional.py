@@ -1083,8 +1083,10 @@ def sliding_window_attention(query, key, value, window, sinks=0, scale=None):
     a prompt over a cache, or one decoding step.  The query at position i
     sees the keys j <= i with j > i - window or j < sinks; what other keys
     and values hold has no part in its output.  O(Tk) memory beside the
-    result, time by the keys seen.  Head dims up to 128; the gradients of
-    key and value are summed over the query heads that read them."""
+    result, time by the keys seen.  Head dims up to 128 (operands are copied
+    where one is no multiple of 4 or rows are not 16-byte aligned); the
+    gradients of key and value are summed over the query heads that read
+    them."""
     if type(window) is not int or window < 1 or window > 1 << 30:
         window = _whole("window", window, 1)
     if type(sinks) is not int or sinks < 0 or sinks > 1 << 30:

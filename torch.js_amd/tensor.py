@@ -2737,8 +2737,8 @@ def topk(x, k, dim=-1, largest=True):
     """Tensor.topk (Tensor.ts:3048-3178) on the device: (values, int32
     indices) of the k largest (smallest) elements along `dim`, sorted by
     value, equal ones by ascending index; NaN counts as the largest, as in
-    PyTorch.  k up to 1024.  The values' gradient goes back to the elements
-    they came from."""
+    PyTorch.  k up to 1024; other dtypes are compared as float32.  The
+    values' gradient goes back to the elements they came from."""
     k = int(k)
     if x.ndim == 0:
         v, i = topk(reshape(x, (1,)), k, 0, largest)
