@@ -665,8 +665,10 @@ __global__ __launch_bounds__(256) void k_win_sums(WinArgs a, const float* __rest
 // Query kernel: dQ^T += K^T dS^T from the stored dS blocks, one wave 32
 // queries, the next tile's operands on their way during a tile's products.
 // Half the products of a tile for the same loads as the forward's: the sizes
-// of k_win_fwd, 58 us, 49 TFLOP/s of the keys seen; 375 us, 87.
-template <int HD>
+// of k_win_fwd, 58 us, 49 TFLOP/s of the keys seen; 375 us, 87.  JOIN: where
+// that leaves CUs idle, a workgroup's waves have a quarter each of the tiles
+// of the same 32 queries and add their sums up in order.
+template <int HD, bool JOIN>
 __global__ __launch_bounds__(256, HD <= 64 ? 3 : HD <= 96 ? 2 : 1) void k_win_dq(WinArgs a) {
   using S_ = Hd<HD>;
   __shared__ __attribute__((aligned(16))) float buf[WAVES][TILE * S_::W];
@@ -674,13 +676,14 @@ __global__ __launch_bounds__(256, HD <= 64 ? 3 : HD <= 96 ? 2 : 1) void k_win_dq
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l32 = lane & 31, h = lane >> 5;
   const int item = xcd_item(blockIdx.x, gridDim.x);
-  const int64_t bhl = item / a.nblk;  // from the launch's first head on
-  const int qb = item % a.nblk;
+  const int per_head = JOIN ? a.nqt : a.nblk;
+  const int64_t bhl = item / per_head;  // from the launch's first head on
+  const int qb = item % per_head;
   const int64_t bh = (int64_t)a.bkv0 * a.G + bhl;
   const int64_t b = bh / a.H, hh = bh % a.H;
   const float* K = a.k + b * a.ks.b + (hh / a.G) * a.ks.h;
-  const int q0 = qb * ROWS + w * TILE, lo = a.off + q0;
-  if (q0 >= a.Tq) return;
+  const int q0 = JOIN ? qb * TILE : qb * ROWS + w * TILE, lo = a.off + q0;
+  if (q0 >= a.Tq) return;  // JOIN: never
   const float* dsrow = a.dsblk + (bhl * a.nqt + q0 / TILE) * a.nsl * (TILE * TILE) + l32 * TILE +
                        h * 16;
   const Tiles tiles(a, lo, min(lo + TILE, a.Tk) - 1);
@@ -702,17 +705,37 @@ __global__ __launch_bounds__(256, HD <= 64 ? 3 : HD <= 96 ? 2 : 1) void k_win_dq
 #pragma unroll
       for (int c = 0; c < S_::NC; ++c) dq[c] = mfma(k[c][s], d[s >> 2][s & 3], dq[c]);
   };
-  float k0[S_::NC][16], k1[S_::NC][16];
-  floatx4 d0[4], d1[4];
-  load(tiles(0), k0, d0);
-  for (int i = 0; i < tiles.n; i += 2) {
-    load(tiles(min(i + 1, tiles.n - 1)), k1, d1);
-    products(tiles(i), k0, d0);
-    load(tiles(min(i + 2, tiles.n - 1)), k0, d0);
-    if (i + 1 < tiles.n) products(tiles(i + 1), k1, d1);
+  const int per = JOIN ? (tiles.n + WAVES - 1) / WAVES : tiles.n;
+  const int i0 = JOIN ? min(w * per, tiles.n) : 0, i1 = min(i0 + per, tiles.n);
+  if (!JOIN || i0 < i1) {
+    float k0[S_::NC][16], k1[S_::NC][16];
+    floatx4 d0[4], d1[4];
+    load(tiles(i0), k0, d0);
+    for (int i = i0; i < i1; i += 2) {
+      load(tiles(min(i + 1, i1 - 1)), k1, d1);
+      products(tiles(i), k0, d0);
+      load(tiles(min(i + 2, i1 - 1)), k0, d0);
+      if (i + 1 < i1) products(tiles(i + 1), k1, d1);
+    }
   }
-  write_rows<HD, false>(buf[w], dq, a.scale, a.out + b * a.o1s.b + hh * a.o1s.h, a.o1s.t, q0, a.Tq,
-                        a.D, l32, h, lane);
+  float* out = a.out + b * a.o1s.b + hh * a.o1s.h;
+  if constexpr (!JOIN) {
+    write_rows<HD, false>(buf[w], dq, a.scale, out, a.o1s.t, q0, a.Tq, a.D, l32, h, lane);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+#pragma unroll
+      for (int c = 0; c < S_::NC; ++c) buf[w][l32 * S_::W + c * 32 + kappa(j, h)] = dq[c][j];
+    __syncthreads();
+    for (int f = threadIdx.x; f < TILE * S_::F4; f += 256) {
+      const int row = f / S_::F4, c4 = f % S_::F4, at = row * S_::W + 4 * c4;
+      if (q0 + row >= a.Tq || 4 * c4 >= a.D) continue;
+      floatx4 sum = *reinterpret_cast<const floatx4*>(&buf[0][at]);
+#pragma unroll
+      for (int i = 1; i < WAVES; ++i) sum += *reinterpret_cast<const floatx4*>(&buf[i][at]);
+      *reinterpret_cast<floatx4*>(out + (int64_t)(q0 + row) * a.o1s.t + 4 * c4) = sum * a.scale;
+    }
+  }
 }
 
 // ------------------------------------------------------------ host
@@ -760,8 +783,14 @@ int launch_bwd(WinArgs a, unsigned keys, float* dq, const int64_t* dq_st) {
   a.nblk = (int)cdiv(a.Tq, ROWS);
   a.out = dq;
   a.o1s = s3(dq_st);
-  const unsigned grid = (unsigned)(a.nbkv * a.G * a.nblk);
-  tjh_launch(k_win_dq<HD>, dim3(grid), dim3(256), 0, stream(), a);
+  const unsigned heads = (unsigned)(a.nbkv * a.G), grid = heads * a.nblk;
+  // the whole backward of one head of 4096, window 2000 (32 workgroups): 171
+  // us, joined 115; 12 of 1024, all seen (96): 116, 102; 8 x 4 of 700, window
+  // 64 (192): 81, 83
+  if (3 * (int64_t)grid <= 2 * (num_cus() > 0 ? num_cus() : 256))
+    tjh_launch(k_win_dq<HD, true>, dim3(heads * a.nqt), dim3(256), 0, stream(), a);
+  else
+    tjh_launch(k_win_dq<HD, false>, dim3(grid), dim3(256), 0, stream(), a);
   return check_launch("window_dq");
 }
 
