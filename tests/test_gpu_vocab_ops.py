@@ -1,6 +1,7 @@
 """Tensor.topk, F.distillation_loss and F.sample_logits against plain numpy in
 64 bits."""
 import math
+import sys
 import types
 
 import numpy as np
@@ -620,6 +621,104 @@ def test_distillation_in_a_graph(torch):
         want.backward()
         assert got[0] == want.item()
         np.testing.assert_array_equal(got[1], e.grad.numpy())
+
+
+class _Memory:
+    """A library that computes nothing: it hands out and takes back addresses
+    and notes the logits that tjh_distill is given."""
+
+    def __init__(self):
+        self.live, self.at, self.read = {}, 1 << 20, []
+
+    def __getattr__(self, name):
+        return lambda *args: 0
+
+    def tjh_malloc(self, n, out):
+        self.at += 1 << 20
+        self.live[self.at] = n
+        out._obj.value = self.at
+        return 0
+
+    def tjh_free(self, p):
+        del self.live[p]
+        return 0
+
+    def tjh_distill(self, px, *args):
+        self.read.append(any(p <= px < p + n for p, n in self.live.items()))
+        return 0
+
+
+@pytest.mark.parametrize("view", ["shifted", "transposed", "columns"])
+def test_distillation_reads_memory_of_its_own(pkg, monkeypatch, view):
+    """Logits that had to be copied are there until the last backward."""
+    from torchjs_amd import _lib as L
+    mem = _Memory()
+    with monkeypatch.context() as m:
+        m.setattr(L, "_lib", mem)
+        m.setitem(sys.modules["torchjs_amd.tensor"]._state, "init", True)
+        v, ids = pkg.empty((2, 3, 4)), pkg.empty((2, 3, 4), "int32")
+        for reduction in ("none", "mean"):
+            w = pkg.empty({"shifted": (2, 4, 9), "transposed": (2, 9, 3), "columns": (2, 3, 18)}[view])
+            y = w.requires_grad_(True)
+            z = {"shifted": lambda: y[:, :3], "transposed": lambda: y.transpose(1, 2),
+                 "columns": lambda: y.view(2, 3, 9, 2)[:, :, :, 0]}[view]()
+            assert z.shape == (2, 3, 9)
+            out = pkg.functional.distillation_loss(z, v, ids, reduction=reduction)
+            del z
+            g = pkg.empty(out.shape)
+            out.backward(g, retain_graph=True)
+            out.backward(g)
+            del out, y, w, g
+        del v, ids
+        assert mem.read == [True] * 6
+
+
+@gpu
+@pytest.mark.parametrize("view", ["shifted", "transposed", "columns", "one column apart"])
+def test_distillation_of_logits_that_are_copied(torch, view):
+    """Views whose rows are not evenly spaced or not dense, with upstream
+    gradients that the forward could not know and other tensors of the
+    copy's size made and dropped before the backward."""
+    F = torch.functional
+    rng = np.random.default_rng(4)
+    b, t, n = 2, 5, 3001
+    full = (rng.standard_normal((b, t + 1, n + 1)) * 2).astype(np.float32)
+    pick = {"shifted": lambda y: y[:, :-1, :n], "transposed": lambda y: y.transpose(1, 2)[:, :, :t],
+            "columns": lambda y: y.view(b, t + 1, (n + 1) // 2, 2)[:, :, :, 0],
+            "one column apart": lambda y: y[:, 1:, 1:]}[view]
+    host = {"shifted": lambda y: y[:, :-1, :n], "transposed": lambda y: y.swapaxes(1, 2)[:, :, :t],
+            "columns": lambda y: y[:, :, ::2], "one column apart": lambda y: y[:, 1:, 1:]}[view]
+    x = np.ascontiguousarray(host(full))
+    rows, c = x.shape[0] * x.shape[1], x.shape[2]
+    v = (rng.standard_normal(x.shape[:2] + (4,)) * 2).astype(np.float32)
+    ids = rng.integers(0, c, v.shape).astype(np.int32)
+    up = rng.standard_normal(x.shape[:2]).astype(np.float32)
+
+    def grads(y, z, reduction, twice):
+        out = F.distillation_loss(z, torch.tensor(v), torch.tensor(ids), 2.0, reduction)
+        del z
+        for _ in range(4):  # takes a freed copy's memory, if there is one
+            torch.full(x.shape, 1e9)
+        if reduction == "none":
+            out.backward(torch.tensor(up))
+        elif twice:
+            out.backward(retain_graph=True)
+            torch.full(x.shape, 1e9)
+            out.backward()
+        else:
+            (out * 0.5 + (y * y).sum() * 0.25).backward()
+        return y.grad.numpy()
+    for reduction, twice in (("none", False), ("mean", False), ("sum", True)):
+        tf, tx = torch.tensor(full, requires_grad=True), torch.tensor(x, requires_grad=True)
+        got = host(grads(tf, pick(tf), reduction, twice))
+        want = grads(tx, tx, reduction, twice)
+        assert got.shape == want.shape and np.isfinite(want).all()
+        # both are off from the formula by at most _bounds times T (q (1 + |ln
+        # q|) + sum p (1 + |ln p|)) <= 2 (2 + ln 4), a row's factor and twice
+        # that where two gradients are added, and by a rounding of the sum
+        # with the other loss's share
+        tol = 2 * _bounds(c, 16) * 6.8 * max(1, np.abs(up).max()) * (2 if twice else 1)
+        assert np.abs(got - want).max() <= tol + 2 * U * np.abs(want).max(), (reduction, twice)
 
 
 # ------------------------------------------------------------------ refusals

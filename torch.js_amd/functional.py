@@ -359,9 +359,11 @@ def distillation_loss(input, teacher_logits, teacher_ids, temperature=1.0, reduc
         if d is None or g is not _T._unit_seed["g"] or me[0] != _T._unit_seed["node"]:
             g = g.contiguous()
             d = grad_buffer()
-            L.check(L.lib().tjh_distill(px, ld, rows, cols, v.data_ptr(), ids.data_ptr(), k, temp,
-                                        red, g.data_ptr(), None, None, d.data_ptr(),
-                                        d._strides[0]), "distillation_loss_backward")
+            # by xd, which may be a copy that lives by this closure alone
+            L.check(L.lib().tjh_distill(xd.data_ptr(), ld, rows, cols, v.data_ptr(),
+                                        ids.data_ptr(), k, temp, red, g.data_ptr(), None, None,
+                                        d.data_ptr(), d._strides[0]),
+                    "distillation_loss_backward")
         return [reshape_raw(d, xs) if len(xs) != 2 else d]
 
     def gbwd(g):  # log_softmax at the ids, weighted by the teacher's probabilities
