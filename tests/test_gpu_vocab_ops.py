@@ -297,6 +297,26 @@ def test_sample_logits_nucleus_in_one_bin(torch, n):
 
 
 @gpu
+@pytest.mark.parametrize("n", [1500, 4000, 16001, 50257, 60001])
+def test_sample_logits_nucleus_ends_among_ties(torch, n):
+    """Logits of a few values: a list holds what can be drawn, and the bin in
+    which the nucleus ends holds more than the short sort takes."""
+    rng = np.random.default_rng(n)
+    rows = 64
+    x = np.full((rows, n), -40, np.float32)
+    for r in range(rows):
+        at = rng.permutation(n)[:min(n, 3900)]
+        x[r, at] = -0.7 * rng.integers(0, 3, at.size)
+    u = rng.random(rows).astype(np.float32)
+    for kw in (dict(top_p=0.35), dict(top_p=0.77), dict(top_p=0.97), dict(top_p=0.6, min_p=0.3),
+               dict(top_p=0.8, top_k=1200)):
+        ref = [sample_ref(x[r], float(u[r]), **kw) for r in range(rows)]
+        for _ in range(2):
+            got = torch.functional.sample_logits(torch.tensor(x), torch.tensor(u), **kw)
+            assert got.numpy().tolist() == ref, kw
+
+
+@gpu
 @pytest.mark.parametrize("n", [9001, 600000, 2 ** 20])
 def test_sample_logits_of_neighbours(torch, n):
     """All that can be drawn stands side by side."""

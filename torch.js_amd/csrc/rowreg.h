@@ -403,10 +403,13 @@ __device__ __forceinline__ u64* sort_list(SelectLds<T, CAP>& s, int c) {
 }
 
 // The elements for which in(j, u, x) holds into the list, in no order (it is
-// sorted next): their number, of which the first CAP were stored.
+// sorted next): their number, of which the first CAP were stored.  The first
+// barrier is for callers that chose this by reading s.count: all waves have
+// read it before it is cleared.
 template <int T, int CAP, class In>
 __device__ __forceinline__ int gather_list(const Row<T, 0>& row, uint32_t nan, In in,
                                            SelectLds<T, CAP>& s) {
+  __syncthreads();
   if (threadIdx.x == 0) s.count = 0;
   __syncthreads();
   row.each([&](int j, int u, float x) {
