@@ -460,3 +460,23 @@ def test_refusals_of_the_library(torch):
     assert forward(d=6) == 5 and forward(d=132) == 5 and forward(ptr=p + 4) == 5
     assert forward(strides=L.i64arr((128, 64, 9))) == 5
     assert forward(tq=0, ptr=None) == 0
+
+
+@gpu
+def test_rows_whose_grid_does_not_fit_are_refused(torch):
+    """2^32 threads or more, by sizes alone: nothing is launched or read."""
+    from torchjs_amd import _lib as L
+    x = torch.zeros(1, 1, 8, 8)
+    p, st = x.data_ptr(), L.i64arr((0, 0, 8))
+    sts = (L.P_i64 * 8)(*[L.ctypes.cast(st, L.P_i64)] * 8)
+
+    def calls(b, h, tq):
+        f = L.lib().tjh_window_forward(p, p, p, p, None, b, h, h, tq, 8, 8, st, st, st, st, 1.0, 3, 0)
+        g = L.lib().tjh_window_backward(p, p, p, p, p, p, p, p, p, b, h, h, tq, 8, 8, sts, 1.0, 3, 0)
+        return f, g
+    # a query takes 512 threads where there are at most four, a tile of up to
+    # 32 takes 256
+    for b, h, tq in ((2 ** 23, 1, 1), (1, 2 ** 23 + 1, 1), (2 ** 22, 1, 2), (2 ** 21, 2, 4),
+                     (1398102, 2, 3), (2 ** 24, 1, 5), (2 ** 12, 2 ** 12, 8), (2 ** 29, 2 ** 29, 8)):
+        assert calls(b, h, tq) == (1, 1), (b, h, tq)
+        assert b"too large" in L.lib().tjh_last_error()

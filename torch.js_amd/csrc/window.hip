@@ -825,9 +825,12 @@ int check_window(const char* who, int64_t B, int64_t H, int64_t Hkv, int64_t Tq,
           (long long)sinks);
   TJH_ARG(H == 0 || (Hkv > 0 && H % Hkv == 0), "%s: %lld heads over %lld", who, (long long)H,
           (long long)Hkv);
-  TJH_ARG(Tk < (int64_t(1) << 30) && H < (int64_t(1) << 30), "%s: too large", who);
-  // a grid has less than 2^32 threads, and Tq <= 4 takes a workgroup of 256 a query
-  TJH_ARG(B * H * (Tq <= 4 ? Tq : cdiv(Tq, TILE)) < (int64_t(1) << 24), "%s: too large", who);
+  TJH_ARG(Tk < (int64_t(1) << 30) && B < (int64_t(1) << 30) && H < (int64_t(1) << 30),
+          "%s: too large", who);
+  // a grid has less than 2^32 threads: up to 4 queries take kFewThreads each in
+  // the forward, a tile of 32 at most 256
+  const int64_t groups = Tq <= 4 ? Tq * (kFewThreads / 256) : cdiv(Tq, TILE);
+  TJH_ARG(groups == 0 || B * H <= ((int64_t(1) << 24) - 1) / groups, "%s: too large", who);
   for (int i = 0; i < n; ++i) TJH_ARG(strides[i], "%s: NULL strides", who);
   bool wide = false;
   for (int i = 0; i < n; ++i) wide |= strides[i][2] >= kMaxRowStride || strides[i][2] < 0;
