@@ -741,6 +741,35 @@ def test_distillation_of_logits_that_are_copied(torch, view):
         assert np.abs(got - want).max() <= tol + 2 * U * np.abs(want).max(), (reduction, twice)
 
 
+@gpu
+@pytest.mark.parametrize("n,k", [(9, 3), (900, 70), (900, 200), (3000, 300), (50257, 600), (60001, 5)])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_distillation_teacher_of_nan_or_infinity(torch, n, k, value):
+    """Such an entry makes its row's loss and whole gradient NaN wherever it
+    stands, and leaves the other rows and entries that are none alone."""
+    rng = np.random.default_rng(k)
+    x, v, _ = _distill_inputs(rng, 6, n, k)
+    ids = rng.integers(0, n, (6, k)).astype(np.int32)
+    v[0, 0] = v[1, k - 1] = v[2, 0] = value
+    v[2, 1:] = -np.inf  # and nothing else
+    v[3, 0] = value
+    ids[3, 0] = n  # none
+    want = distill_ref(x[3:], v[3:], ids[3:], 1.5)
+    tx = torch.tensor(x, requires_grad=True)
+    call = lambda red: torch.functional.distillation_loss(tx, torch.tensor(v), torch.tensor(ids), 1.5, red)
+    out = call("none")
+    out.backward(torch.tensor(np.ones(6, np.float32)))
+    got, grad = out.numpy(), tx.grad.numpy()
+    assert np.isnan(got[:3]).all() and np.isnan(grad[:3]).all()
+    c = _bounds(n, 4 * math.ceil(n / (4 * 64 if n <= 1024 else 4 * 256)) + 4)
+    assert (np.abs(got[3:] - want[0]) <= c * want[3]).all()
+    assert (np.abs(grad[3:] - want[1]) <= c * want[4]).all()
+    assert math.isnan(call("mean").item())
+    (d,) = torch.autograd.grad(call("sum"), tx, create_graph=True)
+    d = d.detach().numpy()
+    assert np.isnan(d[:3]).all() and np.isfinite(d[3:]).all()
+
+
 # ------------------------------------------------------------------ refusals
 
 

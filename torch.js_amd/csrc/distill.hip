@@ -96,21 +96,21 @@ __global__ __launch_bounds__(T, T == 512 ? 4 : 1) void k_distill(DistillArgs a) 
   row.load(a.x + r * a.ld, a.n);
   // the teacher's entries, while the row is on its way
   float mt = -INFINITY;
+  bool bad = false;
   for (int i = t; i < K; i += T) {
     const int32_t c = a.ids[r * K + i];
     const float v = a.v[r * K + i];
     const bool in = (unsigned)c < (unsigned)a.n;
     id[i] = in ? c : -1;
     p[i] = in ? v : -INFINITY;
-    mt = in ? (v != v ? v : fmaxf(mt, v)) : mt;
+    mt = in ? fmaxf(mt, v) : mt;  // NaN takes no part
+    bad |= in && v != v;
   }
   float count = 0.f;  // of valid rows, this thread's part
   if (a.valid && a.d)
     for (int64_t i = t; i < a.rows; i += T) count += a.valid[i];
-  // a NaN entry makes the row's loss and gradient NaN, as log_softmax would
-  const bool nan = b.any(mt != mt);
-  mt = b.max(mt != mt ? -INFINITY : mt);
-  const bool valid = nan || mt > -INFINITY;
+  mt = b.max(mt);
+  const bool valid = b.any(bad) || mt > -INFINITY;
   if (!valid) {
     if (t == 0 && a.loss_rows) a.loss_rows[r] = 0.f;
     if (a.d) {
@@ -125,8 +125,10 @@ __global__ __launch_bounds__(T, T == 512 ? 4 : 1) void k_distill(DistillArgs a) 
     const float e = __builtin_amdgcn_exp2f((p[i] - mt) * c2);
     st += e;
   }
+  // an entry of NaN or +infinity makes this NaN, and with it the row's loss and
+  // whole gradient, as q_j times the sum of the probabilities would be
   st = b.sum(st);
-  const float lst = logf(st), ist = (nan ? NAN : 1.0f) / st;
+  const float lst = logf(st), ist = 1.0f / st;
   // the student's
   float mx = -INFINITY;
   row.each([&](int, int, float x) { mx = fmaxf(mx, x); });
@@ -152,7 +154,7 @@ __global__ __launch_bounds__(T, T == 512 ? 4 : 1) void k_distill(DistillArgs a) 
   if (a.valid) g /= b.sum(count);
   else if (a.denom) g /= a.denom[0];
   g *= a.temp;
-  const float gq = g / s;
+  const float gq = st == st ? g / s : NAN;
   float* __restrict__ d = a.d + r * a.ldd;
   const auto grad = [&](float x) { return __builtin_amdgcn_exp2f((x - mx) * c2) * gq; };
   if (row.edge_index >= 0) d[row.edge_index] = grad(row.edge);

@@ -388,8 +388,9 @@ def _teacher(v, ids, cols, temp, red, rows):
         there = (hid >= 0) & (hid < cols)
         h = np.where(there, h, -np.inf)
         m = h.max(-1, keepdims=True)
-        valid = m > -np.inf
-        e = np.where(valid, np.exp(h - np.where(valid, m, 0.0)), 0.0)
+        valid = m != -np.inf  # a row with NaN or +infinity is NaN throughout
+        with np.errstate(invalid="ignore"):  # infinity less infinity
+            e = np.where(valid, np.exp(h - np.where(valid, m, 0.0)), 0.0)
         p = e / np.where(valid, e.sum(-1, keepdims=True), 1.0)
         lp = np.log(np.where(p > 0, p, 1.0))
         den = max(int(valid.sum()), 1) if red == 1 else rows if red == 3 else 1
