@@ -770,6 +770,37 @@ def test_distillation_teacher_of_nan_or_infinity(torch, n, k, value):
     assert np.isnan(d[:3]).all() and np.isfinite(d[3:]).all()
 
 
+@gpu
+def test_distillation_second_derivative_beside_masked_logits(torch):
+    """Logits of -infinity where the teacher has no probability: entries that
+    are none stand for column 0, others are -infinity or underflow."""
+    rng = np.random.default_rng(16)
+    x, v, ids = _distill_inputs(rng, 3, 9, 4)
+    x[:, 0] = x[2, 7] = -np.inf
+    ids[:] = [[1, -1, 5, 9], [0, 2, 3, 4], [7, 1, 2, 8]]
+    v[1, 0] = -np.inf
+    v[2, 0] = -1000
+    w = rng.standard_normal((3, 9)).astype(np.float32)
+    fin = x > -np.inf
+    q = np.where(fin, np.exp(np.where(fin, x, 0.0).astype(np.float64)), 0.0)
+    q /= q.sum(1, keepdims=True)
+    h = np.where((ids >= 0) & (ids < 9), v.astype(np.float64), -np.inf)
+    p = np.exp(h - h.max(1, keepdims=True))
+    p /= p.sum(1, keepdims=True)
+    first = q.copy()
+    for r in range(3):
+        np.add.at(first[r], np.clip(ids[r], 0, 8), -p[r])
+    for red in ("sum", "none"):
+        tx = torch.tensor(x, requires_grad=True)
+        out = torch.functional.distillation_loss(tx, torch.tensor(v), torch.tensor(ids), 1.0, red)
+        assert np.isfinite(out.numpy()).all()
+        (d,) = torch.autograd.grad(out.sum(), tx, create_graph=True)
+        # a dozen float32 operations on values of at most 4, here and below
+        assert np.abs(d.detach().numpy() - first).max() <= 100 * U
+        (dd,) = torch.autograd.grad((d * torch.tensor(w)).sum(), tx)
+        assert np.abs(dd.numpy() - q * (w - (q * w).sum(1, keepdims=True))).max() <= 100 * U
+
+
 # ------------------------------------------------------------------ refusals
 
 

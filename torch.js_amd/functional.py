@@ -367,10 +367,11 @@ def distillation_loss(input, teacher_logits, teacher_ids, temperature=1.0, reduc
         return [reshape_raw(d, xs) if len(xs) != 2 else d]
 
     def gbwd(g):  # log_softmax at the ids, weighted by the teacher's probabilities
-        p, lp, den = _teacher(v, ids, cols, temp, red, rows)
+        p, lp, drop, den = _teacher(v, ids, cols, temp, red, rows)
 
         def ref(xx):
             lq = _T.gather(log_softmax(mul(xx, 1.0 / temp), -1), -1, p[1])
+            lq = _T.masked_fill(lq, drop, 0.0)  # 0 times -infinity is none
             per = mul(_T.reduce_sum(mul(p[0], sub(lp, lq)), -1), temp * temp)
             return per if red == 0 else mul(_T.reduce_sum(per), 1.0 / den)
         return _T._regrad(ref, [x], g)
@@ -381,8 +382,9 @@ def distillation_loss(input, teacher_logits, teacher_ids, temperature=1.0, reduc
 
 def _teacher(v, ids, cols, temp, red, rows):
     """Constants of the distillation loss for its differentiable backward:
-    ((probabilities, ids inside [0, cols)), their logarithms, the divisor),
-    computed without recording.  Entries that are none have probability 0."""
+    ((probabilities, ids inside [0, cols)), their logarithms, where they are
+    0, the divisor), computed without recording.  Entries that are none have
+    probability 0."""
     with _T.no_grad():
         h, hid = v.numpy().astype(np.float64) / temp, ids.numpy()
         there = (hid >= 0) & (hid < cols)
@@ -393,10 +395,11 @@ def _teacher(v, ids, cols, temp, red, rows):
             e = np.where(valid, np.exp(h - np.where(valid, m, 0.0)), 0.0)
         p = e / np.where(valid, e.sum(-1, keepdims=True), 1.0)
         lp = np.log(np.where(p > 0, p, 1.0))
+        p = p.astype(np.float32)
         den = max(int(valid.sum()), 1) if red == 1 else rows if red == 3 else 1
-        return ((_T.tensor(p.astype(np.float32)),
+        return ((_T.tensor(p),
                  _T.tensor(np.where(there, hid, 0).astype(np.int32), dtype="int32")),
-                _T.tensor(lp.astype(np.float32)), float(den))
+                _T.tensor(lp.astype(np.float32)), _T.tensor(p == 0), float(den))
 
 
 def _setting(name, value, rows, dtype, lo, hi):
