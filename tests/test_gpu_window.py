@@ -414,6 +414,30 @@ def test_graphs_and_eager_work_between(torch):
                 np.testing.assert_array_equal(a.numpy(), w)
 
 
+@gpu
+@pytest.mark.parametrize("hkv", [1, 2])
+def test_second_derivative_beside_what_is_not_seen(torch, hkv):
+    """Keys and values that no query sees may hold anything there too."""
+    q, k, v, g = inputs(16, 1, 2, hkv, 4, 12, 8)
+    f = torch.functional.sliding_window_attention
+    hidden = ~visible(4, 12, 3, 2).any(0)
+    assert hidden.sum() == 4
+
+    def derivatives(fill):
+        x = [q, k.copy(), v.copy()]
+        for y in x[1:]:
+            y[:, :, hidden] = fill
+        ts = [torch.tensor(y, requires_grad=True) for y in x]
+        grads = torch.autograd.grad((f(*ts, 3, 2) * torch.tensor(g)).sum(), ts, create_graph=True)
+        loss = sum(((y * y).sum() for y in grads[1:]), (grads[0] * grads[0]).sum())
+        return [y.detach().numpy() for y in list(grads) + list(torch.autograd.grad(loss, ts))]
+    want = derivatives(0.0)
+    for fill in (np.nan, np.inf, -np.inf, 3e38):
+        for a, w in zip(derivatives(fill), want):
+            assert np.isfinite(w).all()
+            np.testing.assert_array_equal(a, w)
+
+
 # ------------------------------------------------------------------ refusals
 
 

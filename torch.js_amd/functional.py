@@ -1159,9 +1159,14 @@ def sliding_window_attention(query, key, value, window, sinks=0, scale=None):
     def gbwd(g):  # softmax over explicit scores with recording ops
         i = np.arange(Tk - Tq, Tk)[:, None]
         j = np.arange(Tk)
-        drop = _T.tensor(~((j <= i) & ((j > i - window) | (j < sinks))))
+        seen = (j <= i) & ((j > i - window) | (j < sinks))
+        drop = _T.tensor(~seen)
+        unseen = ~seen.any(0)  # by no query: 0 times what they hold is none
 
         def ref(qq, kk, vv):
+            if unseen.any():
+                mask = _T.tensor(unseen[:, None])
+                kk, vv = _T.masked_fill(kk, mask, 0.0), _T.masked_fill(vv, mask, 0.0)
             if H != Hkv:
                 kk, vv = [reshape(_T.expand(reshape(t, (B, Hkv, 1, Tk, D)),
                                             (B, Hkv, H // Hkv, Tk, D)), (B, H, Tk, D))
