@@ -127,3 +127,12 @@ def test_generate_says_when_there_is_nothing_to_draw(torch):
         student.generate(_ids(torch, 1, 5), 3, top_k=4)
     with pytest.raises(ValueError, match="top_p"):
         student.generate(_ids(torch, 1, 5), 3, top_p=2.0)
+
+
+def test_generate_from_a_prompt_with_ids_out_of_range(torch):
+    """A prompt's ids are clamped as the embedding does; only drawn ones of -1
+    say that there was nothing to draw."""
+    _, student = _models(torch)
+    prompt = torch.tensor(np.array([[-1, 5, 9]], np.int32))
+    seq = student.generate(prompt, 4, top_k=5).numpy()
+    assert seq[0, :3].tolist() == [-1, 5, 9] and (seq[0, 3:] >= 0).all()

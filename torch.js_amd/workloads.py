@@ -335,7 +335,7 @@ class GPT2(nn.Module):
                 logits = self.forward_cached(nxt, cache, pos)
                 pos += 1
             res = cat(out, 1)
-            if cut and not greedy and (res.numpy() < 0).any():
+            if cut and not greedy and (res.numpy()[:, T:] < 0).any():
                 raise RuntimeError("generate: logits hold NaN, infinity or nothing to draw")
             return res
 
