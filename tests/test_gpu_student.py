@@ -136,3 +136,11 @@ def test_generate_from_a_prompt_with_ids_out_of_range(torch):
     prompt = torch.tensor(np.array([[-1, 5, 9]], np.int32))
     seq = student.generate(prompt, 4, top_k=5).numpy()
     assert seq[0, :3].tolist() == [-1, 5, 9] and (seq[0, 3:] >= 0).all()
+
+
+def test_generate_at_temperature_zero_is_greedy(torch):
+    _, student = _models(torch)
+    prompt = _ids(torch, 2, 20, 6)
+    want = student.generate(prompt, 12, greedy=True).numpy()
+    for kw in ({}, dict(top_k=3), dict(top_p=0.5)):
+        assert (student.generate(prompt, 12, 0, **kw).numpy() == want).all(), kw

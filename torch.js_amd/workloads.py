@@ -307,7 +307,8 @@ class GPT2(nn.Module):
         GPT-2 path, tests/gpt2.test.ts): the prompt runs once, then each
         new token is one cached step; the next token is drawn by
         multinomial from softmax(logits / temperature) (or argmax when
-        greedy).  With top_k, top_p or min_p it is drawn by F.sample_logits
+        greedy).  With top_k, top_p, min_p or a temperature of 0 (the first
+        of the largest logits) it is drawn by F.sample_logits
         from the logits, without a readback in the loop; logits without a
         distribution (NaN) raise at the end.  Returns the
         [B, T + max_new_tokens] int32 ids."""
@@ -316,7 +317,7 @@ class GPT2(nn.Module):
         total = T + max_new_tokens
         if total > self.ctx:
             raise ValueError("generate: %d positions exceed the context of %d" % (total, self.ctx))
-        cut = top_k != 0 or top_p != 1.0 or min_p != 0.0
+        cut = temperature == 0 or top_k != 0 or top_p != 1.0 or min_p != 0.0
         with no_grad():
             cache = self.new_cache(B, total)
             logits = self.forward_cached(ids, cache, 0)
