@@ -142,5 +142,37 @@ def test_generate_at_temperature_zero_is_greedy(torch):
     _, student = _models(torch)
     prompt = _ids(torch, 2, 20, 6)
     want = student.generate(prompt, 12, greedy=True).numpy()
-    for kw in ({}, dict(top_k=3), dict(top_p=0.5)):
+    for kw in ({}, dict(top_k=3), dict(top_p=0.5), dict(top_k=[4, 0], min_p=0.1)):
         assert (student.generate(prompt, 12, 0, **kw).numpy() == want).all(), kw
+
+
+def test_generate_with_settings_of_each_row(torch):
+    """A number, a list, an array or a tensor for any of the settings."""
+    _, student = _models(torch)
+    prompt = _ids(torch, 2, 20, 7)
+    settings = dict(temperature=[0.7, 1.2], top_k=[0, 9], top_p=[0.8, 1.0], min_p=[0.0, 0.02])
+    one = {name: value[0] for name, value in settings.items()}
+    for name, value in settings.items():
+        dtype = np.int32 if name == "top_k" else np.float32
+        kw = dict(one)
+        kw[name] = np.array([value[0]] * 2, dtype)
+        torch.manual_seed(3)
+        want = student.generate(prompt, 10, **one).numpy()
+        for v in (kw[name], kw[name].tolist(), torch.tensor(kw[name])):
+            kw[name] = v
+            torch.manual_seed(3)
+            # float32 settings in place of Python's: one draw in millions differs
+            assert (student.generate(prompt, 10, **kw).numpy() == want).all(), name
+    torch.manual_seed(4)
+    seq = student.generate(prompt, 10, **settings).numpy()
+    torch.manual_seed(4)
+    with torch.no_grad():
+        cache = student.new_cache(2, 30)
+        logits = student.forward_cached(prompt, cache, 0)
+        for pos in range(20, 30):
+            x, u = logits[:, -1, :].numpy(), torch.rand(2).numpy()
+            want = [sample_ref(x[r], float(u[r]), float(np.float32(settings["temperature"][r])),
+                               settings["top_k"][r], float(np.float32(settings["top_p"][r])),
+                               float(np.float32(settings["min_p"][r]))) for r in range(2)]
+            assert seq[:, pos].tolist() == want, pos
+            logits = student.forward_cached(torch.tensor(seq[:, pos:pos + 1]), cache, pos)

@@ -12,10 +12,13 @@ user would write it (nn modules, functional ops, backward(), optimizers):
 import ctypes
 import math
 
+import numpy as np
+
 from . import _lib as L
 from . import functional as F
 from . import nn
-from .tensor import (_before_write, arange, empty, from_numpy, is_grad_enabled, no_grad, zeros)
+from .tensor import (Tensor, _before_write, arange, empty, from_numpy, is_grad_enabled, no_grad,
+                     zeros)
 
 
 def mlp():
@@ -307,8 +310,8 @@ class GPT2(nn.Module):
         GPT-2 path, tests/gpt2.test.ts): the prompt runs once, then each
         new token is one cached step; the next token is drawn by
         multinomial from softmax(logits / temperature) (or argmax when
-        greedy).  With top_k, top_p, min_p or a temperature of 0 (the first
-        of the largest logits) it is drawn by F.sample_logits
+        greedy).  With top_k, top_p or min_p, a temperature of 0, or one
+        value a row of any of the four, it is drawn by F.sample_logits
         from the logits, without a readback in the loop; logits without a
         distribution (NaN) raise at the end.  Returns the
         [B, T + max_new_tokens] int32 ids."""
@@ -317,7 +320,9 @@ class GPT2(nn.Module):
         total = T + max_new_tokens
         if total > self.ctx:
             raise ValueError("generate: %d positions exceed the context of %d" % (total, self.ctx))
-        cut = temperature == 0 or top_k != 0 or top_p != 1.0 or min_p != 0.0
+        rules = (temperature, top_k, top_p, min_p)
+        cut = any(isinstance(s, Tensor) or np.ndim(s) for s in rules) or \
+            temperature == 0 or top_k != 0 or top_p != 1.0 or min_p != 0.0
         with no_grad():
             cache = self.new_cache(B, total)
             logits = self.forward_cached(ids, cache, 0)
