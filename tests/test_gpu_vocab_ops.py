@@ -846,6 +846,31 @@ def test_refusals(pkg):
         F.distillation_loss(_fake(pkg, 4, 0), v, ids)
 
 
+def test_fractions_are_no_counts(pkg):
+    """They were cut off: of numpy's numbers, of lists, of topk's k."""
+    x, u = _fake(pkg, 4, 10), _fake(pkg, 4)
+    for k in (2.5, np.float32(2.5), np.float64(0.5), [2, 2.5, 3, 4], np.array([1, 2, np.nan, 4]),
+              [1, math.inf, 2, 0.5]):
+        with pytest.raises(ValueError, match="whole number"):
+            pkg.functional.sample_logits(x, u, top_k=k)
+    for k in (math.inf, math.nan, 2 ** 31):
+        with pytest.raises(ValueError, match="must lie in"):
+            pkg.functional.sample_logits(x, u, top_k=k)
+    for k in (2.5, np.float32(0.5)):
+        with pytest.raises(ValueError, match="whole number"):
+            x.topk(k)
+
+
+@gpu
+def test_counts_past_32_bits(torch):
+    """A top_k of a row that int32 does not hold is no rule."""
+    rng = np.random.default_rng(2)
+    x, u = rng.standard_normal((3, 40)).astype(np.float32), rng.random(3).astype(np.float32)
+    for k in (np.array([2 ** 32 + 1, -2 ** 40, 3]), [2.0 ** 40, -1.0, 3.0], [2 ** 31, 0, 3]):
+        got = torch.functional.sample_logits(torch.tensor(x), u, top_k=k)
+        assert got.numpy().tolist() == [sample_ref(x[r], float(u[r]), top_k=(0, 0, 3)[r]) for r in range(3)]
+
+
 @gpu
 def test_refusals_of_the_library(torch):
     from torchjs_amd import _lib as L

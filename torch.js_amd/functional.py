@@ -409,9 +409,17 @@ def _setting(name, value, rows, dtype, lo, hi):
         if not lo <= value <= hi:
             raise ValueError("sample_logits: %s must lie in [%s, %s], got %r"
                              % (name, lo, hi, value))
+        if dtype == "int32" and value != int(value):
+            raise ValueError("sample_logits: %s must be a whole number, got %r" % (name, value))
         return None, value, None
-    t = value if isinstance(value, Tensor) else \
-        _T.tensor(np.asarray(value, dtype=_DT[dtype][1]), dtype=dtype)
+    t = value
+    if not isinstance(t, Tensor):
+        a = np.asarray(value)
+        if dtype == "int32":
+            if a.dtype.kind == "f" and not (a == np.trunc(a)).all():
+                raise ValueError("sample_logits: %s must be whole numbers, got %r" % (name, value))
+            a = np.clip(a, lo, hi)  # outside: no rule, as the ends are
+        t = _T.tensor(a.astype(_DT[dtype][1]), dtype=dtype)
     if t.shape != (rows,):
         raise ValueError("sample_logits: %s has shape %s for %d rows"
                          % (name, list(t.shape), rows))
@@ -459,8 +467,6 @@ def sample_logits(logits, uniforms=None, temperature=1.0, top_k=0, top_p=1.0, mi
         u = (u if u.dtype == "float32" else u.float()).contiguous()
     # the tensors live until the launch is queued
     t, t0, _t = _setting("temperature", temperature, rows, "float32", 0.0, math.inf)
-    if isinstance(top_k, float) and top_k != int(top_k):
-        raise ValueError("sample_logits: top_k must be a whole number, got %r" % (top_k,))
     k, k0, _k = _setting("top_k", top_k, rows, "int32", 0, 2 ** 31 - 1)
     p, p0, _p = _setting("top_p", top_p, rows, "float32", 0.0, 1.0)
     m, m0, _m = _setting("min_p", min_p, rows, "float32", 0.0, 1.0)

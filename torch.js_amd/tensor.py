@@ -2739,6 +2739,8 @@ def topk(x, k, dim=-1, largest=True):
     value, equal ones by ascending index; NaN counts as the largest, as in
     PyTorch.  k up to 1024; other dtypes are compared as float32.  The
     values' gradient goes back to the elements they came from."""
+    if int(k) != k:
+        raise ValueError("topk: k must be a whole number, got %r" % (k,))
     k = int(k)
     if x.ndim == 0:
         v, i = topk(reshape(x, (1,)), k, 0, largest)
