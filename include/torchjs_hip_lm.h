@@ -39,7 +39,8 @@ int tjh_topk_backward(const float* g, const int32_t* indices, int64_t rows, int6
  * counted by the mean.  reduction and s_r (from grad_out, NULL: 1) as
  * tjh_cross_entropy_backward's.  Each of loss_rows [rows], out (the reduced
  * loss; needs loss_rows) and dlogits (row stride ldd) may be NULL; with
- * several the logits are read once.  k <= 1024, else TJH_ERR_UNSUPPORTED. */
+ * several the logits are read once.  temperature from 1e-18 to 1e18; k <= 1024,
+ * else TJH_ERR_UNSUPPORTED. */
 int tjh_distill(const float* logits, int64_t ld, int64_t rows, int64_t cols,
                 const float* teacher, const int32_t* ids, int64_t k, float temperature,
                 int reduction, const float* grad_out, float* loss_rows, float* out,

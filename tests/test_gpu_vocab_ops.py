@@ -846,6 +846,13 @@ def test_refusals(pkg):
         F.distillation_loss(_fake(pkg, 4, 0), v, ids)
 
 
+def test_distillation_temperatures_without_float32_powers(pkg):
+    v, ids = _fake(pkg, 4, 3), _fake(pkg, 4, 3, dtype="int32")
+    for t in (1e-40, 9e-19, 1.1e18, 1e30):
+        with pytest.raises(ValueError, match="temperature"):
+            pkg.functional.distillation_loss(_fake(pkg, 4, 10), v, ids, t)
+
+
 def test_fractions_are_no_counts(pkg):
     """They were cut off: of numpy's numbers, of lists, of topk's k."""
     x, u = _fake(pkg, 4, 10), _fake(pkg, 4)
@@ -859,6 +866,18 @@ def test_fractions_are_no_counts(pkg):
     for k in (2.5, np.float32(0.5)):
         with pytest.raises(ValueError, match="whole number"):
             x.topk(k)
+
+
+@gpu
+@pytest.mark.parametrize("t", [1e-18, 1e18])
+def test_distillation_at_the_ends_of_the_temperatures(torch, t):
+    x, v, ids = _distill_inputs(np.random.default_rng(3), 4, 1500, 6)
+    for reduction in ("mean", "none"):
+        _check_distill(torch, x, v, ids, t, reduction)
+    from torchjs_amd import _lib as L
+    p = torch.zeros(4, 10).data_ptr()
+    for bad in (1e-40, 9e-19, 1.1e18, math.inf, math.nan):
+        assert L.lib().tjh_distill(p, 10, 2, 10, p, p, 1, bad, 1, None, p, p, None, 0) == 1
 
 
 @gpu

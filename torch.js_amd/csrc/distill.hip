@@ -240,7 +240,9 @@ extern "C" int tjh_distill(const float* logits, int64_t ld, int64_t rows, int64_
   const int threads = cols <= 1024 ? 64 : cols <= 4096 ? 256 : cols <= 53248 ? 512 : 1024;
   TJH_ARG(rows * threads < (int64_t(1) << 32), "tjh_distill: too many rows");  // of a grid
   TJH_ARG(reduction >= 0 && reduction <= 3, "tjh_distill: reduction %d", reduction);
-  TJH_ARG(temperature > 0.f && temperature < INFINITY, "tjh_distill: temperature must be positive");
+  // 1 / T and T^2 are numbers
+  TJH_ARG(temperature >= 1e-18f && temperature <= 1e18f,
+          "tjh_distill: temperature must be positive, from 1e-18 to 1e18");
   if (k > kMaxK)
     return set_error(TJH_ERR_UNSUPPORTED, "tjh_distill: %lld teacher entries a row, at most %d",
                      (long long)k, kMaxK);

@@ -317,13 +317,15 @@ def distillation_loss(input, teacher_logits, teacher_ids, temperature=1.0, reduc
     q = softmax(input / T) over its columns, a row's loss is
     T^2 sum p (ln p - ln q).  Entries whose id is outside [0, C) are none; a
     row without any has loss 0 and gradient 0 and is not counted by "mean".
-    Reductions as cross_entropy's.  K up to 1024.  The gradient goes to
-    `input` only; for a scalar loss it is formed in the same pass over the
+    Reductions as cross_entropy's.  K up to 1024, temperatures from 1e-18 to
+    1e18 (sums are float32: the loss is off by some 2^-24 T^2 ln C, a gradient
+    by 2^-24 T times its probabilities).  The gradient goes to `input` only; for a scalar loss it is formed in the same pass over the
     logits."""
     red = _reduction_code(reduction)
     temp = float(temperature)
-    if not (temp > 0.0 and math.isfinite(temp)):
-        raise ValueError("distillation_loss: temperature must be positive, got %r" % (temperature,))
+    if not 1e-18 <= temp <= 1e18:  # 1 / T and T^2 are float32 numbers
+        raise ValueError("distillation_loss: temperature must be positive, from 1e-18 to 1e18, "
+                         "got %r" % (temperature,))
     x, v, ids = input, teacher_logits, _T._idx32(teacher_ids)
     if not isinstance(v, Tensor):
         v = _T.tensor(np.asarray(v, dtype=np.float32))
