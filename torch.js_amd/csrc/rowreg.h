@@ -197,14 +197,6 @@ struct Block {
   __device__ __forceinline__ int sum_i(int v) {
     return across(last_lane(wave_scan(v)), [](int x, int y) { return x + y; });
   }
-  // threads for which p holds, counted over `M` predicates of each
-  template <int M>
-  __device__ __forceinline__ int count(const bool (&p)[M]) {
-    int c = 0;
-#pragma unroll
-    for (int i = 0; i < M; ++i) c += __popcll(__ballot(p[i]));
-    return across(c, [](int x, int y) { return x + y; });
-  }
   // sum of v over the threads before this one; total in *all
   template <class V>
   __device__ __forceinline__ V before(V v, V* all) {

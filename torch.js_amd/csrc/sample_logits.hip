@@ -241,9 +241,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
   float per = 0.f;
   int last = -1;
   u64 above = 0;  // weight of the bins before `last`
-  if (largest) {
-    bound = kth_bound(row, (int)top_k, b);
-  } else if (nucleus) {
+  if (nucleus) {
     // weights by bins of m - x, out to weights of e^-24 or the smallest x
     per = (float)(kBins / fmax(fmin(24.0 * temp, m - (double)mn), 1e-30));
     if (!cut) {
@@ -292,26 +290,15 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
     last = lds.pick;
     // elements of later bins that are not below it do no harm
     if (last < kBins - 1) bound = float_below(m - (last + 1.01) / per);
-  } else if (floor_z > -INFINITY) {
+  } else if (!largest && floor_z > -INFINITY) {
     bound = float_below(m + floor_z);
   }
   int c = -1;  // elements of the list, if there is one
   u64* list = s.list;
-  if (largest) c = gather_above(row, kNanFirst, bound, s);
-  else if (bound > -INFINITY) c = gather_pairs(row, bound, s, b);
+  if (bound > -INFINITY) c = gather_pairs(row, bound, s, b);
   if (c > kCap) c = -1;
   if (largest) {
-    if (c < 0) {
-      Row<T, 0> again;
-      again.load(row.p, n);
-      const u64 thr = kth_by_bisection(again, (int)top_k, kNanFirst, b);
-      gather_list(
-          again, kNanFirst,
-          [&](int j, int e, float x) { return composite(order_key(x), again.index(j, e)) >= thr; },
-          s);
-      c = (int)top_k;
-    }
-    list = sort_list(s, c);
+    list = select_largest(row, (int)top_k, kNanFirst, s, b);
     c = (int)top_k;
   } else if (use_p) {
     // the nucleus ends in bin `last`: (tx, ti) from that bin's elements
