@@ -36,10 +36,11 @@ int tjh_topk_backward(const float* g, const int32_t* indices, int64_t rows, int6
  *   loss_row = T^2 sum_i p_i (ln p_i - ln q[ids_i])
  *   dlogits[r, j] = s_r T (q_j - sum_i p_i [ids_i == j])
  * A row with no entry above -infinity has loss 0 and gradient 0 and is not
- * counted by the mean.  reduction and s_r (from grad_out, NULL: 1) as
- * tjh_cross_entropy_backward's.  Each of loss_rows [rows], out (the reduced
- * loss; needs loss_rows) and dlogits (row stride ldd) may be NULL; with
- * several the logits are read once.  temperature from 1e-18 to 1e18; k <= 1024,
+ * counted by the mean; one with an entry of NaN or +infinity is NaN.
+ * reduction and s_r (from grad_out, NULL: 1) as tjh_cross_entropy_backward's.
+ * Each of loss_rows [rows], out (the reduced loss; needs loss_rows) and
+ * dlogits (row stride ldd) may be NULL; with several the logits are read once
+ * (rows of up to 53248).  temperature from 1e-18 to 1e18; k <= 1024,
  * else TJH_ERR_UNSUPPORTED. */
 int tjh_distill(const float* logits, int64_t ld, int64_t rows, int64_t cols,
                 const float* teacher, const int32_t* ids, int64_t k, float temperature,
@@ -74,15 +75,18 @@ int tjh_sample_logits(const float* logits, int64_t ld, int64_t rows, int64_t col
  * backward, or NULL.  Keys and values that a query does not see have no
  * part in its output, whatever they hold.  Head dims up to 128 that are
  * multiples of 4, rows 16-byte aligned and less than 2^23 elements apart (else
- * TJH_ERR_UNSUPPORTED). */
+ * TJH_ERR_UNSUPPORTED).  B H times Tq / 32, rounded up, below 2^24; with up to
+ * 4 queries B H Tq below 2^23 (else TJH_ERR_INVALID). */
 int tjh_window_forward(const float* q, const float* k, const float* v, float* o, float* lse,
                        int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t D,
                        const int64_t* q_strides, const int64_t* k_strides,
                        const int64_t* v_strides, const int64_t* o_strides, float scale,
                        int64_t window, int64_t sinks);
 /* dq [B,H,Tq,D], dk/dv [B,Hkv,Tk,D] written (not accumulated; with Tq == 0
- * nothing is), summed over the query heads of a key head.  strides[0..7] = q,
- * k, v, o, do_, dq, dk, dv as tjh_sdpa_backward's. */
+ * nothing is), summed over the query heads of a key head.  Scratch of some Tq
+ * (window + sinks) floats a query head, at least for all that read one key
+ * head (TJH_ERR_OOM where they do not fit).  strides[0..7] = q, k, v, o, do_,
+ * dq, dk, dv as tjh_sdpa_backward's. */
 int tjh_window_backward(const float* q, const float* k, const float* v, const float* o,
                         const float* do_, const float* lse, float* dq, float* dk, float* dv,
                         int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t D,

@@ -14,8 +14,10 @@
 // Bound by reading the logits once and, for a gradient, writing it once
 // (8 bytes an element): a workgroup keeps its row in registers (rowreg.h)
 // between the two, takes maximum and sum from there, and forms the row's loss
-// and gradient in the same pass.  (2048, 50257) with 64 entries: 177 us, 4.65
-// TB/s, where a large copy moves 5.2; (509, 32001): 30 us, 4.4.
+// and gradient in the same pass.  (2048, 50257) with 64 entries: 179 us, 4.6
+// TB/s, where a large copy moves 5.2; (509, 32001): 29 us, 4.4.  Rows of more
+// than 53248 are read three times ((1024, 128256): 318 us a call, 3.3 TB/s of
+// one read and the write; the loss alone 165).
 #include "rowreg.h"
 
 #include <math.h>

@@ -6,7 +6,8 @@
 // every load is a whole chunk whatever the row's alignment and chunk order is
 // index order; the up to three elements before the first chunk and after the
 // last one are an extra element of the first six threads.  Rows that outgrow
-// the registers (NV == 0) are read again, from the L2, on every pass.
+// the registers (NV == 0) are read again on every pass, from the L2s only
+// while the rows in flight fit them.
 #pragma once
 
 #include "common.h"

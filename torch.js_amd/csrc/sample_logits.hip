@@ -36,6 +36,9 @@
 // maximum), top_k 50 15, min_p 0.01 16, no rule 27 (of it some 12 the
 // weights, 31 instructions each on four SIMDs), top_k 1000 38, top_p 0.9 40; of
 // 32001, top_p 0.9 32.  4096 rows of 4000: top_k 50 80 us, top_p 0.9 119.
+// 256 rows of 128256, outside the registers: top_k 50 66 us, no rule 69, top_p
+// 0.9 160.  A row with fewer than top_k logits above -infinity leaves the list
+// for topk.hip's bisection: 302 us with 30 of 50257 and top_k 50.
 #include "rowreg.h"
 
 #include <float.h>

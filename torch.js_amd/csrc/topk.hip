@@ -10,7 +10,10 @@
 // takes a lower bound of the k-th value from the threads' maxima, moves the
 // few elements above it into LDS and sorts those (rowreg.h).  64 of each of
 // 2048 rows of 50257: 75 us, 5.5 TB/s; 20 of one row: 9 us, a chain of loads,
-// rounds of the bound and the sort on one CU.
+// rounds of the bound and the sort on one CU.  Rows of more than 53248 are read
+// twice (1024 of 128256: 162 us, 3.2 TB/s counted once).  A row with fewer than
+// k elements above -infinity has no bound, and is longer than the list: some 50
+// passes of the bisection (50 of 50257, 30 of them above it: 311 us, not 10).
 #include "rowreg.h"
 
 namespace tjh {

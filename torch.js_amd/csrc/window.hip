@@ -344,7 +344,10 @@ __global__ __launch_bounds__(256) void k_win_merge(WinArgs a, int64_t n4, int ns
 // its keys over groups of 16 lanes, each with a running softmax of its own
 // over every NG-th key, joined once at the end in a fixed order.  grid.y
 // slices of the keys, joined by k_win_merge, where there are few rows.
-// Bound by the latency of its loads: 48 rows of 260 keys, D 64, 5.7 us.
+// Bound by the latency of its loads where rows are few: 48 of 260 keys, D 64,
+// 5.5 us; by memory where they are many: 64 sequences of 8 heads, 4096 keys, D
+// 128, 355 us, 6.1 TB/s.  Query heads that share keys each fetch them, on
+// different XCDs: 32 over those 8 heads take 1239 us, 1.7 TB/s of the cache.
 constexpr int kFewThreads = 512, kFewGroups = kFewThreads / 16, kFewUnroll = 4;
 
 template <int NC, bool PART>  // NC: 64-column pieces of the head dim

@@ -443,10 +443,11 @@ def sample_logits(logits, uniforms=None, temperature=1.0, top_k=0, top_p=1.0, mi
     whose running sum of weights, in index order, exceeds u times their sum.
     temperature 0 takes the first index of the largest logit.
 
-    Each setting is a number or a tensor [rows] of each row's own; in a
-    tensor a temperature that is not above 0 stands for 0, and a setting out
-    of its range for none.  A row with NaN, +infinity or nothing above
-    -infinity gives -1.  C up to 2^20."""
+    Each setting is a number or a tensor [rows] of each row's own, in which
+    a temperature that is not above 0 (or NaN) stands for 0, a top_p below 0
+    for 0, a min_p above 1 for 1, and any other value out of its range, or
+    NaN, for no rule.  A row with NaN, +infinity or nothing above -infinity
+    gives -1.  C up to 2^20."""
     x = logits
     if x.ndim not in (1, 2) or x.shape[-1] == 0:
         raise ValueError("sample_logits: expected logits [rows, C] or [C], got shape %s"
@@ -1096,11 +1097,16 @@ def sliding_window_attention(query, key, value, window, sinks=0, scale=None):
     are the last Tq of the Tk positions: a whole sequence, the next part of
     a prompt over a cache, or one decoding step.  The query at position i
     sees the keys j <= i with j > i - window or j < sinks; what other keys
-    and values hold has no part in its output.  O(Tk) memory beside the
-    result, time by the keys seen.  Head dims up to 128 (operands are copied
-    where one is no multiple of 4 or rows are not 16-byte aligned); the
-    gradients of key and value are summed over the query heads that read
-    them."""
+    and values hold has no part in its output.  Head dims up to 128 (operands
+    are copied where one is no multiple of 4 or rows are not 16-byte
+    aligned); the gradients of key and value are summed over the query heads
+    that read them.
+
+    Time goes by the keys seen.  Memory beside the result: the partial
+    results of cut key ranges where queries are few; in the backward some Tq
+    (window + sinks) floats a query head, for as many key heads at once as 4
+    GiB hold but never less than one with all of its query heads.  It raises
+    where those do not fit."""
     if type(window) is not int or window < 1 or window > 1 << 30:
         window = _whole("window", window, 1)
     if type(sinks) is not int or sinks < 0 or sinks > 1 << 30:
