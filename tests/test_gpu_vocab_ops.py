@@ -881,6 +881,15 @@ def test_distillation_at_the_ends_of_the_temperatures(torch, t):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [np.int8, np.uint8, np.int16, np.int64, np.uint64, np.float16, np.float32])
+def test_counts_of_any_type(torch, dtype):
+    rng = np.random.default_rng(2)
+    x, u = rng.standard_normal((3, 40)).astype(np.float32), rng.random(3).astype(np.float32)
+    got = torch.functional.sample_logits(torch.tensor(x), u, top_k=np.array([4, 0, 1], dtype))
+    assert got.numpy().tolist() == [sample_ref(x[r], float(u[r]), top_k=(4, 0, 1)[r]) for r in range(3)]
+
+
+@gpu
 def test_counts_past_32_bits(torch):
     """A top_k of a row that int32 does not hold is no rule."""
     rng = np.random.default_rng(2)

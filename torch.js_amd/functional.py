@@ -319,8 +319,8 @@ def distillation_loss(input, teacher_logits, teacher_ids, temperature=1.0, reduc
     row without any has loss 0 and gradient 0 and is not counted by "mean".
     Reductions as cross_entropy's.  K up to 1024, temperatures from 1e-18 to
     1e18 (sums are float32: the loss is off by some 2^-24 T^2 ln C, a gradient
-    by 2^-24 T times its probabilities).  The gradient goes to `input` only; for a scalar loss it is formed in the same pass over the
-    logits."""
+    by 2^-24 T times its probabilities).  The gradient goes to `input` only;
+    for a scalar loss it is formed in the same pass over the logits."""
     red = _reduction_code(reduction)
     temp = float(temperature)
     if not 1e-18 <= temp <= 1e18:  # 1 / T and T^2 are float32 numbers
@@ -418,7 +418,8 @@ def _setting(name, value, rows, dtype, lo, hi):
     if not isinstance(t, Tensor):
         a = np.asarray(value)
         if dtype == "int32":
-            if a.dtype.kind == "f" and not (a == np.trunc(a)).all():
+            a = a.astype(np.float64)
+            if not (a == np.trunc(a)).all():
                 raise ValueError("sample_logits: %s must be whole numbers, got %r" % (name, value))
             a = np.clip(a, lo, hi)  # outside: no rule, as the ends are
         t = _T.tensor(a.astype(_DT[dtype][1]), dtype=dtype)
@@ -1104,9 +1105,9 @@ def sliding_window_attention(query, key, value, window, sinks=0, scale=None):
 
     Time goes by the keys seen.  Memory beside the result: the partial
     results of cut key ranges where queries are few; in the backward some Tq
-    (window + sinks) floats a query head, for as many key heads at once as 4
-    GiB hold but never less than one with all of its query heads.  It raises
-    where those do not fit."""
+    (window + sinks) floats a query head (up to twice that where most of them
+    are sinks), for as many key heads at once as 4 GiB hold but never less
+    than one with all of its query heads.  It raises where those do not fit."""
     if type(window) is not int or window < 1 or window > 1 << 30:
         window = _whole("window", window, 1)
     if type(sinks) is not int or sinks < 0 or sinks > 1 << 30:
