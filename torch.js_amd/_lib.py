@@ -1,5 +1,5 @@
 """ctypes binding of libtorchjs_hip.so (the C ABI declared in
-include/torchjs_hip.h and include/torchjs_hip_lm.h).
+include/torchjs_hip.h, include/torchjs_hip_lm.h and include/torchjs_hip_decode.h).
 
 The library is required: importing the package works without it, but the
 first call that needs the device raises, naming the missing file.  Nothing
@@ -205,6 +205,17 @@ SIGNATURES = {
                     c_vp, c_i64],
     "tjh_sample_logits": [c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_f64, c_i64,
                           c_f64, c_f64, c_vp],
+    "tjh_fp4_quantize": [c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp],
+    "tjh_fp4_dequantize": [c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_i64],
+    "tjh_fp4_linear": [c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_i64],
+    "tjh_fp4_cache_append": [c_vp, c_vp, P_i64, P_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64,
+                             c_i64, c_i64, c_i64, c_vp],
+    "tjh_fp4_cache_read": [c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp],
+    "tjh_fp4_attention": [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64,
+                          c_i64, P_i64, P_i64, c_i64, c_vp, c_f32],
+    "tjh_beam_step": [c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp,
+                      c_vp],
+    "tjh_cache_reorder": [c_int, ctypes.POINTER(c_vp), P_i64, P_i64, P_i64, c_i64, c_i64, c_vp],
     "tjh_adam_step": [c_int, ctypes.POINTER(c_vp), ctypes.POINTER(c_vp), ctypes.POINTER(c_vp),
                       ctypes.POINTER(c_vp), P_i64, P_i64, c_f64, c_f64, c_f64, c_f64, c_f64,
                       c_int],

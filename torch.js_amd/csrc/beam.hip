@@ -1,0 +1,339 @@
+// A beam search's step and the reordering of its caches (beside
+// Tensor.multinomial, src/tensor/Tensor.ts:271-359: the next tokens of several
+// kept sequences instead of one drawn from each).
+//
+// Step: of the continuations (w, v) with the scores s_w + x_wv - ln sum exp x_w,
+// the `keep` largest.  Within a beam their order is that of the logits, so each
+// workgroup of the first kernel takes the largest logits of a piece of a row, with
+// the piece's maximum and sum of exponentials, and one workgroup a search then
+// compares the scores of those in 64 bits.
+#include "rowreg.h"
+
+#include <math.h>
+
+namespace tjh {
+namespace {
+
+using namespace rowreg;
+
+struct BeamArgs {
+  const float* x;
+  const float* scores;
+  const uint8_t* finished;
+  float2* stats;  // [rows, S]: maximum, sum of exponentials from it
+  u64* cand;      // [rows, S, keep]: composites, best first
+  float* out_scores;
+  int32_t *tokens, *parents;
+  uint8_t* out_finished;
+  int64_t ld;
+  int W, V, S, per, keep, eos;
+};
+
+// A piece of a row: `per` columns, fewer at the end.
+template <int T, int NV, int CAP>
+__global__ __launch_bounds__(T, T == 512 ? 4 : 1) void k_beam_pieces(BeamArgs a) {
+  __shared__ SelectLds<T, CAP> s;
+  const int64_t r = blockIdx.x / a.S;
+  if (a.finished && a.finished[r]) return;
+  const int piece = blockIdx.x - (int)r * a.S, c0 = piece * a.per, n = min(a.per, a.V - c0);
+  Block<T> b(s.sm);
+  Row<T, NV> row;
+  row.load(a.x + r * a.ld + c0, n, 0, true);
+  float m = -INFINITY, sum = 0.f;
+  row.each([&](int, int, float x) { m = fmaxf(m, x); });  // NaN takes no part here,
+  m = b.max(m);
+  const float from = m == -INFINITY ? 0.f : m;
+  row.each([&](int, int, float x) { sum += expf(x - from); });  // but in the sum
+  sum = b.sum(sum);
+  const int k = min(a.keep, n);
+  const u64* best = select_largest(row, k, kNanFirst, s, b);
+  u64* to = a.cand + blockIdx.x * (int64_t)a.keep;
+  for (int i = threadIdx.x; i < k; i += T) {
+    const u64 c = best[i];
+    to[i] = composite((uint32_t)(c >> 32), c0 + index_of(c));
+  }
+  if (threadIdx.x == 0) a.stats[blockIdx.x] = make_float2(m, sum);
+}
+
+// Unsigned integer in the order of the scores; 0: no continuation.
+__device__ __forceinline__ u64 score_key(double v) {
+  if (!(v > -INFINITY)) return 0;
+  const u64 u = (u64)__double_as_longlong(v + 0.0);
+  return (u >> 63) ? ~u : u | 0x8000000000000000ull;
+}
+__device__ __forceinline__ double key_score(u64 k) {
+  return __longlong_as_double((long long)((k >> 63) ? k & 0x7fffffffffffffffull : ~k));
+}
+
+constexpr int kMaxBeams = 64, kMaxLists = 1280, kMaxEntries = kMaxBeams * kMaxBeams;
+
+// One workgroup a search.  The lists (a beam's pieces) are in order, so only the
+// `keep` lists with the best heads matter, and of those only what is not below the
+// last of these heads; some tens of entries, ranked by counting.
+__global__ __launch_bounds__(256) void k_beam_merge(BeamArgs a) {
+  __shared__ double from[kMaxBeams];  // a beam's score less its logarithm of the sum
+  __shared__ int state[kMaxBeams];    // 0 goes on, 1 finished, 2 has no continuation
+  __shared__ u64 head[kMaxLists];
+  __shared__ int chosen[kMaxBeams];
+  __shared__ u64 key[kMaxEntries];
+  __shared__ int flat[kMaxEntries];
+  __shared__ u64 bound;
+  __shared__ int count;
+  const int t = threadIdx.x, lists = a.W * a.S;
+  const int64_t r0 = (int64_t)blockIdx.x * a.W;
+  if (t == 0) {
+    bound = 0;
+    count = 0;
+  }
+  if (t < kMaxBeams) chosen[t] = -1;
+  for (int w = t; w < a.W; w += 256) {
+    const double s = a.scores[r0 + w];
+    from[w] = s;
+    if (!(s > -INFINITY)) {
+      state[w] = 2;
+    } else if (a.finished && a.finished[r0 + w]) {
+      state[w] = 1;
+    } else {
+      const float2* st = a.stats + (r0 + w) * a.S;
+      float m = -INFINITY;
+      for (int i = 0; i < a.S; ++i) m = fmaxf(m, st[i].x);
+      double sum = 0.0;
+      for (int i = 0; i < a.S; ++i) {
+        const float2 p = st[i];
+        sum += p.x == -INFINITY ? (double)p.y : (double)p.y * exp((double)p.x - (double)m);
+      }
+      // NaN in the sum, +infinity as the maximum, or nothing above -infinity
+      const bool ok = sum > 0.0 && sum < INFINITY && m < INFINITY && m > -INFINITY;
+      state[w] = ok ? 0 : 2;
+      from[w] = s - ((double)m + log(sum));
+    }
+  }
+  __syncthreads();
+  const auto entry = [&](int list, int i, int* at) -> u64 {  // i-th of a list: key, w V + v
+    const int w = list / a.S, piece = list - w * a.S;
+    if (state[w] == 2) return 0;
+    if (state[w] == 1) {
+      *at = w * a.V + a.eos;
+      return piece == 0 && i == 0 ? score_key(from[w]) : 0;
+    }
+    if (i >= min(a.keep, min(a.per, a.V - piece * a.per))) return 0;
+    const u64 c = a.cand[((r0 + w) * a.S + piece) * a.keep + i];
+    const int v = index_of(c);
+    *at = w * a.V + v;
+    return score_key(from[w] + (double)key_value((uint32_t)(c >> 32)));
+  };
+  int at;
+  for (int i = t; i < lists; i += 256) head[i] = entry(i, 0, &at);
+  __syncthreads();
+  for (int i = t; i < lists; i += 256) {
+    const u64 me = head[i];
+    int rank = 0;
+    for (int j = 0; j < lists; ++j) rank += head[j] > me || (head[j] == me && j < i);
+    if (rank < a.keep) chosen[rank] = i;
+    if (rank == a.keep - 1) bound = me;
+  }
+  __syncthreads();
+  for (int i = t; i < a.keep * a.keep; i += 256) {
+    const int list = chosen[i / a.keep];
+    if (list < 0) continue;
+    const u64 k = entry(list, i % a.keep, &at);
+    if (k != 0 && k >= bound) {
+      const int to = atomicAdd(&count, 1);
+      key[to] = k;
+      flat[to] = at;
+    }
+  }
+  __syncthreads();
+  const int n = count;
+  const int64_t o = (int64_t)blockIdx.x * a.keep;
+  for (int i = t; i < n; i += 256) {
+    const u64 me = key[i];
+    const int f = flat[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += key[j] > me || (key[j] == me && flat[j] < f);
+    if (rank >= a.keep) continue;
+    const int w = f / a.V, v = f - w * a.V;
+    a.out_scores[o + rank] = (float)key_score(me);
+    a.tokens[o + rank] = v;
+    a.parents[o + rank] = w;
+    a.out_finished[o + rank] = v == a.eos || state[w] == 1;
+  }
+  for (int i = n + t; i < a.keep; i += 256) {
+    a.out_scores[o + i] = -INFINITY;
+    a.tokens[o + i] = -1;
+    a.parents[o + i] = min(i, a.W - 1);
+    a.out_finished[o + i] = 1;
+  }
+}
+
+// ---------------------------------------------------------------- reordering
+
+constexpr int kTensors = 32;  // of a launch
+
+struct Moved {
+  char* p;
+  int64_t row, stride;  // bytes of a row, from one block to the next
+  int64_t units;        // 16, 4 or 1 bytes: of a block's moved part
+  int first;            // workgroup of the launch (grid x) at which this tensor begins
+  int per;              // workgroups a block
+  int unit;
+};
+struct ReorderArgs {
+  Moved t[kTensors];
+  const int32_t* parents;
+  int n, W;
+};
+
+// A thread has one unit's place in all beams of a search: it reads what its
+// beams become, then writes those that change, so no other thread's units are
+// touched in between.
+template <int W, class U>
+__device__ __forceinline__ void move_units(char* p, int64_t row, int n, const int* parent) {
+  U v[W];
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    const int from = __builtin_amdgcn_readfirstlane(parent[i]);
+    if (i < n && from != i) v[i] = *reinterpret_cast<const U*>(p + from * row);
+  }
+#pragma unroll
+  for (int i = 0; i < W; ++i)
+    if (i < n && __builtin_amdgcn_readfirstlane(parent[i]) != i)
+      *reinterpret_cast<U*>(p + i * row) = v[i];
+}
+
+template <int W>
+__global__ __launch_bounds__(256) void k_reorder(ReorderArgs a) {
+  __shared__ int parent[W];
+  const int b = blockIdx.y;
+  if (threadIdx.x < W) {
+    const int i = threadIdx.x;
+    int p = i < a.W ? a.parents[(int64_t)b * a.W + i] : i;
+    parent[i] = p >= 0 && p < a.W ? p : i;
+  }
+  __syncthreads();
+  int k = 0;
+  while (k + 1 < a.n && (int)blockIdx.x >= a.t[k + 1].first) ++k;
+  const Moved& t = a.t[k];
+  const int at = blockIdx.x - t.first, block = at / t.per;
+  const int64_t unit = (int64_t)(at - block * t.per) * 256 + threadIdx.x;
+  if (unit >= t.units) return;
+  char* p = t.p + (int64_t)b * a.W * t.row + block * t.stride + unit * t.unit;
+  typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
+  if (t.unit == 16) move_units<W, uintx4>(p, t.row, a.W, parent);
+  else if (t.unit == 4) move_units<W, uint32_t>(p, t.row, a.W, parent);
+  else move_units<W, uint8_t>(p, t.row, a.W, parent);
+}
+
+}  // namespace
+}  // namespace tjh
+
+using namespace tjh;
+
+extern "C" {
+
+int tjh_beam_step(const float* logits, int64_t ld, const float* scores, const uint8_t* finished,
+                  int64_t B, int64_t W, int64_t V, int64_t keep, int64_t eos, float* out_scores,
+                  int32_t* tokens, int32_t* parents, uint8_t* out_finished) {
+  TJH_REQUIRE_INIT();
+  TJH_ARG(B >= 0 && W > 0 && V > 0 && keep >= 0 && ld >= V && eos < V && (!finished || eos >= 0),
+          "tjh_beam_step: bad sizes");
+  if (W > kMaxBeams || keep > kMaxBeams || V > (1 << 20))
+    return set_error(TJH_ERR_UNSUPPORTED,
+                     "tjh_beam_step: %lld beams of %lld tokens, %lld kept (at most %d, 2^20, %d)",
+                     (long long)W, (long long)V, (long long)keep, kMaxBeams, kMaxBeams);
+  TJH_ARG(keep <= W * V, "tjh_beam_step: %lld kept of %lld", (long long)keep, (long long)(W * V));
+  if (B == 0 || keep == 0) return TJH_OK;
+  TJH_ARG(logits && scores && out_scores && tokens && parents && out_finished,
+          "tjh_beam_step: NULL pointer");
+  TJH_ARG(B < (1 << 20), "tjh_beam_step: too many searches");
+  // pieces of a row: as small as one load of each thread while the lists and
+  // the workgroups stay few
+  const int64_t rows = B * W;
+  int per = 53248 - 4;
+  for (const int size : {1024 - 4, 4096 - 4, 16384 - 4}) {
+    const int64_t S = cdiv(V, size);
+    if (S == 1 || (W * S <= 256 && rows * S <= 2 * num_cus())) {
+      per = size;
+      break;
+    }
+  }
+  BeamArgs a{logits, scores, finished, nullptr, nullptr, out_scores, tokens, parents, out_finished,
+             ld, (int)W, (int)V, (int)cdiv(V, per), per, (int)keep, (int)eos};
+  const int64_t pieces = rows * a.S;
+  TJH_ARG(pieces < (1 << 21), "tjh_beam_step: too many searches");
+  Scratch s((size_t)pieces * (sizeof(float2) + keep * sizeof(u64)));
+  if (!s.ok()) return set_error(TJH_ERR_OOM, "tjh_beam_step: no scratch");
+  a.cand = s.as<u64>();
+  a.stats = reinterpret_cast<float2*>(a.cand + pieces * keep);
+  KernelScope ks("beam_step");
+  const dim3 grid((unsigned)pieces);
+  if (per < 1024)
+    tjh_launch(k_beam_pieces<256, 1, 1024>, grid, dim3(256), 0, stream(), a);
+  else if (per < 4096)
+    tjh_launch(k_beam_pieces<256, 4, 4096>, grid, dim3(256), 0, stream(), a);
+  else if (per < 16384)
+    tjh_launch(k_beam_pieces<512, 8, 4096>, grid, dim3(512), 0, stream(), a);
+  else
+    tjh_launch(k_beam_pieces<512, 26, 4096>, grid, dim3(512), 0, stream(), a);
+  const int rc = check_launch("beam_pieces");
+  if (rc != TJH_OK) return rc;
+  tjh_launch(k_beam_merge, dim3((unsigned)B), dim3(256), 0, stream(), a);
+  return check_launch("beam_merge");
+}
+
+int tjh_cache_reorder(int n, void* const* tensors, const int64_t* outers, const int64_t* strides,
+                      const int64_t* sizes, int64_t B, int64_t W, const int32_t* parents) {
+  TJH_REQUIRE_INIT();
+  TJH_ARG(n >= 0 && B >= 0 && W >= 0, "tjh_cache_reorder: bad sizes");
+  if (W > 64)
+    return set_error(TJH_ERR_UNSUPPORTED, "tjh_cache_reorder: %lld beams, at most 64",
+                     (long long)W);
+  if (n == 0 || B == 0 || W < 2) return TJH_OK;
+  TJH_ARG(tensors && outers && strides && sizes && parents, "tjh_cache_reorder: NULL pointer");
+  TJH_ARG(B < 65536, "tjh_cache_reorder: too many searches");
+  for (int i = 0; i < n; ++i)
+    TJH_ARG(outers[i] >= 0 && sizes[i] >= 0 && strides[i] >= sizes[i] &&
+                (tensors[i] || outers[i] * sizes[i] == 0),
+            "tjh_cache_reorder: bad tensor %d", i);
+  KernelScope ks("cache_reorder");
+  int i = 0;
+  while (i < n) {
+    ReorderArgs a{};
+    a.parents = parents;
+    a.W = (int)W;
+    int64_t groups = 0;
+    for (; i < n && a.n < kTensors; ++i) {
+      if (outers[i] * sizes[i] == 0) continue;
+      Moved& t = a.t[a.n];
+      t.p = static_cast<char*>(tensors[i]);
+      t.row = outers[i] * strides[i];
+      t.stride = strides[i];
+      const uint64_t bits = (uint64_t)(uintptr_t)t.p | (uint64_t)strides[i] | (uint64_t)sizes[i];
+      t.unit = (bits & 15) == 0 ? 16 : (bits & 3) == 0 ? 4 : 1;
+      t.units = sizes[i] / t.unit;
+      const int64_t per = cdiv(t.units, 256);
+      TJH_ARG(per * outers[i] < (int64_t(1) << 23), "tjh_cache_reorder: tensor %d is too large", i);
+      if (groups + per * outers[i] >= (int64_t(1) << 23)) break;  // the next launch's
+      t.per = (int)per;
+      t.first = (int)groups;
+      groups += per * outers[i];
+      ++a.n;
+    }
+    if (a.n == 0) continue;
+    const int64_t most = (int64_t(1) << 23) / groups;  // searches of a launch
+    for (int64_t b = 0; b < B; b += most) {
+      const dim3 grid((unsigned)groups, (unsigned)(B - b < most ? B - b : most));
+      ReorderArgs part = a;
+      part.parents = parents + b * W;
+      for (int j = 0; j < a.n; ++j) part.t[j].p += b * W * a.t[j].row;
+      if (W <= 4) tjh_launch(k_reorder<4>, grid, dim3(256), 0, stream(), part);
+      else if (W <= 8) tjh_launch(k_reorder<8>, grid, dim3(256), 0, stream(), part);
+      else if (W <= 16) tjh_launch(k_reorder<16>, grid, dim3(256), 0, stream(), part);
+      else if (W <= 32) tjh_launch(k_reorder<32>, grid, dim3(256), 0, stream(), part);
+      else tjh_launch(k_reorder<64>, grid, dim3(256), 0, stream(), part);
+    }
+  }
+  return check_launch("cache_reorder");
+}
+
+}  // extern "C"

@@ -9,6 +9,7 @@
 
 #include "../../include/torchjs_hip.h"
 #include "../../include/torchjs_hip_lm.h"
+#include "../../include/torchjs_hip_decode.h"
 
 namespace tjh {
 

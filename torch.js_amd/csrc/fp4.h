@@ -1,0 +1,62 @@
+// Four-bit values: a sign and the number of a step of 0, 0.5, 1, 1.5, 2, 3, 4,
+// 6 (one sign bit, two of an exponent, one of a fraction), times a float scale
+// that several share.  The codes are those that gfx950 converts itself, two in
+// one instruction, exactly, to floats or to bfloat16.  Device only.
+#pragma once
+
+#include "common.h"
+#include "wave.h"
+
+namespace tjh {
+namespace fp4 {
+
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
+
+// The eight values of a word, the lowest 4 bits first.
+__device__ __forceinline__ void unpack(uint32_t w, float (&v)[8]) {
+  const floatx2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 0);
+  const floatx2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 1);
+  const floatx2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 2);
+  const floatx2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 3);
+  v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+  v[4] = c.x; v[5] = c.y; v[6] = d.x; v[7] = d.y;
+}
+
+// |x| as an integer in the order of magnitudes, NaN above infinity.
+__device__ __forceinline__ uint32_t magnitude(float x) {
+  return __float_as_uint(x) & 0x7fffffffu;
+}
+
+// The scale of values whose largest magnitude is `top`: top / 6, 0 where they
+// are held as zeros (under 2^-100, so that borders below stay normal floats),
+// NaN where one of them is no number.
+__device__ __forceinline__ float scale_of(uint32_t top) {
+  if (top >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
+  return top < 0x0d800000u ? 0.f : __uint_as_float(top) / 6.f;
+}
+
+// The code of x at a scale.  A step is passed where |x| is above the border
+// halfway to it, or on one whose upper step is even; the sign of |x| - border *
+// scale is exact, as it is rounded once.
+__device__ __forceinline__ uint32_t code_of(float x, float scale) {
+  const float a = fabsf(x);
+  uint32_t c = 0;
+  c += __builtin_fmaf(-0.25f, scale, a) > 0.f;
+  c += __builtin_fmaf(-0.75f, scale, a) >= 0.f;
+  c += __builtin_fmaf(-1.25f, scale, a) > 0.f;
+  c += __builtin_fmaf(-1.75f, scale, a) >= 0.f;
+  c += __builtin_fmaf(-2.5f, scale, a) > 0.f;
+  c += __builtin_fmaf(-3.5f, scale, a) >= 0.f;
+  c += __builtin_fmaf(-5.f, scale, a) > 0.f;
+  if (!(scale > 0.f)) c = 0;
+  return c | (x < 0.f ? 8u : 0u);
+}
+
+// Bytes of a cached position's codes.
+__host__ __device__ inline int row_bytes(int D) { return (D + 31) / 32 * 16; }
+
+}  // namespace fp4
+}  // namespace tjh

@@ -1,0 +1,256 @@
+// Values into four bits and back: weights (tjh_fp4_quantize, _dequantize) and
+// the positions of a key / value cache (tjh_fp4_cache_append, _read).
+#include "fp4.h"
+
+namespace tjh {
+namespace {
+
+using namespace fp4;
+
+constexpr int64_t kGrid = 1 << 21;  // workgroups of a launch: a grid has less than 2^32 threads
+
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v, int lanes) {
+  for (int o = 1; o < lanes; o <<= 1) {
+    const uint32_t w = (uint32_t)__shfl_xor((int)v, o, 64);
+    v = v > w ? v : w;
+  }
+  return v;
+}
+
+// ------------------------------------------------------------------ weights
+
+// 16 lanes a row's 128 columns, 8 columns a lane (one word of codes), 4, 8 or
+// 16 lanes a scale.  Runs once for a layer.
+__global__ __launch_bounds__(256) void k_fp4_quantize(const float* __restrict__ w, int64_t ld,
+                                                      int64_t K, int64_t nb, int64_t items,
+                                                      int lanes, uint32_t* __restrict__ codes,
+                                                      float* __restrict__ scales) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const bool on = at < items;
+  const int64_t block = (on ? at : items - 1) >> 4;  // n nb + b
+  const int i = threadIdx.x & 15;
+  const int64_t n = block / nb, k = (block - n * nb) * 128 + 8 * i;
+  float x[8];
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    x[e] = k + e < K ? w[n * ld + k + e] : 0.f;
+    top = max(top, magnitude(x[e]));
+  }
+  const float scale = scale_of(lanes_max(top, lanes));
+  uint32_t word = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) word |= code_of(x[e], scale) << (4 * e);
+  if (!on) return;
+  codes[block * 16 + 4 * (i & 3) + (i >> 2)] = word;
+  if (i % lanes == 0) scales[(block * 16 + i) / lanes] = scale;
+}
+
+// One word a thread.
+__global__ __launch_bounds__(256) void k_fp4_dequantize(const uint32_t* __restrict__ codes,
+                                                        const float* __restrict__ scales,
+                                                        int64_t K, int64_t nb, int64_t items,
+                                                        int lanes, float* __restrict__ out,
+                                                        int64_t ldo) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= items) return;
+  const int64_t block = at >> 4;
+  const int i = at & 15;
+  const int64_t n = block / nb, k = (block - n * nb) * 128 + 8 * i;
+  const float scale = scales[at / lanes];
+  float v[8];
+  unpack(codes[block * 16 + 4 * (i & 3) + (i >> 2)], v);
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (k + e < K) out[n * ldo + k + e] = v[e] * scale;
+}
+
+// -------------------------------------------------------------------- cache
+
+struct AppendArgs {
+  const float* x[2];
+  uint8_t* codes[2];
+  float* scales[2];
+  int64_t st[2][4];
+  int64_t H, T, L, pos, rows;
+  const int32_t* positions;
+  int D, P;
+};
+
+// LR lanes a position, 4 columns a lane (VEC: as one 16-byte load), rows of K
+// then of V.
+template <int LR, bool VEC>
+__global__ __launch_bounds__(256) void k_fp4_append(AppendArgs a) {
+  const int which = blockIdx.y;
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LR;
+  const bool on = at < a.rows;
+  const int64_t row = on ? at : a.rows - 1;  // (b H + h) T + t
+  const int d = 4 * (threadIdx.x % LR);
+  const int64_t bh = row / a.T, t = row - bh * a.T, b = bh / a.H, h = bh - b * a.H;
+  const int64_t* st = a.st[which];
+  const float* p = a.x[which] + b * st[0] + h * st[1] + t * st[2] + d * st[3];
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+  if (VEC) {
+    if (d < a.D) {
+      const floatx4 v = *reinterpret_cast<const floatx4*>(p);
+      x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (d + e < a.D) x[e] = p[e * st[3]];
+  }
+  const uint32_t top = max(max(magnitude(x[0]), magnitude(x[1])),
+                           max(magnitude(x[2]), magnitude(x[3])));
+  const float scale = scale_of(lanes_max(top, LR));
+  const int64_t to = (a.positions ? (int64_t)a.positions[b] : a.pos) + t;
+  if (!on || to < 0 || to >= a.L) return;
+  const uint32_t c = code_of(x[0], scale) | code_of(x[1], scale) << 4 |
+                     code_of(x[2], scale) << 8 | code_of(x[3], scale) << 12;
+  if (d < 2 * a.P)
+    *reinterpret_cast<uint16_t*>(a.codes[which] + (bh * a.L + to) * a.P + d / 2) = (uint16_t)c;
+  if (d == 0) a.scales[which][bh * a.L + to] = scale;
+}
+
+// 8 columns a thread.
+__global__ __launch_bounds__(256) void k_fp4_read(const uint8_t* __restrict__ codes,
+                                                  const float* __restrict__ scales, int64_t L,
+                                                  int D, int P, int64_t start, int64_t n,
+                                                  int64_t items, float* __restrict__ out) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= items) return;
+  const int per = (D + 7) / 8;
+  const int64_t row = at / per, bh = row / n, from = bh * L + start + row - bh * n;
+  const int d = 8 * (int)(at - row * per);
+  const float scale = scales[from];
+  float v[8];
+  unpack(*reinterpret_cast<const uint32_t*>(codes + from * P + d / 2), v);
+  float* o = out + row * D + d;
+  if (D % 4 == 0) {
+    *reinterpret_cast<floatx4*>(o) = floatx4{v[0], v[1], v[2], v[3]} * scale;
+    if (d + 4 < D) *reinterpret_cast<floatx4*>(o + 4) = floatx4{v[4], v[5], v[6], v[7]} * scale;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (d + e < D) o[e] = v[e] * scale;
+  }
+}
+
+int check_weights(const char* who, int64_t N, int64_t K, int64_t group) {
+  TJH_ARG(N >= 0 && K >= 0 && N < (int64_t(1) << 31) && K < (int64_t(1) << 30), "%s: bad sizes",
+          who);
+  TJH_ARG(group == 32 || group == 64 || group == 128, "%s: groups of %lld columns (32, 64 or 128)",
+          who, (long long)group);
+  return TJH_OK;
+}
+
+}  // namespace
+}  // namespace tjh
+
+using namespace tjh;
+
+extern "C" {
+
+int tjh_fp4_quantize(const float* w, int64_t ld, int64_t N, int64_t K, int64_t group,
+                     uint8_t* codes, float* scales) {
+  TJH_REQUIRE_INIT();
+  const int rc = check_weights("tjh_fp4_quantize", N, K, group);
+  if (rc != TJH_OK) return rc;
+  TJH_ARG(ld >= K, "tjh_fp4_quantize: bad sizes");
+  if (N == 0 || K == 0) return TJH_OK;
+  TJH_ARG(w && codes && scales && aligned16(codes), "tjh_fp4_quantize: NULL or unaligned pointer");
+  const int64_t nb = cdiv(K, 128), step = kGrid * 256;
+  TJH_ARG(nb * 16 <= step, "tjh_fp4_quantize: rows too long");
+  const int64_t rows = step / (nb * 16);  // of one launch
+  KernelScope ks("fp4_quantize");
+  for (int64_t n = 0; n < N; n += rows) {
+    const int64_t m = N - n < rows ? N - n : rows;
+    tjh_launch(k_fp4_quantize, dim3((unsigned)cdiv(m * nb * 16, 256)), dim3(256), 0, stream(),
+               w + n * ld, ld, K, nb, m * nb * 16, (int)group / 8,
+               reinterpret_cast<uint32_t*>(codes) + n * nb * 16, scales + n * nb * 128 / group);
+  }
+  return check_launch("fp4_quantize");
+}
+
+int tjh_fp4_dequantize(const uint8_t* codes, const float* scales, int64_t N, int64_t K,
+                       int64_t group, float* out, int64_t ldo) {
+  TJH_REQUIRE_INIT();
+  const int rc = check_weights("tjh_fp4_dequantize", N, K, group);
+  if (rc != TJH_OK) return rc;
+  TJH_ARG(ldo >= K, "tjh_fp4_dequantize: bad sizes");
+  if (N == 0 || K == 0) return TJH_OK;
+  TJH_ARG(out && codes && scales && aligned16(codes),
+          "tjh_fp4_dequantize: NULL or unaligned pointer");
+  const int64_t nb = cdiv(K, 128), step = kGrid * 256;
+  TJH_ARG(nb * 16 <= step, "tjh_fp4_dequantize: rows too long");
+  const int64_t rows = step / (nb * 16);
+  KernelScope ks("fp4_dequantize");
+  for (int64_t n = 0; n < N; n += rows) {
+    const int64_t m = N - n < rows ? N - n : rows;
+    tjh_launch(k_fp4_dequantize, dim3((unsigned)cdiv(m * nb * 16, 256)), dim3(256), 0, stream(),
+               reinterpret_cast<const uint32_t*>(codes) + n * nb * 16,
+               scales + n * nb * 128 / group, K, nb, m * nb * 16, (int)group / 8, out + n * ldo,
+               ldo);
+  }
+  return check_launch("fp4_dequantize");
+}
+
+int tjh_fp4_cache_append(const float* k, const float* v, const int64_t* k_strides,
+                         const int64_t* v_strides, uint8_t* k_codes, float* k_scales,
+                         uint8_t* v_codes, float* v_scales, int64_t B, int64_t H, int64_t T,
+                         int64_t D, int64_t L, int64_t pos, const int32_t* positions) {
+  TJH_REQUIRE_INIT();
+  TJH_ARG(B >= 0 && H >= 0 && T >= 0 && D > 0 && L >= 0, "tjh_fp4_cache_append: bad sizes");
+  if (D > 128 || L >= (int64_t(1) << 24))
+    return set_error(TJH_ERR_UNSUPPORTED,
+                     "tjh_fp4_cache_append: head dim %lld, length %lld (128, 2^24 - 1 at most)",
+                     (long long)D, (long long)L);
+  TJH_ARG(positions || (pos >= 0 && pos + T <= L), "tjh_fp4_cache_append: positions [%lld, %lld) of %lld",
+          (long long)pos, (long long)(pos + T), (long long)L);
+  if (B == 0 || H == 0 || T == 0 || L == 0) return TJH_OK;
+  TJH_ARG(k && v && k_strides && v_strides && k_codes && k_scales && v_codes && v_scales &&
+              aligned16(k_codes) && aligned16(v_codes),
+          "tjh_fp4_cache_append: NULL or unaligned pointer");
+  AppendArgs a{{k, v}, {k_codes, v_codes}, {k_scales, v_scales}, {}, H, T, L, pos, B * H * T,
+               positions, (int)D, fp4::row_bytes((int)D)};
+  bool vec = D % 4 == 0 && aligned16(k) && aligned16(v);
+  for (int i = 0; i < 4; ++i) {
+    a.st[0][i] = k_strides[i];
+    a.st[1][i] = v_strides[i];
+    vec = vec && (i == 3 ? k_strides[i] == 1 && v_strides[i] == 1
+                         : k_strides[i] % 4 == 0 && v_strides[i] % 4 == 0);
+  }
+  const int lanes = D <= 32 ? 8 : D <= 64 ? 16 : 32;
+  TJH_ARG(cdiv(a.rows * lanes, 256) <= kGrid, "tjh_fp4_cache_append: too many rows");
+  const dim3 grid((unsigned)cdiv(a.rows * lanes, 256), 2), block(256);
+  KernelScope ks("fp4_append");
+  if (lanes == 8 && vec) tjh_launch(k_fp4_append<8, true>, grid, block, 0, stream(), a);
+  else if (lanes == 8) tjh_launch(k_fp4_append<8, false>, grid, block, 0, stream(), a);
+  else if (lanes == 16 && vec) tjh_launch(k_fp4_append<16, true>, grid, block, 0, stream(), a);
+  else if (lanes == 16) tjh_launch(k_fp4_append<16, false>, grid, block, 0, stream(), a);
+  else if (vec) tjh_launch(k_fp4_append<32, true>, grid, block, 0, stream(), a);
+  else tjh_launch(k_fp4_append<32, false>, grid, block, 0, stream(), a);
+  return check_launch("fp4_append");
+}
+
+int tjh_fp4_cache_read(const uint8_t* codes, const float* scales, int64_t B, int64_t H, int64_t L,
+                       int64_t D, int64_t start, int64_t n, float* out) {
+  TJH_REQUIRE_INIT();
+  TJH_ARG(B >= 0 && H >= 0 && D > 0 && start >= 0 && n >= 0 && start + n <= L,
+          "tjh_fp4_cache_read: bad sizes");
+  if (D > 128 || L >= (int64_t(1) << 24))
+    return set_error(TJH_ERR_UNSUPPORTED,
+                     "tjh_fp4_cache_read: head dim %lld, length %lld (128, 2^24 - 1 at most)",
+                     (long long)D, (long long)L);
+  if (B == 0 || H == 0 || n == 0) return TJH_OK;
+  TJH_ARG(codes && scales && out && aligned16(codes) && aligned16(out),
+          "tjh_fp4_cache_read: NULL or unaligned pointer");
+  const int64_t items = B * H * n * cdiv(D, 8);
+  TJH_ARG(cdiv(items, 256) <= kGrid, "tjh_fp4_cache_read: too many rows");
+  KernelScope ks("fp4_read");
+  tjh_launch(k_fp4_read, dim3((unsigned)cdiv(items, 256)), dim3(256), 0, stream(), codes, scales,
+             L, (int)D, fp4::row_bytes((int)D), start, n, items, out);
+  return check_launch("fp4_read");
+}
+
+}  // extern "C"

@@ -55,11 +55,14 @@ struct Row {
     return __uint_as_float(__float_as_uint(p[i]) ^ sign);
   }
 
-  __device__ __forceinline__ void load(const float* row, int cols, uint32_t flip = 0) {
+  // `any` alignment: chunks from the first element on, so that what a thread
+  // holds goes by the elements' places alone (equal rows sum to equal bits)
+  __device__ __forceinline__ void load(const float* row, int cols, uint32_t flip = 0,
+                                       bool any = false) {
     p = row;
     n = cols;
     sign = flip;
-    head = min(cols, (int)((16 - ((uintptr_t)row & 15)) & 15) / 4);
+    head = any ? 0 : min(cols, (int)((16 - ((uintptr_t)row & 15)) & 15) / 4);
     n4 = (n - head) >> 2;
     const int t = threadIdx.x, tail = (n - head) & 3;
     edge_index = t < 3 ? (t < head ? t : -1) : (t - 3 < tail ? head + 4 * n4 + t - 3 : -1);

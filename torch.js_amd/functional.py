@@ -10,6 +10,9 @@ import numpy as np
 
 from . import _lib as L
 from . import tensor as _T
+from .decode_ops import (attention_fp4, beam_step, cache_append_fp4, cache_read_fp4,  # noqa: F401
+                         cache_reorder_, cache_row_bytes, dequantize_fp4, linear_fp4,
+                         quantize_fp4)
 from .tensor import _e_unary_bwd
 from .tensor import (Tensor, _DT, _alias, _contig_strides, _empty_padded, _gemm, _k_binary,
                      _k_contiguous, _k_reduce, _k_scalar, _numel, _record, _view_raw, _wrap_dim,

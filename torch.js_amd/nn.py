@@ -109,7 +109,10 @@ class Module:
             if name not in params:
                 raise KeyError("unexpected key %s in state_dict" % name)
             tgt = params[name]
-            src = value if isinstance(value, Tensor) else from_numpy(np.asarray(value))
+            src = value if isinstance(value, Tensor) else \
+                from_numpy(np.asarray(value), dtype=tgt.dtype)
+            if src.dtype != tgt.dtype:
+                src = src.to(tgt.dtype)
             if tuple(src.shape) != tgt.shape:
                 raise ValueError("size mismatch for %s: %s vs %s" % (name, list(src.shape),
                                                                    list(tgt.shape)))
@@ -134,6 +137,40 @@ class Linear(Module):
         if x.ndim == 1:
             x = x.unsqueeze(0)
         return F.linear(x, self.weight, self.bias)
+
+
+class LinearFP4(Module):
+    """nn.Linear whose weight is held in 4 bits (F.quantize_fp4, F.linear_fp4)
+    and has no gradient; `codes` and `scales` are in the state dict.
+    LinearFP4.of(linear) takes the weight and bias of an nn.Linear."""
+
+    def __init__(self, in_features, out_features, bias=True, group_size=64):
+        super().__init__()
+        self.in_features = in_features
+        self.out_features = out_features
+        self.group_size = group_size
+        w = randn(out_features, in_features).mul(math.sqrt(1.0 / in_features))
+        self._hold(w, Parameter.create(zeros(out_features)) if bias else None)
+
+    def _hold(self, weight, bias):
+        codes, scales = F.quantize_fp4(weight, self.group_size)
+        self.register_parameter("codes", codes)
+        self.register_parameter("scales", scales)
+        self.register_parameter("bias", bias)
+
+    @classmethod
+    def of(cls, linear, group_size=64):
+        self = cls.__new__(cls)
+        Module.__init__(self)
+        self.out_features, self.in_features = linear.weight.shape
+        self.group_size = group_size
+        self._hold(linear.weight, getattr(linear, "bias", None))
+        return self
+
+    def forward(self, x):
+        if x.ndim == 1:
+            x = x.unsqueeze(0)
+        return F.linear_fp4(x, self.codes, self.scales, self.bias, self.group_size)
 
 
 class LayerNorm(Module):
