@@ -85,13 +85,21 @@ class CausalSelfAttention(nn.Module):
         cached keys / values of positions [0, pos) plus their own; the new
         keys and values are appended to the cache.  A prompt (pos 0) is
         causal over itself; a single new token attends to every cached
-        position.  With a window, a prompt may also come in parts."""
+        position.  With a window, or a cache in 4 bits, a prompt may also
+        come in parts."""
         B, T, C = x.shape
         hd = C // self.heads
         q, k, v = self.c_attn(x).split(C, dim=2)
         q = q.view(B, T, self.heads, hd).transpose(1, 2)
         k = k.view(B, T, self.heads, hd).transpose(1, 2)
         v = v.view(B, T, self.heads, hd).transpose(1, 2)
+        if isinstance(cache, KVCacheFP4):
+            if self.window is not None:
+                raise NotImplementedError("KV cache in 4 bits: not with a window")
+            cache.append(layer, k, v, pos)
+            y = cache.attend(layer, q, pos + T)
+            y = y.transpose(1, 2).contiguous().view(B, T, C)
+            return self._project(y, residual)
         keys, values = cache.append(layer, k, v, pos)
         if self.window is not None:
             y = F.sliding_window_attention(q, keys, values, self.window, self.sinks)
@@ -106,7 +114,7 @@ class CausalSelfAttention(nn.Module):
         return self._project(y, residual)
 
     def _project(self, y, residual):
-        if self.fused:
+        if self.fused and type(self.c_proj) is nn.Linear:
             return F._linear_add(y, self.c_proj.weight, self.c_proj.bias, residual)
         out = self.c_proj(y)
         return out if residual is None else residual + out
@@ -120,7 +128,7 @@ class MLPBlock(nn.Module):
         self.c_proj = nn.Linear(4 * d, d)
 
     def forward(self, x, residual=None):
-        if self.fused:
+        if self.fused and type(self.c_fc) is type(self.c_proj) is nn.Linear:
             # c_proj(gelu(c_fc(x))) (+ residual) with GELU and the add fused
             # into the two GEMMs
             return F._mlp_gelu(x, self.c_fc.weight, self.c_fc.bias, self.c_proj.weight,
@@ -251,6 +259,60 @@ class KVCache:
             self.v[layer][:, :, pos:pos + T].copy_(v)
         return self.k[layer][:, :, :pos + T], self.v[layer][:, :, :pos + T]
 
+    def reorder(self, parents, length):
+        """The first `length` positions of row b * W + i become those of row
+        b * W + parents[b, i] (F.cache_reorder_), for a beam search whose W
+        beams are neighbouring rows."""
+        F.cache_reorder_(self._tensors(), parents, length)
+
+    def spread(self, prompt, length):
+        """Copies the first `length` positions of each of another cache's rows
+        to as many neighbouring rows as this one has for it."""
+        with no_grad():
+            for dst, src in zip(self._tensors(), prompt._tensors()):
+                n, rest = src.shape[0], dst.shape[1:]
+                dst = dst.view(n, dst.shape[0] // n, *rest)
+                src = src.view(n, 1, *src.shape[1:])[:, :, :, :length]
+                dst = dst[:, :, :, :length]
+                dst.copy_(src.expand(*dst.shape))
+
+    def _tensors(self):
+        return self.k + self.v
+
+
+class KVCacheFP4(KVCache):
+    """KVCache in 4 bits: codes k, v [B, H, max_len, bytes] and one float32
+    scale a position and head (F.cache_append_fp4), a seventh of the float
+    cache's memory at a head dim of 64.  A position's keys and values are held
+    once they are appended, so attention reads them as they are held, a prompt's
+    own among them."""
+
+    def __init__(self, layers, batch, heads, max_len, head_dim):
+        self.max_len, self.head_dim = max_len, head_dim
+        shape = (batch, heads, max_len)
+        row = (F.cache_row_bytes(head_dim),)
+        self.k = [zeros(*(shape + row), dtype="uint8") for _ in range(layers)]
+        self.v = [zeros(*(shape + row), dtype="uint8") for _ in range(layers)]
+        self.k_scales = [zeros(*shape) for _ in range(layers)]
+        self.v_scales = [zeros(*shape) for _ in range(layers)]
+
+    def append(self, layer, k, v, pos):
+        F.cache_append_fp4(self.k[layer], self.k_scales[layer], self.v[layer],
+                           self.v_scales[layer], k, v, pos)
+
+    def attend(self, layer, q, length, scale=None):
+        """F.attention_fp4 over a layer's first `length` positions."""
+        return F.attention_fp4(q, self.k[layer], self.k_scales[layer], self.v[layer],
+                               self.v_scales[layer], length, scale)
+
+    def read(self, layer, start, stop):
+        """(keys, values) that positions [start, stop) stand for."""
+        return (F.cache_read_fp4(self.k[layer], self.k_scales[layer], self.head_dim, start, stop),
+                F.cache_read_fp4(self.v[layer], self.v_scales[layer], self.head_dim, start, stop))
+
+    def _tensors(self):
+        return self.k + self.v + self.k_scales + self.v_scales
+
 
 class GPT2(nn.Module):
     """GPT-2 with the LM head tied to the token embedding; with `window` and
@@ -265,13 +327,30 @@ class GPT2(nn.Module):
         self.wpe = nn.Embedding(ctx, d)
         self.h = nn.ModuleList([Block(d, heads, fused, window, sinks) for _ in range(layers)])
         self.ln_f = nn.LayerNorm(d)
+        self.head = None  # the LM head in 4 bits (quantize_fp4)
+
+    def quantize_fp4(self, group_size=64, head=True):
+        """Holds the blocks' linear layers in 4 bits (nn.LinearFP4), and with
+        `head` a 4-bit copy of the token table for the logits; the tables that
+        tokens and positions are looked up in stay float."""
+        for blk in self.h:
+            for m, name in ((blk.attn, "c_attn"), (blk.attn, "c_proj"), (blk.mlp, "c_fc"),
+                            (blk.mlp, "c_proj")):
+                if type(getattr(m, name)) is nn.Linear:
+                    setattr(m, name, nn.LinearFP4.of(getattr(m, name), group_size))
+        if head:
+            self.head = nn.LinearFP4.of(self.wte, group_size)
+        return self
+
+    def _logits(self, x):
+        return F.linear(x, self.wte.weight) if self.head is None else self.head(x)
 
     def forward(self, ids):
         x = self._embed(ids, 0)
         for blk in self.h:
             x = blk(x)
         x = self.ln_f(x)
-        return F.linear(x, self.wte.weight)
+        return self._logits(x)
 
     def _embed(self, ids, pos0):
         """wte(ids) + wpe(positions pos0 .. pos0 + T - 1); with `fused` one
@@ -290,9 +369,13 @@ class GPT2(nn.Module):
         teacher's largest ones [B, T, K] (`teacher(ids).topk(K)`)."""
         return F.distillation_loss(self(ids), teacher_logits, teacher_ids, temperature)
 
-    def new_cache(self, batch, max_len=None):
+    def new_cache(self, batch, max_len=None, bits=32):
+        """A cache for `batch` rows: KVCache, or KVCacheFP4 with bits=4."""
+        if bits not in (4, 32):
+            raise ValueError("a KV cache holds 32 or 4 bits, got %r" % (bits,))
         blk = self.h[0].attn
-        return KVCache(len(self.h), batch, blk.heads, max_len or self.ctx, blk.d // blk.heads)
+        kind = KVCache if bits == 32 else KVCacheFP4
+        return kind(len(self.h), batch, blk.heads, max_len or self.ctx, blk.d // blk.heads)
 
     def forward_cached(self, ids, cache, pos):
         """Logits of positions [pos, pos + T) of ids [B, T], the keys and
@@ -302,10 +385,10 @@ class GPT2(nn.Module):
         for i, blk in enumerate(self.h):
             x = blk.forward_cached(x, cache, i, pos)
         x = self.ln_f(x)
-        return F.linear(x, self.wte.weight)
+        return self._logits(x)
 
     def generate(self, ids, max_new_tokens, temperature=1.0, greedy=False, top_k=0, top_p=1.0,
-                 min_p=0.0):
+                 min_p=0.0, beams=1, eos=None, cache_bits=32):
         """Autoregressive decoding with a KV cache (the inference side of the
         GPT-2 path, tests/gpt2.test.ts): the prompt runs once, then each
         new token is one cached step; the next token is drawn by
@@ -313,9 +396,21 @@ class GPT2(nn.Module):
         greedy).  With top_k, top_p or min_p, a temperature of 0, or one
         value a row of any of the four, it is drawn by F.sample_logits
         from the logits, without a readback in the loop; logits without a
-        distribution (NaN) raise at the end.  Returns the
+        distribution (NaN) raise at the end.  With beams > 1, the most
+        probable of the continuations that a search with so many beams keeps
+        (F.beam_step), without drawing; one that ends with the token `eos` is
+        filled up with it.  cache_bits=4 holds the cache in 4 bits.  Returns the
         [B, T + max_new_tokens] int32 ids."""
         from .tensor import cat
+        if beams != 1:
+            rules = (temperature, top_k, top_p, min_p)
+            if greedy or any(isinstance(r, Tensor) or np.ndim(r) for r in rules) or \
+                    rules != (1.0, 0, 1.0, 0.0):
+                raise ValueError("generate: a beam search draws nothing; temperature, greedy, "
+                                 "top_k, top_p and min_p do not apply")
+            return self._search(ids, max_new_tokens, beams, eos, cache_bits)
+        if eos is not None:
+            raise ValueError("generate: eos ends a beam search's sequences; beams is 1")
         B, T = ids.shape
         total = T + max_new_tokens
         if total > self.ctx:
@@ -324,7 +419,7 @@ class GPT2(nn.Module):
         cut = any(isinstance(s, Tensor) or np.ndim(s) for s in rules) or \
             temperature == 0 or top_k != 0 or top_p != 1.0 or min_p != 0.0
         with no_grad():
-            cache = self.new_cache(B, total)
+            cache = self.new_cache(B, total, cache_bits)
             logits = self.forward_cached(ids, cache, 0)
             out = [ids]
             pos = T
@@ -344,6 +439,45 @@ class GPT2(nn.Module):
             if cut and not greedy and (res.numpy()[:, T:] < 0).any():
                 raise RuntimeError("generate: logits hold NaN, infinity or nothing to draw")
             return res
+
+    def _search(self, ids, count, beams, eos, cache_bits):
+        """generate's beam search: the prompt once, its cache copied to the
+        beams, then a step, a reordering of the caches and one token of every
+        beam at a time; the best beam's tokens are followed back at the end,
+        after one readback."""
+        B, T = ids.shape
+        if not 1 < beams <= min(64, self.vocab) or beams != int(beams):
+            raise ValueError("generate: %r beams of %d tokens (from 1 to 64)"
+                             % (beams, self.vocab))
+        if T + count > self.ctx:
+            raise ValueError("generate: %d positions exceed the context of %d"
+                             % (T + count, self.ctx))
+        if not count:
+            return ids if ids.dtype == "int32" else ids.to("int32")
+        with no_grad():
+            prompt = self.new_cache(B, T, cache_bits)
+            logits = self.forward_cached(ids, prompt, 0)[:, -1, :]
+            cache = self.new_cache(B * beams, T + count, cache_bits)
+            cache.spread(prompt, T)
+            scores, tokens, parents, done = F.beam_step(logits, zeros(B, 1), beams, None, eos)
+            steps = [(tokens, parents)]
+            for pos in range(T, T + count - 1):
+                if len(steps) > 1:
+                    cache.reorder(parents, pos)
+                logits = self.forward_cached(tokens.view(B * beams, 1), cache, pos)
+                scores, tokens, parents, done = F.beam_step(
+                    logits.view(B * beams, -1), scores, beams, done if eos is not None else None,
+                    eos)
+                steps.append((tokens, parents))
+            at = np.zeros(B, np.int64)
+            out = np.empty((B, count), np.int32)
+            for i in range(count - 1, -1, -1):
+                tokens, parents = (t.numpy() for t in steps[i])
+                out[:, i] = tokens[np.arange(B), at]
+                at = parents[np.arange(B), at]
+            if (out < 0).any():
+                raise RuntimeError("generate: logits hold NaN, infinity or nothing to choose")
+            return from_numpy(np.concatenate([ids.numpy().astype(np.int32), out], 1))
 
 
 def load_params(model, params):
