@@ -86,26 +86,34 @@ __global__ __launch_bounds__(256) void k_beam_merge(BeamArgs a) {
     count = 0;
   }
   if (t < kMaxBeams) chosen[t] = -1;
-  for (int w = t; w < a.W; w += 256) {
+  // a wave a beam, its lanes the pieces, always added up in one order
+  for (int w = t >> 6; w < a.W; w += 4) {
+    const int lane = t & 63;
     const double s = a.scores[r0 + w];
-    from[w] = s;
+    int st = 0;
+    double less = 0.0;
     if (!(s > -INFINITY)) {
-      state[w] = 2;
+      st = 2;
     } else if (a.finished && a.finished[r0 + w]) {
-      state[w] = 1;
+      st = 1;
     } else {
-      const float2* st = a.stats + (r0 + w) * a.S;
+      const float2* p = a.stats + (r0 + w) * a.S;
       float m = -INFINITY;
-      for (int i = 0; i < a.S; ++i) m = fmaxf(m, st[i].x);
+      for (int i = lane; i < a.S; i += 64) m = fmaxf(m, p[i].x);
+      m = wave_max(m);
       double sum = 0.0;
-      for (int i = 0; i < a.S; ++i) {
-        const float2 p = st[i];
-        sum += p.x == -INFINITY ? (double)p.y : (double)p.y * exp((double)p.x - (double)m);
+      for (int i = lane; i < a.S; i += 64) {
+        const float2 x = p[i];
+        sum += x.x == -INFINITY ? (double)x.y : (double)x.y * exp((double)x.x - (double)m);
       }
+      for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
       // NaN in the sum, +infinity as the maximum, or nothing above -infinity
-      const bool ok = sum > 0.0 && sum < INFINITY && m < INFINITY && m > -INFINITY;
-      state[w] = ok ? 0 : 2;
-      from[w] = s - ((double)m + log(sum));
+      if (!(sum > 0.0 && sum < INFINITY && m < INFINITY && m > -INFINITY)) st = 2;
+      else less = (double)m + log(sum);
+    }
+    if (lane == 0) {
+      state[w] = st;
+      from[w] = s - less;
     }
   }
   __syncthreads();
@@ -128,6 +136,7 @@ __global__ __launch_bounds__(256) void k_beam_merge(BeamArgs a) {
   for (int i = t; i < lists; i += 256) {
     const u64 me = head[i];
     int rank = 0;
+#pragma unroll 8
     for (int j = 0; j < lists; ++j) rank += head[j] > me || (head[j] == me && j < i);
     if (rank < a.keep) chosen[rank] = i;
     if (rank == a.keep - 1) bound = me;
@@ -150,6 +159,7 @@ __global__ __launch_bounds__(256) void k_beam_merge(BeamArgs a) {
     const u64 me = key[i];
     const int f = flat[i];
     int rank = 0;
+#pragma unroll 4
     for (int j = 0; j < n; ++j) rank += key[j] > me || (key[j] == me && flat[j] < f);
     if (rank >= a.keep) continue;
     const int w = f / a.V, v = f - w * a.V;
@@ -252,7 +262,7 @@ int tjh_beam_step(const float* logits, int64_t ld, const float* scores, const ui
   int per = 53248 - 4;
   for (const int size : {1024 - 4, 4096 - 4, 16384 - 4}) {
     const int64_t S = cdiv(V, size);
-    if (S == 1 || (W * S <= 256 && rows * S <= 2 * num_cus())) {
+    if (S == 1 || (W * S <= 256 && rows * S <= 4 * num_cus())) {
       per = size;
       break;
     }

@@ -14,6 +14,10 @@ typedef float floatx2 __attribute__((ext_vector_type(2)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
+typedef float floatx4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef float floatx2u __attribute__((ext_vector_type(2), aligned(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 // The eight values of a word, the lowest 4 bits first.
 __device__ __forceinline__ void unpack(uint32_t w, float (&v)[8]) {
@@ -23,6 +27,55 @@ __device__ __forceinline__ void unpack(uint32_t w, float (&v)[8]) {
   const floatx2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 3);
   v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
   v[4] = c.x; v[5] = c.y; v[6] = d.x; v[7] = d.y;
+}
+
+// The same as a matrix operand.
+__device__ __forceinline__ bf16x8 steps(uint32_t w) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.f, 0);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.f, 1);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.f, 2);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.f, 3);
+  return bf16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+// A float as three bfloat16 parts, eight bits of its significand each: every
+// part is cut off, so that what is left is exact.  A part is the high half of a
+// word; two are packed into one.
+__device__ __forceinline__ float cut(float x) {
+  return __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+}
+__device__ __forceinline__ uint32_t pack_high(float a, float b) {
+  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
+}
+// What is left of x; an infinity is its first part alone.
+__device__ __forceinline__ float rest(float x) {
+  const float h = cut(x);
+  return x == h ? 0.f : x - h;
+}
+__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&part)[3]) {
+  uintx4 p[3];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const float a = rest(x[2 * q]), b = rest(x[2 * q + 1]);
+    p[0][q] = pack_high(x[2 * q], x[2 * q + 1]);
+    p[1][q] = pack_high(a, b);
+    p[2][q] = pack_high(a - cut(a), b - cut(b));
+  }
+#pragma unroll
+  for (int i = 0; i < 3; ++i) part[i] = __builtin_bit_cast(bf16x8, p[i]);
+}
+// The same of numbers that are no infinities.
+__device__ __forceinline__ void split8_finite(const float (&x)[8], bf16x8 (&part)[3]) {
+  uintx4 p[3];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const float a = x[2 * q] - cut(x[2 * q]), b = x[2 * q + 1] - cut(x[2 * q + 1]);
+    p[0][q] = pack_high(x[2 * q], x[2 * q + 1]);
+    p[1][q] = pack_high(a, b);
+    p[2][q] = pack_high(a - cut(a), b - cut(b));
+  }
+#pragma unroll
+  for (int i = 0; i < 3; ++i) part[i] = __builtin_bit_cast(bf16x8, p[i]);
 }
 
 // |x| as an integer in the order of magnitudes, NaN above infinity.

@@ -25,8 +25,8 @@ struct AttArgs {
   const int32_t* lengths;
   int64_t qb, qh, qt, ob, oh, ot;
   int64_t L, length;
-  int B, H, Hkv, Tq, D, P, group;
-  int row_groups, slices;
+  int B, H, Hkv, Tq, D, group;
+  int row_tiles, slices;
   float scale;
 };
 
@@ -36,170 +36,297 @@ __device__ __forceinline__ int length_of(const AttArgs& a, int b) {
   return n < 0 ? 0 : n > a.L ? (int)a.L : n;
 }
 
-// Few queries.  A row is one query of one of the heads that share a key head;
-// a workgroup takes R rows of one key head and a slice of the keys.  LPK lanes
-// have a key, 16 columns each; each lane group walks its own keys, U of them at
-// a time, with sums of its own; the maxima are raised only when a score is
-// 2^kSlack above them, so that sums are rescaled once or twice in a walk.
+// A row is one query of one of the heads that share a key head; a wave takes 16
+// rows of one key head and walks tiles of 32 keys.  No operand changes lanes:
+//
+//   S^T[key, row] = K q^T: lane (j, n) feeds key n of each half tile and row n,
+//     columns 8 NB j + 8 t + e in product t (any order serves that is the same in
+//     both), q as three bfloat16 parts, and gets the scores of row n with the keys
+//     4 j + r of both halves;
+//   O[row, column] = P V: those eight keys are what lane (j, n) feeds of row n, in
+//     three parts, so it feeds the same keys of V: eight words, one of each key,
+//     whose 8 x 8 codes are transposed in registers.
+//
+// Running maxima are raised only when a score is 2^kSlack above them, the same in
+// the four lanes of a row; then the sums are rescaled.
 constexpr float kSlack = 10.f;
-constexpr int kWaves = 4;
+constexpr int kWaves = 4, kTile = 32;
 
-template <int LPK, int R, int U>
-__global__ __launch_bounds__(64 * kWaves) void k_fp4_attend(AttArgs a) {
-  constexpr int SPW = 64 / LPK, kSlots = SPW * kWaves, DP = 16 * LPK, PR = 4 * kWaves;
-  __shared__ float sm[PR][R], sl[PR][R];
-  __shared__ float so[PR][R][DP];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int part = lane % LPK, slot = w * SPW + lane / LPK;
-  int id = blockIdx.x;
-  const int rg = id % a.row_groups;
-  id /= a.row_groups;
-  const int slice = id % a.slices;
-  const int bh = id / a.slices, b = bh / a.Hkv, kh = bh - b * a.Hkv;
-  const int len = length_of(a, b);
-  const int rows = a.group * a.Tq, r0 = rg * R;
-  // keys that each row sees, and all of them together
-  int seen[R], most = 0;
-  float q[R][16];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int row = r0 + r < rows ? r0 + r : rows - 1;
-    const int h = row / a.Tq, i = row - h * a.Tq;
-    seen[r] = max(0, len - a.Tq + i + 1);
-    most = max(most, seen[r]);
-    const float* p = a.q + b * a.qb + (int64_t)(kh * a.group + h) * a.qh + i * a.qt + 16 * part;
-#pragma unroll
-    for (int d = 0; d < 16; ++d)
-      q[r][d] = 16 * part + d < a.D ? p[d] * (a.scale * kLog2e) : 0.f;
+// NB: words of a key that a lane feeds, a quarter of its codes.
+template <int NB>
+struct Dims {
+  static constexpr int CH = NB == 1 ? 4 : NB == 2 ? 8 : 16;  // words of V's rows, over the lanes
+  static constexpr int NT = CH / 2;                          // column tiles
+  static constexpr int DP = 8 * CH;
+  // column of lane n in tile d
+  __device__ __forceinline__ static int column(int n, int d) {
+    return 8 * (n % CH) + n / CH + 16 / CH * d;
   }
-  // this slice's keys: equal runs of the sequence's own
-  const int per = (most + a.slices - 1) / a.slices;
+};
+
+// w[d] = the d-th of the lane's columns: the codes of the eight keys whose words
+// are a[0..8).
+template <int NB>
+__device__ __forceinline__ void transpose(const uint32_t (&a)[8], int n,
+                                          uint32_t (&w)[Dims<NB>::NT]) {
+  uint32_t u[8], v[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {  // columns 0 to 3 and 4 to 7
+    u[i] = __builtin_amdgcn_perm(a[i + 4], a[i], 0x05040100);
+    u[i + 4] = __builtin_amdgcn_perm(a[i + 4], a[i], 0x07060302);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {  // pairs of columns
+    if (i & 2) continue;
+    v[i] = __builtin_amdgcn_perm(u[i + 2], u[i], 0x06020400);
+    v[i + 2] = __builtin_amdgcn_perm(u[i + 2], u[i], 0x07030501);
+  }
+  constexpr uint32_t kLow = 0x0f0f0f0fu;
+  const auto even = [&](uint32_t x, uint32_t y) { return (x & kLow) | ((y << 4) & ~kLow); };
+  const auto odd = [&](uint32_t x, uint32_t y) { return ((x >> 4) & kLow) | (y & ~kLow); };
+  if constexpr (Dims<NB>::CH == 16) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      w[i] = even(v[i], v[i + 1]);
+      w[i + 1] = odd(v[i], v[i + 1]);
+    }
+  } else if constexpr (Dims<NB>::CH == 8) {  // columns n / 8 + 2 d
+    const int s = n < 8 ? 0 : 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = ((v[2 * i] >> s) & kLow) | ((v[2 * i + 1] << (4 - s)) & ~kLow);
+  } else {  // columns n / 4 + 4 d
+    const int s = n & 4;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t x = n < 8 ? v[4 * i] : v[4 * i + 2], y = n < 8 ? v[4 * i + 1] : v[4 * i + 3];
+      w[i] = ((x >> s) & kLow) | ((y << (4 - s)) & ~kLow);
+    }
+  }
+}
+
+template <int NB>
+struct Keys {  // a lane's part of a tile
+  uint32_t k[2][NB], v[8];
+  floatx4 ks[2], vs[2];
+};
+
+template <int NB>
+__device__ __forceinline__ void load_words(uint32_t (&w)[NB], const uint8_t* p) {
+  typedef uint32_t uintx3 __attribute__((ext_vector_type(3), aligned(4)));
+  if constexpr (NB == 4) {
+    const uintx4 x = *reinterpret_cast<const uintx4*>(p);
+    w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+  } else if constexpr (NB == 3) {
+    const uintx3 x = *reinterpret_cast<const uintx3*>(p);
+    w[0] = x.x; w[1] = x.y; w[2] = x.z;
+  } else if constexpr (NB == 2) {
+    const uintx2 x = *reinterpret_cast<const uintx2*>(p);
+    w[0] = x.x; w[1] = x.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+
+// SPLIT: the waves of a workgroup share 16 rows' keys, tile by tile; otherwise
+// each has rows of its own.
+template <int NB, bool SPLIT>
+__global__ __launch_bounds__(64 * kWaves) void k_fp4_attend(AttArgs a) {
+  typedef Dims<NB> Z;
+  constexpr int NT = Z::NT, P = 16 * NB;
+  const int lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int id = blockIdx.x;
+  const int groups = SPLIT ? a.row_tiles : (a.row_tiles + kWaves - 1) / kWaves;
+  const int g = groups - 1 - id % groups;  // the last queries have the most keys: first
+  id /= groups;
+  const int slice = id % a.slices, bh = id / a.slices;
+  const int tile = SPLIT ? g : g * kWaves + w;
+  if (!SPLIT && tile >= a.row_tiles) return;
+  const int b = bh / a.Hkv, kh = bh - b * a.Hkv, len = length_of(a, b);
+  const int rows = a.group * a.Tq, r0 = 16 * tile;
+  // keys that this lane's row sees; that any and that all of the rows see
+  const int row = min(r0 + n, rows - 1), h = row / a.Tq, i = row - h * a.Tq;
+  const int seen = max(0, len - a.Tq + i + 1);
+  const int last = min(r0 + 15, rows - 1), h0 = r0 / a.Tq, h1 = last / a.Tq;
+  const int most = max(0, h0 == h1 ? len - a.Tq + last - h1 * a.Tq + 1 : len);
+  const int least = max(0, len - a.Tq + (h0 == h1 ? r0 - h0 * a.Tq : 0) + 1);
+  const int per = ((most + a.slices - 1) / a.slices + kTile - 1) / kTile * kTile;
   const int from = min(most, slice * per), to = min(most, from + per);
+  bf16x8 q[NB][3];
+  {
+    const float* p = a.q + b * a.qb + (int64_t)(kh * a.group + h) * a.qh + i * a.qt;
+    const float f = a.scale * kLog2e;
+#pragma unroll
+    for (int t = 0; t < NB; ++t) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int d = 8 * (NB * j + t) + e;
+        x[e] = d < a.D ? p[d] * f : 0.f;
+      }
+      split8(x, q[t]);
+    }
+  }
   const int64_t base = (int64_t)bh * a.L;
-  const uint8_t* __restrict__ kc = a.kc + base * a.P + 8 * part;
-  const uint8_t* __restrict__ vc = a.vc + base * a.P + 8 * part;
+  const uint8_t* __restrict__ kc = a.kc + base * P + 4 * NB * j;
+  const uint8_t* __restrict__ vc = a.vc + base * P + 4 * min(n % Z::CH, 4 * NB - 1);
   const float* __restrict__ ks = a.ks + base;
   const float* __restrict__ vs = a.vs + base;
-  const bool held = 8 * part < a.P;
-  float m[R], l[R], o[R][16];
+  const auto load = [&](int t0, Keys<NB>& x) {
+    if (t0 + kTile <= to) {
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    m[r] = -INFINITY;
-    l[r] = 0.f;
+      for (int s = 0; s < 2; ++s) {
+        load_words(x.k[s], kc + (int64_t)(t0 + 16 * s + n) * P);
+        x.ks[s] = *reinterpret_cast<const floatx4u*>(ks + t0 + 16 * s + 4 * j);
+        x.vs[s] = *reinterpret_cast<const floatx4u*>(vs + t0 + 16 * s + 4 * j);
 #pragma unroll
-    for (int d = 0; d < 16; ++d) o[r][d] = 0.f;
-  }
-  for (int t0 = from + slot; __any(t0 < to); t0 += kSlots * U) {
-    uintx2 kw[U], vw[U];
-    float kscale[U], vscale[U];
+        for (int r = 0; r < 4; ++r)
+          x.v[4 * s + r] = *reinterpret_cast<const uint32_t*>(
+              vc + (int64_t)(t0 + 16 * s + 4 * j + r) * P);
+      }
+    } else {  // past the last key: that one again, with weights of 0
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int t = min(t0 + u * kSlots, to - 1);  // past the slice: its last key, not used
-      kw[u] = held ? *reinterpret_cast<const uintx2*>(kc + (int64_t)t * a.P) : uintx2{0, 0};
-      vw[u] = held ? *reinterpret_cast<const uintx2*>(vc + (int64_t)t * a.P) : uintx2{0, 0};
-      kscale[u] = ks[t];
-      vscale[u] = vs[t];
-    }
-    float s[U][R];
+      for (int s = 0; s < 2; ++s) {
+        load_words(x.k[s], kc + (int64_t)min(t0 + 16 * s + n, to - 1) * P);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float k[16];
-      unpack(kw[u].x, reinterpret_cast<float(&)[8]>(k[0]));
-      unpack(kw[u].y, reinterpret_cast<float(&)[8]>(k[8]));
-      const int t = t0 + u * kSlots;
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        float x = 0.f;
-#pragma unroll
-        for (int d = 0; d < 16; ++d) x = __builtin_fmaf(q[r][d], k[d], x);
-        if (LPK > 1) x += dpp_f<kDppXor1>(x);
-        if (LPK > 2) x += dpp_f<kDppXor2>(x);
-        if (LPK > 4) x += dpp_f<0x141>(x);  // row_half_mirror: the other four of eight
-        s[u][r] = t < to && t < seen[r] ? x * kscale[u] : -INFINITY;
+        for (int r = 0; r < 4; ++r) {
+          const int t = min(t0 + 16 * s + 4 * j + r, to - 1);
+          x.ks[s][r] = ks[t];
+          x.vs[s][r] = vs[t];
+          x.v[4 * s + r] = *reinterpret_cast<const uint32_t*>(vc + (int64_t)t * P);
+        }
       }
     }
-    float ms[R];
+  };
+  const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
+  floatx4 o[NT];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      float top = s[0][r];
+  for (int d = 0; d < NT; ++d) o[d] = zero;
+  float m = -INFINITY, l = 0.f;
+  const int step = SPLIT ? kTile * kWaves : kTile;
+  int t0 = from + (SPLIT ? w * kTile : 0);
+  Keys<NB> next;
+  if (t0 < to) load(t0, next);
+  for (; t0 < to; t0 += step) {
+    const Keys<NB> x = next;
+    if (t0 + step < to) load(t0 + step, next);
+    floatx4 s[2] = {zero, zero};
 #pragma unroll
-      for (int u = 1; u < U; ++u) top = fmaxf(top, s[u][r]);
-      if (__any(top > m[r] + kSlack)) {
-        const float up = fmaxf(m[r], top);
-        const float f = up == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[r] - up);
-        m[r] = up;
-        l[r] *= f;
+    for (int part = 2; part >= 0; --part)
 #pragma unroll
-        for (int d = 0; d < 16; ++d) o[r][d] *= f;
+      for (int t = 0; t < NB; ++t)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+          s[y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(steps(x.k[y][t]), q[t][part], s[y], 0, 0, 0);
+    float p[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] = s[e >> 2][e & 3] * x.ks[e >> 2][e & 3];
+    const bool masked = t0 + kTile > min(to, least);
+    bool sees[8];
+    if (masked) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int t = t0 + 16 * (e >> 2) + 4 * j + (e & 3);
+        sees[e] = t < to && t < seen;
+        if (!sees[e]) p[e] = -INFINITY;
       }
-      ms[r] = m[r] == -INFINITY ? 0.f : m[r];
     }
+    float top = p[0];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float v[16];
-      unpack(vw[u].x, reinterpret_cast<float(&)[8]>(v[0]));
-      unpack(vw[u].y, reinterpret_cast<float(&)[8]>(v[8]));
-      const int t = t0 + u * kSlots;
+    for (int e = 1; e < 8; ++e) top = fmaxf(top, p[e]);
+    if (__any(top > m + kSlack)) {
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float up = fmaxf(m, top);
+      const float f = up == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - up);
+      m = up;
+      l *= f;
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const bool sees = t < to && t < seen[r];
-        const float p = sees ? __builtin_amdgcn_exp2f(s[u][r] - ms[r]) : 0.f;
-        const float pv = sees ? p * vscale[u] : 0.f;  // what is not seen may hold NaN
-        l[r] += p;
+      for (int r = 0; r < 4; ++r) {
+        const float fr = __shfl(f, 4 * j + r, 64);
 #pragma unroll
-        for (int d = 0; d < 16; ++d) o[r][d] = __builtin_fmaf(pv, v[d], o[r][d]);
+        for (int d = 0; d < NT; ++d) o[d][r] *= fr;
       }
+    }
+    const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float y = __builtin_amdgcn_exp2f(p[e] - ms);
+      l += y;
+      p[e] = y * x.vs[e >> 2][e & 3];
+    }
+    if (masked) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (!sees[e]) p[e] = 0.f;  // the scale of what is not seen may be NaN
+    }
+    bf16x8 pp[3];
+    split8_finite(p, pp);
+    uint32_t v[NT];
+    transpose<NB>(x.v, n, v);
+#pragma unroll
+    for (int d = 0; d < NT; ++d) {
+      const bf16x8 vb = steps(v[d]);
+#pragma unroll
+      for (int part = 2; part >= 0; --part)
+        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pp[part], vb, o[d], 0, 0, 0);
     }
   }
-  // one sum of each 16 lanes, then of all of them
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    float top = m[r];
-    if (LPK <= 2) top = fmaxf(top, dpp_f<kDppXor2>(top));
-    if (LPK <= 4) top = fmaxf(top, dpp_f<kDppRor4>(top));
-    top = fmaxf(top, dpp_f<kDppRor8>(top));
-    const float f = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[r] - top);
-    const auto join = [&](float x) {
-      if (LPK <= 2) x += dpp_f<kDppXor2>(x);
-      if (LPK <= 4) x += dpp_f<kDppRor4>(x);
-      return x + dpp_f<kDppRor8>(x);
-    };
-    const float sum = join(l[r] * f);
-    const int at = w * 4 + (lane >> 4);
-    if ((lane & 15) == 0) {
-      sm[at][r] = top;
-      sl[at][r] = sum;
-    }
-#pragma unroll
-    for (int d = 0; d < 16; ++d) {
-      const float x = join(o[r][d] * f);
-      if ((lane & 15) < LPK) so[at][r][16 * part + d] = x;
-    }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < R * DP; i += 64 * kWaves) {
-    const int r = i / DP, d = i - r * DP;
-    if (r0 + r >= rows || d >= a.D) continue;
-    float top = -INFINITY;
-    for (int s = 0; s < PR; ++s) top = fmaxf(top, sm[s][r]);
-    const float ts = top == -INFINITY ? 0.f : top;
-    float num = 0.f, den = 0.f;
-    for (int s = 0; s < PR; ++s) {
-      const float f = __builtin_amdgcn_exp2f(sm[s][r] - ts);
-      den = __builtin_fmaf(sl[s][r], f, den);
-      num = __builtin_fmaf(so[s][r][d], f, num);
-    }
-    const int h = (r0 + r) / a.Tq, t = r0 + r - h * a.Tq;
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  // lane (j, n) has the columns of lane n of rows 4 j + r
+  const auto put = [&](int r, int d, float num, float den, float top) {
+    const int at = r0 + r;
+    if (at >= rows || d >= a.D) return;
     if (a.slices == 1) {
+      const int hh = at / a.Tq, t = at - hh * a.Tq;
       // no key seen: zeros
-      a.o[b * a.ob + (int64_t)(kh * a.group + h) * a.oh + t * a.ot + d] = den == 0.f ? 0.f : num / den;
+      a.o[b * a.ob + (int64_t)(kh * a.group + hh) * a.oh + t * a.ot + d] =
+          den == 0.f ? 0.f : num / den;
     } else {
-      const int64_t to = ((int64_t)bh * rows + r0 + r) * a.slices + slice;
-      a.po[to * a.D + d] = num;
+      const int64_t p = ((int64_t)bh * rows + at) * a.slices + slice;
+      a.po[p * a.D + d] = num;
       if (d == 0) {
-        a.pm[to] = top;
-        a.pl[to] = den;
+        a.pm[p] = top;
+        a.pl[p] = den;
       }
+    }
+  };
+  if constexpr (SPLIT) {
+    __shared__ float sm[kWaves][16], sl[kWaves][16];
+    __shared__ float so[kWaves][16][Z::DP + 4];
+    if (lane < 16) {
+      sm[w][n] = m;
+      sl[w][n] = l;
+    }
+#pragma unroll
+    for (int d = 0; d < NT; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) so[w][4 * j + r][Z::column(n, d)] = o[d][r];
+    __syncthreads();
+    const int live = min(16, rows - r0);
+    for (int e = threadIdx.x; e < live * Z::DP; e += 64 * kWaves) {
+      const int r = e / Z::DP, d = e % Z::DP;
+      float top = sm[0][r];
+#pragma unroll
+      for (int y = 1; y < kWaves; ++y) top = fmaxf(top, sm[y][r]);
+      const float ts = top == -INFINITY ? 0.f : top;
+      float num = 0.f, den = 0.f;
+#pragma unroll
+      for (int y = 0; y < kWaves; ++y) {
+        const float f = __builtin_amdgcn_exp2f(sm[y][r] - ts);
+        num = __builtin_fmaf(so[y][r][d], f, num);
+        den = __builtin_fmaf(sl[y][r], f, den);
+      }
+      put(r, d, num, den, top);
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float den = __shfl(l, 4 * j + r, 64), top = __shfl(m, 4 * j + r, 64);
+#pragma unroll
+      for (int d = 0; d < NT; ++d) put(4 * j + r, Z::column(n, d), o[d][r], den, top);
     }
   }
 }
@@ -225,12 +352,13 @@ __global__ __launch_bounds__(128) void k_fp4_join(AttArgs a) {
   a.o[b * a.ob + h * a.oh + t * a.ot + d] = den == 0.f ? 0.f : num / den;
 }
 
-template <int LPK>
-void launch_few(AttArgs& a, int R) {
-  const dim3 grid((unsigned)(a.B * a.Hkv * a.slices * a.row_groups)), block(64 * kWaves);
-  if (R == 1) tjh_launch((k_fp4_attend<LPK, 1, 4>), grid, block, 0, stream(), a);
-  else if (R == 2) tjh_launch((k_fp4_attend<LPK, 2, 4>), grid, block, 0, stream(), a);
-  else tjh_launch((k_fp4_attend<LPK, 4, 2>), grid, block, 0, stream(), a);
+template <int NB>
+void launch_attend(const AttArgs& a, bool split) {
+  const dim3 block(64 * kWaves);
+  const int groups = split ? a.row_tiles : (int)cdiv(a.row_tiles, kWaves);
+  const dim3 grid((unsigned)(a.B * a.Hkv * a.slices * groups));
+  if (split) tjh_launch((k_fp4_attend<NB, true>), grid, block, 0, stream(), a);
+  else tjh_launch((k_fp4_attend<NB, false>), grid, block, 0, stream(), a);
 }
 
 }  // namespace
@@ -267,15 +395,17 @@ extern "C" int tjh_fp4_attention(const float* q, const uint8_t* k_codes, const f
   a.ob = o_strides[0]; a.oh = o_strides[1]; a.ot = o_strides[2];
   a.L = L; a.length = length;
   a.B = (int)B; a.H = (int)H; a.Hkv = (int)Hkv; a.Tq = (int)Tq; a.D = (int)D;
-  a.P = fp4::row_bytes((int)D);
   a.group = (int)(H / Hkv);
   a.scale = scale;
   const int64_t rows = a.group * Tq;
-  const int R = rows == 1 ? 1 : rows == 2 ? 2 : 4;
-  a.row_groups = (int)cdiv(rows, R);
-  // slices of the keys until the CUs have two workgroups each, none under 128 keys
-  const int64_t keys = lengths ? L : length, wgs = B * Hkv * a.row_groups;
-  const int64_t want = cdiv(2 * num_cus(), wgs), can = cdiv(keys, 128);
+  a.row_tiles = (int)cdiv(rows, 16);
+  // the waves of a workgroup share a row tile's keys where there are too few
+  // tiles for a wave on every SIMD; then slices of the keys until the CUs have
+  // two workgroups each, none under 128 keys (a tile of each wave)
+  const int64_t keys = lengths ? L : length, tiles = B * Hkv * a.row_tiles;
+  const bool split = tiles < 4 * num_cus();
+  const int64_t wgs = split ? tiles : B * Hkv * cdiv(a.row_tiles, kWaves);
+  const int64_t want = cdiv(2 * num_cus(), wgs), can = cdiv(keys, split ? 128 : 512);
   a.slices = (int)(want < can ? want : can);
   if (a.slices < 1) a.slices = 1;
   KernelScope ks("fp4_attention");
@@ -288,9 +418,10 @@ extern "C" int tjh_fp4_attention(const float* q, const uint8_t* k_codes, const f
     a.po = a.pl + n;
   }
   TJH_ARG(wgs * a.slices < (int64_t(1) << 23), "tjh_fp4_attention: too many queries");
-  if (D <= 32) launch_few<2>(a, R);
-  else if (D <= 64) launch_few<4>(a, R);
-  else launch_few<8>(a, R);
+  if (D <= 32) launch_attend<1>(a, split);
+  else if (D <= 64) launch_attend<2>(a, split);
+  else if (D <= 96) launch_attend<3>(a, split);
+  else launch_attend<4>(a, split);
   int rc = check_launch("fp4_attend");
   if (rc != TJH_OK || a.slices == 1) return rc;
   tjh_launch(k_fp4_join, dim3((unsigned)(B * H * Tq)), dim3(128), 0, stream(), a);

@@ -15,11 +15,6 @@ namespace {
 
 using namespace fp4;
 
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float floatx4u __attribute__((ext_vector_type(4), aligned(4)));
-typedef float floatx2u __attribute__((ext_vector_type(2), aligned(4)));
-
 struct LinArgs {
   const float* x;
   const uintx4* parts;  // x in fragments (k_split_rows), or NULL
@@ -32,32 +27,19 @@ struct LinArgs {
   int rows;  // of x a workgroup takes (grid y)
 };
 
-// The eight steps of a word as a matrix operand.
-__device__ __forceinline__ bf16x8 steps(uint32_t w) {
-  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.f, 0);
-  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.f, 1);
-  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.f, 2);
-  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.f, 3);
-  return bf16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
-}
-
-// The part-th (0, 1, 2) eight bits of x's significand as a bfloat16 in the high
-// half: each part is cut off, what is left is exact.  An infinity is its first
-// part alone.
-__device__ __forceinline__ uint32_t part_of(float x, int part) {
-  const float h = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
-  const float r = x == h ? 0.f : x - h;
-  const float m = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
-  return __float_as_uint(part == 0 ? x : part == 1 ? r : r - m);
-}
-__device__ __forceinline__ uint32_t pack_high(uint32_t a, uint32_t b) {
-  return __builtin_amdgcn_perm(b, a, 0x07060302);
-}
+// Part `part` of eight floats.
 __device__ __forceinline__ bf16x8 parts_of(const float (&x)[8], int part) {
   uintx4 v;
 #pragma unroll
-  for (int q = 0; q < 4; ++q)
-    v[q] = pack_high(part_of(x[2 * q], part), part_of(x[2 * q + 1], part));
+  for (int q = 0; q < 4; ++q) {
+    float y[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float r = rest(x[2 * q + i]);
+      y[i] = part == 0 ? x[2 * q + i] : part == 1 ? r : r - cut(r);
+    }
+    v[q] = pack_high(y[0], y[1]);
+  }
   return __builtin_bit_cast(bf16x8, v);
 }
 

@@ -11,6 +11,7 @@ value becomes the nearest step, of two that are as near the one whose number is
 even.  Values whose largest magnitude is under 2^-100 are held as zeros; where
 one is NaN or infinite, all that share its scale become NaN."""
 import ctypes
+import functools
 
 import numpy as np
 
@@ -341,41 +342,53 @@ def cache_reorder_(tensors, parents, length=None):
         raise ValueError("%s: expected parents [B, W], got shape %s"
                          % (who, list(parents.shape)))
     B, W = parents.shape
-    n = len(tensors)
-    ptrs, outers, strides, sizes, spans = [], [], [], [], []
+    if length is not None and length != int(length):
+        raise ValueError("%s: %r positions" % (who, length))
     for t in tensors:
-        sh = t._shape
-        if not sh or sh[0] != B * W:
-            raise ValueError("%s: a tensor of shape %s for %d rows" % (who, list(sh), B * W))
-        if not t.is_contiguous():
-            raise ValueError("%s: a tensor of shape %s is not contiguous" % (who, list(sh)))
         if t.requires_grad:
             raise RuntimeError("%s: a tensor that requires grad is changed in place" % who)
-        item = t.itemsize
+    geometry = _reorder_geometry(tuple([(t._shape, t._strides, t._dtype) for t in tensors]), B * W,
+                                 None if length is None else int(length))
+    ptrs = [t.data_ptr() for t in tensors]
+    parents = parents.contiguous()
+    spans = list(zip(ptrs, geometry[0]))
+    spans.append((parents.data_ptr(), 4 * parents.numel()))
+    spans.sort()
+    end = 0
+    for p, size in spans:
+        if size:
+            if p < end:
+                raise ValueError("%s: tensors share memory" % who)
+            end = p + size
+    _T._before_write(*tensors)
+    L.check(L.lib().tjh_cache_reorder(len(ptrs), (ctypes.c_void_p * max(1, len(ptrs)))(*ptrs),
+                                      *geometry[1:], B, W, parents.data_ptr()), who)
+
+
+@functools.lru_cache(maxsize=256)
+def _reorder_geometry(kinds, rows, length):
+    """(bytes of each tensor, blocks a row, bytes of a block, of them moved), the
+    last three as the library takes them, for tensors of these shapes, strides and
+    types."""
+    who = "cache_reorder_"
+    total, outers, strides, sizes = [], [], [], []
+    for sh, st, dtype in kinds:
+        if not sh or sh[0] != rows:
+            raise ValueError("%s: a tensor of shape %s for %d rows" % (who, list(sh), rows))
+        if any(a != b for a, b, n in zip(st, _T._contig_strides(sh), sh) if n != 1) and _numel(sh):
+            raise ValueError("%s: a tensor of shape %s is not contiguous" % (who, list(sh)))
+        item = _T._DT[dtype][0]
         if length is None:
             outer, size = 1, _numel(sh[1:]) * item
             part = size
         else:
-            if len(sh) < 3 or not 0 <= length <= sh[2] or length != int(length):
-                raise ValueError("%s: %r positions of a tensor of shape %s"
+            if len(sh) < 3 or not 0 <= length <= sh[2]:
+                raise ValueError("%s: %d positions of a tensor of shape %s"
                                  % (who, length, list(sh)))
             outer, size = sh[1], _numel(sh[2:]) * item
-            part = int(length) * _numel(sh[3:]) * item
-        p = t.data_ptr()
-        ptrs.append(p)
+            part = length * _numel(sh[3:]) * item
+        total.append(rows * outer * size)
         outers.append(outer)
         strides.append(size)
         sizes.append(part)
-        if t.numel():
-            spans.append((p, p + t.numel() * item))
-    parents = parents.contiguous()
-    if parents.numel():
-        p = parents.data_ptr()
-        spans.append((p, p + 4 * parents.numel()))
-    spans.sort()
-    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-        raise ValueError("%s: tensors share memory" % who)
-    _T._before_write(*tensors)
-    L.check(L.lib().tjh_cache_reorder(n, (ctypes.c_void_p * max(1, n))(*ptrs), L.i64arr(outers),
-                                      L.i64arr(strides), L.i64arr(sizes), B, W,
-                                      parents.data_ptr()), who)
+    return total, L.i64arr(outers), L.i64arr(strides), L.i64arr(sizes)
