@@ -188,7 +188,8 @@ def _linear_case(torch, m, k, n, group, bias, seed=0):
 
 LINEAR = [(1, 1, 1), (1, 31, 3), (2, 128, 16), (3, 129, 17), (5, 768, 2304), (6, 768, 50),
           (10, 300, 65), (16, 1000, 100), (17, 515, 77), (32, 640, 40), (33, 256, 129), (64, 1024, 64),
-          (100, 96, 500), (129, 384, 257), (300, 200, 1030), (1, 4100, 5000), (4, 260, 33000)]
+          (100, 96, 500), (129, 384, 257), (300, 200, 1030), (1, 4100, 5000), (4, 260, 33000),
+          (7, 1300, 17000), (30, 700, 9000), (70, 33, 33000), (1100, 160, 4000), (2050, 300, 1900)]
 
 
 @gpu

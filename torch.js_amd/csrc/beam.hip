@@ -262,7 +262,7 @@ int tjh_beam_step(const float* logits, int64_t ld, const float* scores, const ui
   int per = 53248 - 4;
   for (const int size : {1024 - 4, 4096 - 4, 16384 - 4}) {
     const int64_t S = cdiv(V, size);
-    if (S == 1 || (W * S <= 256 && rows * S <= 4 * num_cus())) {
+    if (S == 1 || (W * S <= 256 && rows * S <= 2 * num_cus())) {
       per = size;
       break;
     }

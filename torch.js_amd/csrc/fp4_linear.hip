@@ -17,31 +17,18 @@ using namespace fp4;
 
 struct LinArgs {
   const float* x;
-  const uintx4* parts;  // x in fragments (k_split_rows), or NULL
+  const uintx4* parts;  // x's parts in fragments, or NULL
   const uint8_t* codes;
   const float* scales;
   const float* bias;
   float* y;
   int64_t ldx, ldy, M, N, K;
-  int nb;    // blocks of 128 columns
-  int rows;  // of x a workgroup takes (grid y)
+  int nb;       // blocks of 128 columns
+  int rows;     // of x a workgroup takes (grid y of k_fp4_rows)
+  int m_tiles;  // 16 rows each (k_fp4_gemm)
 };
 
-// Part `part` of eight floats.
-__device__ __forceinline__ bf16x8 parts_of(const float (&x)[8], int part) {
-  uintx4 v;
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    float y[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float r = rest(x[2 * q + i]);
-      y[i] = part == 0 ? x[2 * q + i] : part == 1 ? r : r - cut(r);
-    }
-    v[q] = pack_high(y[0], y[1]);
-  }
-  return __builtin_bit_cast(bf16x8, v);
-}
+constexpr int kWaves = 8;
 
 // x[k0, k0 + 8) of a row, 0 past K.
 __device__ __forceinline__ void load8(const float* __restrict__ row, int64_t k0, int64_t K,
@@ -60,26 +47,6 @@ __device__ __forceinline__ void load8(const float* __restrict__ row, int64_t k0,
   }
 }
 
-// The parts of x's rows in the order in which the matrix cores take them: for
-// each chunk of R rows, each 32 columns and each 16 of its 3 R (row, part)
-// pairs, part by part, 64 lanes of 8 columns.
-__global__ __launch_bounds__(256) void k_split_rows(const float* __restrict__ x, int64_t ldx,
-                                                    int64_t M, int64_t K, int R, int MT,
-                                                    int kb, int64_t items,
-                                                    uintx4* __restrict__ parts) {
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (at >= items) return;
-  const int lane = at & 63;
-  const int64_t f = at >> 6, chunk = f / ((int64_t)kb * MT);
-  const int rest = (int)(f - chunk * kb * MT), k32 = rest / MT, tile = rest - k32 * MT;
-  const int r = tile * 16 + (lane & 15), part = r / R;
-  int64_t m = chunk * R + r - part * R;
-  m = m < M ? m : M - 1;
-  float v[8];
-  load8(x + m * ldx, 32 * (int64_t)k32 + 8 * (lane >> 4), K, v);
-  parts[at] = __builtin_bit_cast(uintx4, parts_of(v, part));
-}
-
 // The scales of a row's 128 columns, one for each 32.
 template <int G>
 __device__ __forceinline__ floatx4 scales_of(const float* __restrict__ s) {
@@ -91,132 +58,330 @@ __device__ __forceinline__ floatx4 scales_of(const float* __restrict__ s) {
   return floatx4{*s, *s, *s, *s};
 }
 
-// Few rows of x.  A workgroup has 16 NT columns of y, its waves share the
-// columns of x by blocks of 128 and add up through LDS.  A matrix tile's 16
-// rows are (row, part) pairs: one tile holds five rows, MT of them 16 MT / 3.
-template <int G, int MT, int NT, int WAVES, bool SPLIT>
-__global__ __launch_bounds__(64 * WAVES) void k_fp4_rows(LinArgs a) {
-  __shared__ float red[WAVES][MT][16][16];
-  const int lane = threadIdx.x & 63, c = lane & 15, j = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t n0 = (int64_t)blockIdx.x * 16 * NT, m0 = (int64_t)blockIdx.y * a.rows;
-  const int R = (int)(a.M - m0 < a.rows ? a.M - m0 : a.rows);
-  const uint8_t* __restrict__ cp[NT];
-  const float* __restrict__ sp[NT];
+// ----------------------------------------------------------------- few rows
+
+// Parts of x's rows as k_fp4_rows takes them: for each chunk of R rows, each 32
+// columns and each 16 of its 3 R (part, row) pairs, part by part, a matrix
+// operand: lane (j, i) has pair i and columns 8 j to 8 j + 7.
+__global__ __launch_bounds__(256) void k_fp4_split_rows(const float* __restrict__ x, int64_t ldx,
+                                                        int64_t M, int64_t K, int R, int MT,
+                                                        int kb, int64_t items,
+                                                        uintx4* __restrict__ parts) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= items) return;
+  // (chunk, 32 columns, 8 of them, row)
+  const int64_t row8 = at / R;
+  const int r = (int)(at - row8 * R), j = (int)(row8 & 3);
+  const int64_t f = row8 >> 2, chunk = f / kb, k32 = f - chunk * kb;
+  const int64_t m = chunk * R + r;
+  float v[8];
+  load8(x + (m < M ? m : M - 1) * ldx, 32 * k32 + 8 * j, K, v);
+  bf16x8 p[3];
+  split8(v, p);
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int64_t n = n0 + 16 * t + c < a.N ? n0 + 16 * t + c : a.N - 1;
-    cp[t] = a.codes + n * a.nb * 64 + 16 * j;
-    sp[t] = a.scales + n * a.nb * (128 / G);
+  for (int i = 0; i < 3; ++i) {
+    const int pair = i * R + r;
+    parts[(f * MT + (pair >> 4)) * 64 + 16 * j + (pair & 15)] = __builtin_bit_cast(uintx4, p[i]);
   }
-  // this lane's row of x and part of it
-  const int part = SPLIT ? c / a.rows : 0;
-  const float* __restrict__ xr = a.x;
-  if (SPLIT) xr += (m0 + min(c - part * a.rows, R - 1)) * a.ldx;
-  const uintx4* __restrict__ frag = a.parts + (int64_t)blockIdx.y * a.nb * 4 * MT * 64 + lane;
-  floatx4 acc[MT][NT];
+}
+
+// A workgroup's eight waves have 8 / KS tiles of 16 columns of y; KS of them
+// share a tile's columns of x by blocks of 128 and add up through LDS.  x's
+// parts for KB = KS U blocks at a time lie in LDS, split there (SPLIT) or
+// copied; the codes of the next U blocks of a wave are loaded before.  A matrix
+// operand's 16 rows are (part, row) pairs: MT of them hold 16 MT / 3 rows.
+template <int G, int MT, int KS, int U, bool SPLIT>
+__global__ __launch_bounds__(64 * kWaves) void k_fp4_rows(LinArgs a) {
+  constexpr int KB = KS * U, kParts = KB * 4 * MT * 64;
+  constexpr int kRed = kWaves * MT * 64;  // 16-byte items of the sums
+  __shared__ uintx4 lds[kParts > kRed ? kParts : kRed];
+  const int lane = threadIdx.x & 63, c = lane & 15, j = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ks = w % KS;
+  const int64_t m0 = (int64_t)blockIdx.y * a.rows;
+  const int R = (int)(a.M - m0 < a.rows ? a.M - m0 : a.rows);
+  const int64_t n0 = ((int64_t)blockIdx.x * (kWaves / KS) + w / KS) * 16;
+  const int64_t n = n0 + c < a.N ? n0 + c : a.N - 1;
+  const uint8_t* __restrict__ cp = a.codes + n * a.nb * 64 + 16 * j;
+  const float* __restrict__ sp = a.scales + n * a.nb * (128 / G);
+  floatx4 acc[MT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
+  for (int i = 0; i < MT; ++i) acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  uintx4 code[U], next[U];
+  floatx4 s[U], snext[U];
+  const auto load = [&](int b0, uintx4 (&cd)[U], floatx4 (&sc)[U]) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) acc[i][t] = floatx4{0.f, 0.f, 0.f, 0.f};
-  for (int b = w; b < a.nb; b += WAVES) {
-    uintx4 code[NT];
-    floatx4 s[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      code[t] = *reinterpret_cast<const uintx4*>(cp[t] + (int64_t)b * 64);
-      s[t] = scales_of<G>(sp[t] + b * (128 / G));
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      bf16x8 xa[MT];
-      if (SPLIT) {
-        float v[8];
-        load8(xr, 128 * (int64_t)b + 32 * u + 8 * j, a.K, v);
-        xa[0] = parts_of(v, part);
-      } else {
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-          xa[i] = __builtin_bit_cast(bf16x8, frag[((b * 4 + u) * MT + i) * 64]);
+    for (int u = 0; u < U; ++u) {
+      const int b = b0 + u * KS + ks;
+      if (b < a.nb) {
+        cd[u] = *reinterpret_cast<const uintx4*>(cp + (int64_t)b * 64);
+        sc[u] = scales_of<G>(sp + b * (128 / G));
       }
+    }
+  };
+  load(0, next, snext);
+  for (int b0 = 0; b0 < a.nb; b0 += KB) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const bf16x8 wb = steps(code[t][u]);
+    for (int u = 0; u < U; ++u) {
+      code[u] = next[u];
+      s[u] = snext[u];
+    }
+    if (b0 + KB < a.nb) load(b0 + KB, next, snext);
+    if (b0) __syncthreads();
+    const int k32s = 4 * (KB < a.nb - b0 ? KB : a.nb - b0);
+    if (SPLIT) {
+      // 16 octets of columns of a row a time, which lie in one line
+      for (int i = threadIdx.x; i < k32s * 4 * R; i += 64 * kWaves) {
+        const int o = i & 15, r = (i >> 4) % R, k = ((i >> 4) / R) * 16 + o;  // octet
+        float v[8];
+        load8(a.x + (m0 + r) * a.ldx, 128 * (int64_t)b0 + 8 * k, a.K, v);
+        bf16x8 p[3];
+        split8(v, p);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+          const int pair = q * a.rows + r;
+          lds[((k >> 2) * MT + (pair >> 4)) * 64 + 16 * (k & 3) + (pair & 15)] =
+              __builtin_bit_cast(uintx4, p[q]);
+        }
+      }
+    } else {
+      const uintx4* from = a.parts + ((int64_t)blockIdx.y * a.nb + b0) * 4 * MT * 64;
+      for (int i = threadIdx.x; i < k32s * MT * 64; i += 64 * kWaves) lds[i] = from[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = u * KS + ks;
+      if (b0 + at >= a.nb) break;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const bf16x8 wb = steps(code[u][t]);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
+          const bf16x8 xa = __builtin_bit_cast(bf16x8, lds[((at * 4 + t) * MT + i) * 64 + lane]);
           const floatx4 p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-              xa[i], wb, floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+              xa, wb, floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[i][t][r] = __builtin_fmaf(s[t][u], p[r], acc[i][t][r]);
+          for (int r = 0; r < 4; ++r) acc[i][r] = __builtin_fmaf(s[u][t], p[r], acc[i][r]);
         }
       }
     }
   }
+  __syncthreads();
+  float* red = reinterpret_cast<float*>(lds);  // [wave][pair][column]
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    if (t) __syncthreads();
+  for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int r = 0; r < 4; ++r) red[((w * MT + i) * 16 + 4 * j + r) * 16 + c] = acc[i][r];
+  __syncthreads();
+  for (int o = threadIdx.x; o < R * (kWaves / KS) * 16; o += 64 * kWaves) {
+    const int col = o & 15, tile = (o >> 4) % (kWaves / KS), m = (o >> 4) / (kWaves / KS);
+    const int64_t at = ((int64_t)blockIdx.x * (kWaves / KS) + tile) * 16 + col;
+    if (at >= a.N) continue;
+    float v = 0.f;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) red[w][i][4 * j + r][c] = acc[i][t][r];
-    __syncthreads();
-    for (int o = threadIdx.x; o < R * 16; o += 64 * WAVES) {
-      const int m = o >> 4, col = o & 15;
-      const int64_t n = n0 + 16 * t + col;
-      float v = 0.f;
+    for (int p = 2; p >= 0; --p)
 #pragma unroll
-      for (int p = 2; p >= 0; --p) {
-        const int row = p * a.rows + m;
-#pragma unroll
-        for (int q = 0; q < WAVES; ++q) v += red[q][row >> 4][row & 15][col];
-      }
-      if (n < a.N) a.y[(m0 + m) * a.ldy + n] = a.bias ? v + a.bias[n] : v;
-    }
+      for (int q = 0; q < KS; ++q)
+        v += red[((tile * KS + q) * MT * 16 + p * a.rows + m) * 16 + col];
+    a.y[(m0 + m) * a.ldy + at] = a.bias ? v + a.bias[at] : v;
   }
 }
 
-template <int G, int MT, int NT, bool SPLIT>
-void launch_waves(const LinArgs& a, int chunks) {
-  const dim3 grid((unsigned)cdiv(a.N, 16 * NT), (unsigned)chunks);
-  if (a.nb <= 4)
-    tjh_launch((k_fp4_rows<G, MT, NT, 4, SPLIT>), grid, dim3(256), 0, stream(), a);
-  else
-    tjh_launch((k_fp4_rows<G, MT, NT, 8, SPLIT>), grid, dim3(512), 0, stream(), a);
+template <int G, int MT, int KS, bool SPLIT>
+void launch_rows(const LinArgs& a, int chunks) {
+  // 64 KB of parts at most, four blocks a wave
+  constexpr int kFit = 16 / MT / KS, U = kFit < 1 ? 1 : kFit > 4 ? 4 : kFit;
+  const dim3 grid((unsigned)cdiv(a.N, 16 * (kWaves / KS)), (unsigned)chunks);
+  tjh_launch((k_fp4_rows<G, MT, KS, U, SPLIT>), grid, dim3(64 * kWaves), 0, stream(), a);
 }
 
 template <int G, int MT, bool SPLIT>
-void launch_cols(const LinArgs& a, int chunks) {
-  if (a.N * chunks >= 64LL * 2 * num_cus()) launch_waves<G, MT, 4, SPLIT>(a, chunks);
-  else launch_waves<G, MT, 1, SPLIT>(a, chunks);
+void launch_share(const LinArgs& a, int chunks) {
+  // waves share a tile's columns of x until the CUs have a workgroup each
+  const int64_t tiles = cdiv(a.N, 16) * chunks;
+  constexpr int kMost = 16 / MT >= 8 ? 8 : 16 / MT >= 4 ? 4 : 2;
+  const int64_t fit = a.nb < kMost ? a.nb : kMost;
+  if (fit >= 8 && tiles < 2 * num_cus()) launch_rows<G, MT, kMost, SPLIT>(a, chunks);
+  else if (fit >= 4 && tiles < 4 * num_cus())
+    launch_rows<G, MT, kMost < 4 ? kMost : 4, SPLIT>(a, chunks);
+  else if (fit >= 2 && tiles < 8 * num_cus()) launch_rows<G, MT, 2, SPLIT>(a, chunks);
+  else launch_rows<G, MT, 1, SPLIT>(a, chunks);
 }
 
 template <int G>
-int launch_rows(LinArgs a) {
+int few_rows(LinArgs a) {
   if (a.M <= 5) {
-    a.rows = 5;
-    launch_cols<G, 1, true>(a, 1);
+    a.rows = (int)a.M;
+    launch_share<G, 1, true>(a, 1);
     return check_launch("fp4_rows");
   }
   const int chunks = (int)cdiv(a.M, 32);
   a.rows = (int)cdiv(a.M, chunks);
-  const int MT = (int)cdiv(3 * a.rows, 16);
-  const int64_t items = (int64_t)chunks * a.nb * 4 * MT * 64;
+  const int MT = (int)cdiv(3 * a.rows, 16), kb = a.nb * 4;
+  const int64_t items = (int64_t)chunks * kb * 4 * a.rows;
   TJH_ARG(chunks < 65536 && cdiv(items, 256) < (1 << 23), "tjh_fp4_linear: too many rows");
-  Scratch s((size_t)(items ? items : 1) * 16);
+  Scratch s((size_t)(kb ? kb : 1) * chunks * MT * 64 * 16);
   if (!s.ok()) return set_error(TJH_ERR_OOM, "tjh_fp4_linear: no scratch");
-  // a last chunk of fewer rows has its parts as far apart as the others
   if (items)
-    tjh_launch(k_split_rows, dim3((unsigned)cdiv(items, 256)), dim3(256), 0, stream(), a.x, a.ldx,
-               a.M, a.K, a.rows, MT, a.nb * 4, items, s.as<uintx4>());
+    tjh_launch(k_fp4_split_rows, dim3((unsigned)cdiv(items, 256)), dim3(256), 0, stream(), a.x,
+               a.ldx, a.M, a.K, a.rows, MT, kb, items, s.as<uintx4>());
   a.parts = s.as<uintx4>();
   switch (MT) {
-    case 2: launch_cols<G, 2, false>(a, chunks); break;
-    case 3: launch_cols<G, 3, false>(a, chunks); break;
-    case 4: launch_cols<G, 4, false>(a, chunks); break;
-    case 5: launch_cols<G, 5, false>(a, chunks); break;
-    default: launch_cols<G, 6, false>(a, chunks); break;
+    case 2: launch_share<G, 2, false>(a, chunks); break;
+    case 3: launch_share<G, 3, false>(a, chunks); break;
+    case 4: launch_share<G, 4, false>(a, chunks); break;
+    case 5: launch_share<G, 5, false>(a, chunks); break;
+    default: launch_share<G, 6, false>(a, chunks); break;
   }
   return check_launch("fp4_rows");
+}
+
+// ---------------------------------------------------------------- many rows
+
+// Parts of x for k_fp4_gemm: for each 32 columns, each 16 rows and each part a
+// matrix operand.
+__global__ __launch_bounds__(256) void k_fp4_split(const float* __restrict__ x, int64_t ldx,
+                                                   int64_t M, int64_t K, int m_tiles,
+                                                   int64_t items, uintx4* __restrict__ parts) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= items) return;
+  const int lane = at & 63;
+  const int64_t f = at >> 6, k32 = f / m_tiles, m = (f - k32 * m_tiles) * 16 + (lane & 15);
+  float v[8];
+  load8(x + (m < M ? m : M - 1) * ldx, 32 * k32 + 8 * (lane >> 4), K, v);
+  bf16x8 p[3];
+  split8(v, p);
+#pragma unroll
+  for (int i = 0; i < 3; ++i) parts[(f * 3 + i) * 64 + lane] = __builtin_bit_cast(uintx4, p[i]);
+}
+
+// 128 x 256 of y a workgroup, 64 x 64 a wave, 32 columns of x at a time.  x's
+// parts are loaded a step ahead, codes and scales 128 columns ahead, and go
+// through one of two LDS buffers, so one barrier a step.
+template <int G>
+__global__ __launch_bounds__(64 * kWaves, 2) void k_fp4_gemm(LinArgs a) {
+  constexpr int T = 64 * kWaves;
+  __shared__ uintx4 lx[2][8 * 3 * 64];
+  __shared__ uint32_t lw[2][16 * 64];
+  __shared__ float ls[2][256];
+  const int lane = threadIdx.x & 63, c = lane & 15, j = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = w & 1, wn = w >> 1;
+  // each XCD has a run of tiles: row blocks, in each all column blocks
+  const int nt = (int)((a.N + 255) / 256), total = nt * (a.m_tiles / 8);
+  const int per = (total + 7) / 8, t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (t >= total) return;
+  const int mb = t / nt, cb = t - mb * nt;
+  const int64_t n0 = (int64_t)cb * 256;
+  // this thread's codes (of column tiles w and w + 8, as lanes feed them) and
+  // scales (of column threadIdx.x)
+  const uint8_t* __restrict__ cp[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int64_t n = n0 + 16 * (w + 8 * i) + c;
+    cp[i] = a.codes + (n < a.N ? n : a.N - 1) * a.nb * 64 + 16 * j;
+  }
+  const int64_t ns = n0 + (threadIdx.x & 255);
+  const float* __restrict__ sp = a.scales + (ns < a.N ? ns : a.N - 1) * a.nb * (128 / G);
+  const uintx4* __restrict__ from = a.parts + (int64_t)mb * 8 * 3 * 64 + threadIdx.x;
+  const int64_t hop = (int64_t)a.m_tiles * 3 * 64;  // to the next 32 columns
+  floatx4 acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int n = 0; n < 4; ++n) acc[i][n] = floatx4{0.f, 0.f, 0.f, 0.f};
+  uintx4 code[2], cnext[2], xr[3];
+  floatx4 sc, snext;
+  const auto load_w = [&](int b) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) cnext[i] = *reinterpret_cast<const uintx4*>(cp[i] + (int64_t)b * 64);
+    snext = scales_of<G>(sp + b * (128 / G));
+  };
+  // no branches in the loop: the last step and block are loaded twice (with
+  // branches the compiler moves products past them and spills)
+  int left = 4 * a.nb;
+  const auto load_x = [&] {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) xr[i] = from[i * T];
+    --left;
+    from += left > 0 ? hop : 0;
+  };
+  load_x();
+  load_w(0);
+  for (int b = 0; b < a.nb; ++b) {
+    code[0] = cnext[0];
+    code[1] = cnext[1];
+    sc = snext;
+    load_w(b + 1 < a.nb ? b + 1 : b);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int to = u & 1;
+#pragma unroll
+      for (int i = 0; i < 3; ++i) lx[to][threadIdx.x + i * T] = xr[i];
+      lw[to][threadIdx.x] = code[0][u];
+      lw[to][threadIdx.x + T] = code[1][u];
+      ls[to][threadIdx.x & 255] = sc[u];
+      load_x();
+      __syncthreads();
+      bf16x8 xa[4][3];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+          xa[i][p] = __builtin_bit_cast(bf16x8, lx[to][((wm * 4 + i) * 3 + p) * 64 + lane]);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const bf16x8 wb = steps(lw[to][(wn * 4 + n) * 64 + lane]);
+        const float f = ls[to][(wn * 4 + n) * 16 + c];
+        floatx4 y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int p = 2; p >= 0; --p)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            y[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xa[i][p], wb, y[i], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[i][n][r] = __builtin_fmaf(f, y[i][r], acc[i][n][r]);
+        __builtin_amdgcn_sched_barrier(0);  // else all columns' sums are held at once
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const int64_t at = n0 + (wn * 4 + n) * 16 + c;
+    if (at >= a.N) continue;
+    const float bias = a.bias ? a.bias[at] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int64_t m = (int64_t)mb * 128 + wm * 64 + 16 * i + 4 * j + r;
+        if (m < a.M) a.y[m * a.ldy + at] = acc[i][n][r] + bias;
+      }
+  }
+}
+
+template <int G>
+int many_rows(LinArgs a) {
+  a.m_tiles = (int)cdiv(a.M, 128) * 8;
+  const int64_t items = (int64_t)a.m_tiles * a.nb * 4 * 64, tiles = cdiv(a.N, 256) * (a.m_tiles / 8);
+  TJH_ARG(cdiv(items, 256) < (1 << 23) && tiles < (1 << 22), "tjh_fp4_linear: too many rows");
+  Scratch s((size_t)items * 3 * 16);
+  if (!s.ok()) return set_error(TJH_ERR_OOM, "tjh_fp4_linear: no scratch");
+  tjh_launch(k_fp4_split, dim3((unsigned)cdiv(items, 256)), dim3(256), 0, stream(), a.x, a.ldx, a.M,
+             a.K, a.m_tiles, items, s.as<uintx4>());
+  a.parts = s.as<uintx4>();
+  tjh_launch(k_fp4_gemm<G>, dim3((unsigned)(cdiv(tiles, 8) * 8)), dim3(64 * kWaves), 0, stream(), a);
+  return check_launch("fp4_gemm");
+}
+
+template <int G>
+int product(const LinArgs& a) {
+  // whole tiles of many rows where they give half of the CUs one each
+  if (a.M > 64 && a.nb && cdiv(a.M, 128) * cdiv(a.N, 256) * 2 >= num_cus()) return many_rows<G>(a);
+  return few_rows<G>(a);
 }
 
 }  // namespace
@@ -236,9 +401,9 @@ extern "C" int tjh_fp4_linear(const float* x, int64_t ldx, int64_t M, int64_t N,
   if (M == 0 || N == 0) return TJH_OK;
   TJH_ARG(y && (K == 0 || (x && codes && scales && aligned16(codes))),
           "tjh_fp4_linear: NULL or unaligned pointer");
-  LinArgs a{x, nullptr, codes, scales, bias, y, ldx, ldy, M, N, K, (int)cdiv(K, 128), 0};
+  LinArgs a{x, nullptr, codes, scales, bias, y, ldx, ldy, M, N, K, (int)cdiv(K, 128), 0, 0};
   KernelScope ks("fp4_linear");
-  if (group == 32) return launch_rows<32>(a);
-  if (group == 64) return launch_rows<64>(a);
-  return launch_rows<128>(a);
+  if (group == 32) return product<32>(a);
+  if (group == 64) return product<64>(a);
+  return product<128>(a);
 }
