@@ -255,132 +255,178 @@ __global__ __launch_bounds__(256) void k_fp4_split(const float* __restrict__ x, 
   for (int i = 0; i < 3; ++i) parts[(f * 3 + i) * 64 + lane] = __builtin_bit_cast(uintx4, p[i]);
 }
 
-// 128 x 256 of y a workgroup, 64 x 64 a wave, 32 columns of x at a time.  x's
-// parts are loaded a step ahead, codes and scales 128 columns ahead, and go
-// through one of two LDS buffers, so one barrier a step.
-template <int G>
-__global__ __launch_bounds__(64 * kWaves, 2) void k_fp4_gemm(LinArgs a) {
-  constexpr int T = 64 * kWaves;
-  __shared__ uintx4 lx[2][8 * 3 * 64];
-  __shared__ uint32_t lw[2][16 * 64];
-  __shared__ float ls[2][256];
+// 128 x 16 C of y a workgroup, 32 rows of it a wave.  A wave's parts of x come straight
+// from memory as its lanes feed them, one step of 32 columns ahead; codes and
+// scales, which all four waves feed, go through one of two LDS buffers, 128
+// columns at a time and loaded as many ahead.
+constexpr int kGemmWaves = 4, kRowTiles = 2;
+
+template <int G, int C>
+__global__ __launch_bounds__(64 * kGemmWaves, 2) void k_fp4_gemm(LinArgs a) {
+  constexpr int T = 64 * kGemmWaves, kBM = 16 * kRowTiles * kGemmWaves, kBN = 16 * C;
+  constexpr int kItems = (C + kGemmWaves - 1) / kGemmWaves;  // column tiles a wave loads
+  __shared__ uint32_t lw[2][4][C * 64];
+  __shared__ float ls[2][4][kBN];
   const int lane = threadIdx.x & 63, c = lane & 15, j = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = w & 1, wn = w >> 1;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // each XCD has a run of tiles: row blocks, in each all column blocks
-  const int nt = (int)((a.N + 255) / 256), total = nt * (a.m_tiles / 8);
+  const int nt = (int)((a.N + kBN - 1) / kBN), total = nt * (a.m_tiles * 16 / kBM);
   const int per = (total + 7) / 8, t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if (t >= total) return;
   const int mb = t / nt, cb = t - mb * nt;
-  const int64_t n0 = (int64_t)cb * 256;
-  // this thread's codes (of column tiles w and w + 8, as lanes feed them) and
-  // scales (of column threadIdx.x)
-  const uint8_t* __restrict__ cp[2];
+  const int64_t n0 = (int64_t)cb * kBN;
+  const uint8_t* __restrict__ cp[kItems];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t n = n0 + 16 * (w + 8 * i) + c;
+  for (int i = 0; i < kItems; ++i) {
+    // (the last one again where there are fewer)
+    const int64_t n = n0 + 16 * min(w + kGemmWaves * i, C - 1) + c;
     cp[i] = a.codes + (n < a.N ? n : a.N - 1) * a.nb * 64 + 16 * j;
   }
-  const int64_t ns = n0 + (threadIdx.x & 255);
+  const int64_t ns = n0 + threadIdx.x % kBN;
   const float* __restrict__ sp = a.scales + (ns < a.N ? ns : a.N - 1) * a.nb * (128 / G);
-  const uintx4* __restrict__ from = a.parts + (int64_t)mb * 8 * 3 * 64 + threadIdx.x;
   const int64_t hop = (int64_t)a.m_tiles * 3 * 64;  // to the next 32 columns
-  floatx4 acc[4][4];
+  const uintx4* __restrict__ from =
+      a.parts + (int64_t)(mb * (kBM / 16) + w * kRowTiles) * 3 * 64 + lane;
+  floatx4 acc[kRowTiles][C];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < kRowTiles; ++i)
 #pragma unroll
-    for (int n = 0; n < 4; ++n) acc[i][n] = floatx4{0.f, 0.f, 0.f, 0.f};
-  uintx4 code[2], cnext[2], xr[3];
-  floatx4 sc, snext;
+    for (int n = 0; n < C; ++n) acc[i][n] = floatx4{0.f, 0.f, 0.f, 0.f};
+  uintx4 code[kItems], xr[kRowTiles][3];
+  floatx4 sc;
   const auto load_w = [&](int b) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) cnext[i] = *reinterpret_cast<const uintx4*>(cp[i] + (int64_t)b * 64);
-    snext = scales_of<G>(sp + b * (128 / G));
+    for (int i = 0; i < kItems; ++i) code[i] = *reinterpret_cast<const uintx4*>(cp[i] + (int64_t)b * 64);
+    sc = scales_of<G>(sp + b * (128 / G));
   };
   // no branches in the loop: the last step and block are loaded twice (with
   // branches the compiler moves products past them and spills)
   int left = 4 * a.nb;
   const auto load_x = [&] {
 #pragma unroll
-    for (int i = 0; i < 3; ++i) xr[i] = from[i * T];
+    for (int i = 0; i < kRowTiles; ++i)
+#pragma unroll
+      for (int p = 0; p < 3; ++p) xr[i][p] = from[(i * 3 + p) * 64];
     --left;
     from += left > 0 ? hop : 0;
   };
-  load_x();
   load_w(0);
+  load_x();
   for (int b = 0; b < a.nb; ++b) {
-    code[0] = cnext[0];
-    code[1] = cnext[1];
-    sc = snext;
-    load_w(b + 1 < a.nb ? b + 1 : b);
+    const int to = b & 1;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int to = u & 1;
 #pragma unroll
-      for (int i = 0; i < 3; ++i) lx[to][threadIdx.x + i * T] = xr[i];
-      lw[to][threadIdx.x] = code[0][u];
-      lw[to][threadIdx.x + T] = code[1][u];
-      ls[to][threadIdx.x & 255] = sc[u];
-      load_x();
-      __syncthreads();
-      bf16x8 xa[4][3];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int p = 0; p < 3; ++p)
-          xa[i][p] = __builtin_bit_cast(bf16x8, lx[to][((wm * 4 + i) * 3 + p) * 64 + lane]);
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const bf16x8 wb = steps(lw[to][(wn * 4 + n) * 64 + lane]);
-        const float f = ls[to][(wn * 4 + n) * 16 + c];
-        floatx4 y[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int p = 2; p >= 0; --p)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            y[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xa[i][p], wb, y[i], 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[i][n][r] = __builtin_fmaf(f, y[i][r], acc[i][n][r]);
-        __builtin_amdgcn_sched_barrier(0);  // else all columns' sums are held at once
-      }
+      for (int i = 0; i < kItems; ++i)
+        lw[to][u][min(w + kGemmWaves * i, C - 1) * 64 + lane] = code[i][u];
+      ls[to][u][threadIdx.x % kBN] = sc[u];
     }
+    load_w(b + 1 < a.nb ? b + 1 : b);
+    __syncthreads();
+    // The products of a column tile are issued between the sums of the one
+    // before and the conversions of the one after: a wave alone keeps its
+    // matrix cores busy.
+    bf16x8 xa[kRowTiles][3], wb = steps(lw[to][0][lane]);
+    float f = ls[to][0][c], fnext = ls[to][0][16 + c], fy = 0.f;
+    uint32_t word = lw[to][0][64 + lane];
+    floatx4 y[kRowTiles];
+#pragma unroll
+    for (int q = 0; q < 4 * C; ++q) {
+      const int u = q / C, n = q % C;
+      if (n == 0) {
+#pragma unroll
+        for (int i = 0; i < kRowTiles; ++i)
+#pragma unroll
+          for (int p = 0; p < 3; ++p) xa[i][p] = __builtin_bit_cast(bf16x8, xr[i][p]);
+        load_x();
+      }
+      floatx4 z[kRowTiles];
+#pragma unroll
+      for (int i = 0; i < kRowTiles; ++i) z[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int p = 2; p >= 0; --p)
+#pragma unroll
+        for (int i = 0; i < kRowTiles; ++i)
+          z[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xa[i][p], wb, z[i], 0, 0, 0);
+      const float fz = f;
+      if (q + 1 < 4 * C) {
+        wb = steps(word);
+        f = fnext;
+        if (q + 2 < 4 * C) {
+          word = lw[to][(q + 2) / C][(q + 2) % C * 64 + lane];
+          fnext = ls[to][(q + 2) / C][(q + 2) % C * 16 + c];
+        }
+      }
+      if (q > 0) {
+        const int before = (n + C - 1) % C;
+#pragma unroll
+        for (int i = 0; i < kRowTiles; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            acc[i][before][r] = __builtin_fmaf(fy, y[i][r], acc[i][before][r]);
+      }
+      fy = fz;
+#pragma unroll
+      for (int i = 0; i < kRowTiles; ++i) y[i] = z[i];
+#pragma unroll
+      for (int i = 0; i < 3 * kRowTiles; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a product,
+        __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);  // two of the other operations
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int i = 0; i < kRowTiles; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        acc[i][C - 1][r] = __builtin_fmaf(fy, y[i][r], acc[i][C - 1][r]);
   }
 #pragma unroll
-  for (int n = 0; n < 4; ++n) {
-    const int64_t at = n0 + (wn * 4 + n) * 16 + c;
+  for (int n = 0; n < C; ++n) {
+    const int64_t at = n0 + n * 16 + c;
     if (at >= a.N) continue;
     const float bias = a.bias ? a.bias[at] : 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < kRowTiles; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int64_t m = (int64_t)mb * 128 + wm * 64 + 16 * i + 4 * j + r;
+        const int64_t m = (int64_t)mb * kBM + (w * kRowTiles + i) * 16 + 4 * j + r;
         if (m < a.M) a.y[m * a.ldy + at] = acc[i][n][r] + bias;
       }
   }
 }
 
+template <int G, int C>
+void launch_gemm(const LinArgs& a) {
+  const int64_t tiles = cdiv(a.N, 16 * C) * (a.m_tiles / 8);
+  tjh_launch((k_fp4_gemm<G, C>), dim3((unsigned)(cdiv(tiles, 8) * 8)), dim3(64 * kGemmWaves), 0,
+             stream(), a);
+}
+
 template <int G>
 int many_rows(LinArgs a) {
   a.m_tiles = (int)cdiv(a.M, 128) * 8;
-  const int64_t items = (int64_t)a.m_tiles * a.nb * 4 * 64, tiles = cdiv(a.N, 256) * (a.m_tiles / 8);
-  TJH_ARG(cdiv(items, 256) < (1 << 23) && tiles < (1 << 22), "tjh_fp4_linear: too many rows");
+  const int64_t items = (int64_t)a.m_tiles * a.nb * 4 * 64, rows = a.m_tiles / 8;
+  TJH_ARG(cdiv(items, 256) < (1 << 23) && cdiv(a.N, 64) * rows < (1 << 23),
+          "tjh_fp4_linear: too many rows");
   Scratch s((size_t)items * 3 * 16);
   if (!s.ok()) return set_error(TJH_ERR_OOM, "tjh_fp4_linear: no scratch");
   tjh_launch(k_fp4_split, dim3((unsigned)cdiv(items, 256)), dim3(256), 0, stream(), a.x, a.ldx, a.M,
              a.K, a.m_tiles, items, s.as<uintx4>());
   a.parts = s.as<uintx4>();
-  tjh_launch(k_fp4_gemm<G>, dim3((unsigned)(cdiv(tiles, 8) * 8)), dim3(64 * kWaves), 0, stream(), a);
+  // column tiles of the CU that has most
+  const auto load = [&](int C) { return cdiv(cdiv(a.N, 16 * C) * rows, num_cus()) * C; };
+  const int64_t l4 = load(4) * 5 / 4, l8 = load(8), l13 = load(13);
+  if (l13 <= l8 && l13 <= l4) launch_gemm<G, 13>(a);
+  else if (l8 <= l4) launch_gemm<G, 8>(a);
+  else launch_gemm<G, 4>(a);
   return check_launch("fp4_gemm");
 }
 
 template <int G>
 int product(const LinArgs& a) {
   // whole tiles of many rows where they give half of the CUs one each
-  if (a.M > 64 && a.nb && cdiv(a.M, 128) * cdiv(a.N, 256) * 2 >= num_cus()) return many_rows<G>(a);
+  if (a.M > 64 && a.nb && cdiv(a.M, 128) * cdiv(a.N, 64) * 2 >= num_cus()) return many_rows<G>(a);
   return few_rows<G>(a);
 }
 
