@@ -106,12 +106,6 @@ __device__ __forceinline__ void transpose(const uint32_t (&a)[8], int n,
 }
 
 template <int NB>
-struct Keys {  // a lane's part of a tile
-  uint32_t k[2][NB], v[8];
-  floatx4 ks[2], vs[2];
-};
-
-template <int NB>
 __device__ __forceinline__ void load_words(uint32_t (&w)[NB], const uint8_t* p) {
   typedef uint32_t uintx3 __attribute__((ext_vector_type(3), aligned(4)));
   if constexpr (NB == 4) {
@@ -131,7 +125,7 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[NB], const uint8_t* p) 
 // SPLIT: the waves of a workgroup share 16 rows' keys, tile by tile; otherwise
 // each has rows of its own.
 template <int NB, bool SPLIT>
-__global__ __launch_bounds__(64 * kWaves) void k_fp4_attend(AttArgs a) {
+__global__ __launch_bounds__(64 * kWaves, NB < 3 ? 3 : 2) void k_fp4_attend(AttArgs a) {
   typedef Dims<NB> Z;
   constexpr int NT = Z::NT, P = 16 * NB;
   const int lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4;
@@ -153,6 +147,66 @@ __global__ __launch_bounds__(64 * kWaves) void k_fp4_attend(AttArgs a) {
   const int least = max(0, len - a.Tq + (h0 == h1 ? r0 - h0 * a.Tq : 0) + 1);
   const int per = ((most + a.slices - 1) / a.slices + kTile - 1) / kTile * kTile;
   const int from = min(most, slice * per), to = min(most, from + per);
+  const int64_t base = (int64_t)bh * a.L;
+  const uint8_t* __restrict__ kc = a.kc + base * P;
+  const uint8_t* __restrict__ vc = a.vc + base * P;
+  const float* __restrict__ ks = a.ks + base;
+  const float* __restrict__ vs = a.vs + base;
+  const uint32_t kat = n * P + 4 * NB * j, vat = 4 * j * P + 4 * min(n % Z::CH, 4 * NB - 1);
+  // one of keys or values of a tile; a key past the cache's end is its last one,
+  // a key past `to` or not seen is whatever the cache holds: weights of 0 below
+  const int end = (int)a.L;
+  uint32_t kw[2][NB], vw[8];
+  floatx4 kscale[2], vscale[2];
+  const auto load_scales = [&](const float* p, int t0, floatx4 (&x)[2]) {
+    if (t0 + kTile <= end) {
+      const float* at = p + (uint32_t)(t0 + 4 * j);
+#pragma unroll
+      for (int y = 0; y < 2; ++y) x[y] = *reinterpret_cast<const floatx4u*>(at + 16 * y);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        x[e >> 2][e & 3] = p[min(t0 + 16 * (e >> 2) + 4 * j + (e & 3), end - 1)];
+    }
+  };
+  const auto load_k = [&](int t0) {
+    if (t0 + kTile <= end) {
+      const uint8_t* at = kc + ((uint32_t)t0 * P + kat);
+      load_words(kw[0], at);
+      load_words(kw[1], at + 16 * P);
+    } else {
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+        load_words(kw[y], kc + ((uint32_t)min(t0 + 16 * y + n, end - 1) * P + 4 * NB * j));
+    }
+    load_scales(ks, t0, kscale);
+  };
+  const auto load_v = [&](int t0) {
+    if (t0 + kTile <= end) {
+      const uint8_t* at = vc + ((uint32_t)t0 * P + vat);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        vw[e] = *reinterpret_cast<const uint32_t*>(at + (16 * (e >> 2) + (e & 3)) * P);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        vw[e] = *reinterpret_cast<const uint32_t*>(
+            vc + ((uint32_t)min(t0 + 16 * (e >> 2) + 4 * j + (e & 3), end - 1) * P +
+                  4 * min(n % Z::CH, 4 * NB - 1)));
+    }
+    load_scales(vs, t0, vscale);
+  };
+  const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
+  floatx4 o[NT];
+#pragma unroll
+  for (int d = 0; d < NT; ++d) o[d] = zero;
+  float m = -INFINITY, l = 0.f;
+  const int step = SPLIT ? kTile * kWaves : kTile;
+  int t0 = from + (SPLIT ? w * kTile : 0);
+  if (t0 < to) {
+    load_k(t0);
+    load_v(t0);
+  }
   bf16x8 q[NB][3];
   {
     const float* p = a.q + b * a.qb + (int64_t)(kh * a.group + h) * a.qh + i * a.qt;
@@ -163,73 +217,42 @@ __global__ __launch_bounds__(64 * kWaves) void k_fp4_attend(AttArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int d = 8 * (NB * j + t) + e;
-        x[e] = d < a.D ? p[d] * f : 0.f;
+        const float y = p[min(d, a.D - 1)];
+        x[e] = d < a.D ? y * f : 0.f;
       }
       split8(x, q[t]);
     }
   }
-  const int64_t base = (int64_t)bh * a.L;
-  const uint8_t* __restrict__ kc = a.kc + base * P + 4 * NB * j;
-  const uint8_t* __restrict__ vc = a.vc + base * P + 4 * min(n % Z::CH, 4 * NB - 1);
-  const float* __restrict__ ks = a.ks + base;
-  const float* __restrict__ vs = a.vs + base;
-  const auto load = [&](int t0, Keys<NB>& x) {
-    if (t0 + kTile <= to) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        load_words(x.k[s], kc + (int64_t)(t0 + 16 * s + n) * P);
-        x.ks[s] = *reinterpret_cast<const floatx4u*>(ks + t0 + 16 * s + 4 * j);
-        x.vs[s] = *reinterpret_cast<const floatx4u*>(vs + t0 + 16 * s + 4 * j);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          x.v[4 * s + r] = *reinterpret_cast<const uint32_t*>(
-              vc + (int64_t)(t0 + 16 * s + 4 * j + r) * P);
-      }
-    } else {  // past the last key: that one again, with weights of 0
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        load_words(x.k[s], kc + (int64_t)min(t0 + 16 * s + n, to - 1) * P);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int t = min(t0 + 16 * s + 4 * j + r, to - 1);
-          x.ks[s][r] = ks[t];
-          x.vs[s][r] = vs[t];
-          x.v[4 * s + r] = *reinterpret_cast<const uint32_t*>(vc + (int64_t)t * P);
-        }
-      }
-    }
-  };
-  const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
-  floatx4 o[NT];
-#pragma unroll
-  for (int d = 0; d < NT; ++d) o[d] = zero;
-  float m = -INFINITY, l = 0.f;
-  const int step = SPLIT ? kTile * kWaves : kTile;
-  int t0 = from + (SPLIT ? w * kTile : 0);
-  Keys<NB> next;
-  if (t0 < to) load(t0, next);
   for (; t0 < to; t0 += step) {
-    const Keys<NB> x = next;
-    if (t0 + step < to) load(t0 + step, next);
+    const int tn = t0 + step < to ? t0 + step : t0;  // the last tile is loaded twice
     floatx4 s[2] = {zero, zero};
+    {
+      bf16x8 kf[2][NB];
 #pragma unroll
-    for (int part = 2; part >= 0; --part)
+      for (int y = 0; y < 2; ++y)
 #pragma unroll
-      for (int t = 0; t < NB; ++t)
+        for (int t = 0; t < NB; ++t) kf[y][t] = steps(kw[y][t]);
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
-          s[y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(steps(x.k[y][t]), q[t][part], s[y], 0, 0, 0);
+      for (int part = 2; part >= 0; --part)
+#pragma unroll
+        for (int t = 0; t < NB; ++t)
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+            s[y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[y][t], q[t][part], s[y], 0, 0, 0);
+    }
     float p[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) p[e] = s[e >> 2][e & 3] * x.ks[e >> 2][e & 3];
+    for (int e = 0; e < 8; ++e) p[e] = s[e >> 2][e & 3] * kscale[e >> 2][e & 3];
+    load_k(tn);
     const bool masked = t0 + kTile > min(to, least);
-    bool sees[8];
     if (masked) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int t = t0 + 16 * (e >> 2) + 4 * j + (e & 3);
-        sees[e] = t < to && t < seen;
-        if (!sees[e]) p[e] = -INFINITY;
+        if (t >= min(to, seen)) {
+          p[e] = -INFINITY;
+          vscale[e >> 2][e & 3] = 0.f;  // may be NaN
+        }
       }
     }
     float top = p[0];
@@ -254,23 +277,21 @@ __global__ __launch_bounds__(64 * kWaves) void k_fp4_attend(AttArgs a) {
     for (int e = 0; e < 8; ++e) {
       const float y = __builtin_amdgcn_exp2f(p[e] - ms);
       l += y;
-      p[e] = y * x.vs[e >> 2][e & 3];
-    }
-    if (masked) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (!sees[e]) p[e] = 0.f;  // the scale of what is not seen may be NaN
+      p[e] = y * vscale[e >> 2][e & 3];
     }
     bf16x8 pp[3];
     split8_finite(p, pp);
     uint32_t v[NT];
-    transpose<NB>(x.v, n, v);
+    transpose<NB>(vw, n, v);
+    load_v(tn);
 #pragma unroll
-    for (int d = 0; d < NT; ++d) {
-      const bf16x8 vb = steps(v[d]);
+    for (int d = 0; d < NT; d += 2) {  // two chains at a time
+      const bf16x8 vb[2] = {steps(v[d]), steps(v[d + 1])};
 #pragma unroll
       for (int part = 2; part >= 0; --part)
-        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pp[part], vb, o[d], 0, 0, 0);
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+          o[d + y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pp[part], vb[y], o[d + y], 0, 0, 0);
     }
   }
   l += __shfl_xor(l, 16, 64);
@@ -405,7 +426,7 @@ extern "C" int tjh_fp4_attention(const float* q, const uint8_t* k_codes, const f
   const int64_t keys = lengths ? L : length, tiles = B * Hkv * a.row_tiles;
   const bool split = tiles < 4 * num_cus();
   const int64_t wgs = split ? tiles : B * Hkv * cdiv(a.row_tiles, kWaves);
-  const int64_t want = cdiv(2 * num_cus(), wgs), can = cdiv(keys, split ? 128 : 512);
+  const int64_t want = 2 * wgs >= 3 * num_cus() ? 1 : cdiv(2 * num_cus(), wgs), can = cdiv(keys, split ? 128 : 512);
   a.slices = (int)(want < can ? want : can);
   if (a.slices < 1) a.slices = 1;
   KernelScope ks("fp4_attention");
