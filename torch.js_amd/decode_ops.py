@@ -17,7 +17,7 @@ import numpy as np
 
 from . import _lib as L
 from . import tensor as _T
-from .tensor import (Tensor, _alias, _empty_padded, _gemm, _k_contiguous, _numel, _record, empty,
+from .tensor import (Storage, Tensor, _empty_padded, _gemm, _k_contiguous, _numel, _record, empty,
                      reshape_raw)
 
 GROUPS = (32, 64, 128)
@@ -37,17 +37,39 @@ def _weight_shapes(n, k, group):
 
 
 def _weights(who, codes, scales, k, group):
-    """Checks 4-bit weights of k columns; their number of rows."""
-    if not (isinstance(codes, Tensor) and isinstance(scales, Tensor) and codes.ndim == 2 and
-            codes.dtype == "uint8" and scales.dtype == "float32"):
+    """Checks 4-bit weights of k columns; (number of rows, pointer of the codes,
+    of the scales)."""
+    if not (isinstance(codes, Tensor) and isinstance(scales, Tensor)):
+        raise TypeError("%s: codes and scales must be tensors" % who)
+    n = _weight_rows(who, codes._shape, codes._strides, codes._dtype, scales._shape,
+                     scales._strides, scales._dtype, k, group)
+    p = codes.data_ptr()
+    if p & 15:
+        raise ValueError("%s: codes must be 16-byte aligned" % who)
+    return n, p, scales.data_ptr()
+
+
+@functools.lru_cache(maxsize=1024)
+def _weight_rows(who, cs, cst, cd, ss, sst, sd, k, group):
+    if len(cs) != 2 or cd != "uint8" or sd != "float32":
         raise TypeError("%s: codes must be a 2-D uint8 tensor and scales a float32 one" % who)
-    n = codes.shape[0]
-    if (codes.shape, scales.shape) != _weight_shapes(n, k, group):
+    if (cs, ss) != _weight_shapes(cs[0], k, group):
         raise ValueError("%s: codes %s and scales %s do not hold %d columns in groups of %d"
-                         % (who, list(codes.shape), list(scales.shape), k, group))
-    if not (codes.is_contiguous() and scales.is_contiguous()) or codes.data_ptr() & 15:
-        raise ValueError("%s: codes and scales must be contiguous, codes 16-byte aligned" % who)
-    return n
+                         % (who, list(cs), list(ss), k, group))
+    if not (_contiguous(cs, cst) and _contiguous(ss, sst)):
+        raise ValueError("%s: codes and scales must be contiguous" % who)
+    return cs[0]
+
+
+def _contiguous(shape, strides):
+    return not _numel(shape) or all(
+        a == b for a, b, n in zip(strides, _T._contig_strides(shape), shape) if n != 1)
+
+
+@functools.lru_cache(maxsize=1024)
+def _strides(st):
+    """Strides as the C entry points take them."""
+    return L.i64arr(st)
 
 
 def quantize_fp4(weight, group_size=64):
@@ -73,10 +95,9 @@ def dequantize_fp4(codes, scales, in_features, group_size=64):
     stand for."""
     g = _group("dequantize_fp4", group_size)
     k = int(in_features)
-    n = _weights("dequantize_fp4", codes, scales, k, g)
+    n, pc, ps = _weights("dequantize_fp4", codes, scales, k, g)
     out = empty((n, k))
-    L.check(L.lib().tjh_fp4_dequantize(codes.data_ptr(), scales.data_ptr(), n, k, g,
-                                       out.data_ptr(), k), "dequantize_fp4")
+    L.check(L.lib().tjh_fp4_dequantize(pc, ps, n, k, g, out.data_ptr(), k), "dequantize_fp4")
     return out
 
 
@@ -85,24 +106,27 @@ def linear_fp4(x, codes, scales, bias=None, group_size=64):
     quantize_fp4, summed in float32.  The gradient goes to x (through the float
     weight, formed for it) and to bias; the weight has none."""
     g = _group("linear_fp4", group_size)
-    if x.ndim == 0:
+    if not x._shape:
         raise ValueError("linear_fp4: x has no dimensions")
-    if x.dtype != "float32":
+    if x._dtype != "float32":
         x = x.float()
-    k, lead = x.shape[-1], x.shape[:-1]
-    n = _weights("linear_fp4", codes, scales, k, g)
-    if bias is not None and bias.shape != (n,):
-        raise ValueError("linear_fp4: bias of shape %s for %d outputs" % (list(bias.shape), n))
-    xd, px, ld, m, _ = _T._rows_2d(x.detach())
-    b = None
-    if bias is not None:
-        b = bias.detach() if bias.dtype == "float32" else bias.detach().float()
-        b = b.contiguous()
-    y = _empty_padded(m, n) if n % 4 else empty((m, n))
-    L.check(L.lib().tjh_fp4_linear(px, ld, m, n, k, codes.data_ptr(), scales.data_ptr(), g,
-                                   b.data_ptr() if b is not None else None, y.data_ptr(),
+    k, lead = x._shape[-1], x._shape[:-1]
+    n, pc, ps = _weights("linear_fp4", codes, scales, k, g)
+    b = bias
+    if b is not None:
+        if b._shape != (n,):
+            raise ValueError("linear_fp4: bias of shape %s for %d outputs" % (list(b._shape), n))
+        if b._dtype != "float32" or b._strides != (1,):
+            b = b.detach().float().contiguous()
+    # the tensor that holds x's rows lives until the launch is queued
+    xd, px, ld, m, _ = _T._rows_2d(x)
+    pb = b.data_ptr() if b is not None else None
+    y = _empty_padded(m, n) if n % 4 else Tensor(Storage(max(1, m * n) * 4), (m, n))
+    L.check(L.lib().tjh_fp4_linear(px, ld, m, n, k, pc, ps, g, pb, y.data_ptr(),
                                    max(y._strides[0], n)), "linear_fp4")
-    out = reshape_raw(y, lead + (n,))
+    out = reshape_raw(y, lead + (n,)) if len(lead) != 1 else y
+    if not _T._recorded(x, bias):
+        return out
     rx, rb = x.requires_grad, bias is not None and bias.requires_grad
 
     def bwd(gr):
@@ -135,22 +159,34 @@ def cache_row_bytes(head_dim):
 
 
 def _cache(who, codes, scales, d):
-    """Checks a cache of one of keys or values: its (B, H, L)."""
-    if not (isinstance(codes, Tensor) and isinstance(scales, Tensor) and
-            codes._dtype == "uint8" and scales._dtype == "float32"):
-        raise TypeError("%s: a cache's codes must be uint8 and its scales float32 tensors" % who)
-    cs = codes._shape
-    if len(cs) != 4 or cs[3] != cache_row_bytes(d) or scales._shape != cs[:3]:
+    """Checks a cache of one of keys or values: its (B, H, L), its pointers."""
+    if not (isinstance(codes, Tensor) and isinstance(scales, Tensor)):
+        raise TypeError("%s: a cache's codes and scales must be tensors" % who)
+    shape = _cache_shape(who, codes._shape, codes._strides, codes._dtype, scales._shape,
+                         scales._strides, scales._dtype, d)
+    p = codes.data_ptr()
+    if p & 15:
+        raise ValueError("%s: a cache's codes must be 16-byte aligned" % who)
+    return shape, p, scales.data_ptr()
+
+
+@functools.lru_cache(maxsize=1024)
+def _cache_shape(who, cs, cst, cd, ss, sst, sd, d):
+    if cd != "uint8" or sd != "float32":
+        raise TypeError("%s: a cache's codes must be uint8 and its scales float32" % who)
+    if len(cs) != 4 or cs[3] != cache_row_bytes(d) or ss != cs[:3]:
         raise ValueError("%s: codes %s and scales %s do not hold heads of %d columns"
-                         % (who, list(cs), list(scales._shape), d))
-    if not (codes.is_contiguous() and scales.is_contiguous()) or codes.data_ptr() & 15:
-        raise ValueError("%s: a cache must be contiguous, its codes 16-byte aligned" % who)
+                         % (who, list(cs), list(ss), d))
+    if not (_contiguous(cs, cst) and _contiguous(ss, sst)):
+        raise ValueError("%s: a cache must be contiguous" % who)
     return cs[:3]
 
 
 def _per_sequence(who, name, value, b):
     """(number, pointer or None, tensor) of a whole number, or of one of each
     of b sequences."""
+    if type(value) is int and 0 <= value < 1 << 62:
+        return value, None, None
     if isinstance(value, Tensor) or np.ndim(value):
         t = value
         if not isinstance(t, Tensor):
@@ -168,7 +204,7 @@ def _per_sequence(who, name, value, b):
     n = int(value)
     if n != value or n < 0:
         raise ValueError("%s: %s must be a whole number, got %r" % (who, name, value))
-    return n, None, None
+    return min(n, 1 << 62), None, None
 
 
 def cache_append_fp4(k_codes, k_scales, v_codes, v_scales, key, value, pos):
@@ -178,29 +214,32 @@ def cache_append_fp4(k_codes, k_scales, v_codes, v_scales, key, value, pos):
     tensor [B], where each sequence's new positions begin; positions outside
     [0, L) are then not written.  D up to 128."""
     who = "cache_append_fp4"
-    if key.ndim != 4 or key.shape != value.shape:
+    ks = key._shape
+    if len(ks) != 4 or ks != value._shape:
         raise ValueError("%s: key %s and value %s must be [B, H, T, D] alike"
-                         % (who, list(key.shape), list(value.shape)))
-    B, H, T, D = key.shape
+                         % (who, list(ks), list(value._shape)))
+    B, H, T, D = ks
     if not 0 < D <= 128:
         raise NotImplementedError("%s: head dims up to 128, got %d" % (who, D))
-    shape = _cache(who, k_codes, k_scales, D)
-    if _cache(who, v_codes, v_scales, D) != shape or shape[:2] != (B, H):
+    shape, pkc, pks = _cache(who, k_codes, k_scales, D)
+    vshape, pvc, pvs = _cache(who, v_codes, v_scales, D)
+    if vshape != shape or shape[:2] != (B, H):
         raise ValueError("%s: key %s does not fit caches %s and %s"
-                         % (who, list(key.shape), list(k_codes.shape), list(v_codes.shape)))
-    for a, b in ((k_codes, v_codes), (k_scales, v_scales)):
-        if a.numel() and a.data_ptr() == b.data_ptr():
-            raise ValueError("%s: keys and values are one cache" % who)
+                         % (who, list(ks), list(k_codes._shape), list(v_codes._shape)))
+    if (pkc == pvc or pks == pvs) and _numel(shape):
+        raise ValueError("%s: keys and values are one cache" % who)
     n, p, _keep = _per_sequence(who, "pos", pos, B)
     if p is None and n + T > shape[2]:
         raise RuntimeError("KV cache: position %d beyond its length %d" % (n + T, shape[2]))
-    k, v = [(t if t.dtype == "float32" else t.float()).detach() for t in (key, value)]
-    pk, pv = k.data_ptr(), v.data_ptr()
+    if key._dtype != "float32":
+        key = key.float()
+    if value._dtype != "float32":
+        value = value.float()
+    pk, pv = key.data_ptr(), value.data_ptr()
     _T._before_write(k_codes, k_scales, v_codes, v_scales)
     L.check(L.lib().tjh_fp4_cache_append(
-        pk, pv, L.i64arr(k._strides), L.i64arr(v._strides), k_codes.data_ptr(),
-        k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), B, H, T, D, shape[2], n, p),
-        who)
+        pk, pv, _strides(key._strides), _strides(value._strides), pkc, pks, pvc, pvs, B, H, T, D,
+        shape[2], n, p), who)
 
 
 def cache_read_fp4(codes, scales, head_dim, start, stop):
@@ -210,12 +249,12 @@ def cache_read_fp4(codes, scales, head_dim, start, stop):
     d = int(head_dim)
     if not 0 < d <= 128:
         raise NotImplementedError("%s: head dims up to 128, got %d" % (who, d))
-    B, H, n = _cache(who, codes, scales, d)
+    (B, H, n), pc, ps = _cache(who, codes, scales, d)
     if not 0 <= start <= stop <= n:
         raise ValueError("%s: positions [%d, %d) of %d" % (who, start, stop, n))
-    out = empty((B, H, stop - start, d))
-    L.check(L.lib().tjh_fp4_cache_read(codes.data_ptr(), scales.data_ptr(), B, H, n, d, start,
-                                       stop - start, out.data_ptr()), who)
+    out = Tensor(Storage(max(1, B * H * (stop - start) * d) * 4), (B, H, stop - start, d))
+    L.check(L.lib().tjh_fp4_cache_read(pc, ps, B, H, n, d, start, stop - start, out.data_ptr()),
+            who)
     return out
 
 
@@ -229,37 +268,39 @@ def attention_fp4(query, k_codes, k_scales, v_codes, v_scales, length, scale=Non
     Sums are float32; D up to 128.  For inference: a query that needs a gradient
     is refused."""
     who = "attention_fp4"
-    if query.ndim != 4:
-        raise ValueError("%s: expected a [B, H, Tq, D] query, got shape %s"
-                         % (who, list(query.shape)))
+    qs = query._shape
+    if len(qs) != 4:
+        raise ValueError("%s: expected a [B, H, Tq, D] query, got shape %s" % (who, list(qs)))
     if _T._recorded(query):
         raise RuntimeError("%s: no gradient is taken through a cache in 4 bits; run it under "
                            "no_grad()" % who)
-    B, H, Tq, D = query._shape
+    B, H, Tq, D = qs
     if not 0 < D <= 128:
         raise NotImplementedError("%s: head dims up to 128, got %d" % (who, D))
-    shape = _cache(who, k_codes, k_scales, D)
-    if _cache(who, v_codes, v_scales, D) != shape or shape[0] != B:
+    shape, pkc, pks = _cache(who, k_codes, k_scales, D)
+    vshape, pvc, pvs = _cache(who, v_codes, v_scales, D)
+    if vshape != shape or shape[0] != B:
         raise ValueError("%s: query %s does not fit caches %s and %s"
-                         % (who, list(query.shape), list(k_codes.shape), list(v_codes.shape)))
+                         % (who, list(qs), list(k_codes._shape), list(v_codes._shape)))
     Hkv, n = shape[1:]
     if (Hkv == 0) != (H == 0) or (Hkv and H % Hkv):
         raise RuntimeError("%s: %d query heads over %d of keys" % (who, H, Hkv))
     count, p, _keep = _per_sequence(who, "length", length, B)
-    if count > n:
-        raise ValueError("%s: length %d of a cache of %d" % (who, count, n))
-    if p is None and Tq > count:
-        raise RuntimeError("%s: %d queries are not the last of %d positions" % (who, Tq, count))
+    if p is None:
+        if count > n:
+            raise ValueError("%s: length %d of a cache of %d" % (who, count, n))
+        if Tq > count:
+            raise RuntimeError("%s: %d queries are not the last of %d positions"
+                               % (who, Tq, count))
     q = query if query._dtype == "float32" else query.float()
     if q._strides[3] != 1 and D > 1:
         q = _k_contiguous(q)
-    o = empty((B, Tq, H, D))
+    o = Storage(max(1, B * Tq * H * D) * 4)
     st = (Tq * H * D, D, H * D, 1)
     L.check(L.lib().tjh_fp4_attention(
-        q.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
-        v_scales.data_ptr(), o.data_ptr(), B, H, Hkv, Tq, n, D, L.i64arr(q._strides[:3]),
-        L.i64arr(st[:3]), count, p, float(scale) if scale is not None else D ** -0.5), who)
-    return _alias(o, (B, H, Tq, D), st, 0)
+        q.data_ptr(), pkc, pks, pvc, pvs, o.ptr, B, H, Hkv, Tq, n, D, _strides(q._strides),
+        _strides(st), count, p, float(scale) if scale is not None else D ** -0.5), who)
+    return Tensor(o, qs, st)
 
 
 # ------------------------------------------------------------------ beams
@@ -284,12 +325,12 @@ def beam_step(logits, scores, beams=None, finished=None, eos=None):
     who = "beam_step"
     if not isinstance(scores, Tensor):
         scores = _T.tensor(np.asarray(scores, dtype=np.float32))
-    if scores.ndim != 2 or scores.shape[1] == 0:
-        raise ValueError("%s: expected scores [B, W], got shape %s" % (who, list(scores.shape)))
-    B, W = scores.shape
-    ls = logits.shape
-    if logits.ndim not in (2, 3) or ls[-1] == 0 or \
-            (ls[:-1] != (B, W) if logits.ndim == 3 else ls[0] != B * W):
+    ss, ls = scores._shape, logits._shape
+    if len(ss) != 2 or ss[1] == 0:
+        raise ValueError("%s: expected scores [B, W], got shape %s" % (who, list(ss)))
+    B, W = ss
+    if len(ls) not in (2, 3) or ls[-1] == 0 or \
+            (ls[:-1] != ss if len(ls) == 3 else ls[0] != B * W):
         raise ValueError("%s: logits of shape %s for scores %s" % (who, list(ls), [B, W]))
     V = ls[-1]
     keep = W if beams is None else int(beams)
@@ -308,16 +349,22 @@ def beam_step(logits, scores, beams=None, finished=None, eos=None):
             raise ValueError("%s: finished of shape %s for scores %s"
                              % (who, list(finished.shape), [B, W]))
         finished = finished.contiguous()
-    x = logits if logits.dtype == "float32" else logits.float()
-    xd, px, ld, _, _ = _T._rows_2d(x.detach())
-    s = (scores if scores.dtype == "float32" else scores.float()).detach().contiguous()
-    out = empty((B, keep))
-    tokens, parents = empty((B, keep), "int32"), empty((B, keep), "int32")
-    done = empty((B, keep), "bool")
-    L.check(L.lib().tjh_beam_step(px, ld, s.data_ptr(),
+    x = logits if logits._dtype == "float32" else logits.float()
+    if scores._dtype != "float32":
+        scores = scores.float()
+    if not scores.is_contiguous():
+        scores = scores.detach().contiguous()
+    xd, px, ld, _, _ = _T._rows_2d(x)
+    # all four in one allocation
+    n, shape = B * keep, (B, keep)
+    st = Storage(max(1, 13 * n))
+    out, tokens = Tensor(st, shape), Tensor(st, shape, None, n, "int32")
+    parents, done = Tensor(st, shape, None, 2 * n, "int32"), Tensor(st, shape, None, 12 * n, "bool")
+    p = st.ptr
+    L.check(L.lib().tjh_beam_step(px, ld, scores.data_ptr(),
                                   finished.data_ptr() if finished is not None else None, B, W, V,
-                                  keep, -1 if eos is None else int(eos), out.data_ptr(),
-                                  tokens.data_ptr(), parents.data_ptr(), done.data_ptr()), who)
+                                  keep, -1 if eos is None else int(eos), p, p + 4 * n, p + 8 * n,
+                                  p + 12 * n), who)
     return out, tokens, parents, done
 
 
