@@ -91,21 +91,17 @@ __device__ __forceinline__ float scale_of(uint32_t top) {
   return top < 0x0d800000u ? 0.f : __uint_as_float(top) / 6.f;
 }
 
-// The code of x at a scale.  A step is passed where |x| is above the border
-// halfway to it, or on one whose upper step is even; the sign of |x| - border *
-// scale is exact, as it is rounded once.
+// The code of x at a scale, by bisection.  A step is passed where |x| is above the
+// border halfway to it, or on one whose upper step is even; the sign of |x| -
+// border * scale is exact, as it is rounded once.
 __device__ __forceinline__ uint32_t code_of(float x, float scale) {
   const float a = fabsf(x);
-  uint32_t c = 0;
-  c += __builtin_fmaf(-0.25f, scale, a) > 0.f;
-  c += __builtin_fmaf(-0.75f, scale, a) >= 0.f;
-  c += __builtin_fmaf(-1.25f, scale, a) > 0.f;
-  c += __builtin_fmaf(-1.75f, scale, a) >= 0.f;
-  c += __builtin_fmaf(-2.5f, scale, a) > 0.f;
-  c += __builtin_fmaf(-3.5f, scale, a) >= 0.f;
-  c += __builtin_fmaf(-5.f, scale, a) > 0.f;
-  if (!(scale > 0.f)) c = 0;
-  return c | (x < 0.f ? 8u : 0u);
+  const bool b4 = __builtin_fmaf(-1.75f, scale, a) >= 0.f;
+  const bool b2 = __builtin_fmaf(b4 ? -3.5f : -0.75f, scale, a) >= 0.f;
+  const float hi = b4 ? -5.f : -1.25f, lo = b4 ? -2.5f : -0.25f;
+  const bool b1 = __builtin_fmaf(b2 ? hi : lo, scale, a) > 0.f;
+  const uint32_t c = (b4 ? 4u : 0u) | (b2 ? 2u : 0u) | (b1 ? 1u : 0u);
+  return (scale > 0.f ? c : 0u) | (x < 0.f ? 8u : 0u);
 }
 
 // Bytes of a cached position's codes.

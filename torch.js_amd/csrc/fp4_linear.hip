@@ -64,15 +64,15 @@ __device__ __forceinline__ floatx4 scales_of(const float* __restrict__ s) {
 // columns and each 16 of its 3 R (part, row) pairs, part by part, a matrix
 // operand: lane (j, i) has pair i and columns 8 j to 8 j + 7.
 __global__ __launch_bounds__(256) void k_fp4_split_rows(const float* __restrict__ x, int64_t ldx,
-                                                        int64_t M, int64_t K, int R, int MT,
-                                                        int kb, int64_t items,
+                                                        int64_t M, int64_t K, uint32_t R, int MT,
+                                                        uint32_t kb, uint32_t items,
                                                         uintx4* __restrict__ parts) {
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const uint32_t at = blockIdx.x * 256 + threadIdx.x;
   if (at >= items) return;
   // (chunk, 32 columns, 8 of them, row)
-  const int64_t row8 = at / R;
+  const uint32_t row8 = at / R, fu = row8 >> 2;
   const int r = (int)(at - row8 * R), j = (int)(row8 & 3);
-  const int64_t f = row8 >> 2, chunk = f / kb, k32 = f - chunk * kb;
+  const int64_t f = fu, chunk = fu / kb, k32 = fu % kb;
   const int64_t m = chunk * R + r;
   float v[8];
   load8(x + (m < M ? m : M - 1) * ldx, 32 * k32 + 8 * j, K, v);
@@ -224,7 +224,8 @@ int few_rows(LinArgs a) {
   if (!s.ok()) return set_error(TJH_ERR_OOM, "tjh_fp4_linear: no scratch");
   if (items)
     tjh_launch(k_fp4_split_rows, dim3((unsigned)cdiv(items, 256)), dim3(256), 0, stream(), a.x,
-               a.ldx, a.M, a.K, a.rows, MT, kb, items, s.as<uintx4>());
+               a.ldx, a.M, a.K, (uint32_t)a.rows, MT, (uint32_t)kb, (uint32_t)items,
+               s.as<uintx4>());
   a.parts = s.as<uintx4>();
   switch (MT) {
     case 2: launch_share<G, 2, false>(a, chunks); break;
@@ -241,12 +242,13 @@ int few_rows(LinArgs a) {
 // Parts of x for k_fp4_gemm: for each 32 columns, each 16 rows and each part a
 // matrix operand.
 __global__ __launch_bounds__(256) void k_fp4_split(const float* __restrict__ x, int64_t ldx,
-                                                   int64_t M, int64_t K, int m_tiles,
-                                                   int64_t items, uintx4* __restrict__ parts) {
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+                                                   int64_t M, int64_t K, uint32_t m_tiles,
+                                                   uint32_t items, uintx4* __restrict__ parts) {
+  const uint32_t at = blockIdx.x * 256 + threadIdx.x;
   if (at >= items) return;
   const int lane = at & 63;
-  const int64_t f = at >> 6, k32 = f / m_tiles, m = (f - k32 * m_tiles) * 16 + (lane & 15);
+  const uint32_t fu = at >> 6;
+  const int64_t f = fu, k32 = fu / m_tiles, m = (fu % m_tiles) * 16 + (lane & 15);
   float v[8];
   load8(x + (m < M ? m : M - 1) * ldx, 32 * k32 + 8 * (lane >> 4), K, v);
   bf16x8 p[3];
@@ -412,7 +414,7 @@ int many_rows(LinArgs a) {
   Scratch s((size_t)items * 3 * 16);
   if (!s.ok()) return set_error(TJH_ERR_OOM, "tjh_fp4_linear: no scratch");
   tjh_launch(k_fp4_split, dim3((unsigned)cdiv(items, 256)), dim3(256), 0, stream(), a.x, a.ldx, a.M,
-             a.K, a.m_tiles, items, s.as<uintx4>());
+             a.K, (uint32_t)a.m_tiles, (uint32_t)items, s.as<uintx4>());
   a.parts = s.as<uintx4>();
   // column tiles of the CU that has most
   const auto load = [&](int C) { return cdiv(cdiv(a.N, 16 * C) * rows, num_cus()) * C; };
