@@ -29,6 +29,17 @@ struct BeamArgs {
   int W, V, S, per, keep, eos;
 };
 
+// exp(x) for x <= 0 to about a float's step: the rounding of x log2(e) goes back
+// in behind the hardware's power of two (half of expf's instructions, of which a
+// row has one each).
+__device__ __forceinline__ float exp_near(float x) {
+  constexpr float kLog2e = 1.44269502f, kLog2eLow = 1.92596299e-8f, kLn2 = 0.693147182f;
+  const float y = fmaxf(x, -200.f) * kLog2e;  // below, 0 in any case
+  const float low = __builtin_fmaf(x, kLog2eLow, __builtin_fmaf(x, kLog2e, -y));
+  const float e = __builtin_amdgcn_exp2f(y);
+  return x > -100.f ? __builtin_fmaf(e, low * kLn2, e) : x == x ? 0.f : x;
+}
+
 // A piece of a row: `per` columns, fewer at the end.
 template <int T, int NV, int CAP>
 __global__ __launch_bounds__(T, T == 512 ? 4 : 1) void k_beam_pieces(BeamArgs a) {
@@ -43,7 +54,7 @@ __global__ __launch_bounds__(T, T == 512 ? 4 : 1) void k_beam_pieces(BeamArgs a)
   row.each([&](int, int, float x) { m = fmaxf(m, x); });  // NaN takes no part here,
   m = b.max(m);
   const float from = m == -INFINITY ? 0.f : m;
-  row.each([&](int, int, float x) { sum += expf(x - from); });  // but in the sum
+  row.each([&](int, int, float x) { sum += exp_near(x - from); });  // but in the sum
   sum = b.sum(sum);
   const int k = min(a.keep, n);
   const u64* best = select_largest(row, k, kNanFirst, s, b);
@@ -65,56 +76,68 @@ __device__ __forceinline__ double key_score(u64 k) {
   return __longlong_as_double((long long)((k >> 63) ? k & 0x7fffffffffffffffull : ~k));
 }
 
-constexpr int kMaxBeams = 64, kMaxLists = 1280, kMaxEntries = kMaxBeams * kMaxBeams;
+constexpr int kMaxBeams = 64, kMaxEntries = kMaxBeams * kMaxBeams;
+constexpr int kMergeThreads = 512;
+constexpr int kEarly = 3;  // candidates a thread, read before anything else is known
 
 // One workgroup a search.  The lists (a beam's pieces) are in order, so only the
 // `keep` lists with the best heads matter, and of those only what is not below the
 // last of these heads; some tens of entries, ranked by counting.
-__global__ __launch_bounds__(256) void k_beam_merge(BeamArgs a) {
+__global__ __launch_bounds__(kMergeThreads) void k_beam_merge(BeamArgs a) {
   __shared__ double from[kMaxBeams];  // a beam's score less its logarithm of the sum
   __shared__ int state[kMaxBeams];    // 0 goes on, 1 finished, 2 has no continuation
-  __shared__ u64 head[kMaxLists];
   __shared__ int chosen[kMaxBeams];
-  __shared__ u64 key[kMaxEntries];
+  __shared__ u64 early[kEarly * kMergeThreads];
+  __shared__ u64 key[kMaxEntries];  // the lists' heads, then the entries
   __shared__ int flat[kMaxEntries];
   __shared__ u64 bound;
   __shared__ int count;
   const int t = threadIdx.x, lists = a.W * a.S;
   const int64_t r0 = (int64_t)blockIdx.x * a.W;
+  // Most of the time goes by reads one after the other of what other CUs have
+  // just written: where there are few candidates they are all read at once (of
+  // ended beams, whatever stands there).
+  const u64* __restrict__ cand = a.cand + r0 * a.S * a.keep;
+  const int all = lists * a.keep;
+  const bool few = all <= kEarly * kMergeThreads;
+  u64 pre[kEarly];
+  if (few) {
+#pragma unroll
+    for (int i = 0; i < kEarly; ++i)
+      if (t + kMergeThreads * i < all) pre[i] = cand[t + kMergeThreads * i];
+  }
   if (t == 0) {
     bound = 0;
     count = 0;
   }
   if (t < kMaxBeams) chosen[t] = -1;
   // a wave a beam, its lanes the pieces, always added up in one order
-  for (int w = t >> 6; w < a.W; w += 4) {
+  for (int w = t >> 6; w < a.W; w += kMergeThreads / 64) {
     const int lane = t & 63;
+    const float2* p = a.stats + (r0 + w) * a.S;
+    const float2 first = lane < a.S ? p[lane] : make_float2(-INFINITY, 0.f);
+    const bool ended = a.finished && a.finished[r0 + w];
     const double s = a.scores[r0 + w];
-    int st = 0;
-    double less = 0.0;
-    if (!(s > -INFINITY)) {
-      st = 2;
-    } else if (a.finished && a.finished[r0 + w]) {
-      st = 1;
-    } else {
-      const float2* p = a.stats + (r0 + w) * a.S;
-      float m = -INFINITY;
-      for (int i = lane; i < a.S; i += 64) m = fmaxf(m, p[i].x);
-      m = wave_max(m);
-      double sum = 0.0;
-      for (int i = lane; i < a.S; i += 64) {
-        const float2 x = p[i];
-        sum += x.x == -INFINITY ? (double)x.y : (double)x.y * exp((double)x.x - (double)m);
-      }
-      for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
-      // NaN in the sum, +infinity as the maximum, or nothing above -infinity
-      if (!(sum > 0.0 && sum < INFINITY && m < INFINITY && m > -INFINITY)) st = 2;
-      else less = (double)m + log(sum);
-    }
+    float m = first.x;
+    for (int i = lane + 64; i < a.S; i += 64) m = fmaxf(m, p[i].x);
+    m = wave_max(m);
+    const auto term = [&](float2 x) {
+      return x.x == -INFINITY ? (double)x.y : (double)x.y * exp((double)x.x - (double)m);
+    };
+    double sum = term(first);
+    for (int i = lane + 64; i < a.S; i += 64) sum += term(p[i]);
+    for (int o = 1; o < 64 && o < a.S; o <<= 1) sum += __shfl_xor(sum, o, 64);
+    // NaN in the sum, +infinity as the maximum, or nothing above -infinity
+    const bool ok = sum > 0.0 && sum < INFINITY && m < INFINITY && m > -INFINITY;
     if (lane == 0) {
-      state[w] = st;
-      from[w] = s - less;
+      state[w] = !(s > -INFINITY) ? 2 : ended ? 1 : ok ? 0 : 2;
+      from[w] = ended || !ok ? s : s - ((double)m + log(sum));
     }
+  }
+  if (few) {
+#pragma unroll
+    for (int i = 0; i < kEarly; ++i)
+      if (t + kMergeThreads * i < all) early[t + kMergeThreads * i] = pre[i];
   }
   __syncthreads();
   const auto entry = [&](int list, int i, int* at) -> u64 {  // i-th of a list: key, w V + v
@@ -125,24 +148,24 @@ __global__ __launch_bounds__(256) void k_beam_merge(BeamArgs a) {
       return piece == 0 && i == 0 ? score_key(from[w]) : 0;
     }
     if (i >= min(a.keep, min(a.per, a.V - piece * a.per))) return 0;
-    const u64 c = a.cand[((r0 + w) * a.S + piece) * a.keep + i];
+    const u64 c = few ? early[list * a.keep + i] : cand[(int64_t)list * a.keep + i];
     const int v = index_of(c);
     *at = w * a.V + v;
     return score_key(from[w] + (double)key_value((uint32_t)(c >> 32)));
   };
   int at;
-  for (int i = t; i < lists; i += 256) head[i] = entry(i, 0, &at);
+  for (int i = t; i < lists; i += kMergeThreads) key[i] = entry(i, 0, &at);
   __syncthreads();
-  for (int i = t; i < lists; i += 256) {
-    const u64 me = head[i];
+  for (int i = t; i < lists; i += kMergeThreads) {
+    const u64 me = key[i];
     int rank = 0;
 #pragma unroll 8
-    for (int j = 0; j < lists; ++j) rank += head[j] > me || (head[j] == me && j < i);
+    for (int j = 0; j < lists; ++j) rank += key[j] > me || (key[j] == me && j < i);
     if (rank < a.keep) chosen[rank] = i;
     if (rank == a.keep - 1) bound = me;
   }
   __syncthreads();
-  for (int i = t; i < a.keep * a.keep; i += 256) {
+  for (int i = t; i < a.keep * a.keep; i += kMergeThreads) {
     const int list = chosen[i / a.keep];
     if (list < 0) continue;
     const u64 k = entry(list, i % a.keep, &at);
@@ -155,7 +178,7 @@ __global__ __launch_bounds__(256) void k_beam_merge(BeamArgs a) {
   __syncthreads();
   const int n = count;
   const int64_t o = (int64_t)blockIdx.x * a.keep;
-  for (int i = t; i < n; i += 256) {
+  for (int i = t; i < n; i += kMergeThreads) {
     const u64 me = key[i];
     const int f = flat[i];
     int rank = 0;
@@ -168,7 +191,7 @@ __global__ __launch_bounds__(256) void k_beam_merge(BeamArgs a) {
     a.parents[o + rank] = w;
     a.out_finished[o + rank] = v == a.eos || state[w] == 1;
   }
-  for (int i = n + t; i < a.keep; i += 256) {
+  for (int i = n + t; i < a.keep; i += kMergeThreads) {
     a.out_scores[o + i] = -INFINITY;
     a.tokens[o + i] = -1;
     a.parents[o + i] = min(i, a.W - 1);
@@ -260,9 +283,9 @@ int tjh_beam_step(const float* logits, int64_t ld, const float* scores, const ui
   // the workgroups stay few
   const int64_t rows = B * W;
   int per = 53248 - 4;
-  for (const int size : {1024 - 4, 4096 - 4, 16384 - 4}) {
+  for (const int size : {1024 - 4, 4096 - 4, 16384 - 4, 26624 - 4}) {
     const int64_t S = cdiv(V, size);
-    if (S == 1 || (W * S <= 256 && rows * S <= 2 * num_cus())) {
+    if (S == 1 || (W * S <= 64 && rows * S <= 2 * num_cus())) {
       per = size;
       break;
     }
@@ -283,11 +306,13 @@ int tjh_beam_step(const float* logits, int64_t ld, const float* scores, const ui
     tjh_launch(k_beam_pieces<256, 4, 4096>, grid, dim3(256), 0, stream(), a);
   else if (per < 16384)
     tjh_launch(k_beam_pieces<512, 8, 4096>, grid, dim3(512), 0, stream(), a);
+  else if (per < 26624)
+    tjh_launch(k_beam_pieces<512, 13, 4096>, grid, dim3(512), 0, stream(), a);
   else
     tjh_launch(k_beam_pieces<512, 26, 4096>, grid, dim3(512), 0, stream(), a);
   const int rc = check_launch("beam_pieces");
   if (rc != TJH_OK) return rc;
-  tjh_launch(k_beam_merge, dim3((unsigned)B), dim3(256), 0, stream(), a);
+  tjh_launch(k_beam_merge, dim3((unsigned)B), dim3(kMergeThreads), 0, stream(), a);
   return check_launch("beam_merge");
 }
 
