@@ -12,10 +12,10 @@ U = 2.0 ** -24
 VOCAB, CTX, D, HEADS, LAYERS = 211, 64, 96, 3, 2
 
 
-def _model(torch, seed=11):
+def _model(torch, seed=11, **kw):
     from torchjs_amd import workloads as W
     torch.manual_seed(seed)
-    m = W.GPT2(VOCAB, CTX, D, HEADS, LAYERS)
+    m = W.GPT2(VOCAB, CTX, D, HEADS, LAYERS, **kw)
     with torch.no_grad():  # logits that differ by some units
         for p in (m.ln_f.weight, m.ln_f.bias):
             p.copy_(p + 0.1 * torch.randn(*p.shape))
@@ -171,7 +171,16 @@ def test_search(torch, bits, w, quantized):
         assert not at.size or (row[at[0]:] == eos).all()
 
 
-def test_search_finds_more_than_greedy(torch):
+def test_search_with_a_window(torch):
+    m = _model(torch, 5, window=6, sinks=1)
+    ids = _ids(torch, 2, 9, 2)
+    got = m.generate(ids, 12, beams=3).numpy()[:, 9:]
+    want, least = _search_by_hand(torch, m, ids, 12, 3, None, 32)
+    assert least > 100 * U
+    assert (got == want).all()
+
+
+def test_search_is_exhaustive_with_enough_beams(torch):
     """With as many beams as there are continuations the search is exhaustive."""
     from torchjs_amd import workloads as W
     torch.manual_seed(2)

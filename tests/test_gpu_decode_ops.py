@@ -189,7 +189,9 @@ def _linear_case(torch, m, k, n, group, bias, seed=0):
 LINEAR = [(1, 1, 1), (1, 31, 3), (2, 128, 16), (3, 129, 17), (5, 768, 2304), (6, 768, 50),
           (10, 300, 65), (16, 1000, 100), (17, 515, 77), (32, 640, 40), (33, 256, 129), (64, 1024, 64),
           (100, 96, 500), (129, 384, 257), (300, 200, 1030), (1, 4100, 5000), (4, 260, 33000),
-          (7, 1300, 17000), (30, 700, 9000), (70, 33, 33000), (1100, 160, 4000), (2050, 300, 1900)]
+          (7, 1300, 17000), (30, 700, 9000), (70, 33, 33000), (1100, 160, 4000), (2050, 300, 1900),
+          (1900, 100, 1000), (26, 300, 70), (16, 140, 16400), (21, 140, 16400), (26, 140, 16400),
+          (32, 140, 16400)]
 
 
 @gpu
@@ -218,6 +220,9 @@ def test_linear_takes_rows_where_they_stand(torch, m):
     assert one.shape == (30,) and (np.abs(one.numpy() - want[0]) <= tol[0]).all()
     none = torch.functional.linear_fp4(torch.zeros(0, 203), codes, scales)
     assert none.shape == (0, 30)
+    empty, bias = torch.functional.quantize_fp4(torch.zeros(30, 0)), torch.randn(30)
+    y = torch.functional.linear_fp4(torch.zeros(m, 0), *empty, bias)
+    assert (y.numpy() == bias.numpy()).all()
 
 
 @gpu
@@ -401,7 +406,10 @@ ATTEND = [  # b, h, hkv, tq, keys, d
     (1, 4, 2, 3, 70, 96), (2, 2, 2, 7, 7, 64), (1, 3, 3, 33, 33, 64), (1, 4, 4, 31, 90, 128),
     (1, 4, 1, 64, 200, 80), (1, 2, 2, 65, 65, 32), (2, 2, 1, 100, 133, 64), (1, 1, 1, 129, 400, 128),
     (1, 2, 2, 40, 40, 30), (1, 2, 2, 3, 20, 1), (1, 2, 1, 50, 60, 127), (1, 16, 1, 1, 513, 64),
-    (1, 5, 5, 200, 200, 64)]
+    (1, 5, 5, 200, 200, 64),
+    # keys in slices; a wave for each 16 rows; both
+    (1, 4, 2, 1, 1500, 64), (2, 2, 2, 3, 1300, 80), (1, 2, 1, 40, 1100, 32), (3, 8, 1, 1, 2100, 128),
+    (32, 16, 16, 17, 30, 64), (1, 16, 1, 1024, 1030, 32)]
 
 
 @gpu
@@ -417,14 +425,15 @@ def test_attention(torch, b, h, hkv, tq, n, d):
 
 
 @gpu
+@pytest.mark.parametrize("n", [150, 1200])
 @pytest.mark.parametrize("tq", [1, 3, 40])
 @pytest.mark.parametrize("h,hkv,d", [(4, 2, 64), (3, 3, 128)])
-def test_attention_of_ragged_sequences(torch, tq, h, hkv, d):
+def test_attention_of_ragged_sequences(torch, tq, h, hkv, d, n):
     """A length each: none, fewer than there are queries, some, all, and more and
     less than there can be.  Later positions hold NaN."""
     rng = np.random.default_rng(tq)
-    lengths = np.array([0, 1, 2, 39, 41, 150, 999, -3], np.int32)
-    b, n = len(lengths), 150
+    lengths = np.array([0, 1, 2, 39, 41, n, 9999, -3, n - 1], np.int32)
+    b = len(lengths)
     cache, k, v = _filled(torch, b, hkv, n, d, rng, 0.3)
     for i, length in enumerate(lengths):
         for s in (cache[1], cache[3]):

@@ -359,9 +359,11 @@ __global__ __launch_bounds__(128) void k_fp4_join(AttArgs a) {
   if (d >= a.D) return;
   const int64_t p = row * a.slices;
   float top = -INFINITY;
+#pragma unroll 8
   for (int s = 0; s < a.slices; ++s) top = fmaxf(top, a.pm[p + s]);
   const float ts = top == -INFINITY ? 0.f : top;
   float num = 0.f, den = 0.f;
+#pragma unroll 8
   for (int s = 0; s < a.slices; ++s) {
     const float f = __builtin_amdgcn_exp2f(a.pm[p + s] - ts);
     den = __builtin_fmaf(a.pl[p + s], f, den);
@@ -420,13 +422,15 @@ extern "C" int tjh_fp4_attention(const float* q, const uint8_t* k_codes, const f
   a.scale = scale;
   const int64_t rows = a.group * Tq;
   a.row_tiles = (int)cdiv(rows, 16);
-  // the waves of a workgroup share a row tile's keys where there are too few
-  // tiles for a wave on every SIMD; then slices of the keys until the CUs have
-  // two workgroups each, none under 128 keys (a tile of each wave)
+  // The waves of a workgroup share a row tile's keys where there are too few
+  // tiles for a wave on every SIMD.  Then slices of the keys until the CUs have
+  // two workgroups each, if there are more than 1024: joining them is a launch of
+  // its own (12 heads of 64, 1000 keys: 10 us, in eight slices 11.6, in two 12).
   const int64_t keys = lengths ? L : length, tiles = B * Hkv * a.row_tiles;
   const bool split = tiles < 4 * num_cus();
   const int64_t wgs = split ? tiles : B * Hkv * cdiv(a.row_tiles, kWaves);
-  const int64_t want = 2 * wgs >= 3 * num_cus() ? 1 : cdiv(2 * num_cus(), wgs), can = cdiv(keys, split ? 128 : 512);
+  const int64_t want = 2 * wgs >= 3 * num_cus() ? 1 : cdiv(2 * num_cus(), wgs);
+  const int64_t can = keys > 1024 ? cdiv(keys, 512) : 1;
   a.slices = (int)(want < can ? want : can);
   if (a.slices < 1) a.slices = 1;
   KernelScope ks("fp4_attention");

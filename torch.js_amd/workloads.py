@@ -449,6 +449,7 @@ class GPT2(nn.Module):
         if not 1 < beams <= min(64, self.vocab) or beams != int(beams):
             raise ValueError("generate: %r beams of %d tokens (from 1 to 64)"
                              % (beams, self.vocab))
+        beams = int(beams)
         if T + count > self.ctx:
             raise ValueError("generate: %d positions exceed the context of %d"
                              % (T + count, self.ctx))
