@@ -56,9 +56,11 @@ int tjh_fp4_cache_append(const float* k, const float* v, const int64_t* k_stride
                          const int64_t* v_strides, uint8_t* k_codes, float* k_scales,
                          uint8_t* v_codes, float* v_scales, int64_t B, int64_t H, int64_t T,
                          int64_t D, int64_t L, int64_t pos, const int32_t* positions);
-/* out [B, H, n, D], contiguous = the values at positions [start, start + n). */
-int tjh_fp4_cache_read(const uint8_t* codes, const float* scales, int64_t B, int64_t H, int64_t L,
-                       int64_t D, int64_t start, int64_t n, float* out);
+/* out [B, H, n, D], contiguous = the values at positions [start, start + n) of
+ * one of keys or values, and out2 those of the other (codes2 NULL: none). */
+int tjh_fp4_cache_read(const uint8_t* codes, const float* scales, const uint8_t* codes2,
+                       const float* scales2, int64_t B, int64_t H, int64_t L, int64_t D,
+                       int64_t start, int64_t n, float* out, float* out2);
 /* Causal attention of q [B, H, Tq, D] over such a cache of Hkv heads (H a
  * multiple of Hkv; query head h reads head h / (H / Hkv)): the queries are the
  * last Tq of the first `length` positions, or of lengths[b] (taken into [0, L])

@@ -346,6 +346,9 @@ def test_append_and_read(torch, d):
         assert np.array_equal(got, np.where(finite[..., None], val, np.nan).astype(np.float32),
                               equal_nan=True)
     assert F.cache_read_fp4(*cache[:2], d, 3, 3).shape == (b, h, 0, d)
+    both = F.cache_read_fp4(*cache[:2], d, pos, pos + t, cache[2:])
+    for x, one in zip(both, (cache[:2], cache[2:])):
+        assert np.array_equal(x.numpy(), F.cache_read_fp4(*one, d, pos, pos + t).numpy(), equal_nan=True)
 
 
 @gpu
@@ -777,6 +780,7 @@ def _refusals(t):
         (ValueError, lambda F: F.cache_read_fp4(*cache[:2], 64, 3, 10)),
         (ValueError, lambda F: F.cache_read_fp4(*cache[:2], 64, 5, 4)),
         (ValueError, lambda F: F.cache_read_fp4(*cache[:2], 70, 0, 4)),
+        (ValueError, lambda F: F.cache_read_fp4(*cache[:2], 64, 0, 4, (t(2, 2, 8, 32, **u8), t(2, 2, 8)))),
         (ValueError, lambda F: F.attention_fp4(t(2, 3, 64), *cache, 9)),
         (RuntimeError, lambda F: F.attention_fp4(t(2, 3, 3, 64), *cache, 9)),
         (ValueError, lambda F: F.attention_fp4(q, *cache, 10)),
@@ -808,7 +812,7 @@ def _refusals(t):
     ]
 
 
-@pytest.mark.parametrize("i", range(53))
+@pytest.mark.parametrize("i", range(54))
 def test_refusals(pkg, i):
     """Refused by shapes alone, before the library is called."""
     from torchjs_amd import _lib
@@ -817,7 +821,7 @@ def test_refusals(pkg, i):
         def __getattr__(self, name):
             raise AssertionError("%s was called" % name)
     cases = _refusals(lambda *s, **k: _shape_only(pkg, *s, **k))
-    assert len(cases) == 53
+    assert len(cases) == 54
     error, call = cases[i]
     real, _lib.lib = _lib.lib, lambda: Closed()
     try:
@@ -840,7 +844,8 @@ def test_library_refusals(torch):
     assert lib.tjh_fp4_linear(p, 4, 1, 1, 4, p + 4, p, 32, None, p, 1) == 1
     assert lib.tjh_fp4_cache_append(p, p, st, st, p, p, p, p, 1, 1, 2, 4, 3, 2, None) == 1
     assert lib.tjh_fp4_cache_append(p, p, st, st, p, p, p, p, 1, 1, 2, 129, 3, 0, None) == 5
-    assert lib.tjh_fp4_cache_read(p, p, 1, 1, 3, 4, 2, 2, p) == 1
+    assert lib.tjh_fp4_cache_read(p, p, None, None, 1, 1, 3, 4, 2, 2, p, None) == 1
+    assert lib.tjh_fp4_cache_read(p, p, p, None, 1, 1, 3, 4, 0, 2, p, p) == 1
     assert lib.tjh_fp4_attention(p, p, p, p, p, p, 1, 3, 2, 1, 4, 4, st, st, 4, None, 1.0) == 1
     assert lib.tjh_fp4_attention(p, p, p, p, p, p, 1, 2, 2, 1, 4, 4, st, st, 5, None, 1.0) == 1
     assert lib.tjh_fp4_attention(p, p, p, p, p, p, 1, 2, 2, 1, 4, 200, st, st, 4, None, 1.0) == 5

@@ -210,7 +210,8 @@ SIGNATURES = {
     "tjh_fp4_linear": [c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_i64],
     "tjh_fp4_cache_append": [c_vp, c_vp, P_i64, P_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64,
                              c_i64, c_i64, c_i64, c_vp],
-    "tjh_fp4_cache_read": [c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp],
+    "tjh_fp4_cache_read": [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp,
+                           c_vp],
     "tjh_fp4_attention": [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64,
                           c_i64, P_i64, P_i64, c_i64, c_vp, c_f32],
     "tjh_beam_step": [c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp,

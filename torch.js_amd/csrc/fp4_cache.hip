@@ -130,20 +130,26 @@ __global__ __launch_bounds__(256) void k_fp4_append(AppendArgs a) {
   if (d == 0) a.scales[which][place] = scale;
 }
 
-// 8 columns a thread.
-__global__ __launch_bounds__(256) void k_fp4_read(const uint8_t* __restrict__ codes,
-                                                  const float* __restrict__ scales, int64_t L,
-                                                  int D, int P, int64_t start, uint32_t n,
-                                                  uint32_t items, float* __restrict__ out) {
+struct ReadArgs {
+  const uint8_t* codes[2];
+  const float* scales[2];
+  float* out[2];
+  int64_t L, start;
+  uint32_t n, items;
+  int D, P;
+};
+
+// 8 columns a thread, keys (grid y 0) and values.
+__global__ __launch_bounds__(256) void k_fp4_read(ReadArgs a) {
   const uint32_t at = blockIdx.x * 256 + threadIdx.x;
-  if (at >= items) return;
-  const uint32_t per = (D + 7) / 8, rw = at / per, bh = rw / n;
-  const int64_t row = rw, from = bh * L + start + (rw - bh * n);
-  const int d = 8 * (int)(at - rw * per);
-  const float scale = scales[from];
+  if (at >= a.items) return;
+  const uint32_t per = (a.D + 7) / 8, rw = at / per, bh = rw / a.n;
+  const int64_t row = rw, from = bh * a.L + a.start + (rw - bh * a.n);
+  const int d = 8 * (int)(at - rw * per), D = a.D;
+  const float scale = a.scales[blockIdx.y][from];
   float v[8];
-  unpack(*reinterpret_cast<const uint32_t*>(codes + from * P + d / 2), v);
-  float* o = out + row * D + d;
+  unpack(*reinterpret_cast<const uint32_t*>(a.codes[blockIdx.y] + from * a.P + d / 2), v);
+  float* o = a.out[blockIdx.y] + row * D + d;
   if (D % 4 == 0) {
     *reinterpret_cast<floatx4*>(o) = floatx4{v[0], v[1], v[2], v[3]} * scale;
     if (d + 4 < D) *reinterpret_cast<floatx4*>(o + 4) = floatx4{v[4], v[5], v[6], v[7]} * scale;
@@ -256,8 +262,9 @@ int tjh_fp4_cache_append(const float* k, const float* v, const int64_t* k_stride
   return check_launch("fp4_append");
 }
 
-int tjh_fp4_cache_read(const uint8_t* codes, const float* scales, int64_t B, int64_t H, int64_t L,
-                       int64_t D, int64_t start, int64_t n, float* out) {
+int tjh_fp4_cache_read(const uint8_t* codes, const float* scales, const uint8_t* codes2,
+                       const float* scales2, int64_t B, int64_t H, int64_t L, int64_t D,
+                       int64_t start, int64_t n, float* out, float* out2) {
   TJH_REQUIRE_INIT();
   TJH_ARG(B >= 0 && H >= 0 && D > 0 && start >= 0 && n >= 0 && start + n <= L,
           "tjh_fp4_cache_read: bad sizes");
@@ -266,13 +273,17 @@ int tjh_fp4_cache_read(const uint8_t* codes, const float* scales, int64_t B, int
                      "tjh_fp4_cache_read: head dim %lld, length %lld (128, 2^24 - 1 at most)",
                      (long long)D, (long long)L);
   if (B == 0 || H == 0 || n == 0) return TJH_OK;
-  TJH_ARG(codes && scales && out && aligned16(codes) && aligned16(out),
+  TJH_ARG(codes && scales && out && aligned16(codes) && aligned16(out) &&
+              (!codes2 || (scales2 && out2 && aligned16(codes2) && aligned16(out2))),
           "tjh_fp4_cache_read: NULL or unaligned pointer");
   const int64_t items = B * H * n * cdiv(D, 8);
-  TJH_ARG(B < (1 << 29) && H < (1 << 29) && B * H < (1 << 29) && cdiv(items, 256) <= kGrid, "tjh_fp4_cache_read: too many rows");
+  TJH_ARG(B < (1 << 29) && H < (1 << 29) && B * H < (1 << 29) && cdiv(items, 256) <= kGrid,
+          "tjh_fp4_cache_read: too many rows");
+  const ReadArgs a{{codes, codes2}, {scales, scales2}, {out, out2}, L, start, (uint32_t)n,
+                   (uint32_t)items, (int)D, fp4::row_bytes((int)D)};
   KernelScope ks("fp4_read");
-  tjh_launch(k_fp4_read, dim3((unsigned)cdiv(items, 256)), dim3(256), 0, stream(), codes, scales,
-             L, (int)D, fp4::row_bytes((int)D), start, (uint32_t)n, (uint32_t)items, out);
+  tjh_launch(k_fp4_read, dim3((unsigned)cdiv(items, 256), codes2 ? 2 : 1), dim3(256), 0, stream(),
+             a);
   return check_launch("fp4_read");
 }
 

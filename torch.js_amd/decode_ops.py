@@ -242,20 +242,33 @@ def cache_append_fp4(k_codes, k_scales, v_codes, v_scales, key, value, pos):
         shape[2], n, p), who)
 
 
-def cache_read_fp4(codes, scales, head_dim, start, stop):
+def cache_read_fp4(codes, scales, head_dim, start, stop, other=None):
     """The float32 values [B, H, stop - start, head_dim] that positions
-    [start, stop) of a cache's keys or values stand for."""
+    [start, stop) of a cache's keys or values stand for; with `other`, the
+    (codes, scales) of the other of the two, both as a pair."""
     who = "cache_read_fp4"
     d = int(head_dim)
     if not 0 < d <= 128:
         raise NotImplementedError("%s: head dims up to 128, got %d" % (who, d))
-    (B, H, n), pc, ps = _cache(who, codes, scales, d)
-    if not 0 <= start <= stop <= n:
-        raise ValueError("%s: positions [%d, %d) of %d" % (who, start, stop, n))
-    out = Tensor(Storage(max(1, B * H * (stop - start) * d) * 4), (B, H, stop - start, d))
-    L.check(L.lib().tjh_fp4_cache_read(pc, ps, B, H, n, d, start, stop - start, out.data_ptr()),
-            who)
-    return out
+    shape, pc, ps = _cache(who, codes, scales, d)
+    pc2 = ps2 = None
+    if other is not None:
+        shape2, pc2, ps2 = _cache(who, other[0], other[1], d)
+        if shape2 != shape:
+            raise ValueError("%s: caches of shapes %s and %s"
+                             % (who, list(codes._shape), list(other[0]._shape)))
+    B, H, n = shape
+    if not 0 <= start <= stop <= n or start != int(start) or stop != int(stop):
+        raise ValueError("%s: positions [%s, %s) of %d" % (who, start, stop, n))
+    rows = int(stop) - int(start)
+    size, sh = B * H * rows * d, (B, H, rows, d)
+    # both in one allocation, the second one 16-byte aligned
+    second = (size + 3) & ~3
+    st = Storage(max(1, 2 * second if pc2 is not None else size) * 4)
+    L.check(L.lib().tjh_fp4_cache_read(pc, ps, pc2, ps2, B, H, n, d, int(start), rows, st.ptr,
+                                       st.ptr + 4 * second), who)
+    out = Tensor(st, sh)
+    return out if pc2 is None else (out, Tensor(st, sh, None, second))
 
 
 def attention_fp4(query, k_codes, k_scales, v_codes, v_scales, length, scale=None):

@@ -307,8 +307,8 @@ class KVCacheFP4(KVCache):
 
     def read(self, layer, start, stop):
         """(keys, values) that positions [start, stop) stand for."""
-        return (F.cache_read_fp4(self.k[layer], self.k_scales[layer], self.head_dim, start, stop),
-                F.cache_read_fp4(self.v[layer], self.v_scales[layer], self.head_dim, start, stop))
+        return F.cache_read_fp4(self.k[layer], self.k_scales[layer], self.head_dim, start, stop,
+                                (self.v[layer], self.v_scales[layer]))
 
     def _tensors(self):
         return self.k + self.v + self.k_scales + self.v_scales
