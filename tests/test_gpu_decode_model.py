@@ -84,6 +84,56 @@ def test_quantized_model(torch, group):
     assert four.quantize_fp4(group).h[0].attn.c_attn is before
 
 
+@pytest.mark.parametrize("bits", [32, 4])
+@pytest.mark.parametrize("held", ["", "c_attn c_proj c_fc mlp", "c_fc", "c_proj"])
+@pytest.mark.parametrize("B,T,C,heads", [(1, 1, 64, 2), (2, 37, 96, 3), (7, 20, 160, 2)])
+def test_block_is_one_call(torch, monkeypatch, bits, held, B, T, C, heads):
+    """Without a gradient a block with layers or a cache in 4 bits is one call,
+    with bit for bit the values and the cache of its layers one by one; a layer
+    or a cache that a program has replaced takes the layers."""
+    from torchjs_amd import workloads as W
+    nn = torch.nn
+    torch.manual_seed(5)
+    blk = W.Block(C, heads)
+    for m, name, word in ((blk.attn, "c_attn", "c_attn"), (blk.attn, "c_proj", "c_proj"),
+                          (blk.mlp, "c_fc", "c_fc"), (blk.mlp, "c_proj", "mlp")):
+        if word in held.split():
+            setattr(m, name, nn.LinearFP4.of(getattr(m, name), 32))
+    kind = W.KVCacheFP4 if bits == 4 else W.KVCache
+    x = torch.tensor(np.random.default_rng(1).standard_normal((B, T, C)).astype(np.float32))
+    fast, calls = W.Block._infer, []
+    monkeypatch.setattr(W.Block, "_infer", lambda self, *a: calls.append(fast(self, *a)) or calls[-1])
+
+    def run():
+        with torch.no_grad():
+            cache = kind(1, B, heads, 2 * T + 3, C // heads)
+            out = [blk(x), blk.forward_cached(x, cache, 0, 0),
+                   blk.forward_cached(x[:, :1].contiguous(), cache, 0, T)]
+            if bits == 4:
+                out.append(blk.forward_cached(x, cache, 0, T + 1))
+            with pytest.raises(RuntimeError):
+                blk.forward_cached(x[:, :1].contiguous(), cache, 0, 2 * T + 3)
+            return [a.numpy() for a in out + cache._tensors()]
+    got = run()
+    n = 4 if bits == 4 else 3
+    assert all(c is not None for c in calls[:n]) and calls[n] is None
+    with monkeypatch.context() as m:
+        m.setattr(W.Block, "_infer", lambda self, *a: None)
+        want = run()
+    for a, b in zip(got, want):
+        assert np.array_equal(a, b)
+    with torch.no_grad():
+        cache = kind(1, B, heads, T, C // heads)
+        append, seen = cache.append, []
+        cache.append = lambda *a: seen.append(a[3]) or append(*a)
+        assert np.array_equal(blk.forward_cached(x, cache, 0, 0).numpy(), want[1]) and seen == [0]
+        if held:
+            blk.attn.c_attn = type("Mine", (type(blk.attn.c_attn),), {}).of(nn.Linear(C, 3 * C)) \
+                if "c_attn" in held else type("Mine", (nn.Linear,), {})(C, 3 * C)
+            blk(x)
+            assert calls[-1] is None
+
+
 @pytest.mark.parametrize("parts", [(30,), (1,), (7, 1, 20), (33, 5)])
 def test_cached_positions(torch, parts):
     """Each call's logits are those of explicit attention over what the cache

@@ -116,6 +116,12 @@ int attn_one_query(const float* q, const float* k, const float* v, float* o, flo
                    int64_t H, int64_t Tk, int64_t D, const int64_t* qs, const int64_t* ks,
                    const int64_t* vs, const int64_t* os, float scale, int causal);
 
+// tjh_fp4_linear (fp4_linear.hip) with an epilogue: act 1 GELU, 3 adds residual
+// [M, N] (row stride ldr, not overlapping y).
+int fp4_linear(const float* x, int64_t ldx, int64_t M, int64_t N, int64_t K, const uint8_t* codes,
+               const float* scales, int64_t group, const float* bias, float* y, int64_t ldy,
+               const float* residual, int64_t ldr, int act);
+
 // 16-byte alignment of a device pointer (128-bit access paths).
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 

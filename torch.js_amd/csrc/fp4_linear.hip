@@ -9,6 +9,7 @@
 // on the bf16 matrix cores form the float product of each group; the groups'
 // sums are scaled and added up in floats.
 #include "fp4.h"
+#include "ops_math.h"
 
 namespace tjh {
 namespace {
@@ -21,12 +22,22 @@ struct LinArgs {
   const uint8_t* codes;
   const float* scales;
   const float* bias;
+  const float* residual;
   float* y;
-  int64_t ldx, ldy, M, N, K;
+  int64_t ldx, ldy, ldr, M, N, K;
   int nb;       // blocks of 128 columns
   int rows;     // of x a workgroup takes (grid y of k_fp4_chunks)
   int m_tiles;  // 16 rows each (k_fp4_gemm)
+  int act;      // 1: GELU, 3: plus residual
 };
+
+// The end of an element of y.
+__device__ __forceinline__ void finish(const LinArgs& a, int64_t m, int64_t n, float v) {
+  if (a.bias) v += a.bias[n];
+  if (a.act == 1) v = gelu_f(v);
+  else if (a.act == 3) v = a.residual[m * a.ldr + n] + v;
+  a.y[m * a.ldy + n] = v;
+}
 
 constexpr int kWaves = 8;
 
@@ -165,7 +176,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_fp4_rows(LinArgs a) {
     for (int p = 2; p >= 0; --p)
 #pragma unroll
       for (int q = 0; q < KS; ++q) v += red[((tile * KS + q) * 16 + p * R + m) * 16 + col];
-    a.y[m * a.ldy + at] = a.bias ? v + a.bias[at] : v;
+    finish(a, m, at, v);
   }
 }
 
@@ -273,7 +284,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_fp4_chunks(LinArgs a) {
       for (int p = 2; p >= 0; --p)
 #pragma unroll
         for (int q = 0; q < kWaves; ++q) v += red[q][p * a.rows + m][col];
-      if (n < a.N) a.y[(m0 + m) * a.ldy + n] = a.bias ? v + a.bias[n] : v;
+      if (n < a.N) finish(a, m0 + m, n, v);
     }
   }
 }
@@ -464,13 +475,12 @@ __global__ __launch_bounds__(64 * kGemmWaves, 2) void k_fp4_gemm(LinArgs a) {
   for (int n = 0; n < C; ++n) {
     const int64_t at = n0 + n * 16 + c;
     if (at >= a.N) continue;
-    const float bias = a.bias ? a.bias[at] : 0.f;
 #pragma unroll
     for (int i = 0; i < kRowTiles; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int64_t m = (int64_t)mb * kBM + (w * kRowTiles + i) * 16 + 4 * j + r;
-        if (m < a.M) a.y[m * a.ldy + at] = acc[i][n][r] + bias;
+        if (m < a.M) finish(a, m, at, acc[i][n][r]);
       }
   }
 }
@@ -513,14 +523,10 @@ int product(const LinArgs& a) {
 }
 
 }  // namespace
-}  // namespace tjh
 
-using namespace tjh;
-
-extern "C" int tjh_fp4_linear(const float* x, int64_t ldx, int64_t M, int64_t N, int64_t K,
-                              const uint8_t* codes, const float* scales, int64_t group,
-                              const float* bias, float* y, int64_t ldy) {
-  TJH_REQUIRE_INIT();
+int fp4_linear(const float* x, int64_t ldx, int64_t M, int64_t N, int64_t K, const uint8_t* codes,
+               const float* scales, int64_t group, const float* bias, float* y, int64_t ldy,
+               const float* residual, int64_t ldr, int act) {
   TJH_ARG(M >= 0 && N >= 0 && K >= 0 && M < (int64_t(1) << 31) && N < (int64_t(1) << 31) &&
               K < (int64_t(1) << 30) && ldx >= K && ldy >= N,
           "tjh_fp4_linear: bad sizes");
@@ -529,9 +535,19 @@ extern "C" int tjh_fp4_linear(const float* x, int64_t ldx, int64_t M, int64_t N,
   if (M == 0 || N == 0) return TJH_OK;
   TJH_ARG(y && (K == 0 || (x && codes && scales && aligned16(codes))),
           "tjh_fp4_linear: NULL or unaligned pointer");
-  LinArgs a{x, nullptr, codes, scales, bias, y, ldx, ldy, M, N, K, (int)cdiv(K, 128), 0, 0};
+  LinArgs a{x,   nullptr, codes, scales, bias, residual, y, ldx, ldy, ldr, M, N, K,
+            (int)cdiv(K, 128), 0, 0, act};
   KernelScope ks("fp4_linear");
   if (group == 32) return product<32>(a);
   if (group == 64) return product<64>(a);
   return product<128>(a);
+}
+
+}  // namespace tjh
+
+extern "C" int tjh_fp4_linear(const float* x, int64_t ldx, int64_t M, int64_t N, int64_t K,
+                              const uint8_t* codes, const float* scales, int64_t group,
+                              const float* bias, float* y, int64_t ldy) {
+  TJH_REQUIRE_INIT();
+  return tjh::fp4_linear(x, ldx, M, N, K, codes, scales, group, bias, y, ldy, nullptr, 0, 0);
 }

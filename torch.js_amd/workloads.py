@@ -15,6 +15,7 @@ import math
 import numpy as np
 
 from . import _lib as L
+from . import decode_ops
 from . import functional as F
 from . import nn
 from .tensor import (Tensor, _before_write, arange, empty, from_numpy, is_grad_enabled, no_grad,
@@ -163,61 +164,96 @@ class Block(nn.Module):
         """The block as one library call that issues the same launches (a
         decoding step's eight take 225 us of host time one by one), where no
         graph is recorded and the block is made of the plain layers in
-        float32; None anywhere else."""
+        float32, or of their 4-bit forms, with a cache of either; None
+        anywhere else."""
         at, mlp = self.attn, self.mlp
         if type(at) is not CausalSelfAttention or type(mlp) is not MLPBlock or \
                 at.window is not None:
             return None
         mods = (self.ln_1, at, at.c_attn, at.c_proj, self.ln_2, mlp, mlp.c_fc, mlp.c_proj)
-        if not (tuple(map(type, mods)) == _BLOCK_MODULES and at.fused and mlp.fused and
-                x.ndim == 3 and x.dtype == "float32"):
+        kinds = tuple([nn.Linear if type(m) is nn.LinearFP4 else type(m) for m in mods])
+        if not (kinds == _BLOCK_MODULES and at.fused and mlp.fused and x.ndim == 3 and
+                x.dtype == "float32"):
             return None
         if any(k in m.__dict__ for m in mods for k in ("forward", "forward_cached", "_project")):
             return None
         B, T, C = x.shape
-        hd, hid = C // at.heads, mlp.c_fc.weight.shape[0]
+        hd = C // at.heads
+        hid = mlp.c_fc.out_features if type(mlp.c_fc) is nn.LinearFP4 else mlp.c_fc.weight.shape[0]
         ln = ((C,), (C,))
         if not (x.numel() and C == at.d and C % at.heads == 0 and hd % 4 == 0 and
                 hid % 4 == 0 and self.ln_1.normalized_shape == (C,) and
                 self.ln_2.normalized_shape == (C,) and x.is_contiguous()):
             return None
-        w = []
+        w, scales, groups = [], [], []
         for m, shapes in ((mods[0], ln), (mods[2], ((3 * C, C), (3 * C,))),
                           (mods[3], ((C, C), (C,))), (mods[4], ln),
                           (mods[6], ((hid, C), (hid,))), (mods[7], ((C, hid), (C,)))):
-            for t, shape in zip((m.weight, m.bias), shapes):
+            held = type(m) is nn.LinearFP4
+            if held:
+                try:
+                    n, codes, sc = decode_ops._weights("block_infer", m.codes, m.scales,
+                                                       shapes[0][1], m.group_size)
+                except (TypeError, ValueError):
+                    return None
+                if n != shapes[0][0]:
+                    return None
+                w.append(codes)
+                scales.append(sc)
+                groups.append(m.group_size)
+            elif len(shapes[0]) == 2:
+                scales.append(None)
+                groups.append(0)
+            for t, shape in [(m.bias, shapes[1])] if held else zip((m.weight, m.bias), shapes):
                 if t is None:  # a bias, or a norm without weights
                     w.append(None)
                     continue
                 if t.shape != shape or t.dtype != "float32" or not t.is_contiguous():
                     return None
                 w.append(t.data_ptr())
-        kc = vc = None
+        kc = vc = four = None
         max_len = 0
         if cache is not None:
-            if type(cache) is not KVCache or "append" in cache.__dict__ or pos < 0 or \
-                    (pos and T != 1):
+            four = type(cache) is KVCacheFP4
+            if type(cache) not in (KVCache, KVCacheFP4) or "append" in cache.__dict__ or \
+                    "attend" in cache.__dict__ or pos < 0 or (pos and T != 1 and not four):
                 return None
             kc, vc = cache.k[layer], cache.v[layer]
             max_len = cache.max_len
-            for t in (kc, vc):
-                if t.shape != (B, at.heads, max_len, hd) or t.dtype != "float32" or \
-                        not t.is_contiguous() or t.requires_grad:
-                    return None
             if pos + T > max_len:
                 return None
+            if four:
+                if hd > 128:
+                    return None
+                try:
+                    ks, vs = [decode_ops._cache("block_infer", c, s, hd)
+                              for c, s in ((kc, cache.k_scales[layer]), (vc, cache.v_scales[layer]))]
+                except (TypeError, ValueError):
+                    return None
+                if ks[0] != (B, at.heads, max_len) or vs[0] != ks[0]:
+                    return None
+                _before_write(kc, vc, cache.k_scales[layer], cache.v_scales[layer])
+            else:
+                for t in (kc, vc):
+                    if t.shape != (B, at.heads, max_len, hd) or t.dtype != "float32" or \
+                            not t.is_contiguous() or t.requires_grad:
+                        return None
+                _before_write(kc, vc)
         px = x.data_ptr()
         ptrs = w + [px] if cache is None else w + [px, kc.data_ptr(), vc.data_ptr()]
         if any(p is not None and p & 15 for p in ptrs):
             return None
-        if cache is not None:
-            _before_write(kc, vc)
         y = empty((B, T, C))
-        rc = L.lib().tjh_block_infer(
-            px, y.data_ptr(), (ctypes.c_void_p * 12)(*w), B, T, C, at.heads, hid,
-            float(self.ln_1.eps), float(self.ln_2.eps), 1.0 / math.sqrt(hd),
-            kc.data_ptr() if kc is not None else None, vc.data_ptr() if vc is not None else None,
-            max_len, pos)
+        ws = (ctypes.c_void_p * 12)(*w)
+        sizes = (B, T, C, at.heads, hid, float(self.ln_1.eps), float(self.ln_2.eps),
+                 1.0 / math.sqrt(hd))
+        fc = (None, None) if kc is None or four else (kc.data_ptr(), vc.data_ptr())
+        if four or any(groups):
+            qc = (ks[1], ks[2], vs[1], vs[2]) if four else (None,) * 4
+            rc = L.lib().tjh_block_infer_fp4(px, y.data_ptr(), ws, (ctypes.c_void_p * 4)(*scales),
+                                             L.i64arr(groups), *sizes, *fc, *qc, max_len, pos)
+        else:
+            rc = L.lib().tjh_block_infer(px, y.data_ptr(), ws, *sizes, *fc, max_len, pos)
         if rc == L.ERR_OOM:  # no room for the workspace in one piece
             return None
         L.check(rc, "block_infer")
