@@ -86,7 +86,7 @@ def test_quantized_model(torch, group):
 
 @pytest.mark.parametrize("bits", [32, 4])
 @pytest.mark.parametrize("held", ["", "c_attn c_proj c_fc mlp", "c_fc", "c_proj"])
-@pytest.mark.parametrize("B,T,C,heads", [(1, 1, 64, 2), (2, 37, 96, 3), (7, 20, 160, 2)])
+@pytest.mark.parametrize("B,T,C,heads", [(1, 1, 64, 2), (2, 37, 96, 3), (7, 20, 160, 2), (8, 300, 256, 4)])
 def test_block_is_one_call(torch, monkeypatch, bits, held, B, T, C, heads):
     """Without a gradient a block with layers or a cache in 4 bits is one call,
     with bit for bit the values and the cache of its layers one by one; a layer
