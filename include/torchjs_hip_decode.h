@@ -38,7 +38,7 @@ int tjh_fp4_dequantize(const uint8_t* codes, const float* scales, int64_t N, int
                        int64_t group, float* out, int64_t ldo);
 /* y [M, N] (row stride ldy) = x [M, K] (row stride ldx) times the transpose of
  * such weights, plus bias [N] (or NULL); sums are float32.  y does not overlap
- * x.  N and M below 2^31, K below 2^30. */
+ * x.  M below 2^31, N and K below 2^26. */
 int tjh_fp4_linear(const float* x, int64_t ldx, int64_t M, int64_t N, int64_t K,
                    const uint8_t* codes, const float* scales, int64_t group, const float* bias,
                    float* y, int64_t ldy);

@@ -280,6 +280,55 @@ def test_linear_gradients(torch, m, k, n):
 
 
 @gpu
+def test_linear_of_more_rows_than_are_split_at_once(torch):
+    """A GB of x's parts: the rows before and behind its end."""
+    rng = np.random.default_rng(0)
+    m, k, n = 1398144 + 70, 128, 70
+    w = _weight(rng, n, k)
+    codes, scales = torch.functional.quantize_fp4(torch.tensor(w))
+    v = held_weight(w, 64)[2]
+    torch.manual_seed(1)
+    x = torch.randn(m, k)
+    y = torch.functional.linear_fp4(x, codes, scales)
+    for a, b in ((0, 100), (m - 200, m), (m // 2, m // 2 + 50)):
+        xs, ys = x[a:b].numpy().astype(np.float64), y[a:b].numpy()
+        tol = (64 + k / 32 + 52) * U * (np.abs(xs) @ np.abs(v.T))
+        assert (np.abs(ys - xs @ v.T) <= tol).all()
+
+
+@gpu
+def test_linear_gradients_in_a_graph(torch):
+    """A captured forward and backward beside a graph of the same leaves that
+    is still alive; replays follow new values."""
+    F, rng = torch.functional, np.random.default_rng(3)
+    codes, scales = F.quantize_fp4(torch.tensor(_weight(rng, 48, 100)))
+    x, b = torch.randn(9, 100, requires_grad=True), torch.randn(48, requires_grad=True)
+
+    def loss():
+        y = F.linear_fp4(x, codes, scales, b)
+        return (y * y).sum()
+
+    def grads():
+        x.grad = b.grad = None
+        loss().backward()
+        return x.grad, b.grad
+    grads()
+    alive = loss()
+    g = torch.hip.Graph()
+    with torch.hip.graph(g):
+        captured = grads()
+    for i in range(3):
+        with torch.no_grad():
+            x.copy_(torch.randn(9, 100))
+        g.replay()
+        got = [t.numpy().copy() for t in captured]
+        for a, w in zip(got, grads()):
+            assert (a == w.numpy()).all()
+    alive.backward()
+    g.reset()
+
+
+@gpu
 def test_linear_module(torch):
     torch.manual_seed(3)
     nn = torch.nn
@@ -391,6 +440,9 @@ def test_append_where_each_sequence_ends(torch):
                     want[i, :, pos[i] + j] = scale[i, :, j]
                     rows[i, :, pos[i] + j] = packed_rows(code)[i, :, j]
         assert (scales.numpy() == want).all() and (codes.numpy() == rows).all()
+    other = _new_cache(torch, b, h, n, d, 9)
+    F.cache_append_fp4(*other, torch.tensor(k), torch.tensor(v), [int(p) for p in pos])
+    assert all((x.numpy() == y.numpy()).all() for x, y in zip(other, cache))
 
 
 def _filled(torch, b, hkv, n, d, rng, spread=1.0):

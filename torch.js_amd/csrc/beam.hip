@@ -336,6 +336,14 @@ int tjh_cache_reorder(int n, void* const* tensors, const int64_t* outers, const 
     TJH_ARG(outers[i] >= 0 && sizes[i] >= 0 && strides[i] >= sizes[i] &&
                 (tensors[i] || outers[i] * sizes[i] == 0),
             "tjh_cache_reorder: bad tensor %d", i);
+  // all of them before the first launch: a call moves everything or nothing
+  const auto unit_of = [&](int i) {
+    const uint64_t bits = (uint64_t)(uintptr_t)tensors[i] | (uint64_t)strides[i] | (uint64_t)sizes[i];
+    return (bits & 15) == 0 ? 16 : (bits & 3) == 0 ? 4 : 1;
+  };
+  for (int i = 0; i < n; ++i)
+    TJH_ARG(cdiv(sizes[i] / unit_of(i), 256) * outers[i] < (int64_t(1) << 23),
+            "tjh_cache_reorder: tensor %d is too large", i);
   KernelScope ks("cache_reorder");
   int i = 0;
   while (i < n) {
@@ -349,11 +357,9 @@ int tjh_cache_reorder(int n, void* const* tensors, const int64_t* outers, const 
       t.p = static_cast<char*>(tensors[i]);
       t.row = outers[i] * strides[i];
       t.stride = strides[i];
-      const uint64_t bits = (uint64_t)(uintptr_t)t.p | (uint64_t)strides[i] | (uint64_t)sizes[i];
-      t.unit = (bits & 15) == 0 ? 16 : (bits & 3) == 0 ? 4 : 1;
+      t.unit = unit_of(i);
       t.units = sizes[i] / t.unit;
       const int64_t per = cdiv(t.units, 256);
-      TJH_ARG(per * outers[i] < (int64_t(1) << 23), "tjh_cache_reorder: tensor %d is too large", i);
       if (groups + per * outers[i] >= (int64_t(1) << 23)) break;  // the next launch's
       t.per = (int)per;
       t.first = (int)groups;

@@ -526,6 +526,20 @@ void launch_gemm(const LinArgs& a) {
 
 template <int G>
 int many_rows(LinArgs a) {
+  // a GB of parts at a time: long prompts in pieces of rows
+  const int64_t piece = ((int64_t(1) << 30) / (a.nb * 128 * 6) / 128 + 1) * 128;
+  if (a.M > piece) {
+    LinArgs b = a;
+    for (int64_t m = 0; m < a.M; m += piece) {
+      b.M = a.M - m < piece ? a.M - m : piece;
+      b.x = a.x + m * a.ldx;
+      b.y = a.y + m * a.ldy;
+      if (a.residual) b.residual = a.residual + m * a.ldr;
+      const int rc = many_rows<G>(b);
+      if (rc != TJH_OK) return rc;
+    }
+    return TJH_OK;
+  }
   a.m_tiles = (int)cdiv(a.M, 128) * 8;
   const int64_t items = (int64_t)a.m_tiles * a.nb * 4 * 64, rows = a.m_tiles / 8;
   TJH_ARG(cdiv(items, 256) < (1 << 23) && cdiv(a.N, 64) * rows < (1 << 23),
@@ -559,8 +573,8 @@ int product(const LinArgs& a) {
 int fp4_linear(const float* x, int64_t ldx, int64_t M, int64_t N, int64_t K, const uint8_t* codes,
                const float* scales, int64_t group, const float* bias, float* y, int64_t ldy,
                const float* residual, int64_t ldr, int act) {
-  TJH_ARG(M >= 0 && N >= 0 && K >= 0 && M < (int64_t(1) << 31) && N < (int64_t(1) << 31) &&
-              K < (int64_t(1) << 30) && ldx >= K && ldy >= N,
+  TJH_ARG(M >= 0 && N >= 0 && K >= 0 && M < (int64_t(1) << 31) && N < (int64_t(1) << 26) &&
+              K < (int64_t(1) << 26) && ldx >= K && ldy >= N,
           "tjh_fp4_linear: bad sizes");
   TJH_ARG(group == 32 || group == 64 || group == 128,
           "tjh_fp4_linear: groups of %lld columns (32, 64 or 128)", (long long)group);

@@ -193,7 +193,7 @@ def _per_sequence(who, name, value, b):
             a = np.asarray(value)
             if a.dtype.kind not in "iu":
                 raise TypeError("%s: %s must be whole numbers" % (who, name))
-            t = _T.tensor(np.clip(a, -1, 2 ** 31 - 1).astype(np.int32), dtype="int32")
+            t = _T.tensor(np.clip(a, -2 ** 31, 2 ** 31 - 1).astype(np.int32), dtype="int32")
         if t.dtype != "int32":
             raise TypeError("%s: %s must be an int32 tensor, got %s" % (who, name, t.dtype))
         if t.shape != (b,):

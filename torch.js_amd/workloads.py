@@ -171,9 +171,11 @@ class Block(nn.Module):
                 at.window is not None:
             return None
         mods = (self.ln_1, at, at.c_attn, at.c_proj, self.ln_2, mlp, mlp.c_fc, mlp.c_proj)
-        kinds = tuple([nn.Linear if type(m) is nn.LinearFP4 else type(m) for m in mods])
-        if not (kinds == _BLOCK_MODULES and at.fused and mlp.fused and x.ndim == 3 and
-                x.dtype == "float32"):
+        kinds = tuple(map(type, mods))
+        if kinds != _BLOCK_MODULES:  # some layers in 4 bits?
+            if tuple([nn.Linear if k is nn.LinearFP4 else k for k in kinds]) != _BLOCK_MODULES:
+                return None
+        if not (at.fused and mlp.fused and x.ndim == 3 and x.dtype == "float32"):
             return None
         if any(k in m.__dict__ for m in mods for k in ("forward", "forward_cached", "_project")):
             return None
@@ -189,8 +191,8 @@ class Block(nn.Module):
         for m, shapes in ((mods[0], ln), (mods[2], ((3 * C, C), (3 * C,))),
                           (mods[3], ((C, C), (C,))), (mods[4], ln),
                           (mods[6], ((hid, C), (hid,))), (mods[7], ((C, hid), (C,)))):
-            held = type(m) is nn.LinearFP4
-            if held:
+            ts = (m.bias,) if type(m) is nn.LinearFP4 else (m.weight, m.bias)
+            if len(ts) == 1:
                 try:
                     n, codes, sc = decode_ops._weights("block_infer", m.codes, m.scales,
                                                        shapes[0][1], m.group_size)
@@ -201,10 +203,11 @@ class Block(nn.Module):
                 w.append(codes)
                 scales.append(sc)
                 groups.append(m.group_size)
-            elif len(shapes[0]) == 2:
+                shapes = shapes[1:]
+            elif shapes is not ln:
                 scales.append(None)
                 groups.append(0)
-            for t, shape in [(m.bias, shapes[1])] if held else zip((m.weight, m.bias), shapes):
+            for t, shape in zip(ts, shapes):
                 if t is None:  # a bias, or a norm without weights
                     w.append(None)
                     continue
