@@ -40,6 +40,23 @@ __device__ __forceinline__ float exp_near(float x) {
   return x > -100.f ? __builtin_fmaf(e, low * kLn2, e) : x == x ? 0.f : x;
 }
 
+// A bound that a piece's k largest elements are not below, for small k: the k-th
+// largest of a wave's 64 threads' maxima `top`, to the 16 high bits of its key
+// (-infinity where fewer of them are above -infinity).  No barrier; the largest of
+// the waves' bounds leaves some ten of the k more than a bound over all threads
+// would, which takes eight barriers.
+constexpr int kWaveBound = 16;
+__device__ __forceinline__ float wave_bound(float top, int k) {
+  const uint32_t key = order_key(top);
+  uint32_t lo = 0;
+#pragma unroll
+  for (int bit = 31; bit >= 16; --bit) {
+    const uint32_t c = lo | (1u << bit);
+    if (__popcll(__ballot(key >= c)) >= k) lo = c;
+  }
+  return lo > 0x007fffffu ? key_value(lo) : -INFINITY;  // 0x007fffff: the key of -infinity
+}
+
 // A piece of a row: `per` columns, fewer at the end.  Bound for many rows by
 // reading them and then selecting, in step on all CUs: 256 rows of 50257 (51 MB)
 // 20 us, 12.5 of them without the selection; for few by latency, 7 us.
@@ -54,12 +71,23 @@ __global__ __launch_bounds__(T, T == 512 ? 4 : 1) void k_beam_pieces(BeamArgs a)
   row.load(a.x + r * a.ld + c0, n, 0, true);
   float m = -INFINITY, sum = 0.f;
   row.each([&](int, int, float x) { m = fmaxf(m, x); });  // NaN takes no part here,
-  m = b.max(m);
+  const int k = min(a.keep, n);
+  float bound = k <= kWaveBound ? wave_bound(m, k) : -INFINITY;
+  {
+    // both at once, as (larger first) halves
+    u64 v = ((u64)order_key(wave_max(m)) << 32) | order_key(bound);
+    v = b.across(v, [](u64 x, u64 y) {
+      const uint32_t h = max((uint32_t)(x >> 32), (uint32_t)(y >> 32));
+      return ((u64)h << 32) | max((uint32_t)x, (uint32_t)y);
+    });
+    m = key_value((uint32_t)(v >> 32));
+    bound = key_value((uint32_t)v);
+  }
   const float from = m == -INFINITY ? 0.f : m;
   row.each([&](int, int, float x) { sum += exp_near(x - from); });  // but in the sum
   sum = b.sum(sum);
-  const int k = min(a.keep, n);
-  const u64* best = select_largest(row, k, kNanFirst, s, b);
+  if (bound == -INFINITY) bound = kth_bound(row, k, b);
+  const u64* best = select_above(row, k, bound, kNanFirst, s, b);
   u64* to = a.cand + blockIdx.x * (int64_t)a.keep;
   for (int i = threadIdx.x; i < k; i += T) {
     const u64 c = best[i];

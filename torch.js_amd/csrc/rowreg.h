@@ -573,13 +573,13 @@ __device__ __forceinline__ float kth_bound(const Row<T, NV>& row, int k, Block<T
 }
 
 // The row's k largest elements in order, 1 <= k <= min(n, CAP): where they
-// stand.
+// stand, given a bound that they are not below.
 // Where more than CAP elements are above the bound (ties), the exact one
 // comes from bisection.
 template <int T, int NV, int CAP>
-__device__ __forceinline__ u64* select_largest(const Row<T, NV>& row, int k, uint32_t nan,
-                                               SelectLds<T, CAP>& s, Block<T>& b) {
-  const int c = gather_above(row, nan, kth_bound(row, k, b), s);
+__device__ __forceinline__ u64* select_above(const Row<T, NV>& row, int k, float bound,
+                                             uint32_t nan, SelectLds<T, CAP>& s, Block<T>& b) {
+  const int c = gather_above(row, nan, bound, s);
   if (c > CAP) {
     Row<T, 0> again;
     again.load(row.p, row.n, row.sign);
@@ -592,6 +592,12 @@ __device__ __forceinline__ u64* select_largest(const Row<T, NV>& row, int k, uin
         s);
   }
   return sort_list(s, c > CAP ? k : c);
+}
+
+template <int T, int NV, int CAP>
+__device__ __forceinline__ u64* select_largest(const Row<T, NV>& row, int k, uint32_t nan,
+                                               SelectLds<T, CAP>& s, Block<T>& b) {
+  return select_above(row, k, kth_bound(row, k, b), nan, s, b);
 }
 
 }  // namespace rowreg
