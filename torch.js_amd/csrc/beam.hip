@@ -59,7 +59,7 @@ __device__ __forceinline__ float wave_bound(float top, int k) {
 
 // A piece of a row: `per` columns, fewer at the end.  Bound for many rows by
 // reading them and then selecting, in step on all CUs: 256 rows of 50257 (51 MB)
-// 20 us, 12.5 of them without the selection; for few by latency, 7 us.
+// 16.5 us, 12.5 of them without the selection; for few by latency, 6 us.
 template <int T, int NV, int CAP>
 __global__ __launch_bounds__(T, T == 512 ? 4 : 1) void k_beam_pieces(BeamArgs a) {
   __shared__ SelectLds<T, CAP> s;
