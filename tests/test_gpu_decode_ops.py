@@ -726,6 +726,24 @@ def test_reorder_whole_rows_and_many_tensors(torch):
     assert (big.numpy()[4:] == _reordered(x[4:], parents[:1], None)).all()
 
 
+@gpu
+def test_numbers_past_32_bits_are_taken_as_they_are(torch):
+    """Parents of 2^32 are outside [0, W), not 0; a library caller's -2^32 is no
+    token, not the token 0."""
+    x = np.arange(6, dtype=np.float32).reshape(3, 2)
+    t = torch.tensor(x)
+    torch.functional.cache_reorder_(t, np.array([[1, 2 ** 32, -2 ** 32]]))
+    assert (t.numpy() == x[[1, 1, 2]]).all()
+    logits, scores = torch.tensor(np.float32([[2, 1, 0]])), torch.zeros(1, 1)
+    s, d = torch.zeros(1, 2), torch.zeros(1, 2, dtype="uint8")
+    tok, par = torch.zeros(1, 2, dtype="int32"), torch.zeros(1, 2, dtype="int32")
+    lib = torch._lib
+    lib.check(lib.lib().tjh_beam_step(logits.data_ptr(), 3, scores.data_ptr(), None, 1, 1, 3, 2,
+                                      -2 ** 32, s.data_ptr(), tok.data_ptr(), par.data_ptr(),
+                                      d.data_ptr()), "beam_step")
+    assert tok.numpy().tolist() == [[0, 1]] and d.numpy().tolist() == [[0, 0]]
+
+
 # ------------------------------------------------------------------- graphs
 
 

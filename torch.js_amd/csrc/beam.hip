@@ -325,7 +325,7 @@ int tjh_beam_step(const float* logits, int64_t ld, const float* scores, const ui
     }
   }
   BeamArgs a{logits, scores, finished, nullptr, nullptr, out_scores, tokens, parents, out_finished,
-             ld, (int)W, (int)V, (int)cdiv(V, per), per, (int)keep, (int)eos};
+             ld, (int)W, (int)V, (int)cdiv(V, per), per, (int)keep, eos < 0 ? -1 : (int)eos};
   const int64_t pieces = rows * a.S;
   TJH_ARG(pieces < (1 << 21), "tjh_beam_step: too many searches");
   Scratch s((size_t)pieces * (sizeof(float2) + keep * sizeof(u64)));

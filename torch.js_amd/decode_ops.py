@@ -103,8 +103,9 @@ def dequantize_fp4(codes, scales, in_features, group_size=64):
 
 def linear_fp4(x, codes, scales, bias=None, group_size=64):
     """y = x W^T + b for x [..., K] and the 4-bit weight [N, K] of
-    quantize_fp4, summed in float32.  The gradient goes to x (through the float
-    weight, formed for it) and to bias; the weight has none."""
+    quantize_fp4, summed in float32 (a group before its scale: for x under 2^118 in
+    magnitude).  The gradient goes to x (through the float weight, formed for it)
+    and to bias; the weight has none."""
     g = _group("linear_fp4", group_size)
     if not x._shape:
         raise ValueError("linear_fp4: x has no dimensions")
@@ -278,8 +279,9 @@ def attention_fp4(query, k_codes, k_scales, v_codes, v_scales, length, scale=Non
     positions (already in the cache), or of length[b] of sequence b (an int32
     tensor [B], taken into [0, L]); one that sees no key, before the first
     position, gives zeros.  What later positions hold has no part in the result.
-    Sums are float32; D up to 128.  For inference: a query that needs a gradient
-    is refused."""
+    Sums are float32 (a key's before its scale: for queries under 2^118 in
+    magnitude); D up to 128.  For inference: a query that needs a gradient is
+    refused."""
     who = "attention_fp4"
     qs = query._shape
     if len(qs) != 4:
@@ -395,7 +397,7 @@ def cache_reorder_(tensors, parents, length=None):
         a = np.asarray(parents)
         if a.dtype.kind not in "iu":
             raise TypeError("%s: parents must be whole numbers" % who)
-        parents = _T.tensor(a.astype(np.int32), dtype="int32")
+        parents = _T.tensor(np.clip(a, -2 ** 31, 2 ** 31 - 1).astype(np.int32), dtype="int32")
     if parents.dtype != "int32":
         raise TypeError("%s: parents must be int32, got %s" % (who, parents.dtype))
     if parents.ndim != 2:
