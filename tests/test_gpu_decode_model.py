@@ -134,6 +134,38 @@ def test_block_is_one_call(torch, monkeypatch, bits, held, B, T, C, heads):
             assert calls[-1] is None
 
 
+@pytest.mark.parametrize("B,T", [(9, 1), (2, 8), (3, 17)])
+def test_block_with_sums_in_slices(torch, monkeypatch, B, T):
+    """The same where the MLP's last layer has 8192 columns, whose slices are added
+    up before the residual, and replayed in a graph beside another one's workspace."""
+    from torchjs_amd import workloads as W
+    nn = torch.nn
+    torch.manual_seed(6)
+    blk = W.Block(2048, 16)
+    blk.mlp.c_fc = nn.LinearFP4.of(blk.mlp.c_fc)
+    blk.mlp.c_proj = nn.LinearFP4.of(blk.mlp.c_proj)
+    x = torch.randn(B, T, 2048)
+    graphs, outs = [torch.hip.Graph(), torch.hip.Graph()], []
+    with torch.no_grad():
+        blk(x)
+        for g in graphs:
+            with torch.hip.graph(g):
+                outs.append(blk(x))
+        for i in range(3):
+            for g, out in zip(graphs, outs):
+                x.copy_(torch.randn(B, T, 2048))
+                want = blk(x).numpy()
+                g.replay()
+                assert np.array_equal(out.numpy(), want)
+        x.copy_(torch.tensor(np.random.default_rng(2).standard_normal((B, T, 2048)).astype(np.float32)))
+        got = blk(x).numpy()
+        with monkeypatch.context() as m:
+            m.setattr(W.Block, "_infer", lambda self, *a: None)
+            assert np.array_equal(got, blk(x).numpy())
+    for g in graphs:
+        g.reset()
+
+
 @pytest.mark.parametrize("parts", [(30,), (1,), (7, 1, 20), (33, 5)])
 def test_cached_positions(torch, parts):
     """Each call's logits are those of explicit attention over what the cache

@@ -205,6 +205,32 @@ def test_linear(torch, m, k, n, group):
     assert (np.abs(y.numpy() - want) <= tol).all()
 
 
+# some rows by every width and height of tiles, with x cut beforehand or not, and
+# with the columns of x in slices: tiles 16 high by 16, 32, 64 wide, 32 and 64 high,
+# rows that do not fill the last one, slices of unlike lengths, K inside a block
+SOME = [(9, 500, 2000), (9, 500, 6001), (9, 301, 12000), (9, 301, 17000), (40, 300, 5000),
+        (31, 300, 16500), (50, 297, 16000), (6, 4003, 50), (3, 9000, 40), (1, 31993, 17),
+        (7, 8200, 300), (40, 2100, 300), (33, 1153, 1000), (60, 16000, 500), (100, 16001, 1000),
+        (300, 16000, 1000), (700, 5000, 70)]
+
+
+@gpu
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m,k,n", SOME)
+def test_linear_of_some_rows(torch, m, k, n, group):
+    x, b, codes, scales, want, tol = _linear_case(torch, m, k, n, group, n % 2 == 0, 3)
+    tx, tb = torch.tensor(x), torch.tensor(b) if b is not None else None
+    y = torch.functional.linear_fp4(tx, codes, scales, tb, group).numpy()
+    # as in test_linear; a wave's and a slice's sums are fewer than there
+    assert (np.abs(y - want) <= tol).all()
+    again = torch.functional.linear_fp4(tx, codes, scales, tb, group).numpy()
+    assert np.array_equal(y, again)
+    # rows of a wider tensor, and a row's result does not go by its place
+    wide = torch.tensor(np.concatenate([np.full((m, 1), np.nan, np.float32), x[::-1]], 1))
+    y2 = torch.functional.linear_fp4(wide[:, 1:], codes, scales, tb, group).numpy()
+    assert np.array_equal(y2[::-1], y)
+
+
 @gpu
 @pytest.mark.parametrize("m", [2, 9, 70])
 def test_linear_takes_rows_where_they_stand(torch, m):

@@ -10,10 +10,10 @@
 // sums are scaled and added up in floats.  An error of 6e-8 to 1.4e-7 against 64
 // bits (2-norm), a fifth of a float matrix product's with the same weights.
 //
-// Three kernels, by the rows of x:
+// Three kernels, by the rows of x (product() below):
 //   up to 5    k_fp4_rows    bound by reading the weights and by latency
-//   some       k_fp4_chunks  32 rows at a time, latency of a chain of steps
-//   many       k_fp4_gemm    the bf16 matrix cores
+//   some       k_fp4_some    by latency of a chain of steps, by forming x's parts
+//   many       k_fp4_gemm    by the bf16 matrix cores
 #include "fp4.h"
 #include "ops_math.h"
 
@@ -32,9 +32,10 @@ struct LinArgs {
   float* y;
   int64_t ldx, ldy, ldr, M, N, K;
   int nb;       // blocks of 128 columns
-  int rows;     // of x a workgroup takes (grid y of k_fp4_chunks)
-  int m_tiles;  // 16 rows each (k_fp4_gemm)
+  int m_tiles;  // 16 rows each, of `parts`
   int act;      // 1: GELU, 3: plus residual
+  float* sums;  // [slices, M, N] of k_fp4_some, or NULL
+  int per;      // blocks of a slice
 };
 
 // The end of an element of y.
@@ -76,31 +77,6 @@ __device__ __forceinline__ floatx4 scales_of(const float* __restrict__ s) {
 }
 
 // ----------------------------------------------------------------- few rows
-
-// Parts of x's rows as k_fp4_chunks takes them: for each chunk of R rows, each 32
-// columns and each 16 of its 3 R (part, row) pairs, part by part, a matrix
-// operand: lane (j, i) has pair i and columns 8 j to 8 j + 7.
-__global__ __launch_bounds__(256) void k_fp4_split_rows(const float* __restrict__ x, int64_t ldx,
-                                                        int64_t M, int64_t K, uint32_t R, int MT,
-                                                        uint32_t kb, uint32_t items,
-                                                        uintx4* __restrict__ parts) {
-  const uint32_t at = blockIdx.x * 256 + threadIdx.x;
-  if (at >= items) return;
-  // (chunk, 32 columns, 8 of them, row)
-  const uint32_t row8 = at / R, fu = row8 >> 2;
-  const int r = (int)(at - row8 * R), j = (int)(row8 & 3);
-  const int64_t f = fu, chunk = fu / kb, k32 = fu % kb;
-  const int64_t m = chunk * R + r;
-  float v[8];
-  load8(x + (m < M ? m : M - 1) * ldx, 32 * k32 + 8 * j, K, v);
-  bf16x8 p[3];
-  split8(v, p);
-#pragma unroll
-  for (int i = 0; i < 3; ++i) {
-    const int pair = i * R + r;
-    parts[(f * MT + (pair >> 4)) * 64 + 16 * j + (pair & 15)] = __builtin_bit_cast(uintx4, p[i]);
-  }
-}
 
 // Up to five rows of x: a matrix operand's 16 rows are (part, row) pairs.  A
 // workgroup's eight waves have 8 / KS tiles of 16 columns of y; KS of them share
@@ -212,142 +188,10 @@ int few_rows(const LinArgs& a) {
   return check_launch("fp4_rows");
 }
 
-// Some more rows, in chunks of at most 32: a wave has the (part, row) pairs of a
-// chunk, MT operands of 16, and 16 NT columns of y; the eight waves of a workgroup
-// share the columns of x by blocks of 128 and add up through LDS.  x's parts come
-// from memory as lanes feed them, a step of 32 columns ahead, codes a block ahead.
-//
-// Bound by the latency of a wave's steps while the workgroups fit the CUs, by
-// loading the parts (a KB for each NT products) after that: 32 rows, 4096 x 4096
-// 23 us, 16384 x 4096 27 us; with the parts through LDS, a barrier and an exposed
-// load for each two blocks, 51 and 56.
-template <int G, int MT, int NT>
-__global__ __launch_bounds__(64 * kWaves, 2) void k_fp4_chunks(LinArgs a) {
-  __shared__ float red[kWaves][MT * 16][16];
-  const int lane = threadIdx.x & 63, c = lane & 15, j = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t m0 = (int64_t)blockIdx.y * a.rows, n0 = (int64_t)blockIdx.x * 16 * NT;
-  const int R = (int)(a.M - m0 < a.rows ? a.M - m0 : a.rows);
-  const uint8_t* __restrict__ cp[NT];
-  const float* __restrict__ sp[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int64_t n = n0 + 16 * t + c < a.N ? n0 + 16 * t + c : a.N - 1;
-    cp[t] = a.codes + n * a.nb * 64 + 16 * j;
-    sp[t] = a.scales + n * a.nb * (128 / G);
-  }
-  const uintx4* __restrict__ xp = a.parts + (int64_t)blockIdx.y * a.nb * 4 * MT * 64 + lane;
-  floatx4 acc[MT][NT], s[NT], snext[NT];
-  uintx4 code[NT], cnext[NT], x[MT], xn[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int t = 0; t < NT; ++t) acc[i][t] = floatx4{0.f, 0.f, 0.f, 0.f};
-  const auto load_w = [&](int b) {
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      cnext[t] = *reinterpret_cast<const uintx4*>(cp[t] + (int64_t)b * 64);
-      snext[t] = scales_of<G>(sp[t] + b * (128 / G));
-    }
-  };
-  const auto load_x = [&](int k32) {
-#pragma unroll
-    for (int i = 0; i < MT; ++i) xn[i] = xp[((int64_t)k32 * MT + i) * 64];
-  };
-  if (w < a.nb) {
-    load_w(w);
-    load_x(4 * w);
-  }
-  for (int b = w; b < a.nb; b += kWaves) {
-    const int bn = b + kWaves < a.nb ? b + kWaves : b;  // the last block is loaded twice
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      code[t] = cnext[t];
-      s[t] = snext[t];
-    }
-    load_w(bn);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-#pragma unroll
-      for (int i = 0; i < MT; ++i) x[i] = xn[i];
-      load_x(u < 3 ? 4 * b + u + 1 : 4 * bn);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const bf16x8 wb = steps(code[t][u]);
-        floatx4 p[MT];
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-          p[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x[i]), wb,
-                                                         floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            acc[i][t][r] = __builtin_fmaf(s[t][u], p[i][r], acc[i][t][r]);
-      }
-    }
-  }
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    if (t) __syncthreads();
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) red[w][16 * i + 4 * j + r][c] = acc[i][t][r];
-    __syncthreads();
-    for (int o = threadIdx.x; o < R * 16; o += 64 * kWaves) {
-      const int m = o >> 4, col = o & 15;
-      const int64_t n = n0 + 16 * t + col;
-      float v = 0.f;
-#pragma unroll
-      for (int p = 2; p >= 0; --p)
-#pragma unroll
-        for (int q = 0; q < kWaves; ++q) v += red[q][p * a.rows + m][col];
-      if (n < a.N) finish(a, m0 + m, n, v);
-    }
-  }
-}
+// ---------------------------------------------------------------- some rows
 
-template <int G, int MT>
-void launch_chunks(const LinArgs& a, int chunks) {
-  // four column tiles a wave where that leaves the CUs a workgroup each
-  const int64_t wide = cdiv(a.N, 64);
-  if (wide * chunks >= num_cus())
-    tjh_launch((k_fp4_chunks<G, MT, 4>), dim3((unsigned)wide, (unsigned)chunks), dim3(64 * kWaves),
-               0, stream(), a);
-  else
-    tjh_launch((k_fp4_chunks<G, MT, 2>), dim3((unsigned)cdiv(a.N, 32), (unsigned)chunks),
-               dim3(64 * kWaves), 0, stream(), a);
-}
-
-template <int G>
-int some_rows(LinArgs a) {
-  const int chunks = (int)cdiv(a.M, 32);
-  a.rows = (int)cdiv(a.M, chunks);
-  const int MT = (int)cdiv(3 * a.rows, 16), kb = a.nb * 4;
-  const int64_t items = (int64_t)chunks * kb * 4 * a.rows;
-  TJH_ARG(chunks < 65536 && cdiv(items, 256) < (1 << 23), "tjh_fp4_linear: too many rows");
-  Scratch s((size_t)(kb ? kb : 1) * chunks * MT * 64 * 16);
-  if (!s.ok()) return set_error(TJH_ERR_OOM, "tjh_fp4_linear: no scratch");
-  if (items)
-    tjh_launch(k_fp4_split_rows, dim3((unsigned)cdiv(items, 256)), dim3(256), 0, stream(), a.x,
-               a.ldx, a.M, a.K, (uint32_t)a.rows, MT, (uint32_t)kb, (uint32_t)items,
-               s.as<uintx4>());
-  a.parts = s.as<uintx4>();
-  switch (MT) {
-    case 2: launch_chunks<G, 2>(a, chunks); break;
-    case 3: launch_chunks<G, 3>(a, chunks); break;
-    case 4: launch_chunks<G, 4>(a, chunks); break;
-    case 5: launch_chunks<G, 5>(a, chunks); break;
-    default: launch_chunks<G, 6>(a, chunks); break;
-  }
-  return check_launch("fp4_chunks");
-}
-
-// ---------------------------------------------------------------- many rows
-
-// Parts of x for k_fp4_gemm: for each 32 columns, each 16 rows and each part a
-// matrix operand.
+// Parts of x for k_fp4_some and k_fp4_gemm: for each 32 columns, each 16 rows and
+// each part a matrix operand.
 __global__ __launch_bounds__(256) void k_fp4_split(const float* __restrict__ x, int64_t ldx,
                                                    int64_t M, int64_t K, uint32_t m_tiles,
                                                    uint32_t items, uintx4* __restrict__ parts) {
@@ -363,6 +207,225 @@ __global__ __launch_bounds__(256) void k_fp4_split(const float* __restrict__ x, 
 #pragma unroll
   for (int i = 0; i < 3; ++i) parts[(f * 3 + i) * 64 + lane] = __builtin_bit_cast(uintx4, p[i]);
 }
+
+// A wave has RT times 16 rows and NT times 16 columns of y; the eight waves of a
+// workgroup share the columns of x (a slice's of them, grid z) by blocks of 128 and
+// add up through LDS.  x comes from memory as lanes feed it, a step of 32 columns
+// ahead, codes a block ahead; PARTS: cut into its parts by a launch before, else by
+// every wave for itself, which takes 60 instructions for each 16 rows of a step.
+//
+// Bound by the latency of a wave's steps while the workgroups fit the CUs, and by
+// those instructions; by loading the parts (3 KB for 3 NT products) where there are
+// more.  8, 32 and 64 rows: 2304 x 768 4.0, 4.8 and 6.3 us, 4096 x 4096 10.6, 14.7
+// and 19, 16384 x 4096 18, 23 and 33, 50257 x 768 14, 24 and 39 us.
+template <int G, int RT, int NT, bool PARTS>
+__global__ __launch_bounds__(64 * kWaves, 2) void k_fp4_some(LinArgs a) {
+  constexpr int CT = RT * NT <= 8 ? NT : 8 / RT;  // column tiles that are added up at a time
+  __shared__ float red[kWaves][RT * 16][CT * 16 + 4];
+  const int lane = threadIdx.x & 63, c = lane & 15, j = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t m0 = (int64_t)blockIdx.y * (16 * RT), n0 = (int64_t)blockIdx.x * 16 * NT;
+  const int R = (int)(a.M - m0 < 16 * RT ? a.M - m0 : 16 * RT);
+  const uint8_t* __restrict__ cp[NT];
+  const float* __restrict__ sp[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int64_t n = n0 + 16 * t + c < a.N ? n0 + 16 * t + c : a.N - 1;
+    cp[t] = a.codes + n * a.nb * 64 + 16 * j;
+    sp[t] = a.scales + n * a.nb * (128 / G);
+  }
+  const float* __restrict__ xp[RT];
+  const uintx4* __restrict__ pp[RT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    const int64_t m = m0 + 16 * i + c, tile = m0 / 16 + i;
+    xp[i] = a.x + (m < a.M ? m : a.M - 1) * a.ldx + 8 * j;
+    pp[i] = a.parts + (tile < a.m_tiles ? tile : a.m_tiles - 1) * 192 + lane;
+  }
+  floatx4 acc[RT][NT], s[NT], snext[NT];
+  uintx4 code[NT], cnext[NT], pn[RT][3];
+  float xn[RT][8];
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[i][t] = floatx4{0.f, 0.f, 0.f, 0.f};
+  const auto load_w = [&](int b) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      cnext[t] = *reinterpret_cast<const uintx4*>(cp[t] + (int64_t)b * 64);
+      snext[t] = scales_of<G>(sp[t] + b * (128 / G));
+    }
+  };
+  const auto load_x = [&](int k32) {
+    const int64_t k0 = 32 * (int64_t)k32;
+    if (PARTS) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int q = 0; q < 3; ++q) pn[i][q] = pp[i][(int64_t)k32 * a.m_tiles * 192 + q * 64];
+    } else if (k0 + 32 <= a.K) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        const floatx4 p = *reinterpret_cast<const floatx4u*>(xp[i] + k0);
+        const floatx4 q = *reinterpret_cast<const floatx4u*>(xp[i] + k0 + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          xn[i][e] = p[e];
+          xn[i][4 + e] = q[e];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) xn[i][e] = k0 + 8 * j + e < a.K ? xp[i][k0 + e] : 0.f;
+    }
+  };
+  const int first = blockIdx.z * a.per, end = min(first + a.per, a.nb);
+  if (first + w < end) {
+    load_w(first + w);
+    load_x(4 * (first + w));
+  }
+  for (int b = first + w; b < end; b += kWaves) {
+    const int bn = b + kWaves < end ? b + kWaves : b;  // the last block is loaded twice
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      code[t] = cnext[t];
+      s[t] = snext[t];
+    }
+    load_w(bn);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      bf16x8 x[RT][3];
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        if (PARTS) {
+#pragma unroll
+          for (int q = 0; q < 3; ++q) x[i][q] = __builtin_bit_cast(bf16x8, pn[i][q]);
+        } else {
+          split8(xn[i], x[i]);
+        }
+      }
+      load_x(u < 3 ? 4 * b + u + 1 : 4 * bn);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const bf16x8 wb = steps(code[t][u]);
+        floatx4 p[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) p[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 2; q >= 0; --q)
+#pragma unroll
+          for (int i = 0; i < RT; ++i)
+            p[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i][q], wb, p[i], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            acc[i][t][r] = __builtin_fmaf(s[t][u], p[i][r], acc[i][t][r]);
+      }
+    }
+  }
+#pragma unroll
+  for (int t0 = 0; t0 < NT; t0 += CT) {
+    if (t0) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int t = 0; t < CT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) red[w][16 * i + 4 * j + r][16 * t + c] = acc[i][t0 + t][r];
+    __syncthreads();
+    for (int o = threadIdx.x; o < R * CT * 16; o += 64 * kWaves) {
+      const int m = o / (CT * 16), col = o % (CT * 16);
+      const int64_t n = n0 + 16 * t0 + col;
+      if (n >= a.N) continue;
+      float v = 0.f;
+#pragma unroll
+      for (int q = 0; q < kWaves; ++q) v += red[q][m][col];
+      if (a.sums) a.sums[(blockIdx.z * a.M + m0 + m) * a.N + n] = v;
+      else finish(a, m0 + m, n, v);
+    }
+  }
+}
+
+// The slices' sums together, always in one order.
+__global__ __launch_bounds__(256) void k_fp4_sums(LinArgs a, int slices) {
+  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x, m = blockIdx.y;
+  if (n >= a.N) return;
+  float v = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < slices; ++i) v += a.sums[(i * a.M + m) * a.N + n];
+  finish(a, m, n, v);
+}
+
+// How k_fp4_some takes some rows, and what that costs: 20 for a round of
+// workgroups of 16 x 16 of y and eight blocks of columns (1.7 us).  Wider tiles
+// cost less than their products, but fewer workgroups leave CUs idle:
+// 4096 x 4096, 8 rows by 16 columns 10.6 us, by 32 12.1; 6400 x 1600 8.7 and 6.6.
+struct Some {
+  int rt, nt;
+  int64_t slices, cost;
+  bool parts;
+};
+Some plan_some(const LinArgs& a) {
+  const struct {
+    int rt, nt, cost;
+  } tiles[] = {{1, 1, 20}, {1, 2, 25}, {1, 4, 40}, {2, 4, 54}, {4, 4, 84}};
+  const int64_t cus = num_cus(), blocks = cdiv(a.nb, kWaves);
+  Some best{4, 4, 1, INT64_MAX, true};
+  for (const auto& t : tiles) {
+    const int64_t wgs = cdiv(a.M, 16 * t.rt) * cdiv(a.N, 16 * t.nt);
+    if (t.nt < 4 && wgs > cus) continue;
+    // cut by a launch before (4 us) where that is done often: 4096 x 4096, 96 rows
+    // 22.4 us (28 without); 2304 x 768, 8 rows 7 (4.0)
+    const bool parts = t.rt > 1 || wgs > cus;
+    for (int64_t n = 1; n <= 4 && n <= blocks && (n == 1 || wgs * n <= cus); n *= 2) {
+      // adding slices up is a launch: 1000 x 8000, 8 rows 10.5 us by four and 14 by
+      // one; 4096 x 4096 12.7 and 10.6
+      const int64_t cost = cdiv(wgs * n, cus) * cdiv(blocks, n) * t.cost + (n > 1 ? 60 : 0) +
+                           (parts ? 50 : 0);
+      if (cost < best.cost) best = {t.rt, t.nt, n, cost, parts};
+    }
+  }
+  return best;
+}
+
+template <int G>
+int some_rows(LinArgs a, const Some& plan) {
+  a.m_tiles = (int)cdiv(a.M, 16);
+  a.per = (int)(cdiv(cdiv(a.nb, kWaves), plan.slices) * kWaves);
+  const int slices = a.nb ? (int)cdiv(a.nb, a.per) : 1;
+  const dim3 grid((unsigned)cdiv(a.N, 16 * plan.nt), (unsigned)cdiv(a.M, 16 * plan.rt),
+                  (unsigned)slices);
+  const dim3 block(64 * kWaves);
+  const int64_t items = plan.parts ? (int64_t)a.m_tiles * a.nb * 4 * 64 : 0;
+  const int64_t sums = slices > 1 ? slices * a.M * a.N : 0;
+  TJH_ARG(cdiv(a.M, 16 * plan.rt) < 65536 && cdiv(items, 256) < (1 << 23) &&
+              (int64_t)grid.x * grid.y < (1 << 23),
+          "tjh_fp4_linear: too many rows");
+  Scratch s((size_t)items * 48 + (size_t)sums * 4);
+  if (items || sums) {
+    if (!s.ok()) return set_error(TJH_ERR_OOM, "tjh_fp4_linear: no scratch");
+    a.parts = s.as<uintx4>();
+    if (sums) a.sums = s.as<float>() + items * 12;
+  }
+  if (items)
+    tjh_launch(k_fp4_split, dim3((unsigned)cdiv(items, 256)), dim3(256), 0, stream(), a.x, a.ldx,
+               a.M, a.K, (uint32_t)a.m_tiles, (uint32_t)items, s.as<uintx4>());
+  if (plan.rt == 4) tjh_launch((k_fp4_some<G, 4, 4, true>), grid, block, 0, stream(), a);
+  else if (plan.rt == 2) tjh_launch((k_fp4_some<G, 2, 4, true>), grid, block, 0, stream(), a);
+  else if (plan.parts) tjh_launch((k_fp4_some<G, 1, 4, true>), grid, block, 0, stream(), a);
+  else if (plan.nt == 4) tjh_launch((k_fp4_some<G, 1, 4, false>), grid, block, 0, stream(), a);
+  else if (plan.nt == 2) tjh_launch((k_fp4_some<G, 1, 2, false>), grid, block, 0, stream(), a);
+  else tjh_launch((k_fp4_some<G, 1, 1, false>), grid, block, 0, stream(), a);
+  if (sums)
+    tjh_launch(k_fp4_sums, dim3((unsigned)cdiv(a.N, 256), (unsigned)a.M), dim3(256), 0, stream(), a,
+               slices);
+  return check_launch("fp4_some");
+}
+
+// ---------------------------------------------------------------- many rows
 
 // 128 x 16 C of y a workgroup, 32 rows of it a wave.  A wave's parts of x come straight
 // from memory as its lanes feed them, one step of 32 columns ahead; codes and
@@ -524,6 +587,21 @@ void launch_gemm(const LinArgs& a) {
   else tjh_launch((k_fp4_gemm<G, C, false>), grid, block, 0, stream(), a);
 }
 
+// Column tiles of a workgroup of k_fp4_gemm, and what that costs, as for
+// k_fp4_some: by the column tiles of the CU that has most.
+struct Gemm {
+  int C;
+  int64_t cost;
+};
+Gemm plan_gemm(const LinArgs& a) {
+  const int64_t rows = cdiv(a.M, 128);
+  const auto load = [&](int C) { return cdiv(cdiv(a.N, 16 * C) * rows, num_cus()) * C; };
+  const int64_t l4 = load(4) * 5 / 4, l8 = load(8), l13 = load(13);
+  const auto plan = [&](int C, int64_t l) { return Gemm{C, l * a.nb * 7 / 2 + 150}; };
+  if (l13 <= l8 && l13 <= l4) return plan(13, l13);
+  return l8 <= l4 ? plan(8, l8) : plan(4, load(4) * 3 / 2);
+}
+
 template <int G>
 int many_rows(LinArgs a) {
   // a GB of parts at a time: long prompts in pieces of rows
@@ -549,23 +627,26 @@ int many_rows(LinArgs a) {
   tjh_launch(k_fp4_split, dim3((unsigned)cdiv(items, 256)), dim3(256), 0, stream(), a.x, a.ldx, a.M,
              a.K, (uint32_t)a.m_tiles, (uint32_t)items, s.as<uintx4>());
   a.parts = s.as<uintx4>();
-  // column tiles of the CU that has most
-  const auto load = [&](int C) { return cdiv(cdiv(a.N, 16 * C) * rows, num_cus()) * C; };
-  const int64_t l4 = load(4) * 5 / 4, l8 = load(8), l13 = load(13);
-  if (l13 <= l8 && l13 <= l4) launch_gemm<G, 13>(a);
-  else if (l8 <= l4) launch_gemm<G, 8>(a);
+  const int C = plan_gemm(a).C;
+  if (C == 13) launch_gemm<G, 13>(a);
+  else if (C == 8) launch_gemm<G, 8>(a);
   else launch_gemm<G, 4>(a);
   return check_launch("fp4_gemm");
 }
 
 template <int G>
 int product(const LinArgs& a) {
-  if (a.M <= 5) return few_rows<G>(a);
-  // chunks of 32 rows read the weights once each: for up to two of their
-  // workgroups a CU.  16384 x 4096, 64 rows 48 us (tiles of 128 rows: 64), 80 rows
-  // 68 (64); 4096 x 4096, 256 rows 48 (63), 384 rows 68 (65)
-  if (a.nb && cdiv(cdiv(a.M, 32) * cdiv(a.N, 64), num_cus()) > 2) return many_rows<G>(a);
-  return some_rows<G>(a);
+  const Some plan = plan_some(a);
+  // few rows of many columns take k_fp4_rows a barrier and a split for each 16
+  // blocks: 1000 x 8000, 2 rows 10.7 us (11.1 by slices), 4 rows 13.5 (10.9); 1000 x
+  // 16000, one row 15.5 (13.7)
+  if (a.M <= 5 && (plan.slices == 1 || (a.M + 1) * a.nb < 250)) return few_rows<G>(a);
+  // 50257 x 768, 64 rows 38 us by k_fp4_some and 41 by k_fp4_gemm, 96 rows 51 and 42;
+  // 4096 x 4096, 512 rows 62 and 66, 1024 117 and 95.  Over 210 sizes what is taken
+  // is 12% slower than the other at most.
+  const int64_t parts = plan.parts ? a.M * a.nb * 128 * 6 : 0;  // bytes
+  if (a.nb && (parts > (int64_t(1) << 30) || plan_gemm(a).cost < plan.cost)) return many_rows<G>(a);
+  return some_rows<G>(a, plan);
 }
 
 }  // namespace
@@ -582,7 +663,7 @@ int fp4_linear(const float* x, int64_t ldx, int64_t M, int64_t N, int64_t K, con
   TJH_ARG(y && (K == 0 || (x && codes && scales && aligned16(codes))),
           "tjh_fp4_linear: NULL or unaligned pointer");
   LinArgs a{x,   nullptr, codes, scales, bias, residual, y, ldx, ldy, ldr, M, N, K,
-            (int)cdiv(K, 128), 0, 0, act};
+            (int)cdiv(K, 128), 0, act, nullptr, 0};
   KernelScope ks("fp4_linear");
   if (group == 32) return product<32>(a);
   if (group == 64) return product<64>(a);
