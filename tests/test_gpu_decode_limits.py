@@ -1,0 +1,87 @@
+"""Where decoding's operators meet their limits: sums over many thousands of keys,
+infinities, values near the ends of floats, scores that differ by less than 64 bits
+hold, and what a program may put in the place of a model's parts."""
+import numpy as np
+import pytest
+
+from test_gpu_decode_ops import U, _new_cache, held
+
+gpu = pytest.mark.gpu
+
+
+def _attend_some(q, k, v, scale, picks):
+    """Causal attention in 64 bits of the queries (head, number) of q [H, Tq, D] over
+    k, v [Hkv, n, D], and each result's sum of weighted magnitudes and largest score."""
+    group, tq, n = q.shape[0] // k.shape[0], q.shape[1], k.shape[1]
+    out, size, far = [], [], []
+    for h, t in picks:
+        see = n - tq + t + 1
+        s = k[h // group, :see] @ q[h, t].astype(np.float64) * scale
+        p = np.exp(s - s.max())
+        p /= p.sum()
+        out.append(p @ v[h // group, :see])
+        size.append(p @ np.abs(v[h // group, :see]))
+        far.append(np.abs(s).max())
+    return np.array(out), np.array(size), np.array(far)
+
+
+# a wave with 16 rows and all keys; four waves that share them; slices of them
+LONG = [(16, 1, 1024, 32768, 32), (16, 1, 1024, 32768, 64), (16, 1, 1024, 32768, 80),
+        (16, 1, 1024, 16384, 128), (400, 400, 1, 4096, 32), (400, 400, 1, 4096, 64),
+        (400, 400, 1, 4096, 96), (400, 400, 1, 4096, 128), (2, 1, 3, 32768, 64)]
+
+
+@gpu
+@pytest.mark.parametrize("h,hkv,tq,n,d", LONG)
+@pytest.mark.parametrize("values", ["even", "positive"])
+def test_attention_sums_over_many_keys(torch, h, hkv, tq, n, d, values):
+    """Values with a mean, whose sums over the keys grow with their number."""
+    torch.manual_seed(n + d)
+    cache = _new_cache(torch, 1, hkv, n, d)
+    k, v = 0.3 * torch.randn(1, hkv, n, d), torch.randn(1, hkv, n, d)
+    v = v * 0.01 + 1.0 if values == "even" else v.exp()
+    torch.functional.cache_append_fp4(*cache, k, v, 0)
+    q = torch.randn(1, h, tq, d)
+    y = torch.functional.attention_fp4(q, *cache, n).numpy()[0]
+    picks = [(i, t) for i in sorted({0, h // 2, h - 1}) for t in sorted({0, tq // 3, tq - 1})]
+    kv = sorted({i * hkv // h for i, _ in picks})
+    kh, vh = ({i: held(x[0, i].numpy())[2] for i in kv} for x in (k, v))
+    qn, num, den = q.numpy()[0], 0.0, 0.0
+    for i, t in picks:
+        j = i * hkv // h
+        want, _, _ = _attend_some(qn[i:i + 1], kh[j][None], vh[j][None], np.float32(d ** -0.5), [(0, t)])
+        num += ((y[i, t] - want[0]) ** 2).sum()
+        den += (want[0] ** 2).sum()
+    # A sum of 16 tiles takes 48 instructions, each of which cuts off half a step (of
+    # 2 U) on average of a sum that grows to the whole: 24 U.  The float additions
+    # (of c tiles' sums, and of 128 weights before) round to either side: U / sqrt(3)
+    # of a growing sum each, three standard deviations of both sums together.
+    c = n / 512
+    tol = (24 + 3 / 3 ** 0.5 * (2 * (c / 3) ** 0.5 + (128 / 3) ** 0.5)) * U
+    assert np.sqrt(num / den) <= tol
+
+
+@gpu
+@pytest.mark.parametrize("h,hkv,tq,n,d", LONG[1:4] + LONG[5:])
+@pytest.mark.parametrize("slope", [6, -6])
+def test_attention_with_maxima_that_move_over_many_keys(torch, h, hkv, tq, n, d, slope):
+    """Scores that rise along the keys raise the maxima of sums already put aside;
+    falling ones leave them."""
+    rng = np.random.default_rng(n + d)
+    u = rng.standard_normal(d)
+    k = (np.linspace(-slope, slope, n)[:, None] * u + 0.1 * rng.standard_normal((n, d))).astype(np.float32)
+    v = rng.standard_normal((n, d)).astype(np.float32)
+    q = (u / d * rng.uniform(1, 3, (h, tq, 1)) + 0.1 / d * rng.standard_normal((h, tq, d))).astype(np.float32)
+    cache = _new_cache(torch, 1, hkv, n, d)
+    tk, tv = (torch.tensor(np.broadcast_to(x, (1, hkv, n, d)).copy()) for x in (k, v))
+    torch.functional.cache_append_fp4(*cache, tk, tv, 0)
+    y = torch.functional.attention_fp4(torch.tensor(q[None]), *cache, n, scale=2.0).numpy()[0]
+    kk, vv = held(k)[2][None], held(v)[2][None]
+    for i in sorted({0, h // 2, h - 1}):
+        for t in sorted({0, tq // 3, tq - 1}):
+            want, size, far = _attend_some(q[i:i + 1], kk, vv, 2.0, [(0, t)])
+            s = np.abs(kk[0]) @ np.abs(q[i, t].astype(np.float64)) * 2.0
+            # a score's roundings, of its products and of its distance from the
+            # maximum; the sums as above, no value's part off by more
+            off = ((d + 4) * s.max() + 4 * far[0]) * U
+            assert (np.abs(y[i, t] - want[0]) <= (2 * off + 2 * (48 + n / 512 + 128) * U) * size[0]).all()

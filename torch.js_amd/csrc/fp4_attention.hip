@@ -47,6 +47,13 @@ __device__ __forceinline__ int length_of(const AttArgs& a, int b) {
 //     three parts, so it feeds the same keys of V: eight words, one of each key,
 //     whose 8 x 8 codes are transposed in registers.
 //
+// A matrix instruction cuts off what does not reach a sum's last bit.  Over thousands
+// of keys a row's sum would outgrow what the third parts of P add to it, always to
+// the same side where V's columns have a mean: 7e-6 of the result at 32768 keys of a
+// wave.  So O (and the sum of the weights) goes on for kFold tiles only, and is then
+// rounded to the float sum of those before, which waits in LDS: 1e-7, for 1 to 3% of
+// the time over thousands of keys and none where a wave has fewer tiles.
+//
 // Running maxima are raised only when a score is 2^kSlack above them, the same in
 // the four lanes of a row; then the sums are rescaled.  A key takes 2 (D / 2 + 4)
 // bytes and three products for 2 D / 512 of a matrix instruction each, so up to 16
@@ -61,6 +68,7 @@ __device__ __forceinline__ int length_of(const AttArgs& a, int b) {
 // positions 10.7 us.
 constexpr float kSlack = 10.f;
 constexpr int kWaves = 4, kTile = 32;
+constexpr int kFold = 16;  // tiles; 8: 1% slower, 32: 1% faster at twice the error
 
 // NB: words of a key that a lane feeds, a quarter of its codes.
 template <int NB>
@@ -135,7 +143,7 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[NB], const uint8_t* p) 
 // SPLIT: the waves of a workgroup share 16 rows' keys, tile by tile; otherwise
 // each has rows of its own.
 template <int NB, bool SPLIT>
-__global__ __launch_bounds__(64 * kWaves, NB < 3 ? 3 : 2) void k_fp4_attend(AttArgs a) {
+__global__ __launch_bounds__(64 * kWaves, NB < 4 ? 3 : 2) void k_fp4_attend(AttArgs a) {
   typedef Dims<NB> Z;
   constexpr int NT = Z::NT, P = 16 * NB;
   const int lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4;
@@ -211,6 +219,21 @@ __global__ __launch_bounds__(64 * kWaves, NB < 3 ? 3 : 2) void k_fp4_attend(AttA
 #pragma unroll
   for (int d = 0; d < NT; ++d) o[d] = zero;
   float m = -INFINITY, l = 0.f;
+  // O and l of the tiles before the last fold, and by what maxima raised since scale
+  // them; SPLIT: then what the waves add up, a wave's in its own place
+  __shared__ floatx4 lds[kWaves][SPLIT ? 4 * (Z::DP + 4) : NT * 64];
+  __shared__ float lds_l[kWaves][64];
+  floatx4* const before = lds[w] + lane;
+  float raised = 1.f;
+  bool folded = false;
+  const auto add_before = [&] {
+    floatx4 f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) f[r] = __shfl(raised, 4 * j + r, 64);
+#pragma unroll
+    for (int d = 0; d < NT; ++d) o[d] += before[64 * d] * f;
+    l += lds_l[w][lane] * raised;
+  };
   const int step = SPLIT ? kTile * kWaves : kTile;
   int t0 = from + (SPLIT ? w * kTile : 0);
   if (t0 < to) {
@@ -233,75 +256,91 @@ __global__ __launch_bounds__(64 * kWaves, NB < 3 ? 3 : 2) void k_fp4_attend(AttA
       split8(x, q[t]);
     }
   }
-  for (; t0 < to; t0 += step) {
-    const int tn = t0 + step < to ? t0 + step : t0;  // the last tile is loaded twice
-    floatx4 s[2] = {zero, zero};
-    {
-      bf16x8 kf[2][NB];
-#pragma unroll
-      for (int y = 0; y < 2; ++y)
-#pragma unroll
-        for (int t = 0; t < NB; ++t) kf[y][t] = steps(kw[y][t]);
-#pragma unroll
-      for (int part = 2; part >= 0; --part)
-#pragma unroll
-        for (int t = 0; t < NB; ++t)
-#pragma unroll
-          for (int y = 0; y < 2; ++y)
-            s[y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[y][t], q[t][part], s[y], 0, 0, 0);
-    }
-    float p[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) p[e] = s[e >> 2][e & 3] * kscale[e >> 2][e & 3];
-    load_k(tn);
-    const bool masked = t0 + kTile > min(to, least);
-    if (masked) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int t = t0 + 16 * (e >> 2) + 4 * j + (e & 3);
-        if (t >= min(to, seen)) {
-          p[e] = -INFINITY;
-          vscale[e >> 2][e & 3] = 0.f;  // may be NaN
-        }
-      }
-    }
-    float top = p[0];
-#pragma unroll
-    for (int e = 1; e < 8; ++e) top = fmaxf(top, p[e]);
-    if (__any(top > m + kSlack)) {
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float up = fmaxf(m, top);
-      const float f = up == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - up);
-      m = up;
-      l *= f;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float fr = __shfl(f, 4 * j + r, 64);
-#pragma unroll
-        for (int d = 0; d < NT; ++d) o[d][r] *= fr;
-      }
-    }
-    const float ms = m == -INFINITY ? 0.f : m;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float y = __builtin_amdgcn_exp2f(p[e] - ms);
-      l += y;
-      p[e] = y * vscale[e >> 2][e & 3];
-    }
-    bf16x8 pp[3];
-    split8_finite(p, pp);
-    uint32_t v[NT];
-    transpose<NB>(vw, n, v);
-    load_v(tn);
-#pragma unroll
-    for (int d = 0; d < NT; d += 2) {  // two chains at a time
-      const bf16x8 vb[2] = {steps(v[d]), steps(v[d + 1])};
-#pragma unroll
-      for (int part = 2; part >= 0; --part)
+  while (t0 < to) {
+    const int stop = min(to, t0 + kFold * step);
+    for (; t0 < stop; t0 += step) {
+      const int tn = t0 + step < to ? t0 + step : t0;  // the last tile is loaded twice
+      floatx4 s[2] = {zero, zero};
+      {
+        bf16x8 kf[2][NB];
 #pragma unroll
         for (int y = 0; y < 2; ++y)
-          o[d + y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pp[part], vb[y], o[d + y], 0, 0, 0);
+#pragma unroll
+          for (int t = 0; t < NB; ++t) kf[y][t] = steps(kw[y][t]);
+#pragma unroll
+        for (int part = 2; part >= 0; --part)
+#pragma unroll
+          for (int t = 0; t < NB; ++t)
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+              s[y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[y][t], q[t][part], s[y], 0, 0, 0);
+      }
+      float p[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p[e] = s[e >> 2][e & 3] * kscale[e >> 2][e & 3];
+      load_k(tn);
+      const bool masked = t0 + kTile > min(to, least);
+      if (masked) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int t = t0 + 16 * (e >> 2) + 4 * j + (e & 3);
+          if (t >= min(to, seen)) {
+            p[e] = -INFINITY;
+            vscale[e >> 2][e & 3] = 0.f;  // may be NaN
+          }
+        }
+      }
+      float top = p[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) top = fmaxf(top, p[e]);
+      if (__any(top > m + kSlack)) {
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float up = fmaxf(m, top);
+        const float f = up == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - up);
+        m = up;
+        l *= f;
+        raised *= f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float fr = __shfl(f, 4 * j + r, 64);
+#pragma unroll
+          for (int d = 0; d < NT; ++d) o[d][r] *= fr;
+        }
+      }
+      const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = __builtin_amdgcn_exp2f(p[e] - ms);
+        l += y;
+        p[e] = y * vscale[e >> 2][e & 3];
+      }
+      bf16x8 pp[3];
+      split8_finite(p, pp);
+      uint32_t v[NT];
+      transpose<NB>(vw, n, v);
+      load_v(tn);
+#pragma unroll
+      for (int d = 0; d < NT; d += 2) {  // two chains at a time
+        const bf16x8 vb[2] = {steps(v[d]), steps(v[d + 1])};
+#pragma unroll
+        for (int part = 2; part >= 0; --part)
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+            o[d + y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pp[part], vb[y], o[d + y], 0, 0, 0);
+      }
+    }
+    if (folded) add_before();
+    if (t0 < to) {
+#pragma unroll
+      for (int d = 0; d < NT; ++d) {
+        before[64 * d] = o[d];
+        o[d] = zero;
+      }
+      lds_l[w][lane] = l;
+      l = 0.f;
+      raised = 1.f;
+      folded = true;
     }
   }
   l += __shfl_xor(l, 16, 64);
@@ -326,7 +365,7 @@ __global__ __launch_bounds__(64 * kWaves, NB < 3 ? 3 : 2) void k_fp4_attend(AttA
   };
   if constexpr (SPLIT) {
     __shared__ float sm[kWaves][16], sl[kWaves][16];
-    __shared__ float so[kWaves][16][Z::DP + 4];
+    float(*const so)[16][Z::DP + 4] = reinterpret_cast<float(*)[16][Z::DP + 4]>(lds);
     if (lane < 16) {
       sm[w][n] = m;
       sl[w][n] = l;
