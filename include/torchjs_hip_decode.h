@@ -65,7 +65,8 @@ int tjh_fp4_cache_read(const uint8_t* codes, const float* scales, const uint8_t*
  * multiple of Hkv; query head h reads head h / (H / Hkv)): the queries are the
  * last Tq of the first `length` positions, or of lengths[b] (taken into [0, L])
  * of sequence b.  The query at position i sees the keys j <= i; one that sees
- * none (at a position before the first) gives zeros.  o = softmax(scale q k^T) v
+ * none (at a position before the first) gives zeros; one all of whose scores are
+ * -infinity has no distribution and gives NaN.  o = softmax(scale q k^T) v
  * [B, H, Tq, D]; strides of q and o for the B, H and T axes, D contiguous.  What
  * positions past a sequence's length hold has no part in it. */
 int tjh_fp4_attention(const float* q, const uint8_t* k_codes, const float* k_scales,

@@ -85,3 +85,35 @@ def test_attention_with_maxima_that_move_over_many_keys(torch, h, hkv, tq, n, d,
             # maximum; the sums as above, no value's part off by more
             off = ((d + 4) * s.max() + 4 * far[0]) * U
             assert (np.abs(y[i, t] - want[0]) <= (2 * off + 2 * (48 + n / 512 + 128) * U) * size[0]).all()
+
+
+@gpu
+@pytest.mark.parametrize("b,h,hkv,tq,n,d", [
+    (1, 1, 1, 1, 3, 1), (2, 3, 3, 5, 40, 64), (2, 4, 2, 1, 1500, 80), (1, 2, 2, 40, 1100, 32),
+    (2, 16, 16, 512, 530, 32), (32, 16, 16, 17, 30, 128)])
+def test_attention_of_infinite_queries(torch, b, h, hkv, tq, n, d):
+    """Where all scores that a query sees are -infinity, or one is +infinity, there is
+    no distribution: NaN.  A query that sees no key gives zeros all the same, and the
+    other queries are what they are without it."""
+    rng = np.random.default_rng(n)
+    cache = _new_cache(torch, b, hkv, n, d)
+    k, v = rng.standard_normal((2, b, hkv, n, d)).astype(np.float32)
+    k[..., 0] = -1 - np.abs(k[..., 0])  # not held as zeros, beside values of up to some units
+    assert (held(k)[2][..., 0] < 0).all()
+    torch.functional.cache_append_fp4(*cache, torch.tensor(k), torch.tensor(v), 0)
+    lengths = np.full(b, n, np.int32)
+    lengths[b - 1] = n if b == 1 else tq // 2  # some queries there see nothing
+    q = rng.standard_normal((b, h, tq, d)).astype(np.float32)
+    plain = torch.functional.attention_fp4(torch.tensor(q), *cache, torch.tensor(lengths, dtype="int32")).numpy()
+    assert not np.isnan(plain).any()
+    sees = (lengths[:, None] - tq + np.arange(tq) >= 0)[:, None, :]
+    for sign in (1, -1):
+        odd = rng.random((b, h, tq)) < 0.5
+        odd[0, 0, 0] = True
+        q2 = q.copy()
+        q2[..., 0] = np.where(odd, sign * np.float32(np.inf), q[..., 0])
+        y = torch.functional.attention_fp4(torch.tensor(q2), *cache,
+                                           torch.tensor(lengths, dtype="int32")).numpy()
+        assert np.isnan(y[odd & sees]).all()
+        assert (y[odd & ~sees] == 0).all()
+        assert np.array_equal(y[~odd], plain[~odd])

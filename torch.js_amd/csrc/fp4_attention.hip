@@ -351,9 +351,9 @@ __global__ __launch_bounds__(64 * kWaves, NB < 4 ? 3 : 2) void k_fp4_attend(AttA
     if (at >= rows || d >= a.D) return;
     if (a.slices == 1) {
       const int hh = at / a.Tq, t = at - hh * a.Tq;
-      // no key seen: zeros
+      // zeros where no key is seen, NaN where all scores are -infinity
       a.o[b * a.ob + (int64_t)(kh * a.group + hh) * a.oh + t * a.ot + d] =
-          den == 0.f ? 0.f : num / den;
+          len - a.Tq + t < 0 ? 0.f : num / den;
     } else {
       const int64_t p = ((int64_t)bh * rows + at) * a.slices + slice;
       a.po[p * a.D + d] = num;
@@ -422,7 +422,8 @@ __global__ __launch_bounds__(128) void k_fp4_join(AttArgs a) {
   const int64_t bh = row / a.Tq;
   const int t = (int)(row - bh * a.Tq);
   const int64_t b = bh / a.H, h = bh - b * a.H;
-  a.o[b * a.ob + h * a.oh + t * a.ot + d] = den == 0.f ? 0.f : num / den;
+  const bool none = length_of(a, (int)b) - a.Tq + t < 0;
+  a.o[b * a.ob + h * a.oh + t * a.ot + d] = none ? 0.f : num / den;
 }
 
 template <int NB>

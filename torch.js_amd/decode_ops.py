@@ -278,7 +278,8 @@ def attention_fp4(query, k_codes, k_scales, v_codes, v_scales, length, scale=Non
     h // (H // Hkv)).  The queries are the last Tq of the cache's first `length`
     positions (already in the cache), or of length[b] of sequence b (an int32
     tensor [B], taken into [0, L]); one that sees no key, before the first
-    position, gives zeros.  What later positions hold has no part in the result.
+    position, gives zeros, and one all of whose scores are -infinity NaN.  What
+    later positions hold has no part in the result.
     Sums are float32 (a key's before its scale: for queries under 2^118 in
     magnitude); D up to 128.  For inference: a query that needs a gradient is
     refused."""
