@@ -68,7 +68,10 @@ int tjh_fp4_cache_read(const uint8_t* codes, const float* scales, const uint8_t*
  * none (at a position before the first) gives zeros; one all of whose scores are
  * -infinity has no distribution and gives NaN.  o = softmax(scale q k^T) v
  * [B, H, Tq, D]; strides of q and o for the B, H and T axes, D contiguous.  What
- * positions past a sequence's length hold has no part in it. */
+ * positions past a sequence's length hold has no part in it.  Sums are float32:
+ * a key's before its scale, for |q| under 2^118; a row's, of weights up to 2^10
+ * times the values of up to 2^24 positions, before it is divided by the sum of
+ * the weights, for values under 2^94. */
 int tjh_fp4_attention(const float* q, const uint8_t* k_codes, const float* k_scales,
                       const uint8_t* v_codes, const float* v_scales, float* o, int64_t B,
                       int64_t H, int64_t Hkv, int64_t Tq, int64_t L, int64_t D,

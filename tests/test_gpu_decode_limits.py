@@ -117,3 +117,33 @@ def test_attention_of_infinite_queries(torch, b, h, hkv, tq, n, d):
         assert np.isnan(y[odd & sees]).all()
         assert (y[odd & ~sees] == 0).all()
         assert np.array_equal(y[~odd], plain[~odd])
+
+
+@gpu
+@pytest.mark.parametrize("far", [2.0 ** 94, 2.0 ** -99])
+@pytest.mark.parametrize("n,tq", [(2 ** 24 - 1, 1), (32768, 1), (2000, 1), (4096, 20000)])
+def test_attention_of_the_largest_and_smallest_values(torch, n, tq, far):
+    """Values just inside the range, of one sign, over the longest cache: in every
+    part of the keys the first tiles' scores are as far below the rest as leaves the
+    running maximum where it is, so that weights are as large as they can be."""
+    d = 32
+    cache = _new_cache(torch, 1, 1, n, d)
+    scale = np.float32(far * (1 - 2.0 ** -20) / 6)
+    cache[0].fill_(0x22)  # every column 1
+    cache[2].fill_(0x77)  # every column 6
+    cache[3].fill_(float(scale))
+    # scores of 9.75 in powers of two, but 0 at the start of each run of 512 keys
+    # (slices are longer than that, and a wave's tiles 32 keys)
+    k_scales = np.full(n + 512, 9.75 / 32 * np.log(2), np.float32)
+    k_scales.reshape(-1)[:(n + 511) // 512 * 512].reshape(-1, 512)[::1 if tq > 1 else 8, :128] = 0
+    cache[1].copy_(torch.tensor(k_scales[:n].reshape(1, 1, n)))
+    q = torch.ones(1, 1, tq, d)
+    y = torch.functional.attention_fp4(q, *cache, torch.tensor(np.full(1, n, np.int32), dtype="int32")
+                                       if tq > n else n, scale=1.0).numpy()[0, 0]
+    want = 6 * float(scale)
+    assert np.isfinite(y).all()
+    # equal values, so no error of a weight counts: cut-offs and float sums of 16
+    # tiles, of up to 16 of those, and of up to 512 slices, numerator and denominator
+    tol = 2 * (48 + 128 + 16 + 512) * U * want
+    sees = np.arange(tq) - tq + n >= 0
+    assert (np.abs(y[sees] - want) <= tol).all() and (y[~sees] == 0).all()

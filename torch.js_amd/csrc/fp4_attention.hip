@@ -54,8 +54,9 @@ __device__ __forceinline__ int length_of(const AttArgs& a, int b) {
 // rounded to the float sum of those before, which waits in LDS: 1e-7, for 1 to 3% of
 // the time over thousands of keys and none where a wave has fewer tiles.
 //
-// Running maxima are raised only when a score is 2^kSlack above them, the same in
-// the four lanes of a row; then the sums are rescaled.  A key takes 2 (D / 2 + 4)
+// Running maxima are raised only when a score is kSlack above them, the same in the
+// four lanes of a row; then the sums are rescaled.  So a weight is up to 2^kSlack, and
+// a row's sum finite for 2^24 keys with values under 2^94.  A key takes 2 (D / 2 + 4)
 // bytes and three products for 2 D / 512 of a matrix instruction each, so up to 16
 // rows (a group's heads, or some queries) cost as much as one.
 //

@@ -281,8 +281,9 @@ def attention_fp4(query, k_codes, k_scales, v_codes, v_scales, length, scale=Non
     position, gives zeros, and one all of whose scores are -infinity NaN.  What
     later positions hold has no part in the result.
     Sums are float32 (a key's before its scale: for queries under 2^118 in
-    magnitude); D up to 128.  For inference: a query that needs a gradient is
-    refused."""
+    magnitude; a row's before its weights are divided by their sum: for values
+    under 2^94 in the cache); D up to 128.  For inference: a query that needs a
+    gradient is refused."""
     who = "attention_fp4"
     qs = query._shape
     if len(qs) != 4:
