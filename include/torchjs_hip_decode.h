@@ -81,7 +81,8 @@ int tjh_fp4_attention(const float* q, const uint8_t* k_codes, const float* k_sca
 /* One step of a beam search: of the continuations (w, v) of a search's W beams
  * by V tokens, with scores[b, w] + x[v] - ln sum exp x (x the beam's row of
  * logits [B, W, V] at row stride ld), the `keep` largest in descending order,
- * equal ones by ascending (w, v): scores, tokens, parents (w), all [B, keep].  A
+ * equal ones by ascending w, of a beam by descending x, then by ascending v:
+ * scores, tokens, parents (w), all [B, keep].  A
  * beam with finished[b, w] != 0 (finished may be NULL) goes on as (eos, its
  * score) alone.  out_finished: the parent's flag, or 1 where the token is eos
  * (eos < 0: no such token, finished must be NULL).  A beam whose score is

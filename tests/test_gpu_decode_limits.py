@@ -147,3 +147,29 @@ def test_attention_of_the_largest_and_smallest_values(torch, n, tq, far):
     tol = 2 * (48 + 128 + 16 + 512) * U * want
     sees = np.arange(tq) - tq + n >= 0
     assert (np.abs(y[sees] - want) <= tol).all() and (y[~sees] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("b,w,n", [(1, 1, 2), (1, 1, 3), (2, 3, 9), (1, 4, 2500), (40, 8, 1300),
+                                   (2, 16, 50257), (1, 64, 5000)])
+@pytest.mark.parametrize("levels", [5, 1000])
+def test_beam_step_of_logits_nearer_than_a_score(torch, b, w, n, levels):
+    """Logits that differ by less than the last bit of a 64-bit score: equal scores, by
+    beam, then by logit, then by token; fewer beams are the first of more."""
+    rng = np.random.default_rng(n)
+    x = (np.float32(1e-20) * (rng.integers(0, levels, (b, w, n)) - levels // 2)).astype(np.float32)
+    x[:, :, 1:n // 2:1 + n // 3] = rng.choice(np.float32([-2, 0, 1]), x[:, :, 1:n // 2:1 + n // 3].shape)
+    x[:] = x[:, :1]  # equal rows: beams that tie
+    scores = np.full((b, w), -2.0, np.float32)
+    size = x + np.float32(1) - np.float32(1)  # as scores tell logits apart
+    flat = [a.reshape(b, -1) for a in
+            np.broadcast_arrays(-size, np.arange(w)[None, :, None], -x, np.arange(n)[None, None, :])]
+    most = min(64, w * n)
+    got = [a.numpy() for a in torch.functional.beam_step(torch.tensor(x), torch.tensor(scores), most)]
+    for i in range(b):
+        order = np.lexsort([a[i] for a in flat[::-1]])[:most]
+        assert (got[1][i] == order % n).all() and (got[2][i] == order // n).all()
+    for keep in sorted({1, 2, 5, w} & set(range(most))):
+        few = torch.functional.beam_step(torch.tensor(x), torch.tensor(scores), keep)
+        for a, c in zip(few, got):
+            assert np.array_equal(a.numpy(), c[:, :keep])

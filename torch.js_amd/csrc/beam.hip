@@ -6,7 +6,9 @@
 // the `keep` largest.  Within a beam their order is that of the logits, so each
 // workgroup of the first kernel takes the largest logits of a piece of a row, with
 // the piece's maximum and sum of exponentials, and one workgroup a search then
-// compares the scores of those in 64 bits.
+// compares the scores of those in 64 bits.  Logits that differ by less than such a
+// score holds keep their order within a beam, in which a piece hands them on: so the
+// first continuations are the same for every `keep`.
 #include "rowreg.h"
 
 #include <math.h>
@@ -121,7 +123,7 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(BeamArgs a) {
   __shared__ int chosen[kMaxBeams];
   __shared__ u64 early[kEarly * kMergeThreads];
   __shared__ u64 key[kMaxEntries];  // the lists' heads, then the entries
-  __shared__ int flat[kMaxEntries];
+  __shared__ int place[kMaxEntries];  // an entry's: list keep + i
   __shared__ u64 bound;
   __shared__ int count;
   const int t = threadIdx.x, lists = a.W * a.S;
@@ -172,53 +174,61 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(BeamArgs a) {
       if (t + kMergeThreads * i < all) early[t + kMergeThreads * i] = pre[i];
   }
   __syncthreads();
-  const auto entry = [&](int list, int i, int* at) -> u64 {  // i-th of a list: key, w V + v
+  const auto candidate = [&](int at) { return few ? early[at] : cand[at]; };
+  const auto entry = [&](int list, int i) -> u64 {  // the i-th of a list
     const int w = list / a.S, piece = list - w * a.S;
     if (state[w] == 2) return 0;
-    if (state[w] == 1) {
-      *at = w * a.V + a.eos;
-      return piece == 0 && i == 0 ? score_key(from[w]) : 0;
-    }
+    if (state[w] == 1) return piece == 0 && i == 0 ? score_key(from[w]) : 0;
     if (i >= min(a.keep, min(a.per, a.V - piece * a.per))) return 0;
-    const u64 c = few ? early[list * a.keep + i] : cand[(int64_t)list * a.keep + i];
-    const int v = index_of(c);
-    *at = w * a.V + v;
-    return score_key(from[w] + (double)key_value((uint32_t)(c >> 32)));
+    return score_key(from[w] + (double)key_value((uint32_t)(candidate(list * a.keep + i) >> 32)));
   };
-  int at;
-  for (int i = t; i < lists; i += kMergeThreads) key[i] = entry(i, 0, &at);
+  // how many entries j in [0, n), at the places at(j), come before the i-th: of equal
+  // scores by beam, then as the logits order them (an ended beam has one entry)
+  const auto rank_of = [&](int i, int n, const auto& at) {
+    const u64 me = key[i];
+    int rank = 0, same = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) {
+      rank += key[j] > me;
+      same += key[j] == me;
+    }
+    if (same > 1) {
+      const int w = at(i) / (a.S * a.keep);
+      for (int j = 0; j < n; ++j) {
+        if (j == i || key[j] != me) continue;
+        const int o = at(j) / (a.S * a.keep);
+        rank += o < w || (o == w && candidate(at(j)) > candidate(at(i)));
+      }
+    }
+    return rank;
+  };
+  for (int i = t; i < lists; i += kMergeThreads) key[i] = entry(i, 0);
   __syncthreads();
   for (int i = t; i < lists; i += kMergeThreads) {
-    const u64 me = key[i];
-    int rank = 0;
-#pragma unroll 8
-    for (int j = 0; j < lists; ++j) rank += key[j] > me || (key[j] == me && j < i);
+    if (key[i] == 0) continue;
+    const int rank = rank_of(i, lists, [&](int j) { return j * a.keep; });
     if (rank < a.keep) chosen[rank] = i;
-    if (rank == a.keep - 1) bound = me;
+    if (rank == a.keep - 1) bound = key[i];
   }
   __syncthreads();
   for (int i = t; i < a.keep * a.keep; i += kMergeThreads) {
     const int list = chosen[i / a.keep];
     if (list < 0) continue;
-    const u64 k = entry(list, i % a.keep, &at);
+    const u64 k = entry(list, i % a.keep);
     if (k != 0 && k >= bound) {
       const int to = atomicAdd(&count, 1);
       key[to] = k;
-      flat[to] = at;
+      place[to] = list * a.keep + i % a.keep;
     }
   }
   __syncthreads();
   const int n = count;
   const int64_t o = (int64_t)blockIdx.x * a.keep;
   for (int i = t; i < n; i += kMergeThreads) {
-    const u64 me = key[i];
-    const int f = flat[i];
-    int rank = 0;
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) rank += key[j] > me || (key[j] == me && flat[j] < f);
+    const int rank = rank_of(i, n, [&](int j) { return place[j]; });
     if (rank >= a.keep) continue;
-    const int w = f / a.V, v = f - w * a.V;
-    a.out_scores[o + rank] = (float)key_score(me);
+    const int w = place[i] / (a.S * a.keep), v = state[w] == 1 ? a.eos : index_of(candidate(place[i]));
+    a.out_scores[o + rank] = (float)key_score(key[i]);
     a.tokens[o + rank] = v;
     a.parents[o + rank] = w;
     a.out_finished[o + rank] = v == a.eos || state[w] == 1;

@@ -328,7 +328,9 @@ def beam_step(logits, scores, beams=None, finished=None, eos=None):
     [B, W, V] (or [B * W, V]) of the beams' next tokens and their scores [B, W],
     sums of logarithms of probabilities.  Of the continuations (w, v), which
     have score scores[w] + log_softmax(logits[w])[v], takes the `beams` (W
-    unless given) largest, equal ones by ascending (w, v).  Returns (scores,
+    unless given) largest.  Scores are compared in 64 bits; equal ones go by
+    ascending w, of a beam by descending logit, then by ascending v, whatever
+    `beams` is.  Returns (scores,
     tokens, parents, finished), each [B, beams]: int32 tokens and the beams that
     they continue, and whether the new beam has ended, as its token is `eos` or
     its parent had ended.  finished [B, W] (bool): a beam that has ended goes on
