@@ -4,7 +4,7 @@ hold, and what a program may put in the place of a model's parts."""
 import numpy as np
 import pytest
 
-from test_gpu_decode_ops import U, _new_cache, held
+from test_gpu_decode_ops import U, _new_cache, _shape_only, held
 
 gpu = pytest.mark.gpu
 
@@ -173,3 +173,44 @@ def test_beam_step_of_logits_nearer_than_a_score(torch, b, w, n, levels):
         few = torch.functional.beam_step(torch.tensor(x), torch.tensor(scores), keep)
         for a, c in zip(few, got):
             assert np.array_equal(a.numpy(), c[:, :keep])
+
+
+# ------------------------------------------------- what a program puts in place
+
+
+class _Closed:
+    """The library where nothing is to be called."""
+
+    def __getattr__(self, name):
+        raise AssertionError("%s was called" % name)
+
+
+@pytest.mark.parametrize("value,error", [
+    (np.full((6, 64), 3.7, np.float32), TypeError), (np.full((6, 64), 3.0), TypeError),
+    (np.full((6, 64), 256), ValueError), (np.full((6, 64), -1), ValueError),
+    (np.full((6, 64), "a"), TypeError), ("float32", TypeError), ("int32", TypeError)])
+def test_codes_of_another_type_are_not_converted(pkg, monkeypatch, value, error):
+    from torchjs_amd import _lib
+    m = pkg.nn.Module()
+    m.register_parameter("codes", _shape_only(pkg, 6, 64, dtype="uint8"))
+    if isinstance(value, str):
+        value = _shape_only(pkg, 6, 64, dtype=value, ptr=8192)
+    monkeypatch.setattr(_lib, "lib", _Closed)
+    with pytest.raises(error):
+        m.load_state_dict({"codes": value})
+
+
+@gpu
+def test_states_of_other_types(torch):
+    """Whole numbers that a type holds, and any numbers for floats."""
+    m = torch.nn.LinearFP4(70, 6, group_size=32)
+    codes = np.random.default_rng(0).integers(0, 256, (6, 64))
+    m.load_state_dict({"codes": codes, "scales": np.arange(24).reshape(6, 4), "bias": [1, 2, 3, 4, 5, 6]})
+    assert (m.codes.numpy() == codes).all() and m.codes.dtype == "uint8"
+    assert (m.scales.numpy() == np.arange(24).reshape(6, 4)).all() and m.scales.dtype == "float32"
+    assert m.bias.numpy().tolist() == [1, 2, 3, 4, 5, 6]
+    m.load_state_dict({"bias": torch.tensor(np.arange(6, dtype=np.int32)),
+                       "scales": np.full((6, 4), 0.1)})
+    assert m.bias.numpy().tolist() == list(range(6)) and (m.scales.numpy() == np.float32(0.1)).all()
+    with pytest.raises(ValueError):
+        m.load_state_dict({"codes": codes[:, :32]})

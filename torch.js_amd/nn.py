@@ -109,16 +109,31 @@ class Module:
             if name not in params:
                 raise KeyError("unexpected key %s in state_dict" % name)
             tgt = params[name]
-            src = value if isinstance(value, Tensor) else \
-                from_numpy(np.asarray(value), dtype=tgt.dtype)
-            if src.dtype != tgt.dtype:
-                src = src.to(tgt.dtype)
+            src = _state_value(name, value, tgt.dtype)
             if tuple(src.shape) != tgt.shape:
                 raise ValueError("size mismatch for %s: %s vs %s" % (name, list(src.shape),
                                                                    list(tgt.shape)))
             from .tensor import _copy_into
             _copy_into(tgt, src)
         return self
+
+
+def _state_value(name, value, dtype):
+    """A state's value as a tensor of its parameter's type.  Numbers become
+    float32; a parameter of whole numbers (4-bit codes) takes only those that
+    its type holds."""
+    if isinstance(value, Tensor):
+        if value.dtype != dtype and dtype != "float32":
+            raise TypeError("%s holds %s, got a tensor of %s" % (name, dtype, value.dtype))
+        return value.to(dtype)
+    a = np.asarray(value)
+    if a.dtype.kind not in ("fiub" if dtype == "float32" else "iub"):
+        raise TypeError("%s holds %s, got values of %s" % (name, dtype, a.dtype))
+    if dtype != "float32" and a.size:
+        lo, hi = {"uint8": (0, 255), "bool": (0, 1), "int32": (-2 ** 31, 2 ** 31 - 1)}[dtype]
+        if a.min() < lo or a.max() > hi:
+            raise ValueError("%s holds %s, got values from %s to %s" % (name, dtype, a.min(), a.max()))
+    return from_numpy(a, dtype=dtype)
 
 
 class Linear(Module):
