@@ -214,3 +214,39 @@ def test_states_of_other_types(torch):
     assert m.bias.numpy().tolist() == list(range(6)) and (m.scales.numpy() == np.float32(0.1)).all()
     with pytest.raises(ValueError):
         m.load_state_dict({"codes": codes[:, :32]})
+
+
+@gpu
+def test_a_subclass_of_linear_keeps_the_fused_layers(torch, monkeypatch):
+    """One that changes nothing takes the products with the GELU and the residual
+    in them, forward and backward; one with a forward of its own is called."""
+    from torchjs_amd import workloads as W
+    F, nn = torch.functional, torch.nn
+    mine = type("Mine", (nn.Linear,), {})
+    twice = type("Twice", (nn.Linear,), {"forward": lambda self, x: nn.Linear.forward(self, x) * 2.0})
+    x = np.random.default_rng(0).standard_normal((2, 9, 64)).astype(np.float32)
+    seen = []
+    for name in ("_linear_add", "_mlp_gelu"):
+        real = getattr(F, name)
+        monkeypatch.setattr(F, name, lambda *a, real=real, name=name: seen.append(name) or real(*a))
+
+    def run(kind):
+        torch.manual_seed(1)
+        blk = W.Block(64, 2)
+        if kind is not None:
+            for m, part in ((blk.attn, "c_proj"), (blk.mlp, "c_fc"), (blk.mlp, "c_proj")):
+                old = getattr(m, part)
+                new = kind(old.in_features, old.out_features)
+                new.load_state_dict(old.state_dict())
+                setattr(m, part, new)
+        del seen[:]
+        t = torch.tensor(x, requires_grad=True)
+        y = blk(t)
+        (y * y).sum().backward()
+        return [y.numpy(), t.grad.numpy()] + [p.grad.numpy() for p in blk.parameters()], list(seen)
+    want, calls = run(None)
+    assert calls == ["_linear_add", "_mlp_gelu"]
+    got, same = run(mine)
+    assert same == calls and all(np.array_equal(a, b) for a, b in zip(got, want))
+    got, none = run(twice)
+    assert none == [] and not np.array_equal(got[0], want[0])
