@@ -250,3 +250,22 @@ def test_a_subclass_of_linear_keeps_the_fused_layers(torch, monkeypatch):
     assert same == calls and all(np.array_equal(a, b) for a, b in zip(got, want))
     got, none = run(twice)
     assert none == [] and not np.array_equal(got[0], want[0])
+
+
+@gpu
+def test_quantized_model_with_subclasses_of_linear(torch):
+    """One that changes nothing is held in 4 bits as nn.Linear is, one with a forward
+    of its own stays."""
+    from torchjs_amd import workloads as W
+    nn = torch.nn
+    mine = type("Mine", (nn.Linear,), {})
+    twice = type("Twice", (nn.Linear,), {"forward": lambda self, x: nn.Linear.forward(self, x) * 2.0})
+    m = W.GPT2(50, 8, 64, 2, 1)
+    m.h[0].attn.c_attn, m.h[0].mlp.c_fc = mine(64, 192), twice(64, 256)
+    want = m.h[0].attn.c_attn.weight.numpy()
+    m.quantize_fp4(32)
+    four = m.h[0].attn.c_attn
+    assert type(four) is nn.LinearFP4 and type(m.h[0].mlp.c_fc) is twice
+    got = torch.functional.dequantize_fp4(four.codes, four.scales, 64, 32).numpy()
+    assert (got == held(want.reshape(192, 2, 32))[2].reshape(192, 64).astype(np.float32)).all()
+    assert m(torch.tensor(np.zeros((1, 8), np.int32))).shape == (1, 8, 50)

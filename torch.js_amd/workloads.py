@@ -377,13 +377,14 @@ class GPT2(nn.Module):
         self.head = None  # the LM head in 4 bits (quantize_fp4)
 
     def quantize_fp4(self, group_size=64, head=True):
-        """Holds the blocks' linear layers in 4 bits (nn.LinearFP4), and with
-        `head` a 4-bit copy of the token table for the logits; the tables that
-        tokens and positions are looked up in stay float."""
+        """Holds the blocks' linear layers in 4 bits (nn.LinearFP4; a layer with a
+        forward of its own stays as it is), and with `head` a 4-bit copy of the
+        token table for the logits; the tables that tokens and positions are
+        looked up in stay float."""
         for blk in self.h:
             for m, name in ((blk.attn, "c_attn"), (blk.attn, "c_proj"), (blk.mlp, "c_fc"),
                             (blk.mlp, "c_proj")):
-                if type(getattr(m, name)) is nn.Linear:
+                if _plain_linear(getattr(m, name)):
                     setattr(m, name, nn.LinearFP4.of(getattr(m, name), group_size))
         if head:
             self.head = nn.LinearFP4.of(self.wte, group_size)
