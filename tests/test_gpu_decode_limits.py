@@ -269,3 +269,28 @@ def test_quantized_model_with_subclasses_of_linear(torch):
     got = torch.functional.dequantize_fp4(four.codes, four.scales, 64, 32).numpy()
     assert (got == held(want.reshape(192, 2, 32))[2].reshape(192, 64).astype(np.float32)).all()
     assert m(torch.tensor(np.zeros((1, 8), np.int32))).shape == (1, 8, 50)
+
+
+def test_a_window_and_a_cache_in_four_bits(pkg, monkeypatch):
+    """Refused before the library is called, wherever the two meet."""
+    from torchjs_amd import _lib, workloads as W
+
+    def make(kind, **kw):
+        m = kind.__new__(kind)
+        pkg.nn.Module.__init__(m)
+        for name, value in kw.items():
+            setattr(m, name, value)
+        return m
+    attn = make(W.CausalSelfAttention, window=8, sinks=0, d=64, heads=2, fused=True)
+    blk = make(W.Block, attn=attn)
+    model = make(W.GPT2, h=[make(W.Block, attn=make(W.CausalSelfAttention, window=None, d=64, heads=2)), blk],
+                 ctx=16, vocab=50)
+    cache = W.KVCacheFP4.__new__(W.KVCacheFP4)
+    x, ids = _shape_only(pkg, 1, 4, 64), _shape_only(pkg, 1, 4, dtype="int32")
+    monkeypatch.setattr(_lib, "lib", _Closed)
+    for call in (lambda: model.new_cache(1, bits=4), lambda: model.forward_cached(ids, cache, 0),
+                 lambda: blk.forward_cached(x, cache, 0, 0), lambda: attn.forward_cached(x, cache, 0, 0),
+                 lambda: model.generate(ids, 3, cache_bits=4),
+                 lambda: model.generate(ids, 3, beams=2, cache_bits=4)):
+        with pytest.raises(NotImplementedError):
+            call()

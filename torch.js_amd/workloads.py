@@ -60,6 +60,14 @@ def _plain_linear(m):
         kind.__call__ is nn.Linear.__call__
 
 
+def _check_cache(cache, *attns):
+    """Refuses, before anything is launched, a cache that the attention layers do
+    not read."""
+    if isinstance(cache, KVCacheFP4) or cache is KVCacheFP4:
+        if any(getattr(a, "window", None) is not None for a in attns):
+            raise NotImplementedError("KV cache in 4 bits: not with a window")
+
+
 class CausalSelfAttention(nn.Module):
     """With `window`, each position sees the last `window` positions and the
     first `sinks` ones (F.sliding_window_attention) in place of all earlier
@@ -96,6 +104,7 @@ class CausalSelfAttention(nn.Module):
         causal over itself; a single new token attends to every cached
         position.  With a window, or a cache in 4 bits, a prompt may also
         come in parts."""
+        _check_cache(cache, self)
         B, T, C = x.shape
         hd = C // self.heads
         q, k, v = self.c_attn(x).split(C, dim=2)
@@ -103,8 +112,6 @@ class CausalSelfAttention(nn.Module):
         k = k.view(B, T, self.heads, hd).transpose(1, 2)
         v = v.view(B, T, self.heads, hd).transpose(1, 2)
         if isinstance(cache, KVCacheFP4):
-            if self.window is not None:
-                raise NotImplementedError("KV cache in 4 bits: not with a window")
             cache.append(layer, k, v, pos)
             y = cache.attend(layer, q, pos + T)
             y = y.transpose(1, 2).contiguous().view(B, T, C)
@@ -271,6 +278,7 @@ class Block(nn.Module):
         return y
 
     def forward_cached(self, x, cache, layer, pos):
+        _check_cache(cache, self.attn)
         if not is_grad_enabled():
             y = self._infer(x, cache, layer, pos)
             if y is not None:
@@ -423,12 +431,14 @@ class GPT2(nn.Module):
             raise ValueError("a KV cache holds 32 or 4 bits, got %r" % (bits,))
         blk = self.h[0].attn
         kind = KVCache if bits == 32 else KVCacheFP4
+        _check_cache(kind, *[getattr(b, "attn", None) for b in self.h])
         return kind(len(self.h), batch, blk.heads, max_len or self.ctx, blk.d // blk.heads)
 
     def forward_cached(self, ids, cache, pos):
         """Logits of positions [pos, pos + T) of ids [B, T], the keys and
         values of earlier positions read from (and these appended to) the
         cache."""
+        _check_cache(cache, *[getattr(b, "attn", None) for b in self.h])
         x = self._embed(ids, pos)
         for i, blk in enumerate(self.h):
             x = blk.forward_cached(x, cache, i, pos)
