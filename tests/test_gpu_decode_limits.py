@@ -294,3 +294,38 @@ def test_a_window_and_a_cache_in_four_bits(pkg, monkeypatch):
                  lambda: model.generate(ids, 3, beams=2, cache_bits=4)):
         with pytest.raises(NotImplementedError):
             call()
+
+
+@gpu
+def test_models_with_a_head_of_their_own(torch):
+    """A subclass's `head`, a layer or a method, has no part in the model's logits, and
+    it keeps it when its layers are held in 4 bits."""
+    from torchjs_amd import workloads as W
+
+    class Own(W.GPT2):
+        def __init__(self, *a):
+            super().__init__(*a)
+            self.head = torch.nn.Linear(64, 3)
+
+    class Method(W.GPT2):
+        def head(self, ids):
+            return 7
+
+    def make(kind):
+        torch.manual_seed(4)
+        return kind(50, 16, 64, 2, 1)
+    plain, own, method = make(W.GPT2), make(Own), make(Method)
+    ids = torch.tensor(np.arange(8, dtype=np.int32).reshape(2, 4))
+    assert method.head(ids) == 7
+    for m in (own, method):
+        assert np.array_equal(m(ids).numpy(), plain(ids).numpy())
+        for kw in (dict(greedy=True), dict(beams=2)):
+            assert np.array_equal(m.generate(ids, 5, **kw).numpy(), plain.generate(ids, 5, **kw).numpy())
+        before = m.h[0].attn.c_attn
+        with pytest.raises(ValueError):
+            m.quantize_fp4()
+        assert m.h[0].attn.c_attn is before
+        m.quantize_fp4(head=False)
+        assert np.array_equal(m(ids).numpy(), make(W.GPT2).quantize_fp4(head=False)(ids).numpy())
+    assert type(own.head) is torch.nn.Linear and plain.head is None
+    assert type(plain.quantize_fp4().quantize_fp4().head) is torch.nn.LinearFP4

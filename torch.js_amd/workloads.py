@@ -373,6 +373,8 @@ class GPT2(nn.Module):
     """GPT-2 with the LM head tied to the token embedding; with `window` and
     `sinks`, attention over a sliding window (CausalSelfAttention)."""
 
+    head = None  # the LM head in 4 bits (quantize_fp4); a subclass's own is not used here
+
     def __init__(self, vocab=50257, ctx=1024, d=768, heads=12, layers=12, fused=True, window=None,
                  sinks=0):
         super().__init__()
@@ -382,13 +384,14 @@ class GPT2(nn.Module):
         self.wpe = nn.Embedding(ctx, d)
         self.h = nn.ModuleList([Block(d, heads, fused, window, sinks) for _ in range(layers)])
         self.ln_f = nn.LayerNorm(d)
-        self.head = None  # the LM head in 4 bits (quantize_fp4)
 
     def quantize_fp4(self, group_size=64, head=True):
         """Holds the blocks' linear layers in 4 bits (nn.LinearFP4; a layer with a
         forward of its own stays as it is), and with `head` a 4-bit copy of the
         token table for the logits; the tables that tokens and positions are
         looked up in stay float."""
+        if head and self.head is not None and not isinstance(self.head, nn.LinearFP4):
+            raise ValueError("quantize_fp4: the model has another head; pass head=False")
         for blk in self.h:
             for m, name in ((blk.attn, "c_attn"), (blk.attn, "c_proj"), (blk.mlp, "c_fc"),
                             (blk.mlp, "c_proj")):
@@ -399,7 +402,7 @@ class GPT2(nn.Module):
         return self
 
     def _logits(self, x):
-        return F.linear(x, self.wte.weight) if self.head is None else self.head(x)
+        return self.head(x) if isinstance(self.head, nn.LinearFP4) else F.linear(x, self.wte.weight)
 
     def forward(self, ids):
         x = self._embed(ids, 0)
