@@ -329,3 +329,21 @@ def test_models_with_a_head_of_their_own(torch):
         assert np.array_equal(m(ids).numpy(), make(W.GPT2).quantize_fp4(head=False)(ids).numpy())
     assert type(own.head) is torch.nn.Linear and plain.head is None
     assert type(plain.quantize_fp4().quantize_fp4().head) is torch.nn.LinearFP4
+
+
+@gpu
+def test_a_model_with_caches_of_its_own(torch):
+    """A new_cache that knows of no bits, as models had before there were any."""
+    from torchjs_amd import workloads as W
+
+    class Own(W.GPT2):
+        def new_cache(self, batch, max_len=None):
+            return W.KVCache(len(self.h), batch, 2, max_len, 32)
+
+    def make(kind):
+        torch.manual_seed(4)
+        return kind(50, 16, 64, 2, 1)
+    plain, own = make(W.GPT2), make(Own)
+    ids = torch.tensor(np.arange(8, dtype=np.int32).reshape(2, 4))
+    for kw in (dict(greedy=True), dict(top_k=1), dict(beams=2)):
+        assert np.array_equal(own.generate(ids, 5, **kw).numpy(), plain.generate(ids, 5, **kw).numpy())

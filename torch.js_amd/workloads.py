@@ -480,7 +480,8 @@ class GPT2(nn.Module):
         cut = any(isinstance(s, Tensor) or np.ndim(s) for s in rules) or \
             temperature == 0 or top_k != 0 or top_p != 1.0 or min_p != 0.0
         with no_grad():
-            cache = self.new_cache(B, total, cache_bits)
+            # (a model's own new_cache may know of no bits)
+            cache = self.new_cache(B, total, *([] if cache_bits == 32 else [cache_bits]))
             logits = self.forward_cached(ids, cache, 0)
             out = [ids]
             pos = T
@@ -517,9 +518,10 @@ class GPT2(nn.Module):
         if not count:
             return ids if ids.dtype == "int32" else ids.to("int32")
         with no_grad():
-            prompt = self.new_cache(B, T, cache_bits)
+            bits = [] if cache_bits == 32 else [cache_bits]
+            prompt = self.new_cache(B, T, *bits)
             logits = self.forward_cached(ids, prompt, 0)[:, -1, :]
-            cache = self.new_cache(B * beams, T + count, cache_bits)
+            cache = self.new_cache(B * beams, T + count, *bits)
             cache.spread(prompt, T)
             scores, tokens, parents, done = F.beam_step(logits, zeros(B, 1), beams, None, eos)
             steps = [(tokens, parents)]
