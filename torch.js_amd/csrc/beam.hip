@@ -109,6 +109,21 @@ __device__ __forceinline__ double key_score(u64 k) {
 }
 
 constexpr int kMaxBeams = 64, kMaxEntries = kMaxBeams * kMaxBeams;
+constexpr int kTokenBits = 20;
+
+// The order of continuations of equal scores as one integer, the first one's the
+// largest: ascending beams, then descending logits, then ascending tokens.
+__device__ __forceinline__ u64 tie_of(int w, uint32_t logit, int v) {
+  const uint32_t last = (1u << kTokenBits) - 1;
+  return ((u64)(kMaxBeams - 1 - w) << (32 + kTokenBits)) | ((u64)logit << kTokenBits) | (last - v);
+}
+__device__ __forceinline__ int beam_of(u64 tie) {
+  return kMaxBeams - 1 - (int)(tie >> (32 + kTokenBits));
+}
+__device__ __forceinline__ int token_of(u64 tie) {
+  const uint32_t last = (1u << kTokenBits) - 1;
+  return last - ((uint32_t)tie & last);
+}
 constexpr int kMergeThreads = 512;
 constexpr int kEarly = 3;  // candidates a thread, read before anything else is known
 
@@ -123,7 +138,7 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(BeamArgs a) {
   __shared__ int chosen[kMaxBeams];
   __shared__ u64 early[kEarly * kMergeThreads];
   __shared__ u64 key[kMaxEntries];  // the lists' heads, then the entries
-  __shared__ int place[kMaxEntries];  // an entry's: list keep + i
+  __shared__ u64 tie[kMaxEntries];
   __shared__ u64 bound;
   __shared__ int count;
   const int t = threadIdx.x, lists = a.W * a.S;
@@ -174,39 +189,36 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(BeamArgs a) {
       if (t + kMergeThreads * i < all) early[t + kMergeThreads * i] = pre[i];
   }
   __syncthreads();
-  const auto candidate = [&](int at) { return few ? early[at] : cand[at]; };
-  const auto entry = [&](int list, int i) -> u64 {  // the i-th of a list
+  const auto entry = [&](int list, int i, u64* at) -> u64 {  // the i-th of a list: key, tie
     const int w = list / a.S, piece = list - w * a.S;
     if (state[w] == 2) return 0;
-    if (state[w] == 1) return piece == 0 && i == 0 ? score_key(from[w]) : 0;
+    if (state[w] == 1) {
+      *at = tie_of(w, 0, a.eos);
+      return piece == 0 && i == 0 ? score_key(from[w]) : 0;
+    }
     if (i >= min(a.keep, min(a.per, a.V - piece * a.per))) return 0;
-    return score_key(from[w] + (double)key_value((uint32_t)(candidate(list * a.keep + i) >> 32)));
+    const u64 c = few ? early[list * a.keep + i] : cand[(int64_t)list * a.keep + i];
+    *at = tie_of(w, (uint32_t)(c >> 32), index_of(c));
+    return score_key(from[w] + (double)key_value((uint32_t)(c >> 32)));
   };
-  // how many entries j in [0, n), at the places at(j), come before the i-th: of equal
-  // scores by beam, then as the logits order them (an ended beam has one entry)
-  const auto rank_of = [&](int i, int n, const auto& at) {
-    const u64 me = key[i];
-    int rank = 0, same = 0;
+  // how many of the entries [0, n) come before the i-th; without a branch, so that
+  // the reads go on: 4096 entries in 0.9 ms, with one 2.2 (3.4 where all are equal)
+  const auto rank_of = [&](int i, int n) {
+    const u64 me = key[i], mine = tie[i];
+    int rank = 0;
 #pragma unroll 8
-    for (int j = 0; j < n; ++j) {
-      rank += key[j] > me;
-      same += key[j] == me;
-    }
-    if (same > 1) {
-      const int w = at(i) / (a.S * a.keep);
-      for (int j = 0; j < n; ++j) {
-        if (j == i || key[j] != me) continue;
-        const int o = at(j) / (a.S * a.keep);
-        rank += o < w || (o == w && candidate(at(j)) > candidate(at(i)));
-      }
-    }
+    for (int j = 0; j < n; ++j) rank += (key[j] > me) | ((key[j] == me) & (tie[j] > mine));
     return rank;
   };
-  for (int i = t; i < lists; i += kMergeThreads) key[i] = entry(i, 0);
+  u64 at = 0;
+  for (int i = t; i < lists; i += kMergeThreads) {
+    key[i] = entry(i, 0, &at);
+    tie[i] = at;
+  }
   __syncthreads();
   for (int i = t; i < lists; i += kMergeThreads) {
     if (key[i] == 0) continue;
-    const int rank = rank_of(i, lists, [&](int j) { return j * a.keep; });
+    const int rank = rank_of(i, lists);
     if (rank < a.keep) chosen[rank] = i;
     if (rank == a.keep - 1) bound = key[i];
   }
@@ -214,20 +226,20 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(BeamArgs a) {
   for (int i = t; i < a.keep * a.keep; i += kMergeThreads) {
     const int list = chosen[i / a.keep];
     if (list < 0) continue;
-    const u64 k = entry(list, i % a.keep);
+    const u64 k = entry(list, i % a.keep, &at);
     if (k != 0 && k >= bound) {
       const int to = atomicAdd(&count, 1);
       key[to] = k;
-      place[to] = list * a.keep + i % a.keep;
+      tie[to] = at;
     }
   }
   __syncthreads();
   const int n = count;
   const int64_t o = (int64_t)blockIdx.x * a.keep;
   for (int i = t; i < n; i += kMergeThreads) {
-    const int rank = rank_of(i, n, [&](int j) { return place[j]; });
+    const int rank = rank_of(i, n);
     if (rank >= a.keep) continue;
-    const int w = place[i] / (a.S * a.keep), v = state[w] == 1 ? a.eos : index_of(candidate(place[i]));
+    const int w = beam_of(tie[i]), v = token_of(tie[i]);
     a.out_scores[o + rank] = (float)key_score(key[i]);
     a.tokens[o + rank] = v;
     a.parents[o + rank] = w;
