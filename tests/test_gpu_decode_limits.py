@@ -9,6 +9,14 @@ from test_gpu_decode_ops import U, _new_cache, _shape_only, held
 gpu = pytest.mark.gpu
 
 
+@pytest.fixture
+def large(torch):
+    """For tests of large tensors: their memory does not stay in the allocator's
+    cache, whose blocks others' workspaces would be counted by."""
+    yield
+    torch.hip.empty_cache()
+
+
 def _attend_some(q, k, v, scale, picks):
     """Causal attention in 64 bits of the queries (head, number) of q [H, Tq, D] over
     k, v [Hkv, n, D], and each result's sum of weighted magnitudes and largest score."""
@@ -34,7 +42,7 @@ LONG = [(16, 1, 1024, 32768, 32), (16, 1, 1024, 32768, 64), (16, 1, 1024, 32768,
 @gpu
 @pytest.mark.parametrize("h,hkv,tq,n,d", LONG)
 @pytest.mark.parametrize("values", ["even", "positive"])
-def test_attention_sums_over_many_keys(torch, h, hkv, tq, n, d, values):
+def test_attention_sums_over_many_keys(torch, large, h, hkv, tq, n, d, values):
     """Values with a mean, whose sums over the keys grow with their number."""
     torch.manual_seed(n + d)
     cache = _new_cache(torch, 1, hkv, n, d)
@@ -64,7 +72,7 @@ def test_attention_sums_over_many_keys(torch, h, hkv, tq, n, d, values):
 @gpu
 @pytest.mark.parametrize("h,hkv,tq,n,d", LONG[1:4] + LONG[5:])
 @pytest.mark.parametrize("slope", [6, -6])
-def test_attention_with_maxima_that_move_over_many_keys(torch, h, hkv, tq, n, d, slope):
+def test_attention_with_maxima_that_move_over_many_keys(torch, large, h, hkv, tq, n, d, slope):
     """Scores that rise along the keys raise the maxima of sums already put aside;
     falling ones leave them."""
     rng = np.random.default_rng(n + d)
@@ -122,7 +130,7 @@ def test_attention_of_infinite_queries(torch, b, h, hkv, tq, n, d):
 @gpu
 @pytest.mark.parametrize("far", [2.0 ** 94, 2.0 ** -99])
 @pytest.mark.parametrize("n,tq", [(2 ** 24 - 1, 1), (32768, 1), (2000, 1), (4096, 20000)])
-def test_attention_of_the_largest_and_smallest_values(torch, n, tq, far):
+def test_attention_of_the_largest_and_smallest_values(torch, large, n, tq, far):
     """Values just inside the range, of one sign, over the longest cache: in every
     part of the keys the first tiles' scores are as far below the rest as leaves the
     running maximum where it is, so that weights are as large as they can be."""
