@@ -130,8 +130,8 @@ constexpr int kEarly = 3;  // candidates a thread, read before anything else is 
 // One workgroup a search.  The lists (a beam's pieces) are in order, so only the
 // `keep` lists with the best heads matter, and of those only what is not below the
 // last of these heads; some tens of entries, ranked by counting.  A chain of reads
-// of what other CUs wrote, barriers and 64-bit logarithms: 6 us for one search with
-// four beams, 9 us for 32 with eight.
+// of what other CUs wrote, barriers and 64-bit logarithms: 5.7 us for one search
+// with four beams, 5.9 us for 32 with eight.
 __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(BeamArgs a) {
   __shared__ double from[kMaxBeams];  // a beam's score less its logarithm of the sum
   __shared__ int state[kMaxBeams];    // 0 goes on, 1 finished, 2 has no continuation

@@ -61,10 +61,10 @@ __device__ __forceinline__ int length_of(const AttArgs& a, int b) {
 // rows (a group's heads, or some queries) cost as much as one.
 //
 // Bound for one query by reading the cache: 32 sequences of 4096 to 8192 positions,
-// 32 heads over 8 of 128, 217 MB: 50.5 us, 4.3 TB/s (with float multiply-adds in
+// 32 heads over 8 of 128, 217 MB: 51 us, 4.3 TB/s (with float multiply-adds in
 // place of the matrix cores 131); for many by issuing some 260 vector instructions
 // a tile beside its 42 to 48 products: the last 1999 of 4095 positions, 16 heads
-// over 4 of 80: 192 us, 165 TFLOP/s, more than the float matrix cores' 154 (by
+// over 4 of 80: 178 us, 178 TFLOP/s, more than the float matrix cores' 154 (by
 // float multiply-adds 1600).  Few short sequences by latency: 48 heads of 64, 1000
 // positions 10.7 us.
 constexpr float kSlack = 10.f;
