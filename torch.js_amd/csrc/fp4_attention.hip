@@ -51,7 +51,7 @@ __device__ __forceinline__ int length_of(const AttArgs& a, int b) {
 // of keys a row's sum would outgrow what the third parts of P add to it, always to
 // the same side where V's columns have a mean: 7e-6 of the result at 32768 keys of a
 // wave.  So O (and the sum of the weights) goes on for kFold tiles only, and is then
-// rounded to the float sum of those before, which waits in LDS: 1e-7, for 1 to 3% of
+// rounded to the float sum of those before, which waits in LDS: 1e-7, for up to 3% of
 // the time over thousands of keys and none where a wave has fewer tiles.
 //
 // Running maxima are raised only when a score is kSlack above them, the same in the
